@@ -65,12 +65,20 @@ _PROTOTYPES: dict[str, list] = {
     "gdn2_packed_sizes": [_P] + [_I64] * 3 + [_P] * 3,
     "gdn2_packed_forward": [_P] * 14 + [_I64] * 3 + [_INT] * 3 + [_F32, _INT, _P],
     "gdn2_packed_backward": [_P] * 22 + [_I64] * 3 + [_INT, _INT, _F32, _P],
+    "gdn2_rotary": [_P] * 8 + [_I64] * 8 + [_INT] * 3 + [_P],
+    "gdn2_append_tokens": [_P] * 6 + [_I64] * 5 + [_INT, _P],
+    "gdn2_tree_workspace_bytes": [_I64] * 4,
+    "gdn2_tree_attention": [_P] * 11 + [_I64] * 10 + [_INT, _F32, _P],
+    "gdn2_attention_stat_rows": [_P] + [_I64] * 2,
+    "gdn2_attention_forward": [_P] * 7 + [_I64] * 5 + [_INT, _F32, _P],
+    "gdn2_attention_backward": [_P] * 12 + [_I64] * 5 + [_INT, _F32, _P],
     "gdn2_profile_enable": [_INT],
     "gdn2_profile_chunk_kernels": [_P] * 4,
 }
 _RESTYPES = {"gdn2_status_string": ctypes.c_char_p, "gdn2_last_cuda_error": ctypes.c_char_p,
              "gdn2_chunk_workspace_bytes": ctypes.c_int64, "gdn2_chunk_scratch_bytes": ctypes.c_int64,
-             "gdn2_tensor_maps_encoded": ctypes.c_int64}
+             "gdn2_tensor_maps_encoded": ctypes.c_int64, "gdn2_tree_workspace_bytes": ctypes.c_int64,
+             "gdn2_attention_stat_rows": ctypes.c_int64}
 
 
 def library_path() -> pathlib.Path:
@@ -159,6 +167,12 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 def ptr(tensor: torch.Tensor | None) -> int | None:
     return None if tensor is None else tensor.data_ptr()
+
+
+def int64s(*values: int) -> ctypes.Array:
+    """A host array of 64-bit integers (strides, bounds); it lives as long as the call that takes it."""
+
+    return (ctypes.c_int64 * len(values))(*values)
 
 
 def stream_ptr(device: torch.device) -> int:

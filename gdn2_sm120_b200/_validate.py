@@ -114,6 +114,46 @@ def byte_span(tensor: torch.Tensor) -> tuple[int, int]:
     return lo, lo + tensor.numel() * tensor.element_size()
 
 
+def extent(tensor: torch.Tensor) -> tuple[int, int]:
+    """Half-open byte interval from the first to the last element of a strided tensor."""
+
+    lo = tensor.data_ptr()
+    if tensor.numel() == 0:
+        return lo, lo
+    return lo, lo + (sum((n - 1) * s for n, s in zip(tensor.shape, tensor.stride())) + 1) * tensor.element_size()
+
+
+def heads_tensor(name: str, tensor, device, dtype) -> None:
+    """Validate one ``[B, T, H, D]`` operand of attention: a view is fine where every row of channels is 16-byte
+    aligned (the kernels' tiled copies need that) and no two elements share a place."""
+
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if tensor.ndim != 4:
+        raise ValueError(f"{name} must be a rank-4 [B, T, H, D] tensor")
+    if dtype not in _LOW_PRECISION:
+        raise TypeError("attention takes torch.float16 or torch.bfloat16")
+    if tensor.dtype != dtype:
+        raise TypeError(f"{name} must have q's dtype")
+    if not tensor.is_cuda or tensor.device != device:
+        raise ValueError("all inputs must be CUDA tensors on the same device")
+    dim = tensor.shape[3]
+    if not 0 < dim <= 128 or dim % 8:
+        raise NotImplementedError("attention takes head dimensions that are multiples of 8, up to 128")
+    if tensor.stride(3) != 1:
+        raise ValueError(f"the channels of {name} must be contiguous")
+    if tensor.data_ptr() % 16 or any(n > 1 and (s <= 0 or s % 8) for n, s in zip(tensor.shape[:3], tensor.stride())):
+        raise ValueError(f"every row of {name} must be 16-byte aligned and have a place of its own")
+
+
+def head_strides(tensor: torch.Tensor) -> tuple[int, int, int]:
+    """Batch, token and head stride in elements; a dimension of size 1 gets that of a contiguous tensor."""
+
+    _, time, heads, dim = tensor.shape
+    dense = (time * heads * dim, heads * dim, dim)
+    return tuple(d if n <= 1 else s for n, s, d in zip(tensor.shape, tensor.stride(), dense))
+
+
 def spans_overlap(left: tuple[int, int], right: tuple[int, int]) -> bool:
     """True when two non-empty half-open intervals intersect."""
 

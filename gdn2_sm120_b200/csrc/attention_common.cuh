@@ -1,0 +1,195 @@
+// What the kernels of causal attention share: which rows a work item has, tensor maps, products of 16-bit operands.
+#pragma once
+
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "chunk_common.cuh"
+#include "tc05.cuh"
+
+namespace gdn2 {
+namespace attn {
+
+constexpr int kTileRows = 256;   // query rows of a work item of the forward: two tiles of 128
+constexpr int kMaxSequences = GDN2_PACKED_MAX_SEQUENCES;   // in a launch, whose parameters hold their table
+
+// Sequences of one launch: `n` equally long ones (a [n, time] batch), or the entries of a table, longest first.  Row
+// statistics (one float a query row) lie per head in tiles of 256 rows; tile numbers run through all sequences.
+struct Sequences {
+  struct Entry { int row0, len, tile0, pad; };
+  int n, time, packed;        // time: rows of a sequence where not packed
+  int tiles, tiles_each;      // of all, of one where not packed
+  int64_t stat_rows;          // rows of a head's statistics: of all launches of a call
+  int64_t stat_row0;          // of this launch
+  Entry e[kMaxSequences];
+};
+
+struct Item {
+  int row0, batch;   // where the sequence's first row is in the tensor maps
+  int len, tile;     // of the sequence; number of the 256-row tile in it
+  int64_t row;       // first row of the sequence in [rows][heads][dim]
+  int64_t stat;      // first row of the sequence's statistics
+};
+
+// tile t of the launch; `last_first`: a sequence's last tiles come first
+__device__ __forceinline__ Item find_item(const Sequences& s, int t, bool last_first) {
+  Item it;
+  if (!s.packed) {
+    const int tile = t / s.n;
+    it.batch = t - tile * s.n;
+    it.tile = last_first ? s.tiles_each - 1 - tile : tile;
+    it.row0 = 0;
+    it.len = s.time;
+    it.row = int64_t(it.batch) * s.time;
+    it.stat = s.stat_row0 + int64_t(it.batch) * s.tiles_each * kTileRows;
+    return it;
+  }
+  int lo = 0, hi = s.n - 1;
+  while (lo < hi) {  // last entry with tile0 <= t
+    const int mid = (lo + hi + 1) >> 1;
+    if (s.e[mid].tile0 <= t) lo = mid; else hi = mid - 1;
+  }
+  const Sequences::Entry x = s.e[lo];
+  const int each = (x.len + kTileRows - 1) / kTileRows, tile = t - x.tile0;
+  it.batch = 0;
+  it.tile = last_first ? each - 1 - tile : tile;
+  it.row0 = x.row0;
+  it.len = x.len;
+  it.row = x.row0;
+  it.stat = s.stat_row0 + int64_t(x.tile0) * kTileRows;
+  return it;
+}
+
+// Items are in the order of their work, the longest first.  CTA c of n takes them by turns that go up and down, c,
+// 2n - 1 - c, 2n + c, ...: the sums come out nearly equal without a counter.
+__device__ __forceinline__ int64_t item_of_turn(int turn) {
+  const int64_t n = gridDim.x, c = blockIdx.x;
+  return turn * n + ((turn & 1) ? n - 1 - c : c);
+}
+
+// Waits of a CTA are bounded: whoever waits in vain says so, and all others stop waiting too.
+struct Waiter {
+  volatile int* failed;
+  // by whole warps, whose lanes agree on what came of it
+  __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) const {
+    return __all_sync(0xffffffffu, tc::mbar_try_wait(bar, parity) || wait_on(bar, parity));
+  }
+  __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity) const {
+#pragma unroll 1
+    for (uint32_t i = 0; i < (1u << 20); ++i) {
+      if (tc::mbar_try_wait(bar, parity)) return true;
+      if ((i & 63) == 63 && *failed) return false;
+    }
+    *failed = 1;
+    return false;
+  }
+};
+
+// Registers move from the warps that copy and issue to those that compute; the sum stays what the CTA was launched with.
+template <int N>
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// ---- 16-bit products ---------------------------------------------------------------------------------------
+// Tiles of [rows][64] channels in lines of 128 bytes whose 16-byte pieces are permuted by the line (the 128-byte
+// swizzle of the tiled copies); a tile of 128 channels is two of them.  One copy serves both ways of reading it:
+//   K-major (contraction over channels): 8-line atoms, 1024 bytes apart; 16 channels are 32 bytes of a line.
+//   MN-major (contraction over rows): an atom is 64 channels x 8 rows; 16 rows are 2048 bytes; the next 64 channels
+//   are the next slab.
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile, uint32_t slab_bytes, int kstep) {
+  return tc::smem_desc_at(tile, uint32_t(kstep >> 2) * slab_bytes + uint32_t(kstep & 3) * 32u, 16, 1024, 2);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, uint32_t slab_bytes, int kstep) {
+  return tc::smem_desc_at(tile, uint32_t(kstep) * 2048u, slab_bytes, 1024, 2);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t id, uint32_t accumulate,
+                                       uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(id), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t id, uint32_t accumulate,
+                                       uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(id), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+
+template <typename T> struct Format;
+template <> struct Format<__nv_bfloat16> { static constexpr uint32_t code = tc::kFmtBF16, exponent = 0x7f80u; };
+template <> struct Format<__half> { static constexpr uint32_t code = tc::kFmtF16, exponent = 0x7c00u; };
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  const typename Pair<T>::type v = Pair<T>::make(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// [batch][rows][heads][dim] with any strides that are multiples of 16 bytes, in boxes of 64 channels x box_rows rows
+// of one head.  Channels from dim on and rows behind a batch entry's last one arrive as zeros.
+inline bool encode_heads_map(CUtensorMap* tm, const void* base, const int64_t* strides, int64_t batch, int64_t rows,
+                             int64_t heads, int dim, int dtype, int box_rows) {
+  const cuuint64_t dims[4] = {cuuint64_t(dim), cuuint64_t(heads), cuuint64_t(rows), cuuint64_t(batch)};
+  const cuuint64_t bytes[3] = {cuuint64_t(strides[2]) * 2, cuuint64_t(strides[1]) * 2, cuuint64_t(strides[0]) * 2};
+  const cuuint32_t box[4] = {64, 1, cuuint32_t(box_rows), 1};
+  return encode_cached(tm, 4, dtype == GDN2_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                       base, dims, bytes, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// rows of a head's statistics for all sequences of a call
+inline int64_t stat_rows(const int64_t* bounds, int64_t n_seq, int64_t time) {
+  auto padded = [](int64_t n) { return (n + kTileRows - 1) / kTileRows * kTileRows; };
+  if (bounds == nullptr) return n_seq * padded(time);
+  int64_t rows = 0;
+  for (int64_t i = 0; i < n_seq; ++i) rows += padded(bounds[i + 1] - bounds[i]);
+  return rows;
+}
+
+// The launches of a call: one for a batch of equally long sequences (bounds null, `time` rows each), one for every
+// kMaxSequences packed ones.  Fills *s for each and calls launch(); it follows from the bounds alone, so that forward
+// and backward agree on where a row's statistics are.
+template <typename Launch>
+inline int for_groups(const int64_t* bounds, int64_t n_seq, int64_t time, Sequences* s, Launch launch) {
+  s->stat_rows = stat_rows(bounds, n_seq, time);
+  s->stat_row0 = 0;
+  if (bounds == nullptr) {
+    s->packed = 0;
+    s->n = int(n_seq);
+    s->time = int(time);
+    s->tiles_each = int((time + kTileRows - 1) / kTileRows);
+    s->tiles = s->tiles_each * s->n;
+    return launch();
+  }
+  s->packed = 1;
+  s->time = 0;
+  s->tiles_each = 0;
+  for (int64_t first = 0; first < n_seq; first += kMaxSequences) {
+    const int count = int(n_seq - first < kMaxSequences ? n_seq - first : kMaxSequences);
+    const int64_t* b = bounds + first;
+    int order[kMaxSequences];
+    for (int i = 0; i < count; ++i) order[i] = i;
+    std::stable_sort(order, order + count, [&](int x, int y) { return b[x + 1] - b[x] > b[y + 1] - b[y]; });
+    s->n = s->tiles = 0;
+    for (int i = 0; i < count; ++i) {
+      const int len = int(b[order[i] + 1] - b[order[i]]);
+      if (len == 0) break;   // sorted: nothing but empty ones from here on
+      s->e[s->n++] = Sequences::Entry{int(b[order[i]]), len, s->tiles, 0};
+      s->tiles += (len + kTileRows - 1) / kTileRows;
+    }
+    if (s->n > 0) {
+      const int status = launch();
+      if (status != GDN2_OK) return status;
+    }
+    s->stat_row0 += int64_t(s->tiles) * kTileRows;
+  }
+  return GDN2_OK;
+}
+
+}  // namespace attn
+}  // namespace gdn2

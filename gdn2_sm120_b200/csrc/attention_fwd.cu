@@ -1,0 +1,411 @@
+// Causal attention over whole prompts, forward, on the tensor cores.
+//
+//   s_ij = scale q_i . k_j (j <= i)    m_i = max_j s_ij    o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i)
+//
+// One pass over keys and values with a running maximum and sum.  A work item is 256 query rows of one head, two tiles
+// of 128, against tiles of 128 keys.  The two tiles take turns: while the tensor cores form one's O += P V and next
+// S = Q K^T, four warps turn the other's S into P, a row a thread.  Bound by both at once: a tile of 128 x 128 x 128
+// takes the tensor cores 1024 clocks for its two products and the special-function unit 1024 for its exponentials.
+//
+// TMEM (512 columns): S0 S1 O0 O1, 128 each; P (16-bit) overlays the first half of its S and is the A operand of P V
+// from there.  Products are issued in an order that needs no further waits: S_t(j+1) after O_t += P_t(j) V, so an S
+// that has arrived says that the O before it has, too.  O is scaled down only when a row's maximum has grown by 2^8
+// since the last time (weights stay below 2^8, sums in 32 bits), by the row's own thread.
+
+#include "attention_common.cuh"
+
+namespace gdn2 {
+namespace attn {
+
+namespace {
+
+constexpr int kThreads = 384;    // warps 0-3, 4-7: the rows of the two tiles; 8: products; 9: copies; 10, 11: look at values
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescale = 8.f;  // in powers of two
+
+template <int DP>
+struct FwdConfig {
+  static constexpr int kTileBytes = 128 * DP * 2;
+  static constexpr int kSlab = 128 * 128;               // 64 channels of 128 rows
+  static constexpr int kStages = DP == 128 ? 5 : 8;
+  static constexpr int kBytes = (2 + kStages) * kTileBytes + 1024 /* alignment */ + 512;
+};
+
+struct FwdParams {
+  CUtensorMap q, k, v;
+  void* out;
+  float* lse;          // [heads][stat rows] in powers of two, or null
+  int heads, kv_heads, group, dim, turns;
+  int64_t items;
+  float scale_log2;    // positive
+  uint32_t negate;     // the scale is negative: Q counts with its sign changed
+  Sequences seq;
+};
+
+struct FwdBars {
+  uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2];
+  uint64_t raw;        // a tile that is mended before the products may read it
+  uint64_t drained;
+  uint64_t kv_full[8], kv_empty[8];
+  uint32_t tmem;
+  int failed;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __grid_constant__ FwdParams p) {
+  using C = FwdConfig<DP>;
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_tiles = smem;
+  uint8_t* kv_tiles = smem + 2 * C::kTileBytes;
+  FwdBars& bar = *reinterpret_cast<FwdBars*>(smem + (2 + C::kStages) * C::kTileBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      tc::mbar_init(&bar.q_full[t], 1);
+      tc::mbar_init(&bar.q_empty[t], 1);
+      tc::mbar_init(&bar.s_full[t], 1);
+      tc::mbar_init(&bar.p_ready[t], 4);
+      tc::mbar_init(&bar.o_full[t], 1);
+    }
+    tc::mbar_init(&bar.raw, 1);
+    tc::mbar_init(&bar.drained, 1);
+    for (int s = 0; s < C::kStages; ++s) {
+      tc::mbar_init(&bar.kv_full[s], 1);
+      tc::mbar_init(&bar.kv_empty[s], 1);
+    }
+    bar.failed = 0;
+    tc::fence_mbar_init();
+  }
+  if (warp == 8) {
+    tc::tmem_alloc(&bar.tmem, 512);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = bar.tmem;
+  const Waiter waiter{&bar.failed};
+
+  // an item's head, rows and numbers of key tiles
+  auto item_at = [&](int64_t index, int* head) {
+    const int t = int(index / p.heads);
+    *head = int(index - int64_t(t) * p.heads);
+    return find_item(p.seq, t, true);
+  };
+  auto key_tiles = [](const Item& it, int t) {  // of the first or second query tile
+    const int tile = 2 * it.tile + t;
+    return tile * 128 < it.len ? tile + 1 : 0;
+  };
+
+  // 384 threads of 168 registers = 256 of 208 + 128 of 88
+  if (warp >= 8) {
+    give_registers<88>();
+    if (warp == 9) {
+      // ---- copies ------------------------------------------------------------------------------------------
+      const uint32_t leader = tc::elect_leader();
+      int filled = 0, loaded[2] = {0, 0}, mended = 0;
+      bool ok = true;
+      auto load = [&](const CUtensorMap* map, uint8_t* to, int head, int row, int batch, uint64_t* full) {
+        tc::mbar_arrive_expect_tx(full, C::kTileBytes, leader);
+  #pragma unroll
+        for (int slab = 0; slab < DP / 64; ++slab) {
+          tc::tma_load_4d(to + slab * C::kSlab, map, slab * 64, head, row, batch, full, leader);
+        }
+      };
+      for (int turn = 0; turn < p.turns && ok; ++turn) {
+        const int64_t index = item_of_turn(turn);
+        if (index >= p.items) continue;
+        int head;
+        const Item it = item_at(index, &head);
+        const int kv_head = head / p.group;
+        const int n = max(key_tiles(it, 0), key_tiles(it, 1));
+        for (int j = 0; j < n && ok; ++j) {
+          if (j == 0) {
+            for (int t = 0; t < 2 && ok; ++t) {
+              if (key_tiles(it, t) == 0) continue;
+              if (loaded[t] > 0) ok = waiter.wait(&bar.q_empty[t], (loaded[t] - 1) & 1);
+              if (!ok) break;
+              load(&p.q, q_tiles + t * C::kTileBytes, head, it.row0 + (2 * it.tile + t) * 128, it.batch, &bar.q_full[t]);
+              ++loaded[t];
+              if (t == 0) {  // the first product needs no more than this
+                const int s = filled % C::kStages;
+                if (filled >= C::kStages) ok = waiter.wait(&bar.kv_empty[s], (filled / C::kStages - 1) & 1);
+                if (!ok) break;
+                load(&p.k, kv_tiles + s * C::kTileBytes, kv_head, it.row0, it.batch, &bar.kv_full[s]);
+                ++filled;
+              }
+            }
+          } else {
+            const int s = filled % C::kStages;
+            if (filled >= C::kStages) ok = waiter.wait(&bar.kv_empty[s], (filled / C::kStages - 1) & 1);
+            if (!ok) break;
+            load(&p.k, kv_tiles + s * C::kTileBytes, kv_head, it.row0 + j * 128, it.batch, &bar.kv_full[s]);
+            ++filled;
+          }
+          if (!ok) break;
+          const int s = filled % C::kStages;
+          if (filled >= C::kStages) ok = waiter.wait(&bar.kv_empty[s], (filled / C::kStages - 1) & 1);
+          if (!ok) break;
+          uint8_t* to = kv_tiles + s * C::kTileBytes;
+          const int valid = it.len - j * 128;   // rows of the sequence
+          if (p.seq.packed && valid < 128) {
+            // rows of the next sequence: their weights are 0, but 0 * inf and 0 * NaN are not
+            load(&p.v, to, kv_head, it.row0 + j * 128, it.batch, &bar.raw);
+            ok = waiter.wait(&bar.raw, mended & 1);
+            ++mended;
+  #pragma unroll
+            for (int slab = 0; slab < DP / 64; ++slab) {
+              uint4* lines = reinterpret_cast<uint4*>(to + slab * C::kSlab);
+              for (int x = valid * 8 + lane; x < 128 * 8; x += 32) lines[x] = make_uint4(0, 0, 0, 0);
+            }
+            tc::fence_async_smem();
+            __syncwarp();
+            tc::mbar_arrive(&bar.kv_full[s], leader);
+          } else {
+            load(&p.v, to, kv_head, it.row0 + j * 128, it.batch, &bar.kv_full[s]);
+          }
+          ++filled;
+        }
+      }
+      if (!ok) {  // copies under way end before the CTA does
+        for (int back = 1; back <= C::kStages && back <= filled; ++back) {
+          const int x = filled - back;
+          for (int i = 0; i < 4096 && !tc::mbar_try_wait(&bar.kv_full[x % C::kStages], (x / C::kStages) & 1); ++i) {}
+        }
+        for (int t = 0; t < 2; ++t) {
+          for (int i = 0; loaded[t] > 0 && i < 4096 && !tc::mbar_try_wait(&bar.q_full[t], (loaded[t] - 1) & 1); ++i) {}
+        }
+      }
+    } else if (warp == 8) {
+      // ---- products ----------------------------------------------------------------------------------------
+      const uint32_t leader = tc::elect_leader();
+      const uint32_t id_s = tc::idesc(128, 128, Format<T>::code, tc::kMajorK, tc::kMajorK, p.negate);
+      const uint32_t id_o = tc::idesc(128, DP, Format<T>::code, tc::kMajorK, tc::kMajorMN);
+      const uint32_t q_base = tc::smem_u32(q_tiles), kv_base = tc::smem_u32(kv_tiles);
+      int used = 0, q_used[2] = {0, 0}, p_used[2] = {0, 0};
+      bool ok = true;
+      auto scores = [&](int t, int s) {
+  #pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          mma_ss(tmem + t * 128, desc_k(q_base + t * C::kTileBytes, C::kSlab, ks), desc_k(kv_base + s * C::kTileBytes, C::kSlab, ks),
+                 id_s, ks > 0, leader);
+        }
+        tc::mma_commit(&bar.s_full[t], leader);
+      };
+      for (int turn = 0; turn < p.turns && ok; ++turn) {
+        const int64_t index = item_of_turn(turn);
+        if (index >= p.items) continue;
+        int head;
+        const Item it = item_at(index, &head);
+        const int n_t[2] = {key_tiles(it, 0), key_tiles(it, 1)};
+        const int n = max(n_t[0], n_t[1]);
+        auto full = [&](int x) { return waiter.wait(&bar.kv_full[x % C::kStages], (x / C::kStages) & 1); };
+        if (!(ok = full(used))) break;
+  #pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (n_t[t] == 0 || !ok) continue;
+          if (!(ok = waiter.wait(&bar.q_full[t], q_used[t] & 1))) continue;
+          tc::tc_fence_after();
+          scores(t, used % C::kStages);
+          if (n_t[t] == 1) tc::mma_commit(&bar.q_empty[t], leader);
+        }
+        if (!ok) break;
+        tc::mma_commit(&bar.kv_empty[used % C::kStages], leader);
+        for (int j = 0; j < n && ok; ++j) {
+          const int xv = used + 2 * j + 1, xk = xv + 1;
+          if (!(ok = full(xv))) break;
+          if (j + 1 < n && !(ok = full(xk))) break;
+          const uint32_t v_tile = kv_base + (xv % C::kStages) * C::kTileBytes;
+  #pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j < n_t[t] && ok) {
+              if (!(ok = waiter.wait(&bar.p_ready[t], p_used[t] & 1))) continue;
+              ++p_used[t];
+              tc::tc_fence_after();
+  #pragma unroll
+              for (int ks = 0; ks < 8; ++ks) {
+                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, desc_mn(v_tile, C::kSlab, ks), id_o, j > 0 || ks > 0, leader);
+              }
+              if (j + 1 == n_t[t]) tc::mma_commit(&bar.o_full[t], leader);
+            }
+            if (t == 1) tc::mma_commit(&bar.kv_empty[xv % C::kStages], leader);
+            if (j + 1 < n_t[t]) {
+              scores(t, xk % C::kStages);
+              if (j + 2 == n_t[t]) tc::mma_commit(&bar.q_empty[t], leader);
+            }
+          }
+          if (j + 1 < n) tc::mma_commit(&bar.kv_empty[xk % C::kStages], leader);
+        }
+        used += 2 * n;
+        for (int t = 0; t < 2; ++t) q_used[t] += n_t[t] > 0;
+      }
+      if (!ok) {  // products under way end before the CTA does
+        tc::mma_commit(&bar.drained, leader);
+        for (int i = 0; i < 4096 && !tc::mbar_try_wait(&bar.drained, 0); ++i) {}
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---- weights: a row a thread ---------------------------------------------------------------------------
+    take_registers<208>();
+    const int t = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lane_base = uint32_t(warp & 3) << 21;   // 32 lanes of TMEM, in bits 16 and up
+    const uint32_t s_at = tmem + lane_base + t * 128, o_at = tmem + lane_base + 256 + t * 128;
+    const float c = p.scale_log2;
+    int seen = 0, outs = 0;
+    bool ok = true;
+    for (int turn = 0; turn < p.turns; ++turn) {
+      const int64_t index = item_of_turn(turn);
+      if (index >= p.items) continue;
+      int head;
+      const Item it = item_at(index, &head);
+      const int n = key_tiles(it, t);
+      if (n == 0) {
+        if (p.lse != nullptr) p.lse[head * p.seq.stat_rows + it.stat + (2 * it.tile + t) * 128 + row] = INFINITY;
+        continue;
+      }
+      float m = -INFINITY;
+      float2 sum2[2] = {{0.f, 0.f}, {0.f, 0.f}};
+      for (int j = 0; j < n && ok; ++j) {
+        if (!(ok = waiter.wait(&bar.s_full[t], seen & 1))) break;
+        ++seen;
+        tc::tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tc::tmem_ld32(s_at + x * 32, s[x]);
+        tc::tmem_wait_ld();
+        if (j + 1 == n) {   // the tile on the diagonal; what lies behind the sequence's end lies behind every row
+#pragma unroll
+          for (int x = 0; x < 128; ++x) {
+            if (x > row) s[x >> 5][x & 31] = 0xff800000u;
+          }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < 128; ++x) top = fmaxf(top, __uint_as_float(s[x >> 5][x & 31]));
+        if (j == 0) {
+          m = top;
+        } else {
+          const bool grown = (top - m) * c > kRescale;
+          if (__any_sync(0xffffffffu, grown)) {
+            const float f = grown ? exp2_approx((m - top) * c) : 1.f;
+            if (grown) m = top;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) sum2[x] = mul2(sum2[x], twice(f));
+#pragma unroll
+            for (int x = 0; x < DP / 32; ++x) {
+              uint32_t o[32];
+              tc::tmem_ld32(o_at + x * 32, o);
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+              tc::tmem_st32(o_at + x * 32, o);
+            }
+          }
+        }
+        // exp2(s c - m c); a row that has seen nothing but -inf so far has weights 0
+        const float2 minus = twice(m == -INFINITY ? 0.f : -m * c), by = twice(c);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint32_t w[32];
+#pragma unroll
+          for (int y = 0; y < 32; ++y) {
+            const int at = x * 64 + y * 2;
+            const float2 e = exp2_2(fma2(make_float2(__uint_as_float(s[at >> 5][at & 31]), __uint_as_float(s[at >> 5][(at & 31) + 1])), by, minus));
+            sum2[y & 1] = add2(sum2[y & 1], e);
+            w[y] = pack_pair<T>(e.x, e.y);   // the sum has them as they were, the product rounded to the values' type
+          }
+          tc::tmem_st32(s_at + x * 32, w);
+        }
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        __syncwarp();
+        tc::mbar_arrive(&bar.p_ready[t], lane == 0);
+      }
+      if (ok) ok = waiter.wait(&bar.o_full[t], outs & 1);
+      ++outs;
+      tc::tc_fence_after();
+      const int i = (2 * it.tile + t) * 128 + row;
+      const bool there = i < it.len;
+      const float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+      const float inv = ok ? 1.f / sum : NAN;
+      T* to = static_cast<T*>(p.out) + ((it.row + i) * p.heads + head) * p.dim;
+#pragma unroll
+      for (int x = 0; x < DP / 32; ++x) {
+        uint32_t o[32];
+        tc::tmem_ld32(o_at + x * 32, o);
+        tc::tmem_wait_ld();
+        if (there) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            if (x * 32 + y * 8 < p.dim) {
+              uint4 w;
+              w.x = pack_pair<T>(__uint_as_float(o[y * 8]) * inv, __uint_as_float(o[y * 8 + 1]) * inv);
+              w.y = pack_pair<T>(__uint_as_float(o[y * 8 + 2]) * inv, __uint_as_float(o[y * 8 + 3]) * inv);
+              w.z = pack_pair<T>(__uint_as_float(o[y * 8 + 4]) * inv, __uint_as_float(o[y * 8 + 5]) * inv);
+              w.w = pack_pair<T>(__uint_as_float(o[y * 8 + 6]) * inv, __uint_as_float(o[y * 8 + 7]) * inv);
+              *reinterpret_cast<uint4*>(to + x * 32 + y * 8) = w;
+            }
+          }
+        }
+      }
+      tc::tc_fence_before();
+      // rows behind the end: a backward gives them weights exp2(0 - inf) = 0
+      if (p.lse != nullptr) {
+        p.lse[head * p.seq.stat_rows + it.stat + i] =
+            !there ? INFINITY : ok ? m * c + log2f(sum) : NAN;
+      }
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int DP>
+int launch_typed(const FwdParams& p, cudaStream_t stream) {
+  using C = FwdConfig<DP>;
+  const void* kernel = reinterpret_cast<const void*>(&attention_forward_kernel<T, DP>);
+  const cudaError_t err = ensure_dynamic_smem(kernel, C::kBytes);
+  if (err != cudaSuccess) { record_cuda_error(err); return GDN2_ERR_LAUNCH; }
+  int sms = 0;
+  const int status = multiprocessors(&sms);
+  if (status != GDN2_OK) return status;
+  FwdParams q = p;
+  const int64_t grid = p.items < sms ? p.items : sms;
+  q.turns = int((p.items + grid - 1) / grid);
+  attention_forward_kernel<T, DP><<<unsigned(grid), kThreads, C::kBytes, stream>>>(q);
+  return check_launch();
+}
+
+}  // namespace
+
+int launch_attention_forward(const void* q, const void* k, const void* v, void* out, float* lse, const int64_t* strides,
+                             const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, int dim,
+                             int dtype, float scale, cudaStream_t stream) {
+  FwdParams p;
+  const int64_t batch = bounds != nullptr ? 1 : n_seq;
+  if (!encode_heads_map(&p.q, q, strides, batch, time, heads, dim, dtype, 128) ||
+      !encode_heads_map(&p.k, k, strides + 3, batch, time, kv_heads, dim, dtype, 128) ||
+      !encode_heads_map(&p.v, v, strides + 6, batch, time, kv_heads, dim, dtype, 128)) {
+    return GDN2_ERR_LAUNCH;
+  }
+  p.out = out; p.lse = lse;
+  p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.dim = dim;
+  // the sign goes to the product, and a scale of 0 stays a positive number, so that -inf * scale masks as ever
+  p.negate = scale < 0.f;
+  p.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
+  return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {
+    p.items = int64_t(p.seq.tiles) * heads;
+    if (dtype == GDN2_BF16) return dim <= 64 ? launch_typed<__nv_bfloat16, 64>(p, stream) : launch_typed<__nv_bfloat16, 128>(p, stream);
+    return dim <= 64 ? launch_typed<__half, 64>(p, stream) : launch_typed<__half, 128>(p, stream);
+  });
+}
+
+}  // namespace attn
+}  // namespace gdn2

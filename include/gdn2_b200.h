@@ -430,6 +430,80 @@ int gdn2_chunk_forward_static(const void* q, const void* k, const void* v, const
  */
 int gdn2_chunk_static_read_status(void* stream);
 
+/*
+ * Operators of an attention layer that stands between Gated DeltaNet-2 layers.  No counterparts in the
+ * reference.  Tensors are [B, T, H, D] like the others here, but may be views: strides are given in
+ * elements, the innermost one is 1.  Attention takes any D that is a multiple of 8, up to
+ * GDN2_ATTENTION_MAX_DIM, bf16 or fp16, pointers aligned to 16 bytes and strides of whole 16 bytes;
+ * query head h reads key head h / (heads / kv_heads).
+ */
+#define GDN2_ATTENTION_MAX_DIM 128
+
+/*
+ * Rotary positions of queries [B, T, q_heads, dim] and keys [B, T, k_heads, dim] (bf16, fp16 or fp32): channel
+ * pairs i < pairs turn by the angle whose cosine and sine are cos[p][i], sin[p][i] ([table][pairs] fp32),
+ *   y_a = x_a c - x_b s,  y_b = x_b c + x_a s,
+ * (a, b) = (i, i + pairs), or (2i, 2i + 1) where `interleaved`; the other channels are copied.
+ * p = positions[b * position_stride + t], or t where positions is NULL; a p outside the table makes the
+ * token's rotated channels NaN.  `inverse` turns the other way: the gradient.  strides: batch, token and head
+ * of q, k, q_out, k_out.  q_out == q and k_out == k works in place.
+ */
+int gdn2_rotary(const void* q, const void* k, void* q_out, void* k_out, const float* cos, const float* sin,
+                const int64_t* positions, const int64_t* strides, int64_t position_stride,
+                int64_t batch, int64_t time, int64_t q_heads, int64_t k_heads, int64_t dim,
+                int64_t pairs, int64_t table, int interleaved, int inverse, int dtype, void* stream);
+
+/*
+ * A paged cache is two contiguous tensors [pages][page][kv_heads][dim].  Copies the keys and values of
+ * `tokens` tokens to their slots, slot = page number * page + place in the page; tokens whose slot is
+ * negative or behind the cache are left out.  No two tokens may have the same slot.  strides: token and
+ * head of k, of v.
+ */
+int gdn2_append_tokens(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* slots,
+                       const int64_t* strides, int64_t tokens, int64_t pages, int64_t page,
+                       int64_t kv_heads, int64_t dim, int dtype, void* stream);
+
+/*
+ * Attention of `drafted` tokens of each sequence over its lengths[b] cached tokens (token t in page
+ * page_table[b * table_stride + t / page]) and over those drafted ones that its mask row names:
+ * mask[b * mask_stride + i * drafted + j] != 0, or j <= i where mask is NULL.  q [B, drafted, heads, dim],
+ * k and v [B, drafted, kv_heads, dim] are not in the cache; out [B, drafted, heads, dim] is contiguous.
+ * A row that sees nothing gives 0.  A page number outside the cache, or a length that `columns` pages cannot
+ * hold, makes the sequence's output NaN.  strides: batch, token and head of q, k, v.  workspace:
+ * gdn2_tree_workspace_bytes (a negative status if the sizes are wrong), dead when the call's kernels have run.
+ */
+int64_t gdn2_tree_workspace_bytes(int64_t drafted, int64_t heads, int64_t kv_heads, int64_t dim);
+int gdn2_tree_attention(const void* q, const void* k, const void* v, const void* k_pages,
+                        const void* v_pages, const int* page_table, const int* lengths, const void* mask,
+                        void* out, void* workspace, const int64_t* strides, int64_t table_stride,
+                        int64_t mask_stride, int64_t batch, int64_t drafted, int64_t heads,
+                        int64_t kv_heads, int64_t dim, int64_t pages, int64_t page, int64_t columns,
+                        int dtype, float scale, void* stream);
+
+/*
+ * Causal attention over whole sequences: n_seq of `time` tokens each (bounds NULL), or n_seq packed ones
+ * that are rows bounds[i] .. bounds[i + 1] of [1, time, H, D] tensors (host array of n_seq + 1).
+ * out [.., heads, dim] is contiguous.  `statistics` (NULL for inference): heads * gdn2_attention_stat_rows
+ * floats that a backward needs.  Rows of `out` that belong to no sequence are not written.
+ * strides: batch, token and head of q, k, v.
+ */
+int64_t gdn2_attention_stat_rows(const int64_t* bounds, int64_t n_seq, int64_t time);
+int gdn2_attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics,
+                           const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time,
+                           int64_t heads, int64_t kv_heads, int64_t dim, int dtype, float scale,
+                           void* stream);
+
+/*
+ * Its gradients.  out and statistics are the forward's; dq, dk, dv contiguous; scratch has the size of
+ * statistics.  strides: batch, token and head of q, k, v, d_out.  No atomics: the same inputs give the same
+ * bits.
+ */
+int gdn2_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out,
+                            const float* statistics, float* scratch, void* dq, void* dk, void* dv,
+                            const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time,
+                            int64_t heads, int64_t kv_heads, int64_t dim, int dtype, float scale,
+                            void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif
