@@ -25,7 +25,6 @@ namespace {
 
 constexpr int kThreads = 384;    // warps 0-3: even steps; 4-7: odd ones; 8: products; 9: copies
 constexpr int kStep = 64;        // rows of a step
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <int DP>
 struct BwdConfig {

@@ -11,6 +11,7 @@
 namespace gdn2 {
 namespace attn {
 
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTileRows = 256;   // query rows of a work item of the forward: two tiles of 128
 constexpr int kMaxSequences = GDN2_PACKED_MAX_SEQUENCES;   // in a launch, whose parameters hold their table
 
@@ -129,6 +130,67 @@ template <typename T>
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   const typename Pair<T>::type v = Pair<T>::make(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// One tile of scores becomes weights, a row a thread: S (128 columns of TMEM at s_at) is read, masked, and overlaid by
+// P = exp2(S c - m c) in 16 bits.  m is the row's reference so far and `sum` the sum of its weights; both and O (DP columns
+// at o_at, as it is after all tiles before this one) follow a maximum that has grown by more than 2^kRescale: weights stay
+// below that and sums in 32 bits lose nothing.
+constexpr float kRescale = 8.f;
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+template <typename T, int DP, typename Mask>
+__device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, bool first, float& m, float2 (&sum)[2],
+                                       Mask mask) {
+  uint32_t s[4][32];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) tc::tmem_ld32(s_at + x * 32, s[x]);
+  tc::tmem_wait_ld();
+  mask(s);
+  float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int x = 0; x < 128; x += 2) {
+    tops[(x >> 1) & 3] = max3(tops[(x >> 1) & 3], __uint_as_float(s[x >> 5][x & 31]), __uint_as_float(s[x >> 5][(x & 31) + 1]));
+  }
+  const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
+  if (first) {
+    m = top;
+  } else {
+    const bool grown = (top - m) * c > kRescale;
+    if (__any_sync(0xffffffffu, grown)) {
+      const float f = grown ? exp2_approx((m - top) * c) : 1.f;
+      if (grown) m = top;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) sum[x] = mul2(sum[x], twice(f));
+#pragma unroll
+      for (int x = 0; x < DP / 32; ++x) {
+        uint32_t o[32];
+        tc::tmem_ld32(o_at + x * 32, o);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+        tc::tmem_st32(o_at + x * 32, o);
+      }
+    }
+  }
+  // a row that has seen nothing but -inf so far has weights 0
+  const float2 minus = twice(m == -INFINITY ? 0.f : -m * c), by = twice(c);
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    uint32_t w[32];
+#pragma unroll
+    for (int y = 0; y < 32; ++y) {
+      const int at = x * 64 + y * 2;
+      const float2 e = exp2_2(fma2(make_float2(__uint_as_float(s[at >> 5][at & 31]), __uint_as_float(s[at >> 5][(at & 31) + 1])), by, minus));
+      sum[y & 1] = add2(sum[y & 1], e);
+      w[y] = pack_pair<T>(e.x, e.y);   // the sum has them as they were, the product rounded to the values' type
+    }
+    tc::tmem_st32(s_at + x * 32, w);
+  }
+  tc::tmem_wait_st();
 }
 
 // [batch][rows][heads][dim] with any strides that are multiples of 16 bytes, in boxes of 64 channels x box_rows rows

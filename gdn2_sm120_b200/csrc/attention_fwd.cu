@@ -20,8 +20,6 @@ namespace attn {
 namespace {
 
 constexpr int kThreads = 384;    // warps 0-3, 4-7: the rows of the two tiles; 8: products; 9: copies; 10, 11: look at values
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescale = 8.f;  // in powers of two
 
 template <int DP>
 struct FwdConfig {
@@ -272,54 +270,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
         if (!(ok = waiter.wait(&bar.s_full[t], seen & 1))) break;
         ++seen;
         tc::tc_fence_after();
-        uint32_t s[4][32];
+        soften<T, DP>(s_at, o_at, c, j == 0, m, sum2, [&](uint32_t (&s)[4][32]) {
+          if (j + 1 == n) {   // the tile on the diagonal; what lies behind the sequence's end lies behind every row
 #pragma unroll
-        for (int x = 0; x < 4; ++x) tc::tmem_ld32(s_at + x * 32, s[x]);
-        tc::tmem_wait_ld();
-        if (j + 1 == n) {   // the tile on the diagonal; what lies behind the sequence's end lies behind every row
-#pragma unroll
-          for (int x = 0; x < 128; ++x) {
-            if (x > row) s[x >> 5][x & 31] = 0xff800000u;
-          }
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int x = 0; x < 128; ++x) top = fmaxf(top, __uint_as_float(s[x >> 5][x & 31]));
-        if (j == 0) {
-          m = top;
-        } else {
-          const bool grown = (top - m) * c > kRescale;
-          if (__any_sync(0xffffffffu, grown)) {
-            const float f = grown ? exp2_approx((m - top) * c) : 1.f;
-            if (grown) m = top;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) sum2[x] = mul2(sum2[x], twice(f));
-#pragma unroll
-            for (int x = 0; x < DP / 32; ++x) {
-              uint32_t o[32];
-              tc::tmem_ld32(o_at + x * 32, o);
-              tc::tmem_wait_ld();
-#pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-              tc::tmem_st32(o_at + x * 32, o);
+            for (int x = 0; x < 128; ++x) {
+              if (x > row) s[x >> 5][x & 31] = 0xff800000u;
             }
           }
-        }
-        // exp2(s c - m c); a row that has seen nothing but -inf so far has weights 0
-        const float2 minus = twice(m == -INFINITY ? 0.f : -m * c), by = twice(c);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          uint32_t w[32];
-#pragma unroll
-          for (int y = 0; y < 32; ++y) {
-            const int at = x * 64 + y * 2;
-            const float2 e = exp2_2(fma2(make_float2(__uint_as_float(s[at >> 5][at & 31]), __uint_as_float(s[at >> 5][(at & 31) + 1])), by, minus));
-            sum2[y & 1] = add2(sum2[y & 1], e);
-            w[y] = pack_pair<T>(e.x, e.y);   // the sum has them as they were, the product rounded to the values' type
-          }
-          tc::tmem_st32(s_at + x * 32, w);
-        }
-        tc::tmem_wait_st();
+        });
         tc::tc_fence_before();
         __syncwarp();
         tc::mbar_arrive(&bar.p_ready[t], lane == 0);

@@ -11,21 +11,28 @@
 //
 //                   o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i),   s_ij = scale q_i . k_j,  m_i = max_j s_ij
 //
-//                 and 0 where nothing is seen.  One pass over the cache with a running maximum and sum; the heads of a
-//                 group are rows of one product with their shared key head, so the cache is read once for every 64 rows
-//                 (drafted tokens x heads of a group).  Bound by HBM up to there: 64 rows take 64 flop a byte.
-//                 All (sequence, key head, 64-token tile) are one list that the CTAs share evenly, so neither
+//                 and 0 where nothing is seen.  One pass with a running maximum and sum.  The heads of a group are rows
+//                 of one product with their shared key head, so a key is read once for 256 rows (drafted tokens x heads
+//                 of a group).  Bound by HBM: the 64 KiB of a tile of 128 tokens take an SM's share of HBM 2700 clocks,
+//                 its products 1024 for up to 128 rows and 2048 for up to 256, the few rows of plain decoding too.
+//                 All (sequence, key head, block of rows, tile) are one list that the CTAs share evenly, so neither
 //                 unequal lengths nor few sequences leave SMs idle, and the host need not know the lengths.  A CTA
 //                 whose part begins or ends inside a sequence leaves (O, m, l) in the workspace; tree_join_kernel joins
 //                 these in the order of the tiles: the same inputs give the same bits.
-//                 The products are mma.sync m16n8k16: tiles of 16 rows fit one to a few drafted tokens, where an
-//                 instruction of the tcgen05 kind has 64 rows at least and its sums in another memory.
+//
+// A CTA: two chains of four warps turn scores into weights, a row a thread.  Up to 128 rows both work on the same rows,
+// on every other tile, and their (O, m, l) are joined at the end; above, each has 128 rows and all tiles.  Four warps
+// bring in rows with 16-byte asynchronous copies, since pages of any size make no box for a tiled copy; one issues the
+// products.  TMEM: S0 S1 O0 O1, 128 columns each, P over S.
 
 #include <algorithm>
 
-#include "common.cuh"
+#include "attention_common.cuh"
 
 namespace gdn2 {
+
+using attn::Format;
+using attn::pack_pair;
 
 namespace {
 
@@ -55,64 +62,59 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 }
 
 // ---- tree attention ----------------------------------------------------------------------------------
-constexpr int kTile = 64;      // tokens of a tile
-constexpr int kStages = 3;     // tiles in flight: 96 KiB of keys and values of 128 channels, two CTAs to an SM
-constexpr int kThreads = 128;
-constexpr float kLog2e = 1.4426950408889634f;
-
+constexpr int kTile = 128;     // tokens of a tile
+constexpr int kThreads = 512;  // warps 0-3, 4-7: weights; 8-11: copies; 12: products
+constexpr int kJoinThreads = 128;
 struct TreeParams {
   const void *q, *k, *v;
   const void *k_pages, *v_pages;
   void* out;
   const int *table, *lengths;
   const uint8_t* mask;                       // [batch or 1][drafted][drafted], or null: j <= i
-  float* partials;                           // [CTA][2][rows][DP + 2]
+  float* partials;                           // [CTA][2][rows of a block][DP], then [CTA][2][rows of a block][m, l]
   int64_t q_stride[3], k_stride[3], v_stride[3];  // batch, token, head, in elements
   int64_t table_stride, mask_stride, pages;
   int batch, drafted, heads, kv_heads, group, dim, page, columns;
   int rows, row_blocks, ctas;
-  float scale_log2;
+  float scale_log2;                          // positive
+  uint32_t negate;                           // the scale is negative: Q counts with its sign changed
 };
 
-// One (sequence, key head, block of rows) after the other, tile by tile
-struct Cursor {
-  int b, head, block;   // block of rows
-  int tile, tiles, context_tiles, length;
+// A sequence's cached tokens and then its drafted ones, in tiles; kRows rows of one key head
+struct Unit {
+  int b, head, block;
+  int length, tiles;
   bool bad;             // the sequence's length is none that its page table can hold
 };
 
-__device__ __forceinline__ void read_length(const TreeParams& p, Cursor& c) {
-  if (c.b < p.batch) {
-    const int n = p.lengths[c.b], most = p.columns * p.page;
-    c.bad = n < 0 || n > most;
-    c.length = c.bad ? 0 : n;
-    c.context_tiles = (c.length + kTile - 1) / kTile;
-    c.tiles = c.context_tiles + (p.drafted + kTile - 1) / kTile;
-  }
+__device__ __forceinline__ void read_length(const TreeParams& p, Unit& u) {
+  const int n = u.b < p.batch ? p.lengths[u.b] : 0;
+  u.bad = n < 0 || n > p.columns * p.page;
+  u.length = u.bad ? 0 : n;
+  u.tiles = (u.length + p.drafted + kTile - 1) / kTile;
 }
 
-__device__ __forceinline__ void advance(const TreeParams& p, Cursor& c) {
-  if (++c.tile < c.tiles) return;
-  c.tile = 0;
-  if (++c.block < p.row_blocks) return;
-  c.block = 0;
-  if (++c.head < p.kv_heads) return;
-  c.head = 0;
-  ++c.b;
-  read_length(p, c);
+__device__ __forceinline__ void next_unit(const TreeParams& p, Unit& u) {
+  if (++u.block < p.row_blocks) return;
+  u.block = 0;
+  if (++u.head < p.kv_heads) return;
+  u.head = 0;
+  ++u.b;
+  read_length(p, u);
 }
 
 // tiles of sequence b, for all its key heads and blocks of rows
 __device__ __forceinline__ int64_t tiles_of(const TreeParams& p, int b) {
-  Cursor c{b, 0, 0, 0, 0, 0, 0, false};
-  read_length(p, c);
-  return int64_t(c.tiles) * p.kv_heads * p.row_blocks;
+  Unit u{b, 0, 0, 0, 0, false};
+  read_length(p, u);
+  return int64_t(u.tiles) * p.kv_heads * p.row_blocks;
 }
 
 // CTAs that have a part of `total` tiles: each of them a tile at least
 __device__ __forceinline__ int64_t sharing(const TreeParams& p, int64_t total) { return total < p.ctas ? total : p.ctas; }
 
 // Sum over all threads of the CTA (every one of them gets it) and of those before this one
+template <int kWarps>
 __device__ __forceinline__ int64_t cta_scan(int64_t x, int64_t* before, int64_t* shared) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t sum = x;
@@ -126,7 +128,7 @@ __device__ __forceinline__ int64_t cta_scan(int64_t x, int64_t* before, int64_t*
   __syncthreads();
   int64_t total = 0, earlier = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     if (w == warp) earlier = total;
     total += shared[w];
   }
@@ -137,484 +139,557 @@ __device__ __forceinline__ int64_t cta_scan(int64_t x, int64_t* before, int64_t*
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
-  const typename Pair<T>::type v = Pair<T>::make(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// Arrives on an mbarrier, which counts on it, when all copies of this thread so far have.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
 }
 
-// a 16-bit float that is infinite or NaN: its exponent bits are all ones
-template <typename T> struct Exponent;
-template <> struct Exponent<__nv_bfloat16> { static constexpr uint32_t bits = 0x7f80; };
-template <> struct Exponent<__half> { static constexpr uint32_t bits = 0x7c00; };
-template <typename T>
-__device__ __forceinline__ bool any_not_finite(uint32_t pair) {
-  constexpr uint32_t e = Exponent<T>::bits;
-  return (pair & e) == e || ((pair >> 16) & e) == e;
-}
+// both chains
+__device__ __forceinline__ void sync_chains() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// Shared memory of a CTA: kStages of (K, V) tiles, rows of DP channels whose 16-byte pieces are permuted by the row;
-// where the rows' addresses are; what the warps that share rows exchange.
-template <int DP, int WM>
-struct TreeSmem {
-  static constexpr int kRows = 16 * WM, kWN = 4 / WM;
-  uint8_t kv[kStages][2][kTile * DP * 2];
-  const uint8_t* at[kStages + 1][kTile][2];  // addresses of a token's key and value; null: zeros
-  int64_t scan[kThreads / 32], found[2];
-  int bad[kStages + 1][kTile / 32];          // by locating warp
-  float m[kWN][kRows], l[kWN][kRows];
-  float o[kWN > 1 ? kRows : 1][DP];
+// The key of a page number outside the cache: 128 channels of NaN, in either type
+#define GDN2_NAN4 {~0u, ~0u, ~0u, ~0u}
+__device__ const uint4 g_nan_row[16] = {GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4,
+                                        GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4};
+#undef GDN2_NAN4
+
+// RT: tiles of 128 rows that a CTA has, 1 or 2; QR: rows of queries that a tile has in shared memory.  Where that is 32
+// the product reads on behind them: what its other rows are nobody looks at.
+template <int DP, int RT, int QR>
+struct TreeConfig {
+  static constexpr int kTileBytes = kTile * DP * 2;
+  static constexpr int kSlab = kTile * 128;                    // 64 channels of 128 rows
+  static constexpr int kRows = 128 * RT;
+  static constexpr int kQuerySlab = QR * 128, kQueryBytes = QR * DP * 2;
+  // Queries of two units, so that the copies need not wait between two; those of 256 rows of 128 channels leave no room.
+  static constexpr int kQueries = RT == 2 ? 1 : 2;
+  static constexpr int kStages = DP == 64 ? 8 : QR == 32 ? 6 : 5;
+  static constexpr int kBytes = RT * kQueries * kQueryBytes + kStages * kTileBytes + 2560;
 };
 
-template <int DP>
-__device__ __forceinline__ uint32_t piece(int row, int c) {  // byte offset of 16-byte piece c of a row
-  return uint32_t(row * DP * 2 + ((c ^ (row & 7)) << 4));
-}
+struct TreeBars {
+  uint64_t s_full[2], p_ready[2], o_full[2], q_empty[2], drained;
+  uint64_t kv_full[8], kv_empty[8];
+  int64_t scan[kThreads / 32], found[2];
+  uint32_t tmem;
+  int failed;
+  int strange;          // a drafted value was infinite or NaN
+  float2 ml[2][128];    // what the chains of the same rows tell each other
+};
+static_assert(sizeof(TreeBars) <= 2560, "");
 
-// 16 * WM rows a CTA; the 4 / WM warps of the same rows share a tile's tokens.
-template <typename T, int DP, int WM>
-__global__ void __launch_bounds__(kThreads, 2) tree_kernel(const TreeParams p) {
-  using Smem = TreeSmem<DP, WM>;
-  constexpr int kRows = Smem::kRows, kWN = Smem::kWN;
-  constexpr int kOwn = kTile / kWN;       // tokens of a tile that a warp works on
-  constexpr int kKSteps = DP / 16, kNB = kOwn / 8, kDB = DP / 8;
-  extern __shared__ __align__(128) uint8_t raw[];
-  Smem& sm = *reinterpret_cast<Smem*>(raw);
+template <typename T, int DP, int RT, int QR>
+__global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ TreeParams p) {
+  using C = TreeConfig<DP, RT, QR>;
+  extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
+  const uint32_t q_base = tc::smem_u32(smem), kv_base = q_base + RT * C::kQueries * C::kQueryBytes;
+  TreeBars& bar = *reinterpret_cast<TreeBars*>(smem + RT * C::kQueries * C::kQueryBytes + C::kStages * C::kTileBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int wm = warp % WM, wn = warp / WM;
-  const int quad = lane >> 2, in_quad = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+  if (tid == 0) {
+    for (int t = 0; t < 2; ++t) {
+      tc::mbar_init(&bar.s_full[t], 1);
+      tc::mbar_init(&bar.p_ready[t], 4);
+      tc::mbar_init(&bar.o_full[t], 1);
+    }
+    for (int x = 0; x < C::kQueries; ++x) tc::mbar_init(&bar.q_empty[x], 1);
+    tc::mbar_init(&bar.drained, 1);
+    for (int s = 0; s < C::kStages; ++s) {
+      tc::mbar_init(&bar.kv_full[s], 128);
+      tc::mbar_init(&bar.kv_empty[s], 1);
+    }
+    bar.failed = bar.strange = 0;
+    tc::fence_mbar_init();
+  }
+  if (warp == 12) {
+    tc::tmem_alloc(&bar.tmem, 512);
+    tc::tmem_relinquish();
+  }
   // this CTA's part of all tiles
-  int64_t total = 0, before;
+  int64_t total = 0, before, own = 0;
   for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-    const int b = b0 + tid;
-    total += cta_scan(b < p.batch ? tiles_of(p, b) : 0, &before, sm.scan);
+    own = b0 + tid < p.batch ? tiles_of(p, b0 + tid) : 0;
+    total += cta_scan<kThreads / 32>(own, &before, bar.scan);
   }
   const int64_t ctas = sharing(p, total);
-  if (blockIdx.x >= ctas) return;
+  const bool idle = blockIdx.x >= ctas;
   const int64_t begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
-  Cursor first{0, 0, 0, 0, 0, 0, 0, false};
-  {
+  if (!idle) {
     int64_t base = 0;
     for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-      const int b = b0 + tid;
-      const int64_t own = b < p.batch ? tiles_of(p, b) : 0;
-      const int64_t sum = cta_scan(own, &before, sm.scan);
+      int64_t sum = total;
+      if (p.batch > kThreads) {
+        own = b0 + tid < p.batch ? tiles_of(p, b0 + tid) : 0;
+        sum = cta_scan<kThreads / 32>(own, &before, bar.scan);
+      }
       const int64_t from = base + before;
       if (own > 0 && begin >= from && begin < from + own) {  // one thread of all
-        sm.found[0] = b;
-        sm.found[1] = begin - from;
+        bar.found[0] = b0 + tid;
+        bar.found[1] = begin - from;
       }
       base += sum;
       if (begin < base) break;
     }
-    __syncthreads();
-    first.b = int(sm.found[0]);
-    const int64_t rest = sm.found[1];
-    read_length(p, first);
-    const int64_t unit = rest / first.tiles;
-    first.tile = int(rest - unit * first.tiles);
-    first.head = int(unit / p.row_blocks);
-    first.block = int(unit - int64_t(first.head) * p.row_blocks);
   }
-  const int n_tiles = int(end - begin);
-
-  // where the rows of a tile are: a thread a token
-  auto locate = [&](const Cursor& c, int slot) {
-    if (tid < kTile) {
-      const uint8_t *k = nullptr, *v = nullptr;
-      bool bad = c.bad;
-      if (c.tile < c.context_tiles) {
-        const int t = c.tile * kTile + tid;
-        if (t < c.length) {
-          const int column = t / p.page;
-          const int64_t page = p.table[c.b * p.table_stride + column];
-          if (page >= 0 && page < p.pages) {
-            const int64_t row = (page * p.page + (t - column * p.page)) * p.kv_heads + c.head;
-            k = static_cast<const uint8_t*>(p.k_pages) + row * p.dim * 2;
-            v = static_cast<const uint8_t*>(p.v_pages) + row * p.dim * 2;
-          } else {
-            bad = true;
-          }
-        }
-      } else {
-        const int j = (c.tile - c.context_tiles) * kTile + tid;
-        if (j < p.drafted) {
-          k = static_cast<const uint8_t*>(p.k) + 2 * (c.b * p.k_stride[0] + j * p.k_stride[1] + c.head * p.k_stride[2]);
-          v = static_cast<const uint8_t*>(p.v) + 2 * (c.b * p.v_stride[0] + j * p.v_stride[1] + c.head * p.v_stride[2]);
-        }
-      }
-      sm.at[slot][tid][0] = k;
-      sm.at[slot][tid][1] = v;
-      const bool any = __any_sync(0xffffffffu, bad);
-      if (lane == 0) sm.bad[slot][warp] = any;
-    }
-  };
-  constexpr int kPieces = DP / 8;              // 16-byte pieces of a row
-  const int my_piece = tid % kPieces, my_row = tid / kPieces;
-  const bool piece_there = my_piece * 8 < p.dim;
-  auto fetch = [&](int stage, int slot) {
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(sm.kv[stage][which]));
-#pragma unroll
-      for (int r = 0; r < kTile; r += kThreads / kPieces) {
-        const uint8_t* row = sm.at[slot][r + my_row][which];
-        const bool there = piece_there && row != nullptr;
-        cp_async16(to + piece<DP>(r + my_row, my_piece), there ? row + my_piece * 16 : static_cast<const uint8_t*>(p.k), there);
-      }
-    }
-  };
-
-  Cursor ahead = first;   // the tile whose rows are looked up next
-  int located = 0;
-  for (; located < kStages && located < n_tiles; ++located) {
-    locate(ahead, located);
-    advance(p, ahead);
-  }
+  tc::tc_fence_before();
   __syncthreads();
-  for (int i = 0; i < kStages - 1; ++i) {
-    if (i < n_tiles) fetch(i, i);
-    cp_async_commit();
+  tc::tc_fence_after();
+  const uint32_t tmem = bar.tmem;
+  if (idle) {
+    if (warp == 12) tc::tmem_dealloc(tmem, 512);
+    return;
   }
+  const attn::Waiter waiter{&bar.failed};
+  Unit u{int(bar.found[0]), 0, 0, 0, 0, false};
+  read_length(p, u);
+  const int64_t unit0 = bar.found[1] / u.tiles;
+  int tile = int(bar.found[1] - unit0 * u.tiles);     // the first of this CTA's tiles of the unit
+  u.head = int(unit0 / p.row_blocks);
+  u.block = int(unit0 - int64_t(u.head) * p.row_blocks);
+  int rest = int(end - begin);                        // tiles of this CTA that are left
+  // tiles of 128 rows that a unit has
+  auto row_tiles = [&](const Unit& x) { return RT == 2 && p.rows - x.block * C::kRows > 128 ? 2 : 1; };
 
-  Cursor c = first;
-  uint32_t qf[kKSteps][4];
-  float o[kDB][4];
-  float m[2], l[2];
-  int seg_row = 0;        // first of this warp's rows
-  bool starts_here = false, fresh_segment = true;
-
-  for (int i = 0; i < n_tiles; ++i) {
-    const int stage = i % kStages, slot = i % (kStages + 1);
-    if (fresh_segment) {
-      fresh_segment = false;
-      starts_here = c.tile == 0;
-      seg_row = c.block * kRows + 16 * wm;
+  // 512 threads of 128 registers = 256 of 200 + 128 of 64 + 128 of 48
+  if (warp >= 12) {
+    attn::give_registers<48>();
+    if (warp == 12) {
+      // ---- products --------------------------------------------------------------------------------------
+      const uint32_t leader = tc::elect_leader();
+      const uint32_t id_s = tc::idesc(128, 128, Format<T>::code, tc::kMajorK, tc::kMajorK, p.negate);
+      const uint32_t id_o = tc::idesc(128, DP, Format<T>::code, tc::kMajorK, tc::kMajorMN);
+      int used = 0, p_used[2] = {0, 0}, queries = 0;   // which of the kQueries
+      bool ok = true;
+      auto full = [&](int x) {
+        const bool r = waiter.wait(&bar.kv_full[x % C::kStages], (x / C::kStages) & 1);
+        tc::fence_async_smem();   // what the copies wrote is read by the products
+        return r;
+      };
+      auto scores = [&](int t, int x) {   // S_t from the keys in stage x
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = seg_row + quad + 8 * half;
-        const bool there = r < p.rows;
-        const int n = there ? r / p.group : 0, g = there ? r - n * p.group : 0;
-        const T* row = static_cast<const T*>(p.q) + c.b * p.q_stride[0] + n * p.q_stride[1] +
-                       int64_t(c.head * p.group + g) * p.q_stride[2];
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          attn::mma_ss(tmem + t * 128, attn::desc_k(q_base + (RT == 2 ? t : queries) * C::kQueryBytes, C::kQuerySlab, ks),
+                       attn::desc_k(kv_base + (x % C::kStages) * C::kTileBytes, C::kSlab, ks), id_s, ks > 0, leader);
+        }
+        tc::mma_commit(&bar.s_full[t], leader);
+      };
+      auto outputs = [&](int t, int x, bool first) {   // O_t += P_t V
+        if (!waiter.wait(&bar.p_ready[t], p_used[t] & 1)) return false;
+        ++p_used[t];
+        tc::tc_fence_after();
 #pragma unroll
-        for (int s = 0; s < kKSteps; ++s) {
-#pragma unroll
-          for (int kh = 0; kh < 2; ++kh) {
-            const int col = s * 16 + kh * 8 + in_quad * 2;
-            qf[s][kh * 2 + half] = there && col < p.dim ? *reinterpret_cast<const uint32_t*>(row + col) : 0u;
+        for (int ks = 0; ks < kTile / 16; ++ks) {
+          attn::mma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, attn::desc_mn(kv_base + (x % C::kStages) * C::kTileBytes, C::kSlab, ks),
+                       id_o, !first || ks > 0, leader);
+        }
+        return true;
+      };
+      while (rest > 0 && ok) {
+        const int n = min(rest, u.tiles - tile), chains = row_tiles(u);
+        // the order of the copies is that of use: K0, K1 V0, K2 V1, ...
+        auto k_of = [&](int j) { return used + max(2 * j - 1, 0); };
+        auto v_of = [&](int j) { return used + min(2 * j + 2, 2 * n - 1); };
+        if (RT == 1) {
+          // chains by turns: S(j + 2) is issued behind O += P(j) V, whose P lies in its place
+          for (int j = 0; j < min(n, 2) && ok; ++j) {
+            if (!(ok = full(k_of(j)))) break;
+            scores(j, k_of(j));
+            tc::mma_commit(&bar.kv_empty[k_of(j) % C::kStages], leader);
+          }
+          if (n <= 2) tc::mma_commit(&bar.q_empty[queries], leader);
+          for (int j = 0; j < n && ok; ++j) {
+            const int t = j & 1, xv = v_of(j), xk = k_of(j + 2);
+            if (!(ok = full(xv)) || !(ok = outputs(t, xv, j < 2))) break;
+            tc::mma_commit(&bar.kv_empty[xv % C::kStages], leader);
+            if (j + 2 >= n) {
+              tc::mma_commit(&bar.o_full[t], leader);
+            } else {
+              if (!(ok = full(xk))) break;
+              scores(t, xk);
+              tc::mma_commit(&bar.kv_empty[xk % C::kStages], leader);
+              if (j + 3 == n) tc::mma_commit(&bar.q_empty[queries], leader);
+            }
+          }
+        } else {
+          if (!(ok = full(used))) break;
+          for (int t = 0; t < chains; ++t) scores(t, used);
+          tc::mma_commit(&bar.kv_empty[used % C::kStages], leader);
+          if (n == 1) tc::mma_commit(&bar.q_empty[queries], leader);
+          for (int j = 0; j < n && ok; ++j) {
+            const int xv = v_of(j), xk = k_of(j + 1);
+            if ((j + 1 < n && !(ok = full(xk))) || !(ok = full(xv))) break;
+            for (int t = 0; t < chains && ok; ++t) {
+              if (!(ok = outputs(t, xv, j == 0))) break;
+              if (j + 1 == n) tc::mma_commit(&bar.o_full[t], leader);
+              if (t + 1 == chains) tc::mma_commit(&bar.kv_empty[xv % C::kStages], leader);
+              if (j + 1 < n) scores(t, xk);
+            }
+            if (j + 1 < n) tc::mma_commit(&bar.kv_empty[xk % C::kStages], leader);
+            if (j + 2 == n) tc::mma_commit(&bar.q_empty[queries], leader);
           }
         }
-        m[half] = -INFINITY;
-        l[half] = 0.f;
+        used += 2 * n;
+        if (++queries == C::kQueries) queries = 0;
+        rest -= n;
+        tile = 0;
+        if (rest > 0) next_unit(p, u);
       }
-#pragma unroll
-      for (int d = 0; d < kDB; ++d) { o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f; }
-    }
-    cp_async_wait<kStages - 2>();
-    __syncthreads();   // the tile is there, and nobody reads the one before it any more
-    if (i + kStages - 1 < n_tiles) fetch((i + kStages - 1) % kStages, (i + kStages - 1) % (kStages + 1));
-    cp_async_commit();
-    const bool bad = (sm.bad[slot][0] | sm.bad[slot][1]) != 0;
-    const bool drafted_tile = c.tile >= c.context_tiles;
-    const int first_token = (drafted_tile ? c.tile - c.context_tiles : c.tile) * kTile + wn * kOwn;
-    const uint32_t k_tile = static_cast<uint32_t>(__cvta_generic_to_shared(sm.kv[stage][0]));
-    const uint32_t v_tile = static_cast<uint32_t>(__cvta_generic_to_shared(sm.kv[stage][1]));
-
-    // S = Q K^T
-    float s[kNB][4];
-#pragma unroll
-    for (int n = 0; n < kNB; ++n) { s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f; }
-#pragma unroll
-    for (int ks = 0; ks < kKSteps; ++ks) {
-#pragma unroll
-      for (int n = 0; n < kNB; n += 2) {
-        uint32_t kf[4];  // tokens n*8.. and (n+1)*8.., channels ks*16 + 0..7 and 8..15
-        ldmatrix4(kf, k_tile + piece<DP>(wn * kOwn + n * 8 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
-        mma16816<T>(s[n], qf[ks], kf[0], kf[1]);
-        mma16816<T>(s[n + 1], qf[ks], kf[2], kf[3]);
+      if (!ok) {  // products under way end before the CTA does
+        tc::mma_commit(&bar.drained, leader);
+        for (int i = 0; i < 4096 && !tc::mbar_try_wait(&bar.drained, 0); ++i) {}
       }
+      __syncwarp();
     }
-    // what a row sees of the tile
-    auto sees = [&](int row, int token) {
-      if (!drafted_tile) return token < c.length;
-      if (token >= p.drafted || row >= p.rows) return false;
-      const int n = row / p.group;
-      if (p.mask == nullptr) return token <= n;
-      return p.mask[c.b * p.mask_stride + int64_t(n) * p.drafted + token] != 0;
+  } else if (warp >= 8) {
+    // ---- copies: a warp has 32 rows of every tile, half a warp (128 channels) or a quarter copies a row at a time -----
+    attn::give_registers<64>();
+    constexpr int kPieces = DP / 8, kAtOnce = 32 / kPieces;
+    const int mine = (warp - 8) * 32, piece = lane % kPieces, sub = lane / kPieces;
+    const bool piece_there = piece * 8 < p.dim;
+    const uint64_t anything = reinterpret_cast<uintptr_t>(g_nan_row);   // an address for copies of nothing
+    int filled = 0, units = 0;
+    bool ok = true;
+    // a row of 16-byte pieces, lines of 128 bytes permuted by the row
+    auto to = [&](uint32_t base, uint32_t slab, int row) {
+      return base + uint32_t(piece >> 3) * slab + uint32_t(row) * 128u + ((uint32_t(piece ^ row) & 7u) << 4);
     };
-    const bool whole = !drafted_tile && (c.tile + 1) * kTile <= c.length;
+    // copies this warp's rows of a tile; `at` is where row `mine + lane` is, null for zeros
+    auto copy = [&](uint32_t base, uint32_t slab, const void* at) {
+      const uint32_t lo = uint32_t(reinterpret_cast<uintptr_t>(at)), hi = uint32_t(reinterpret_cast<uintptr_t>(at) >> 32);
 #pragma unroll
-    for (int n = 0; n < kNB; ++n) {
+      for (int i = 0; i < 32; i += 8 * kAtOnce) {
+        uint64_t row[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[n][e] *= p.scale_log2;
-        if (!whole && !sees(seg_row + quad + 8 * (e >> 1), first_token + n * 8 + in_quad * 2 + (e & 1))) s[n][e] = -INFINITY;
+        for (int x = 0; x < 8; ++x) {
+          const int r = i + x * kAtOnce + sub;
+          row[x] = (uint64_t(__shfl_sync(0xffffffffu, hi, r)) << 32) | __shfl_sync(0xffffffffu, lo, r);
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const bool there = piece_there && row[x] != 0;
+          cp_async16(to(base, slab, mine + i + x * kAtOnce + sub), reinterpret_cast<const uint8_t*>(there ? row[x] : anything) + piece * 16, there);
+        }
       }
-    }
-    // running maximum and sum of the two rows of this thread's quad
-    uint32_t pf[kNB][2];
+    };
+    // An infinite or NaN value of a drafted token (this warp's rows from `first` on) must reach the rows that see it and no
+    // others, but in the product it would meet every row (0 * NaN): it leaves the tile, and is added to those rows at the end.
+    auto sift = [&](uint32_t base, int first) {
+      for (int i = 0; i < 32; i += kAtOnce) {
+        if (i + sub < first) continue;
+        const uint32_t at = to(base, C::kSlab, mine + i + sub);
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+        bool any = false;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int n = 0; n < kNB; ++n) top = fmaxf(top, fmaxf(s[n][2 * half], s[n][2 * half + 1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float now = fmaxf(m[half], top);
-      const float base = now == -INFINITY ? 0.f : now;   // nothing seen yet: every weight is exp(-inf) = 0
-      const float keep = exp2_approx(m[half] - base);
-      m[half] = now;
-      float sum = 0.f;
-#pragma unroll
-      for (int n = 0; n < kNB; ++n) {
-        const float a = exp2_approx(s[n][2 * half] - base), b = exp2_approx(s[n][2 * half + 1] - base);
-        sum += a + b;
-        pf[n][half] = pack_pair<T>(a, b);   // weights at most 1, rounded to the values' type for the product
+        for (int j = 0; j < 4; ++j) {
+          if ((w[j] & Format<T>::exponent) == Format<T>::exponent) { w[j] &= 0xffff0000u; any = true; }
+          if (((w[j] >> 16) & Format<T>::exponent) == Format<T>::exponent) { w[j] &= 0xffffu; any = true; }
+        }
+        if (any) {
+          asm volatile("st.shared.v4.b32 [%4], {%0, %1, %2, %3};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(at) : "memory");
+          *static_cast<volatile int*>(&bar.strange) = 1;
+        }
       }
-      l[half] = l[half] * keep + sum;       // (of this thread's columns; the quad's are added at the end)
-#pragma unroll
-      for (int d = 0; d < kDB; ++d) { o[d][2 * half] *= keep; o[d][2 * half + 1] *= keep; }
-    }
-    if (bad) l[0] = l[1] = NAN;             // a page or a length that cannot be: the sequence's output is NaN
-    // An infinite or NaN value of a drafted token must reach the rows that see it and no others, but in the product below
-    // it would meet every row (0 * NaN): it is added to those rows here and leaves the tile.
-    if (drafted_tile) {
-      bool strange = false;
-      for (int x = tid; x < kTile * DP / 8; x += kThreads) {
-        const uint4 w = *reinterpret_cast<const uint4*>(sm.kv[stage][1] + x * 16);
-        strange = strange || any_not_finite<T>(w.x) || any_not_finite<T>(w.y) || any_not_finite<T>(w.z) || any_not_finite<T>(w.w);
+    };
+    auto page_of = [&](const Unit& x, int tile) {   // the page of row mine + lane, looked up a tile ahead
+      const int t = tile * kTile + mine + lane;
+      return t < x.length ? p.table[x.b * p.table_stride + t / p.page] : 0;
+    };
+    // the stage of the next copy, when its tile has been used
+    auto stage = [&]() {
+      const int s = filled % C::kStages;
+      if (filled >= C::kStages) ok = waiter.wait(&bar.kv_empty[s], (filled / C::kStages - 1) & 1);
+      ++filled;
+      return s;
+    };
+    int page = page_of(u, tile);
+    while (rest > 0 && ok) {
+      const int n = min(rest, u.tiles - tile);
+      Unit next = u;
+      if (rest > n) next_unit(p, next);
+      // the queries come with the first keys
+      const int place = units % C::kQueries;
+      if (units >= C::kQueries && !(ok = waiter.wait(&bar.q_empty[place], (units / C::kQueries - 1) & 1))) break;
+      ++units;
+      for (int x = 0; x < RT; ++x) {
+        if (mine >= QR) break;
+        const int r = u.block * C::kRows + x * 128 + mine + lane;
+        const int i = r / p.group, g = r - i * p.group;
+        const T* at = static_cast<const T*>(p.q) + u.b * p.q_stride[0] + i * p.q_stride[1] + int64_t(u.head * p.group + g) * p.q_stride[2];
+        copy(q_base + (RT == 2 ? x : place) * C::kQueryBytes, C::kQuerySlab, r < p.rows ? at : nullptr);
       }
-      if (__syncthreads_or(strange)) {
-        for (int j = 0; j < kOwn; ++j) {
-          const int row_in_tile = wn * kOwn + j;
-          const bool lo = sees(seg_row + quad, first_token + j), hi = sees(seg_row + quad + 8, first_token + j);
-#pragma unroll
-          for (int d = 0; d < kDB; ++d) {
-            const uint32_t pair = *reinterpret_cast<const uint32_t*>(sm.kv[stage][1] + piece<DP>(row_in_tile, d) + in_quad * 4);
-            const float2 x = unpack2<T>(pair);
-            if (!isfinite(x.x)) { if (lo) o[d][0] += x.x; if (hi) o[d][2] += x.x; }
-            if (!isfinite(x.y)) { if (lo) o[d][1] += x.y; if (hi) o[d][3] += x.y; }
+      const uint8_t* v_at = nullptr;
+      int first = 32;     // of this warp's rows of values, the first drafted one
+      for (int x = 0; x <= n && ok; ++x) {
+        const uint8_t *k_now = nullptr, *v_now = nullptr;
+        int first_now = 32;
+        if (x < n) {
+          const int t = (tile + x) * kTile + mine + lane, j = t - u.length;
+          if (j < 0) {
+            const int64_t row = (int64_t(page) * p.page + t % p.page) * p.kv_heads + u.head;
+            const bool there = page >= 0 && page < p.pages;
+            k_now = there ? static_cast<const uint8_t*>(p.k_pages) + row * p.dim * 2 : reinterpret_cast<const uint8_t*>(g_nan_row);
+            v_now = there ? static_cast<const uint8_t*>(p.v_pages) + row * p.dim * 2 : nullptr;
+          } else if (j < p.drafted) {
+            k_now = static_cast<const uint8_t*>(p.k) + 2 * (u.b * p.k_stride[0] + j * p.k_stride[1] + u.head * p.k_stride[2]);
+            v_now = static_cast<const uint8_t*>(p.v) + 2 * (u.b * p.v_stride[0] + j * p.v_stride[1] + u.head * p.v_stride[2]);
+          }
+          first_now = u.length - (tile + x) * kTile - mine;
+          page = x + 1 < n ? page_of(u, tile + x + 1) : page_of(next, 0);
+          const int s = stage();
+          if (!ok) break;
+          copy(kv_base + s * C::kTileBytes, C::kSlab, k_now);
+          cp_async_arrive(&bar.kv_full[s]);
+        }
+        if (x > 0) {
+          const int s = stage();
+          if (!ok) break;
+          copy(kv_base + s * C::kTileBytes, C::kSlab, v_at);
+          if (first < 32) {
+            cp_async_wait_all();
+            sift(kv_base + s * C::kTileBytes, first);
+            tc::mbar_arrive(&bar.kv_full[s]);
+          } else {
+            cp_async_arrive(&bar.kv_full[s]);
           }
         }
-        __syncthreads();
-        for (int x = tid; x < kTile * DP; x += kThreads) {
-          uint16_t* e = reinterpret_cast<uint16_t*>(sm.kv[stage][1]) + x;
-          if ((*e & Exponent<T>::bits) == Exponent<T>::bits) *e = 0;
-        }
-        __syncthreads();
+        v_at = v_now;
+        first = first_now;
       }
+      rest -= n;
+      tile = 0;
+      u = next;
     }
-    // O += P V
+    cp_async_wait_all();
+  } else {
+    // ---- weights: a row a thread ---------------------------------------------------------------------------
+    attn::take_registers<200>();
+    const int t = warp >> 2, row = tid & 127;
+    const uint32_t lane_base = uint32_t(warp & 3) << 21;   // 32 lanes of TMEM, in bits 16 and up
+    const uint32_t s_at = tmem + lane_base + t * 128, o_at = tmem + lane_base + 256 + t * 128;
+    int seen = 0, outs = 0;
+    bool ok = true, split = false;   // the unit began in another CTA
+    split = tile != 0;
+    while (rest > 0) {
+      const int n = min(rest, u.tiles - tile), chains = row_tiles(u);
+      const int local = (RT == 2 ? t * 128 : 0) + row, r = u.block * C::kRows + local;   // row in the block, of all
+      const int token = r / p.group;
+      const bool there = r < p.rows, any_there = r - lane < p.rows;
+      const bool takes_part = RT == 1 || t < chains;
+      float m = -INFINITY;
+      float2 sum2[2] = {{0.f, 0.f}, {0.f, 0.f}};
+      int mine = 0;
+      for (int j = RT == 1 ? t : 0; j < n && takes_part; j += RT == 1 ? 2 : 1) {
+        if (!ok || !(ok = waiter.wait(&bar.s_full[t], seen & 1))) break;
+        ++seen;
+        tc::tc_fence_after();
+        if (any_there) {
+          const int first_token = (tile + j) * kTile;
+          attn::soften<T, DP>(s_at, o_at, p.scale_log2, mine == 0, m, sum2, [&](uint32_t (&s)[4][32]) {
+            if (first_token + kTile <= u.length) return;
+            // drafted tokens, or the end
+            const uint8_t* mask = p.mask == nullptr || !there ? nullptr : p.mask + u.b * p.mask_stride + int64_t(token) * p.drafted;
 #pragma unroll
-    for (int ks = 0; ks < kOwn / 16; ++ks) {
-      const uint32_t pa[4] = {pf[2 * ks][0], pf[2 * ks][1], pf[2 * ks + 1][0], pf[2 * ks + 1][1]};
+            for (int x = 0; x < 4; ++x) {
+              uint32_t sees = 0;
+#pragma unroll 8
+              for (int y = 0; y < 32; ++y) {
+                const int d = first_token + x * 32 + y - u.length;
+                bool see = d < 0;
+                if (!see && d < p.drafted && there) see = p.mask == nullptr ? d <= token : mask[d] != 0;
+                sees |= uint32_t(see) << y;
+              }
 #pragma unroll
-      for (int d = 0; d < kDB; d += 2) {
-        uint32_t vf[4];  // channels d*8.. (tokens 0..7, 8..15), channels (d+1)*8.. (the same)
-        ldmatrix4_trans(vf, v_tile + piece<DP>(wn * kOwn + ks * 16 + (lane & 15), d + (lane >> 4)));
-        mma16816<T>(o[d], pa, vf[0], vf[1]);
-        mma16816<T>(o[d + 1], pa, vf[2], vf[3]);
-      }
-    }
-    const bool last_tile = c.tile + 1 == c.tiles, last = i + 1 == n_tiles;
-    if (last_tile || last) {
-      // the end of this CTA's part of the segment
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-      }
-      if constexpr (kWN > 1) {   // warps that share the rows
-        if (in_quad == 0) {
-          sm.m[wn][16 * wm + quad] = m[0];
-          sm.m[wn][16 * wm + quad + 8] = m[1];
+              for (int y = 0; y < 32; ++y) {
+                if (!((sees >> y) & 1)) s[x][y] = 0xff800000u;
+              }
+            }
+          });
         }
-        __syncthreads();
+        ++mine;
+        tc::tc_fence_before();
+        __syncwarp();
+        tc::mbar_arrive(&bar.p_ready[t], lane == 0);
+      }
+      if (mine > 0) {
+        if (ok) ok = waiter.wait(&bar.o_full[t], outs & 1);
+        ++outs;
+      }
+      tc::tc_fence_after();
+      float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+      // the columns of this thread: all, or where both chains have its row a half of the sum of both
+      constexpr int kCols = RT == 1 ? DP / 2 : DP;
+      const int col0 = RT == 1 ? t * kCols : 0;
+      float f[2] = {1.f, 1.f};
+      bool has[2] = {true, true};
+      if (RT == 1) {
+        bar.ml[t][row] = make_float2(mine > 0 ? m : -INFINITY, mine > 0 ? sum : 0.f);
+        tc::tc_fence_before();
+        sync_chains();
+        tc::tc_fence_after();
+        const float2 a = bar.ml[0][row], b = bar.ml[1][row];
+        m = fmaxf(a.x, b.x);
+        has[1] = n > 1;
+        f[0] = m == -INFINITY ? 0.f : exp2_approx((a.x - m) * p.scale_log2);
+        f[1] = m == -INFINITY ? 0.f : exp2_approx((b.x - m) * p.scale_log2);
+        sum = a.y * f[0] + b.y * f[1];
+        if (isnan(a.y) || isnan(b.y)) sum = NAN;
+      }
+      const bool whole = !split && tile + n == u.tiles;
+      // nothing seen: the sum is 0 and so is the output
+      const float inv = !ok || u.bad ? NAN : !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+      const int64_t slot = int64_t(blockIdx.x) * 2 + (split ? 0 : 1);
+      float* part = p.partials + (slot * C::kRows + local) * DP;
+      const bool strange = *static_cast<volatile int*>(&bar.strange) != 0;
+      if (takes_part && any_there) {
+        const int g = r - token * p.group;
+        T* to = static_cast<T*>(p.out) + (int64_t(u.b) * p.drafted + token) * p.heads * p.dim + int64_t(u.head * p.group + g) * p.dim;
+#pragma unroll 1
+        for (int x = col0; x < col0 + kCols; x += 32) {
+          uint32_t raw[32];
+          float o[32];
+          tc::tmem_ld32(tmem + lane_base + 256 + (RT == 1 ? 0 : t * 128) + x, raw);
+          tc::tmem_wait_ld();
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int r = 16 * wm + quad + 8 * half;
-          float top = -INFINITY;
+          for (int y = 0; y < 32; ++y) o[y] = __uint_as_float(raw[y]);
+          if (RT == 1) {
 #pragma unroll
-          for (int w = 0; w < kWN; ++w) top = fmaxf(top, sm.m[w][r]);
-          const float f = top == -INFINITY ? 0.f : exp2_approx(m[half] - top);
-          m[half] = top;
-          l[half] *= f;
+            for (int y = 0; y < 32; ++y) o[y] *= f[0];
+            if (has[1]) {
+              tc::tmem_ld32(tmem + lane_base + 256 + 128 + x, raw);
+              tc::tmem_wait_ld();
 #pragma unroll
-          for (int d = 0; d < kDB; ++d) { o[d][2 * half] *= f; o[d][2 * half + 1] *= f; }
-          if (in_quad == 0) sm.l[wn][r] = l[half];
-        }
-        for (int w = 1; w < kWN; ++w) {
-          if (wn == w) {
+              for (int y = 0; y < 32; ++y) o[y] = fmaf(__uint_as_float(raw[y]), f[1], o[y]);
+            }
+          }
+          if (!there) continue;
+          if (strange) {
+            for (int d = max(0, tile * kTile - u.length); d < min(p.drafted, (tile + n) * kTile - u.length); ++d) {
+              if (!(p.mask == nullptr ? d <= token : p.mask[u.b * p.mask_stride + int64_t(token) * p.drafted + d] != 0)) continue;
+              const T* v = static_cast<const T*>(p.v) + u.b * p.v_stride[0] + d * p.v_stride[1] + u.head * p.v_stride[2];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-#pragma unroll
-              for (int d = 0; d < kDB; ++d) {
-                float2* at = reinterpret_cast<float2*>(&sm.o[16 * wm + quad + 8 * half][d * 8 + in_quad * 2]);
-                float2 x = make_float2(o[d][2 * half], o[d][2 * half + 1]);
-                if (w > 1) { x.x += at->x; x.y += at->y; }
-                *at = x;
+              for (int y = 0; y < 32; ++y) {
+                const float value = x + y < p.dim ? to_float(v[x + y]) : 0.f;
+                if (!isfinite(value)) o[y] += value;
               }
             }
           }
-          __syncthreads();
-        }
-        if (wn == 0) {
+          if (whole) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int r = 16 * wm + quad + 8 * half;
-            l[half] = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWN; ++w) l[half] += sm.l[w][r];
-#pragma unroll
-            for (int d = 0; d < kDB; ++d) {
-              const float2 x = *reinterpret_cast<const float2*>(&sm.o[r][d * 8 + in_quad * 2]);
-              o[d][2 * half] += x.x;
-              o[d][2 * half + 1] += x.y;
-            }
-          }
-        }
-      }
-      if (wn == 0) {
-        const bool whole_segment = starts_here && last_tile;
-        float* part = p.partials + (int64_t(blockIdx.x) * 2 + (starts_here ? 1 : 0)) * kRows * (DP + 2);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int r = seg_row + quad + 8 * half;
-          if (whole_segment) {
-            if (r < p.rows) {
-              const int n = r / p.group, g = r - n * p.group;
-              // nothing seen: the sum is 0 and so is the output
-              const float inv = l[half] == 0.f ? 0.f : 1.f / l[half];
-              T* to = static_cast<T*>(p.out) + (int64_t(c.b) * p.drafted + n) * p.heads * p.dim +
-                      int64_t(c.head * p.group + g) * p.dim;
-#pragma unroll
-              for (int d = 0; d < kDB; ++d) {
-                const int col = d * 8 + in_quad * 2;
-                if (col < p.dim) *reinterpret_cast<uint32_t*>(to + col) = pack_pair<T>(o[d][2 * half] * inv, o[d][2 * half + 1] * inv);
+            for (int y = 0; y < 32; y += 8) {
+              if (x + y < p.dim) {
+                uint4 w;
+                w.x = pack_pair<T>(o[y] * inv, o[y + 1] * inv);
+                w.y = pack_pair<T>(o[y + 2] * inv, o[y + 3] * inv);
+                w.z = pack_pair<T>(o[y + 4] * inv, o[y + 5] * inv);
+                w.w = pack_pair<T>(o[y + 6] * inv, o[y + 7] * inv);
+                *reinterpret_cast<uint4*>(to + x + y) = w;
               }
             }
           } else {
-            const int lr = 16 * wm + quad + 8 * half;
-            float* row = part + int64_t(lr) * DP;
 #pragma unroll
-            for (int d = 0; d < kDB; ++d) *reinterpret_cast<float2*>(row + d * 8 + in_quad * 2) = make_float2(o[d][2 * half], o[d][2 * half + 1]);
-            if (in_quad == 0) *reinterpret_cast<float2*>(part + kRows * DP + 2 * lr) = make_float2(m[half], l[half]);
+            for (int y = 0; y < 32; y += 4) *reinterpret_cast<float4*>(part + x + y) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
           }
         }
+        if (!whole && there && col0 == 0) {
+          float* ml = p.partials + int64_t(p.ctas) * 2 * C::kRows * DP + (slot * C::kRows + local) * 2;
+          *reinterpret_cast<float2*>(ml) = make_float2(m == -INFINITY ? m : m * p.scale_log2, inv * sum);
+        }
       }
-      fresh_segment = true;
+      tc::tc_fence_before();
+      if (RT == 1) sync_chains();   // the other chain has read this one's O
+      rest -= n;
+      tile = 0;
+      split = false;
+      if (rest > 0) next_unit(p, u);
     }
-    advance(p, c);
-    if (located < n_tiles) {
-      // the slot of the tile before this one: every thread has read it before this iteration's barrier
-      locate(ahead, located % (kStages + 1));
-      advance(p, ahead);
-      ++located;
-    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 512);
   }
 }
 
-// Joins what several CTAs have of one (sequence, key head, block of rows): a CTA each.
+// Joins what several CTAs have of a unit: a warp a row, in the order of the tiles.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) tree_join_kernel(const TreeParams p, int rows_of_block) {
-  __shared__ int64_t scan[kThreads / 32];
+__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ TreeParams p, int block_rows, int ctas_of_unit) {
+  __shared__ int64_t scan[kJoinThreads / 32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int unit = blockIdx.x;
+  const int unit = int(blockIdx.x) / ctas_of_unit;
   const int block = unit % p.row_blocks, head = unit / p.row_blocks % p.kv_heads, b = unit / p.row_blocks / p.kv_heads;
   int64_t total = 0, from = 0, before;
-  for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
+  for (int b0 = 0; b0 < p.batch; b0 += kJoinThreads) {
     const int x = b0 + int(threadIdx.x);
     const int64_t own = x < p.batch ? tiles_of(p, x) : 0;
-    total += cta_scan(own, &before, scan);
-    int64_t sum_before = cta_scan(x < b ? own : 0, &before, scan);
-    from += sum_before;
+    total += cta_scan<kJoinThreads / 32>(own, &before, scan);
+    from += cta_scan<kJoinThreads / 32>(x < b ? own : 0, &before, scan);
   }
-  Cursor c{b, 0, 0, 0, 0, 0, 0, false};
-  read_length(p, c);
-  const int64_t t0 = from + (int64_t(head) * p.row_blocks + block) * c.tiles, t1 = t0 + c.tiles;
+  Unit u{b, 0, 0, 0, 0, false};
+  read_length(p, u);
+  const int64_t t0 = from + (int64_t(head) * p.row_blocks + block) * u.tiles, t1 = t0 + u.tiles;
   const int64_t ctas = sharing(p, total), c0 = ((t0 + 1) * ctas - 1) / total, c1 = (t1 * ctas - 1) / total;
   if (c0 == c1) return;   // one CTA had it all
-  const int row0 = block * rows_of_block;
-  const int64_t size = int64_t(rows_of_block) * (DP + 2);
-  constexpr int kQuads = DP / 4;
-  for (int x = threadIdx.x; x < rows_of_block * kQuads; x += kThreads) {
-    const int lr = x / kQuads, d = (x - lr * kQuads) * 4, r = row0 + lr;
-    if (r >= p.rows || d >= p.dim) continue;
-    float top = -INFINITY;
-    for (int64_t i = c0; i <= c1; ++i) {
-      const float* part = p.partials + (i * 2 + (i == c0 ? 1 : 0)) * size;
-      top = fmaxf(top, part[rows_of_block * DP + 2 * lr]);
-    }
-    float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t i = c0; i <= c1; ++i) {
-      const float* part = p.partials + (i * 2 + (i == c0 ? 1 : 0)) * size;
-      const float2 ml = *reinterpret_cast<const float2*>(part + rows_of_block * DP + 2 * lr);
-      const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
-      sum += isnan(ml.y) ? ml.y : ml.y * f;
-      const float4 v = *reinterpret_cast<const float4*>(part + int64_t(lr) * DP + d);
-      acc[0] += v.x * f; acc[1] += v.y * f; acc[2] += v.z * f; acc[3] += v.w * f;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int n = r / p.group, g = r - n * p.group;
-    T* to = static_cast<T*>(p.out) + (int64_t(b) * p.drafted + n) * p.heads * p.dim + int64_t(head * p.group + g) * p.dim + d;
-    *reinterpret_cast<uint2*>(to) = make_uint2(pack_pair<T>(acc[0] * inv, acc[1] * inv), pack_pair<T>(acc[2] * inv, acc[3] * inv));
+  const int lane = threadIdx.x & 31;
+  const int local = (int(blockIdx.x) - unit * ctas_of_unit) * (kJoinThreads / 32) + int(threadIdx.x >> 5);
+  const int r = block * block_rows + local;
+  if (local >= block_rows || r >= p.rows) return;
+  const float* all_ml = p.partials + int64_t(p.ctas) * 2 * block_rows * DP;
+  // the part of CTA i: its last unit where the unit began there, its first one otherwise
+  auto row_of = [&](int64_t i) { return (i * 2 + (i == c0 ? 1 : 0)) * block_rows + local; };
+  float top = -INFINITY;
+  for (int64_t i = c0 + lane; i <= c1; i += 32) top = fmaxf(top, all_ml[row_of(i) * 2]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  constexpr int kOwn = DP / 32;
+  float sum = 0.f, acc[kOwn];
+#pragma unroll
+  for (int y = 0; y < kOwn; ++y) acc[y] = 0.f;
+#pragma unroll 4
+  for (int64_t i = c0; i <= c1; ++i) {
+    const float2 ml = *reinterpret_cast<const float2*>(all_ml + row_of(i) * 2);
+    const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
+    sum += isnan(ml.y) ? ml.y : ml.y * f;
+    const float* o = p.partials + row_of(i) * DP + lane * kOwn;
+#pragma unroll
+    for (int y = 0; y < kOwn; ++y) acc[y] = fmaf(o[y], f, acc[y]);
   }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int n = r / p.group, g = r - n * p.group, d = lane * kOwn;
+  if (d >= p.dim) return;
+  T* to = static_cast<T*>(p.out) + (int64_t(b) * p.drafted + n) * p.heads * p.dim + int64_t(head * p.group + g) * p.dim + d;
+#pragma unroll
+  for (int y = 0; y < kOwn; y += 2) *reinterpret_cast<uint32_t*>(to + y) = pack_pair<T>(acc[y] * inv, acc[y + 1] * inv);
 }
 
-// rows of a block: as few as hold all rows, 64 at most
-int block_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// rows of a block
+int block_rows(int64_t rows) { return rows <= 128 ? 128 : 256; }
 
-template <typename T, int DP, int WM>
+template <typename T, int DP, int RT, int QR>
 int launch_tree_typed(const TreeParams& p, cudaStream_t stream) {
-  constexpr int kBytes = int(sizeof(TreeSmem<DP, WM>));
-  const void* kernel = reinterpret_cast<const void*>(&tree_kernel<T, DP, WM>);
-  const cudaError_t err = ensure_dynamic_smem(kernel, kBytes);
+  using C = TreeConfig<DP, RT, QR>;
+  const void* kernel = reinterpret_cast<const void*>(&tree_kernel<T, DP, RT, QR>);
+  const cudaError_t err = ensure_dynamic_smem(kernel, C::kBytes);
   if (err != cudaSuccess) { record_cuda_error(err); return GDN2_ERR_LAUNCH; }
-  tree_kernel<T, DP, WM><<<unsigned(p.ctas), kThreads, kBytes, stream>>>(p);
+  const int per_unit = (std::min(p.rows, C::kRows) + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
+  const int64_t joining = int64_t(p.batch) * p.kv_heads * p.row_blocks * per_unit;
+  if (joining > int64_t(0x7fffffff)) return GDN2_ERR_TOO_LARGE;
+  tree_kernel<T, DP, RT, QR><<<unsigned(p.ctas), kThreads, C::kBytes, stream>>>(p);
   const int status = check_launch();
   if (status != GDN2_OK) return status;
-  const int64_t units = int64_t(p.batch) * p.kv_heads * p.row_blocks;
-  return launch_beside(&tree_join_kernel<T, DP>, unsigned(units), kThreads, 0, stream, p, 16 * WM);
+  return launch_beside(&tree_join_kernel<T, DP>, unsigned(joining), kJoinThreads, 0, stream, p, C::kRows, per_unit);
 }
 
 template <typename T>
 int launch_tree_dim(const TreeParams& p, cudaStream_t stream) {
-  const int rows = block_rows(p.rows);
   if (p.dim <= 64) {
-    return rows == 16 ? launch_tree_typed<T, 64, 1>(p, stream) : rows == 32 ? launch_tree_typed<T, 64, 2>(p, stream)
-                                                                            : launch_tree_typed<T, 64, 4>(p, stream);
+    return p.rows <= 128 ? launch_tree_typed<T, 64, 1, 128>(p, stream) : launch_tree_typed<T, 64, 2, 128>(p, stream);
   }
-  return rows == 16 ? launch_tree_typed<T, 128, 1>(p, stream) : rows == 32 ? launch_tree_typed<T, 128, 2>(p, stream)
-                                                                           : launch_tree_typed<T, 128, 4>(p, stream);
+  return p.rows <= 32 ? launch_tree_typed<T, 128, 1, 32>(p, stream)
+                      : p.rows <= 128 ? launch_tree_typed<T, 128, 1, 128>(p, stream) : launch_tree_typed<T, 128, 2, 128>(p, stream);
 }
 
 }  // namespace
@@ -644,13 +719,8 @@ int launch_append(const void* k, const void* v, void* k_pages, void* v_pages, co
   return check_launch();
 }
 
-// CTAs of a call: two an SM, which the tiles share whatever their number
-int tree_ctas(int* ctas) {
-  int sms = 0;
-  const int status = multiprocessors(&sms);
-  *ctas = 2 * sms;
-  return status;
-}
+// CTAs of a call: one an SM, which the tiles share whatever their number
+int tree_ctas(int* ctas) { return multiprocessors(ctas); }
 
 int64_t tree_workspace_bytes(int64_t rows, int dim, int ctas) {
   return int64_t(ctas) * 2 * block_rows(rows) * ((dim <= 64 ? 64 : 128) + 2) * 4;
@@ -674,7 +744,9 @@ int launch_tree(const void* q, const void* k, const void* v, const void* k_pages
   const int status = tree_ctas(&p.ctas);
   if (status != GDN2_OK) return status;
   if (int64_t(batch) * kv_heads * p.row_blocks > int64_t(0x7fffffff)) return GDN2_ERR_TOO_LARGE;
-  p.scale_log2 = scale * kLog2e;
+  // the sign goes to the product, and a scale of 0 stays a positive number, so that -inf * scale masks as ever
+  p.negate = scale < 0.f;
+  p.scale_log2 = fmaxf(fabsf(scale) * attn::kLog2e, 1e-30f);
   return dtype == GDN2_BF16 ? launch_tree_dim<__nv_bfloat16>(p, stream) : launch_tree_dim<__half>(p, stream);
 }
 
