@@ -23,7 +23,7 @@ namespace attn {
 
 namespace {
 
-constexpr int kThreads = 384;    // warps 0-3: even steps; 4-7: odd ones; 8: products; 9: copies
+constexpr int kThreads = 640;    // warps 0-7: even steps; 8-15: odd ones; 16: products; 17: copies
 constexpr int kStep = 64;        // rows of a step
 
 template <int DP>
@@ -31,7 +31,7 @@ struct BwdConfig {
   static constexpr int kStayBytes = 128 * DP * 2, kStaySlab = 128 * 128;
   static constexpr int kGoBytes = kStep * DP * 2, kGoSlab = kStep * 128;
   static constexpr int kStages = DP == 128 ? 4 : 6;
-  static constexpr int kBytes = 2 * kStayBytes + kStages * (2 * kGoBytes + 2 * kStep * 4) + 1024 /* alignment */ + 512;
+  static constexpr int kBytes = 2 * kStayBytes + kStages * (2 * kGoBytes + 2 * kStep * 4) + 512;
 };
 
 struct BwdParams {
@@ -78,8 +78,7 @@ __device__ __forceinline__ bool bwd_item(const BwdParams& p, int turn, BwdItem* 
 template <typename T, int DP, bool kKeys>
 __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const __grid_constant__ BwdParams p) {
   using C = BwdConfig<DP>;
-  extern __shared__ uint8_t raw_smem[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
   uint8_t* stay = smem;
   uint8_t* go = smem + 2 * C::kStayBytes;
   float* stats = reinterpret_cast<float*>(go + C::kStages * 2 * C::kGoBytes);   // [stage][lse, delta][64]
@@ -90,12 +89,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
     tc::mbar_init(&bar.stay_full, 1);
     tc::mbar_init(&bar.stay_empty, 1);
     tc::mbar_init(&bar.acc_full, 1);
-    tc::mbar_init(&bar.acc_empty, 8);
+    tc::mbar_init(&bar.acc_empty, 16);
     tc::mbar_init(&bar.raw, 1);
     tc::mbar_init(&bar.drained, 1);
     for (int b = 0; b < 2; ++b) {
       tc::mbar_init(&bar.s_full[b], 1);
-      tc::mbar_init(&bar.ds_ready[b], 4);
+      tc::mbar_init(&bar.ds_ready[b], 8);
     }
     for (int s = 0; s < C::kStages; ++s) {
       tc::mbar_init(&bar.go_full[s], 1);
@@ -104,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
     bar.failed = 0;
     tc::fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == 16) {
     tc::tmem_alloc(&bar.tmem, 512);
     tc::tmem_relinquish();
   }
@@ -114,10 +113,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
   const uint32_t tmem = bar.tmem;
   const Waiter waiter{&bar.failed};
 
-  if (warp >= 8) {
-    // 384 threads of 168 registers = 256 of 208 + 128 of 88
-    give_registers<88>();
-    if (warp == 9) {
+  if (warp >= 16) {
+    give_registers();
+    if (warp == 17) {
       // ---- copies ----------------------------------------------------------------------------------------
       const uint32_t leader = tc::elect_leader();
       int filled = 0, stayed = 0, mended = 0;
@@ -182,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
         }
         for (int i = 0; stayed > 0 && i < 4096 && !tc::mbar_try_wait(&bar.stay_full, (stayed - 1) & 1); ++i) {}
       }
-    } else if (warp == 8) {
+    } else if (warp == 16) {
       // ---- products --------------------------------------------------------------------------------------
       const uint32_t leader = tc::elect_leader();
       const uint32_t id_s = tc::idesc(128, kStep, Format<T>::code, tc::kMajorK, tc::kMajorK, p.negate);
@@ -219,10 +217,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
           const uint32_t p_at = tmem + 256 + b * 128, ds_at = p_at + 64;
           if (kKeys) {
 #pragma unroll
-            for (int ks = 0; ks < kStep / 16; ++ks) mma_ts(tmem, p_at + ks * 8, desc_mn(ys, C::kGoSlab, ks), id_acc, i > 0 || ks > 0, leader);
+            for (int ks = 0; ks < kStep / 16; ++ks) mma_ts(tmem, p_at + (ks >> 1) * 32 + (ks & 1) * 8, desc_mn(ys, C::kGoSlab, ks), id_acc, i > 0 || ks > 0, leader);
           }
 #pragma unroll
-          for (int ks = 0; ks < kStep / 16; ++ks) mma_ts(tmem + 128, ds_at + ks * 8, desc_mn(xs, C::kGoSlab, ks), id_acc, i > 0 || ks > 0, leader);
+          for (int ks = 0; ks < kStep / 16; ++ks) mma_ts(tmem + 128, ds_at + (ks >> 1) * 32 + (ks & 1) * 8, desc_mn(xs, C::kGoSlab, ks), id_acc, i > 0 || ks > 0, leader);
           tc::mma_commit(&bar.go_empty[x % C::kStages], leader);
           if (i + 1 == w.steps) {
             tc::mma_commit(&bar.acc_full, leader);
@@ -240,11 +238,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
       __syncwarp();
     }
   } else {
-    // ---- weights: a row a thread ---------------------------------------------------------------------------
-    take_registers<208>();
-    const int b = warp >> 2, row = threadIdx.x & 127;
+    // ---- weights: two threads a row ------------------------------------------------------------------------
+    take_registers();
+    const int b = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & 127;   // two threads a row, 32 columns each
     const uint32_t lane_base = uint32_t(warp & 3) << 21;   // 32 lanes of TMEM, in bits 16 and up
-    const uint32_t s_at = tmem + lane_base + 256 + b * 128, dp_at = s_at + 64;
+    const uint32_t s_at = tmem + lane_base + 256 + b * 128 + half * 32, dp_at = s_at + 64;
     int used = 0, seen = 0, outs = 0;
     bool ok = true;
     for (int turn = 0; turn < p.turns; ++turn) {
@@ -265,35 +263,31 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
         const int from = w.tile * 128 + row - at;
         const bool diagonal = kKeys ? at < w.tile * 128 + 128 : at + kStep > w.tile * 128;
         const float* st = stats + ((used + i) % C::kStages) * 2 * kStep;
-        uint32_t pw[32], dsw[32];
+        uint32_t s[32], dp[32], pw[16], dsw[16];
+        tc::tmem_ld32(s_at, s);
+        tc::tmem_ld32(dp_at, dp);
+        tc::tmem_wait_ld();
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t s[32], dp[32];
-          tc::tmem_ld32(s_at + half * 32, s);
-          tc::tmem_ld32(dp_at + half * 32, dp);
-          tc::tmem_wait_ld();
-#pragma unroll
-          for (int y = 0; y < 32; y += 2) {
-            const int x = half * 32 + y;
-            float2 l = twice(lse), d = twice(delta);
-            if (kKeys) {
-              l = *reinterpret_cast<const float2*>(st + x);
-              d = *reinterpret_cast<const float2*>(st + kStep + x);
-            }
-            const float2 sc = fma2(make_float2(__uint_as_float(s[y]), __uint_as_float(s[y + 1])), twice(p.scale_log2), minus2(make_float2(0.f, 0.f), l));
-            float2 e = exp2_2(sc);
-            float2 ds = mul2(e, minus2(make_float2(__uint_as_float(dp[y]), __uint_as_float(dp[y + 1])), d));
-            if (diagonal) {
-              if (kKeys ? x < from : x > from) { e.x = 0.f; ds.x = 0.f; }
-              if (kKeys ? x + 1 < from : x + 1 > from) { e.y = 0.f; ds.y = 0.f; }
-            }
-            // both are rounded to the inputs' type for their products, the sums are in 32 bits
-            if (kKeys) pw[x / 2] = pack_pair<T>(e.x, e.y);
-            dsw[x / 2] = pack_pair<T>(ds.x, ds.y);
+        for (int y = 0; y < 32; y += 2) {
+          const int x = half * 32 + y;
+          float2 l = twice(lse), d = twice(delta);
+          if (kKeys) {
+            l = *reinterpret_cast<const float2*>(st + x);
+            d = *reinterpret_cast<const float2*>(st + kStep + x);
           }
+          const float2 sc = fma2(make_float2(__uint_as_float(s[y]), __uint_as_float(s[y + 1])), twice(p.scale_log2), minus2(make_float2(0.f, 0.f), l));
+          float2 e = exp2_2(sc);
+          float2 ds = mul2(e, minus2(make_float2(__uint_as_float(dp[y]), __uint_as_float(dp[y + 1])), d));
+          if (diagonal) {
+            if (kKeys ? x < from : x > from) { e.x = 0.f; ds.x = 0.f; }
+            if (kKeys ? x + 1 < from : x + 1 > from) { e.y = 0.f; ds.y = 0.f; }
+          }
+          // both are rounded to the inputs' type for their products, the sums are in 32 bits
+          if (kKeys) pw[y / 2] = pack_pair<T>(e.x, e.y);
+          dsw[y / 2] = pack_pair<T>(ds.x, ds.y);
         }
-        if (kKeys) tc::tmem_st32(s_at, pw);
-        tc::tmem_st32(dp_at, dsw);
+        if (kKeys) tc::tmem_st16(s_at, pw);
+        tc::tmem_st16(dp_at, dsw);
         tc::tmem_wait_st();
         tc::tc_fence_before();
         __syncwarp();
@@ -303,23 +297,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
       if (ok) ok = waiter.wait(&bar.acc_full, outs & 1);
       ++outs;
       tc::tc_fence_after();
-      // keys: the first four warps have dv, the others dk; queries: a half of dq's channels each
+      // keys: eight warps have dv, the others dk, a thread half of a row's channels; queries: a quarter of dq's
       const int i = w.tile * 128 + row;
       const bool there = i < w.at.len;
       const float by = !ok ? NAN : kKeys && b == 0 ? 1.f : p.scale;
       const int64_t out_row = ((w.at.row + i) * (kKeys ? p.kv_heads : p.heads) + w.head) * p.dim;
       T* to = static_cast<T*>(kKeys ? (b == 0 ? p.dv : p.dk) : p.dq) + out_row;
       const uint32_t acc = tmem + lane_base + (kKeys ? b * 128 : 128);
-      constexpr int kCols = kKeys ? DP : DP / 2;
-      const int col0 = kKeys ? 0 : b * kCols;
+      constexpr int kCols = kKeys ? DP / 2 : DP / 4;
+      const int col0 = kKeys ? half * kCols : (2 * b + half) * kCols;
 #pragma unroll
-      for (int x = 0; x < kCols; x += 32) {
-        uint32_t o[32];
-        tc::tmem_ld32(acc + col0 + x, o);
+      for (int x = 0; x < kCols; x += 16) {
+        uint32_t o[16];
+        tc::tmem_ld16(acc + col0 + x, o);
         tc::tmem_wait_ld();
         if (there) {
 #pragma unroll
-          for (int y = 0; y < 32; y += 8) {
+          for (int y = 0; y < 16; y += 8) {
             if (col0 + x + y < p.dim) {
               uint4 v;
               v.x = pack_pair<T>(__uint_as_float(o[y]) * by, __uint_as_float(o[y + 1]) * by);
@@ -338,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }

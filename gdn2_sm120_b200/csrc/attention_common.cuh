@@ -87,11 +87,10 @@ struct Waiter {
   }
 };
 
-// Registers move from the warps that copy and issue to those that compute; the sum stays what the CTA was launched with.
-template <int N>
-__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// Registers move from the warps that copy and issue to those that compute; the sum stays what the CTA was launched with:
+// 640 threads of 96 = 512 of 104 + 128 of 64.
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 104;"); }
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
 
 // ---- 16-bit products ---------------------------------------------------------------------------------------
 // Tiles of [rows][64] channels in lines of 128 bytes whose 16-byte pieces are permuted by the line (the 128-byte
@@ -132,33 +131,60 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// One tile of scores becomes weights, a row a thread: S (128 columns of TMEM at s_at) is read, masked, and overlaid by
-// P = exp2(S c - m c) in 16 bits.  m is the row's reference so far and `sum` the sum of its weights; both and O (DP columns
-// at o_at, as it is after all tiles before this one) follow a maximum that has grown by more than 2^kRescale: weights stay
-// below that and sums in 32 bits lose nothing.
+// One tile of 128 x 128 scores becomes weights.  Two threads have a row, 64 columns each (of chain `id`, 256 threads), so
+// that eight warps and not four hide the latencies of one chain: 3900 clocks a tile with four (1950 with two chains).
+// S is read from TMEM, masked, and P = exp2(S c - m c) in 16 bits lies over the first half of its own 64 columns.  m is the
+// row's reference so far and `sum` this thread's part of its weights; both and O (as it is after all tiles before this one)
+// follow a maximum that has grown by more than 2^kRescale: weights stay below that and sums in 32 bits lose nothing.  Only
+// then, and at the first tile, do the two threads have to tell each other their maxima.
 constexpr float kRescale = 8.f;
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// what the two threads of a row tell each other
+struct Exchange { float x[2][128]; };
+
+struct Half {
+  int id, half, row;       // chain, columns, row
+  int threads;             // of the chain that have rows: all of some warps
+  Exchange* exchange;
+  __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory"); }
+  // the other thread's value
+  __device__ __forceinline__ float other(float mine) const {
+    exchange->x[half][row] = mine;
+    sync();
+    const float r = exchange->x[half ^ 1][row];
+    sync();
+    return r;
+  }
+  __device__ __forceinline__ bool any(bool x) const {   // of the chain
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %3, 0;\n\tbar.red.or.pred p, %1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(r) : "r"(id + 1), "r"(threads), "r"(uint32_t(x)) : "memory");
+    return r != 0;
+  }
+};
+
 template <typename T, int DP, typename Mask>
-__device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, bool first, float& m, float2 (&sum)[2],
+__device__ __forceinline__ void soften(const Half& h, uint32_t s_at, uint32_t o_at, float c, bool first, float& m, float2 (&sum)[2],
                                        Mask mask) {
-  uint32_t s[4][32];
+  uint32_t s[2][32];
 #pragma unroll
-  for (int x = 0; x < 4; ++x) tc::tmem_ld32(s_at + x * 32, s[x]);
+  for (int x = 0; x < 2; ++x) tc::tmem_ld32(s_at + x * 32, s[x]);
   tc::tmem_wait_ld();
   mask(s);
   float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int x = 0; x < 128; x += 2) {
+  for (int x = 0; x < 64; x += 2) {
     tops[(x >> 1) & 3] = max3(tops[(x >> 1) & 3], __uint_as_float(s[x >> 5][x & 31]), __uint_as_float(s[x >> 5][(x & 31) + 1]));
   }
-  const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
+  float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
   if (first) {
-    m = top;
-  } else {
+    m = fmaxf(top, h.other(top));
+  } else if (h.any((top - m) * c > kRescale)) {
+    top = fmaxf(top, h.other(top));
     const bool grown = (top - m) * c > kRescale;
     if (__any_sync(0xffffffffu, grown)) {
       const float f = grown ? exp2_approx((m - top) * c) : 1.f;
@@ -166,13 +192,13 @@ __device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, bo
 #pragma unroll
       for (int x = 0; x < 2; ++x) sum[x] = mul2(sum[x], twice(f));
 #pragma unroll
-      for (int x = 0; x < DP / 32; ++x) {
-        uint32_t o[32];
-        tc::tmem_ld32(o_at + x * 32, o);
+      for (int x = 0; x < DP / 2; x += 16) {
+        uint32_t o[16];
+        tc::tmem_ld16(o_at + x, o);
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-        tc::tmem_st32(o_at + x * 32, o);
+        for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+        tc::tmem_st16(o_at + x, o);
       }
     }
   }
@@ -180,15 +206,14 @@ __device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, bo
   const float2 minus = twice(m == -INFINITY ? 0.f : -m * c), by = twice(c);
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    uint32_t w[32];
+    uint32_t w[16];
 #pragma unroll
-    for (int y = 0; y < 32; ++y) {
-      const int at = x * 64 + y * 2;
-      const float2 e = exp2_2(fma2(make_float2(__uint_as_float(s[at >> 5][at & 31]), __uint_as_float(s[at >> 5][(at & 31) + 1])), by, minus));
+    for (int y = 0; y < 16; ++y) {
+      const float2 e = exp2_2(fma2(make_float2(__uint_as_float(s[x][2 * y]), __uint_as_float(s[x][2 * y + 1])), by, minus));
       sum[y & 1] = add2(sum[y & 1], e);
       w[y] = pack_pair<T>(e.x, e.y);   // the sum has them as they were, the product rounded to the values' type
     }
-    tc::tmem_st32(s_at + x * 32, w);
+    tc::tmem_st16(s_at + x * 16, w);
   }
   tc::tmem_wait_st();
 }

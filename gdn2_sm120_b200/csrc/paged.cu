@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 
 // ---- tree attention ----------------------------------------------------------------------------------
 constexpr int kTile = 128;     // tokens of a tile
-constexpr int kThreads = 512;  // warps 0-3, 4-7: weights; 8-11: copies; 12: products
+constexpr int kThreads = 640;  // warps 0-7, 8-15: weights; 16, 17: keys and values; 18: queries; 19: products
 constexpr int kJoinThreads = 128;
 struct TreeParams {
   const void *q, *k, *v;
@@ -76,6 +76,8 @@ struct TreeParams {
   int64_t table_stride, mask_stride, pages;
   int batch, drafted, heads, kv_heads, group, dim, page, columns;
   int rows, row_blocks, ctas;
+  int box;                                   // rows of a tiled copy, or 0: none fits the pages
+  CUtensorMap k_map, v_map;
   float scale_log2;                          // positive
   uint32_t negate;                           // the scale is negative: Q counts with its sign changed
 };
@@ -136,6 +138,46 @@ __device__ __forceinline__ int64_t cta_scan(int64_t x, int64_t* before, int64_t*
   return total;
 }
 
+// This CTA's part of all tiles: its first unit and tile, and how many tiles; false if there are fewer tiles than CTAs.
+template <int kWarps>
+struct Share { int64_t scan[kWarps], found[2]; };
+template <int kWarps>
+__device__ __forceinline__ bool part_of_cta(const TreeParams& p, Share<kWarps>& shared, Unit& u, int& tile, int& rest) {
+  const int tid = threadIdx.x;
+  int64_t total = 0, before, own = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32 * kWarps) {
+    own = b0 + tid < p.batch ? tiles_of(p, b0 + tid) : 0;
+    total += cta_scan<kWarps>(own, &before, shared.scan);
+  }
+  const int64_t ctas = sharing(p, total);
+  if (blockIdx.x >= ctas) return false;
+  const int64_t begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
+  int64_t base = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32 * kWarps) {
+    int64_t sum = total;
+    if (p.batch > 32 * kWarps) {   // otherwise all of them have just been looked at
+      own = b0 + tid < p.batch ? tiles_of(p, b0 + tid) : 0;
+      sum = cta_scan<kWarps>(own, &before, shared.scan);
+    }
+    const int64_t from = base + before;
+    if (own > 0 && begin >= from && begin < from + own) {  // one thread of all
+      shared.found[0] = b0 + tid;
+      shared.found[1] = begin - from;
+    }
+    base += sum;
+    if (begin < base) break;
+  }
+  __syncthreads();
+  u = Unit{int(shared.found[0]), 0, 0, 0, 0, false};
+  read_length(p, u);
+  const int64_t unit = shared.found[1] / u.tiles;
+  tile = int(shared.found[1] - unit * u.tiles);
+  u.head = int(unit / p.row_blocks);
+  u.block = int(unit - int64_t(u.head) * p.row_blocks);
+  rest = int(end - begin);
+  return true;
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
@@ -146,13 +188,180 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 }
 
 // both chains
-__device__ __forceinline__ void sync_chains() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void sync_chains() { asm volatile("bar.sync 3, 512;" ::: "memory"); }
 
 // The key of a page number outside the cache: 128 channels of NaN, in either type
 #define GDN2_NAN4 {~0u, ~0u, ~0u, ~0u}
 __device__ const uint4 g_nan_row[16] = {GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4,
                                         GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NAN4};
 #undef GDN2_NAN4
+
+// A warp copies 32 rows of DP channels, half of it or a quarter a row at a time: `at` is where row `first + lane` is, null
+// for zeros.  In shared memory a slab has 64 channels, in lines of 128 bytes whose 16-byte pieces are permuted by the line.
+template <int DP>
+__device__ __forceinline__ uint32_t place_of(uint32_t base, uint32_t slab, int row, int piece) {
+  return base + uint32_t(piece >> 3) * slab + uint32_t(row) * 128u + ((uint32_t(piece ^ row) & 7u) << 4);
+}
+template <int DP>
+__device__ __forceinline__ void copy_rows(uint32_t base, uint32_t slab, int first, int dim, const void* at) {
+  constexpr int kPieces = DP / 8, kAtOnce = 32 / kPieces;
+  const int lane = threadIdx.x & 31, piece = lane % kPieces, sub = lane / kPieces;
+  const uint64_t anything = reinterpret_cast<uintptr_t>(g_nan_row);   // an address for copies of nothing
+  const uint32_t lo = uint32_t(reinterpret_cast<uintptr_t>(at)), hi = uint32_t(reinterpret_cast<uintptr_t>(at) >> 32);
+#pragma unroll
+  for (int i = 0; i < 32; i += 8 * kAtOnce) {
+    uint64_t row[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int r = i + x * kAtOnce + sub;
+      row[x] = (uint64_t(__shfl_sync(0xffffffffu, hi, r)) << 32) | __shfl_sync(0xffffffffu, lo, r);
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const bool there = piece * 8 < dim && row[x] != 0;
+      cp_async16(place_of<DP>(base, slab, first + i + x * kAtOnce + sub, piece),
+                 reinterpret_cast<const uint8_t*>(there ? row[x] : anything) + piece * 16, there);
+    }
+  }
+}
+
+// An infinite or NaN value of a drafted token must reach the rows that see it and no others, but in the product it would
+// meet every row (0 * NaN): it leaves the tile, and is added to those rows at the end.  Rows first .. last - 1, by the warp
+// that copied them; true for a thread that found one.
+template <typename T, int DP>
+__device__ __forceinline__ bool sift(uint32_t base, uint32_t slab, int first, int last) {
+  constexpr int kPieces = DP / 8, kAtOnce = 32 / kPieces;
+  const int lane = threadIdx.x & 31, piece = lane % kPieces, sub = lane / kPieces;
+  bool found = false;
+  __syncwarp();
+  for (int r = first + sub; r < last; r += kAtOnce) {
+    const uint32_t at = place_of<DP>(base, slab, r, piece);
+    uint32_t w[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if ((w[j] & Format<T>::exponent) == Format<T>::exponent) { w[j] &= 0xffff0000u; any = true; }
+      if (((w[j] >> 16) & Format<T>::exponent) == Format<T>::exponent) { w[j] &= 0xffffu; any = true; }
+    }
+    if (any) {
+      asm volatile("st.shared.v4.b32 [%4], {%0, %1, %2, %3};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(at) : "memory");
+      found = true;
+    }
+  }
+  return found;
+}
+
+// a tiled copy into shared memory that is given by its address there
+__device__ __forceinline__ void tma_load_page(uint32_t to, const CUtensorMap* map, int c, int head, int row, int page,
+                                              uint64_t* full, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+      "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3, %4, %5}], [%6];\n\t}"
+      ::"r"(to), "l"(map), "r"(c), "r"(head), "r"(row), "r"(page), "r"(tc::smem_u32(full)), "r"(leader)
+      : "memory");
+}
+
+// The keys and values of all tiles of a CTA, brought in by kWarps warps that share the rows of every tile, in the order K0,
+// K1 V0, K2 V1, ... of a unit, into kStages places by turns.  full[] counts all their threads, empty[] says that a place has
+// been used.
+template <typename T, int DP, int kStages, int kWarps>
+__device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int tile, int rest, int warp, uint32_t kv_base, uint64_t* full,
+                                            uint64_t* empty, const attn::Waiter& waiter, int* strange) {
+  constexpr int kTileBytes = kTile * DP * 2;
+  constexpr uint32_t kSlab = kTile * 128;
+  constexpr int kMine = kTile / kWarps, kParts = kMine / 32;
+  const int mine = warp * kMine, lane = threadIdx.x & 31;
+  const uint32_t leader = tc::elect_leader();
+  int filled = 0;
+  bool ok = true;
+  struct Pages { int of[kParts]; };    // of rows mine + lane, mine + 32 + lane, ... of a tile
+  auto pages_of = [&](const Unit& x, int tile) {
+    Pages r;
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const int t = tile * kTile + mine + i * 32 + lane;
+      r.of[i] = t < x.length ? p.table[x.b * p.table_stride + t / p.page] : 0;
+    }
+    return r;
+  };
+  auto fetch = [&](bool keys, int tile, const Pages& pages) {
+    const int s = filled % kStages;
+    if (filled >= kStages) ok = waiter.wait(&empty[s], (filled / kStages - 1) & 1);
+    if (!ok) return;
+    ++filled;
+    const uint32_t base = kv_base + s * kTileBytes;
+    const int t0 = tile * kTile + mine;
+    bool good = true;
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) good = good && pages.of[i] >= 0 && pages.of[i] < p.pages;
+    if (p.box > 0 && t0 + kMine <= u.length && __all_sync(0xffffffffu, good)) {
+      // all cached: boxes of p.box rows, of which none reaches into another page
+      if (leader) tc::mbar_arrive_expect_tx(&full[s], kMine * DP * 2);
+      else tc::mbar_arrive(&full[s]);
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        for (int r = 0; r < 32; r += p.box) {
+          const int page = __shfl_sync(0xffffffffu, pages.of[i], r), row = (t0 + i * 32 + r) % p.page;
+#pragma unroll
+          for (int slab = 0; slab < DP / 64; ++slab) {
+            tma_load_page(base + slab * kSlab + uint32_t(mine + i * 32 + r) * 128u, keys ? &p.k_map : &p.v_map, slab * 64, u.head, row, page, &full[s],
+                          leader);
+          }
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const int t = t0 + i * 32 + lane, j = t - u.length;
+      const uint8_t* at = nullptr;
+      if (j < 0) {
+        const int64_t row = (int64_t(pages.of[i]) * p.page + t % p.page) * p.kv_heads + u.head;
+        if (pages.of[i] >= 0 && pages.of[i] < p.pages) at = static_cast<const uint8_t*>(keys ? p.k_pages : p.v_pages) + row * p.dim * 2;
+        else if (keys) at = reinterpret_cast<const uint8_t*>(g_nan_row);
+      } else if (j < p.drafted) {
+        const int64_t* stride = keys ? p.k_stride : p.v_stride;
+        at = static_cast<const uint8_t*>(keys ? p.k : p.v) + 2 * (u.b * stride[0] + j * stride[1] + u.head * stride[2]);
+      }
+      copy_rows<DP>(base, kSlab, mine + i * 32, p.dim, at);
+    }
+    if (!keys && t0 + kMine > u.length) {
+      cp_async_wait_all();
+      if (sift<T, DP>(base, kSlab, mine + max(0, u.length - t0), mine + kMine)) *static_cast<volatile int*>(strange) = 1;
+      tc::mbar_arrive(&full[s]);
+    } else {
+      cp_async_arrive(&full[s]);
+    }
+  };
+  Pages pages = pages_of(u, tile);
+  while (rest > 0 && ok) {
+    const int n = min(rest, u.tiles - tile);
+    Unit next = u;
+    if (rest > n) next_unit(p, next);
+    Pages before = pages;
+    for (int x = 0; x <= n && ok; ++x) {
+      const Pages now = pages;
+      if (x < n) {
+        pages = x + 1 < n ? pages_of(u, tile + x + 1) : pages_of(next, 0);   // looked up a tile ahead
+        fetch(true, tile + x, now);
+      }
+      if (x > 0 && ok) fetch(false, tile + x - 1, before);
+      before = now;
+    }
+    rest -= n;
+    tile = 0;
+    u = next;
+  }
+  cp_async_wait_all();
+  if (!ok) {  // tiled copies under way end before the CTA does
+    for (int back = 1; back <= kStages && back <= filled; ++back) {
+      const int x = filled - back;
+      for (int i = 0; i < 4096 && !tc::mbar_try_wait(&full[x % kStages], (x / kStages) & 1); ++i) {}
+    }
+  }
+}
 
 // RT: tiles of 128 rows that a CTA has, 1 or 2; QR: rows of queries that a tile has in shared memory.  Where that is 32
 // the product reads on behind them: what its other rows are nobody looks at.
@@ -165,19 +374,18 @@ struct TreeConfig {
   // Queries of two units, so that the copies need not wait between two; those of 256 rows of 128 channels leave no room.
   static constexpr int kQueries = RT == 2 ? 1 : 2;
   static constexpr int kStages = DP == 64 ? 8 : QR == 32 ? 6 : 5;
-  static constexpr int kBytes = RT * kQueries * kQueryBytes + kStages * kTileBytes + 2560;
+  static constexpr int kBytes = RT * kQueries * kQueryBytes + kStages * kTileBytes + 768 + 2 * int(sizeof(attn::Exchange));
 };
 
 struct TreeBars {
-  uint64_t s_full[2], p_ready[2], o_full[2], q_empty[2], drained;
+  uint64_t s_full[2], p_ready[2], o_full[2], q_full[2], q_empty[2], drained;
   uint64_t kv_full[8], kv_empty[8];
-  int64_t scan[kThreads / 32], found[2];
+  Share<kThreads / 32> share;
   uint32_t tmem;
   int failed;
   int strange;          // a drafted value was infinite or NaN
-  float2 ml[2][128];    // what the chains of the same rows tell each other
 };
-static_assert(sizeof(TreeBars) <= 2560, "");
+static_assert(sizeof(TreeBars) <= 768, "");
 
 template <typename T, int DP, int RT, int QR>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ TreeParams p) {
@@ -185,82 +393,55 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
   const uint32_t q_base = tc::smem_u32(smem), kv_base = q_base + RT * C::kQueries * C::kQueryBytes;
   TreeBars& bar = *reinterpret_cast<TreeBars*>(smem + RT * C::kQueries * C::kQueryBytes + C::kStages * C::kTileBytes);
+  attn::Exchange* exchange = reinterpret_cast<attn::Exchange*>(smem + RT * C::kQueries * C::kQueryBytes + C::kStages * C::kTileBytes + 768);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (tid == 0) {
     for (int t = 0; t < 2; ++t) {
       tc::mbar_init(&bar.s_full[t], 1);
-      tc::mbar_init(&bar.p_ready[t], 4);
+      tc::mbar_init(&bar.p_ready[t], 8);
       tc::mbar_init(&bar.o_full[t], 1);
     }
-    for (int x = 0; x < C::kQueries; ++x) tc::mbar_init(&bar.q_empty[x], 1);
+    for (int x = 0; x < C::kQueries; ++x) {
+      tc::mbar_init(&bar.q_full[x], 32);
+      tc::mbar_init(&bar.q_empty[x], 1);
+    }
     tc::mbar_init(&bar.drained, 1);
     for (int s = 0; s < C::kStages; ++s) {
-      tc::mbar_init(&bar.kv_full[s], 128);
+      tc::mbar_init(&bar.kv_full[s], 64);
       tc::mbar_init(&bar.kv_empty[s], 1);
     }
     bar.failed = bar.strange = 0;
     tc::fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == 19) {
     tc::tmem_alloc(&bar.tmem, 512);
     tc::tmem_relinquish();
   }
-  // this CTA's part of all tiles
-  int64_t total = 0, before, own = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-    own = b0 + tid < p.batch ? tiles_of(p, b0 + tid) : 0;
-    total += cta_scan<kThreads / 32>(own, &before, bar.scan);
-  }
-  const int64_t ctas = sharing(p, total);
-  const bool idle = blockIdx.x >= ctas;
-  const int64_t begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
-  if (!idle) {
-    int64_t base = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-      int64_t sum = total;
-      if (p.batch > kThreads) {
-        own = b0 + tid < p.batch ? tiles_of(p, b0 + tid) : 0;
-        sum = cta_scan<kThreads / 32>(own, &before, bar.scan);
-      }
-      const int64_t from = base + before;
-      if (own > 0 && begin >= from && begin < from + own) {  // one thread of all
-        bar.found[0] = b0 + tid;
-        bar.found[1] = begin - from;
-      }
-      base += sum;
-      if (begin < base) break;
-    }
-  }
+  Unit u;
+  int tile, rest;   // the first of this CTA's tiles of the unit; how many there are left of all its tiles
+  const bool idle = !part_of_cta<kThreads / 32>(p, bar.share, u, tile, rest);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = bar.tmem;
   if (idle) {
-    if (warp == 12) tc::tmem_dealloc(tmem, 512);
+    if (warp == 19) tc::tmem_dealloc(tmem, 512);
     return;
   }
   const attn::Waiter waiter{&bar.failed};
-  Unit u{int(bar.found[0]), 0, 0, 0, 0, false};
-  read_length(p, u);
-  const int64_t unit0 = bar.found[1] / u.tiles;
-  int tile = int(bar.found[1] - unit0 * u.tiles);     // the first of this CTA's tiles of the unit
-  u.head = int(unit0 / p.row_blocks);
-  u.block = int(unit0 - int64_t(u.head) * p.row_blocks);
-  int rest = int(end - begin);                        // tiles of this CTA that are left
   // tiles of 128 rows that a unit has
   auto row_tiles = [&](const Unit& x) { return RT == 2 && p.rows - x.block * C::kRows > 128 ? 2 : 1; };
 
-  // 512 threads of 128 registers = 256 of 200 + 128 of 64 + 128 of 48
-  if (warp >= 12) {
-    attn::give_registers<48>();
-    if (warp == 12) {
+  if (warp >= 16) {
+    attn::give_registers();
+    if (warp == 19) {
       // ---- products --------------------------------------------------------------------------------------
       const uint32_t leader = tc::elect_leader();
       const uint32_t id_s = tc::idesc(128, 128, Format<T>::code, tc::kMajorK, tc::kMajorK, p.negate);
       const uint32_t id_o = tc::idesc(128, DP, Format<T>::code, tc::kMajorK, tc::kMajorMN);
-      int used = 0, p_used[2] = {0, 0}, queries = 0;   // which of the kQueries
+      int used = 0, p_used[2] = {0, 0}, units = 0, queries = 0;   // which of the kQueries
       bool ok = true;
       auto full = [&](int x) {
         const bool r = waiter.wait(&bar.kv_full[x % C::kStages], (x / C::kStages) & 1);
@@ -281,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         tc::tc_fence_after();
 #pragma unroll
         for (int ks = 0; ks < kTile / 16; ++ks) {
-          attn::mma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, attn::desc_mn(kv_base + (x % C::kStages) * C::kTileBytes, C::kSlab, ks),
+          attn::mma_ts(tmem + 256 + t * 128, tmem + t * 128 + (ks >> 2) * 64 + (ks & 3) * 8, attn::desc_mn(kv_base + (x % C::kStages) * C::kTileBytes, C::kSlab, ks),
                        id_o, !first || ks > 0, leader);
         }
         return true;
@@ -291,6 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         // the order of the copies is that of use: K0, K1 V0, K2 V1, ...
         auto k_of = [&](int j) { return used + max(2 * j - 1, 0); };
         auto v_of = [&](int j) { return used + min(2 * j + 2, 2 * n - 1); };
+        if (!(ok = waiter.wait(&bar.q_full[queries], (units / C::kQueries) & 1))) break;
         if (RT == 1) {
           // chains by turns: S(j + 2) is issued behind O += P(j) V, whose P lies in its place
           for (int j = 0; j < min(n, 2) && ok; ++j) {
@@ -331,6 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           }
         }
         used += 2 * n;
+        ++units;
         if (++queries == C::kQueries) queries = 0;
         rest -= n;
         tile = 0;
@@ -341,134 +524,35 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         for (int i = 0; i < 4096 && !tc::mbar_try_wait(&bar.drained, 0); ++i) {}
       }
       __syncwarp();
+    } else if (warp == 18) {
+      // ---- queries ---------------------------------------------------------------------------------------
+      int units = 0;
+      while (rest > 0) {
+        const int n = min(rest, u.tiles - tile), place = units % C::kQueries;
+        if (units >= C::kQueries && !waiter.wait(&bar.q_empty[place], (units / C::kQueries - 1) & 1)) break;
+        ++units;
+        for (int x = 0; x < RT * QR; x += 32) {
+          const int r = u.block * C::kRows + x + lane;
+          const int i = r / p.group, g = r - i * p.group;
+          const T* at = static_cast<const T*>(p.q) + u.b * p.q_stride[0] + i * p.q_stride[1] + int64_t(u.head * p.group + g) * p.q_stride[2];
+          copy_rows<DP>(q_base + (RT == 2 ? (x / QR) * C::kQueryBytes : place * C::kQueryBytes), C::kQuerySlab, x % QR, p.dim, r < p.rows ? at : nullptr);
+        }
+        cp_async_arrive(&bar.q_full[place]);
+        rest -= n;
+        tile = 0;
+        if (rest > 0) next_unit(p, u);
+      }
+      cp_async_wait_all();
+    } else {
+      bring_tiles<T, DP, C::kStages, 2>(p, u, tile, rest, warp - 16, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange);
     }
-  } else if (warp >= 8) {
-    // ---- copies: a warp has 32 rows of every tile, half a warp (128 channels) or a quarter copies a row at a time -----
-    attn::give_registers<64>();
-    constexpr int kPieces = DP / 8, kAtOnce = 32 / kPieces;
-    const int mine = (warp - 8) * 32, piece = lane % kPieces, sub = lane / kPieces;
-    const bool piece_there = piece * 8 < p.dim;
-    const uint64_t anything = reinterpret_cast<uintptr_t>(g_nan_row);   // an address for copies of nothing
-    int filled = 0, units = 0;
-    bool ok = true;
-    // a row of 16-byte pieces, lines of 128 bytes permuted by the row
-    auto to = [&](uint32_t base, uint32_t slab, int row) {
-      return base + uint32_t(piece >> 3) * slab + uint32_t(row) * 128u + ((uint32_t(piece ^ row) & 7u) << 4);
-    };
-    // copies this warp's rows of a tile; `at` is where row `mine + lane` is, null for zeros
-    auto copy = [&](uint32_t base, uint32_t slab, const void* at) {
-      const uint32_t lo = uint32_t(reinterpret_cast<uintptr_t>(at)), hi = uint32_t(reinterpret_cast<uintptr_t>(at) >> 32);
-#pragma unroll
-      for (int i = 0; i < 32; i += 8 * kAtOnce) {
-        uint64_t row[8];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int r = i + x * kAtOnce + sub;
-          row[x] = (uint64_t(__shfl_sync(0xffffffffu, hi, r)) << 32) | __shfl_sync(0xffffffffu, lo, r);
-        }
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const bool there = piece_there && row[x] != 0;
-          cp_async16(to(base, slab, mine + i + x * kAtOnce + sub), reinterpret_cast<const uint8_t*>(there ? row[x] : anything) + piece * 16, there);
-        }
-      }
-    };
-    // An infinite or NaN value of a drafted token (this warp's rows from `first` on) must reach the rows that see it and no
-    // others, but in the product it would meet every row (0 * NaN): it leaves the tile, and is added to those rows at the end.
-    auto sift = [&](uint32_t base, int first) {
-      for (int i = 0; i < 32; i += kAtOnce) {
-        if (i + sub < first) continue;
-        const uint32_t at = to(base, C::kSlab, mine + i + sub);
-        uint32_t w[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-        bool any = false;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if ((w[j] & Format<T>::exponent) == Format<T>::exponent) { w[j] &= 0xffff0000u; any = true; }
-          if (((w[j] >> 16) & Format<T>::exponent) == Format<T>::exponent) { w[j] &= 0xffffu; any = true; }
-        }
-        if (any) {
-          asm volatile("st.shared.v4.b32 [%4], {%0, %1, %2, %3};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(at) : "memory");
-          *static_cast<volatile int*>(&bar.strange) = 1;
-        }
-      }
-    };
-    auto page_of = [&](const Unit& x, int tile) {   // the page of row mine + lane, looked up a tile ahead
-      const int t = tile * kTile + mine + lane;
-      return t < x.length ? p.table[x.b * p.table_stride + t / p.page] : 0;
-    };
-    // the stage of the next copy, when its tile has been used
-    auto stage = [&]() {
-      const int s = filled % C::kStages;
-      if (filled >= C::kStages) ok = waiter.wait(&bar.kv_empty[s], (filled / C::kStages - 1) & 1);
-      ++filled;
-      return s;
-    };
-    int page = page_of(u, tile);
-    while (rest > 0 && ok) {
-      const int n = min(rest, u.tiles - tile);
-      Unit next = u;
-      if (rest > n) next_unit(p, next);
-      // the queries come with the first keys
-      const int place = units % C::kQueries;
-      if (units >= C::kQueries && !(ok = waiter.wait(&bar.q_empty[place], (units / C::kQueries - 1) & 1))) break;
-      ++units;
-      for (int x = 0; x < RT; ++x) {
-        if (mine >= QR) break;
-        const int r = u.block * C::kRows + x * 128 + mine + lane;
-        const int i = r / p.group, g = r - i * p.group;
-        const T* at = static_cast<const T*>(p.q) + u.b * p.q_stride[0] + i * p.q_stride[1] + int64_t(u.head * p.group + g) * p.q_stride[2];
-        copy(q_base + (RT == 2 ? x : place) * C::kQueryBytes, C::kQuerySlab, r < p.rows ? at : nullptr);
-      }
-      const uint8_t* v_at = nullptr;
-      int first = 32;     // of this warp's rows of values, the first drafted one
-      for (int x = 0; x <= n && ok; ++x) {
-        const uint8_t *k_now = nullptr, *v_now = nullptr;
-        int first_now = 32;
-        if (x < n) {
-          const int t = (tile + x) * kTile + mine + lane, j = t - u.length;
-          if (j < 0) {
-            const int64_t row = (int64_t(page) * p.page + t % p.page) * p.kv_heads + u.head;
-            const bool there = page >= 0 && page < p.pages;
-            k_now = there ? static_cast<const uint8_t*>(p.k_pages) + row * p.dim * 2 : reinterpret_cast<const uint8_t*>(g_nan_row);
-            v_now = there ? static_cast<const uint8_t*>(p.v_pages) + row * p.dim * 2 : nullptr;
-          } else if (j < p.drafted) {
-            k_now = static_cast<const uint8_t*>(p.k) + 2 * (u.b * p.k_stride[0] + j * p.k_stride[1] + u.head * p.k_stride[2]);
-            v_now = static_cast<const uint8_t*>(p.v) + 2 * (u.b * p.v_stride[0] + j * p.v_stride[1] + u.head * p.v_stride[2]);
-          }
-          first_now = u.length - (tile + x) * kTile - mine;
-          page = x + 1 < n ? page_of(u, tile + x + 1) : page_of(next, 0);
-          const int s = stage();
-          if (!ok) break;
-          copy(kv_base + s * C::kTileBytes, C::kSlab, k_now);
-          cp_async_arrive(&bar.kv_full[s]);
-        }
-        if (x > 0) {
-          const int s = stage();
-          if (!ok) break;
-          copy(kv_base + s * C::kTileBytes, C::kSlab, v_at);
-          if (first < 32) {
-            cp_async_wait_all();
-            sift(kv_base + s * C::kTileBytes, first);
-            tc::mbar_arrive(&bar.kv_full[s]);
-          } else {
-            cp_async_arrive(&bar.kv_full[s]);
-          }
-        }
-        v_at = v_now;
-        first = first_now;
-      }
-      rest -= n;
-      tile = 0;
-      u = next;
-    }
-    cp_async_wait_all();
   } else {
-    // ---- weights: a row a thread ---------------------------------------------------------------------------
-    attn::take_registers<200>();
-    const int t = warp >> 2, row = tid & 127;
+    // ---- weights: two threads a row ------------------------------------------------------------------------
+    attn::take_registers();
+    const int t = warp >> 3, half = (warp >> 2) & 1, row = tid & 127;
     const uint32_t lane_base = uint32_t(warp & 3) << 21;   // 32 lanes of TMEM, in bits 16 and up
-    const uint32_t s_at = tmem + lane_base + t * 128, o_at = tmem + lane_base + 256 + t * 128;
+    const uint32_t s_at = tmem + lane_base + t * 128 + half * 64, o_at = tmem + lane_base + 256 + t * 128 + half * (DP / 2);
+    attn::Half h{t, half, row, 0, exchange + t};
     int seen = 0, outs = 0;
     bool ok = true, split = false;   // the unit began in another CTA
     split = tile != 0;
@@ -478,6 +562,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       const int token = r / p.group;
       const bool there = r < p.rows, any_there = r - lane < p.rows;
       const bool takes_part = RT == 1 || t < chains;
+      // warps without a row have nothing to do but to keep count
+      h.threads = 64 * min(4, (p.rows - u.block * C::kRows - (RT == 2 ? t * 128 : 0) + 31) / 32);
       float m = -INFINITY;
       float2 sum2[2] = {{0.f, 0.f}, {0.f, 0.f}};
       int mine = 0;
@@ -486,13 +572,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         ++seen;
         tc::tc_fence_after();
         if (any_there) {
-          const int first_token = (tile + j) * kTile;
-          attn::soften<T, DP>(s_at, o_at, p.scale_log2, mine == 0, m, sum2, [&](uint32_t (&s)[4][32]) {
-            if (first_token + kTile <= u.length) return;
+          const int first_token = (tile + j) * kTile + half * 64;
+          attn::soften<T, DP>(h, s_at, o_at, p.scale_log2, mine == 0, m, sum2, [&](uint32_t (&s)[2][32]) {
+            if (first_token + 64 <= u.length) return;
             // drafted tokens, or the end
             const uint8_t* mask = p.mask == nullptr || !there ? nullptr : p.mask + u.b * p.mask_stride + int64_t(token) * p.drafted;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
+            for (int x = 0; x < 2; ++x) {
               uint32_t sees = 0;
 #pragma unroll 8
               for (int y = 0; y < 32; ++y) {
@@ -519,23 +605,26 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       }
       tc::tc_fence_after();
       float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-      // the columns of this thread: all, or where both chains have its row a half of the sum of both
-      constexpr int kCols = RT == 1 ? DP / 2 : DP;
-      const int col0 = RT == 1 ? t * kCols : 0;
+      if (any_there) sum += h.other(sum);
+      // the columns of this thread: half of its row's, or where both chains have the row a quarter of the sum of both
+      constexpr int kCols = RT == 1 ? DP / 4 : DP / 2;
+      const int col0 = RT == 1 ? (2 * t + half) * kCols : half * kCols;
       float f[2] = {1.f, 1.f};
       bool has[2] = {true, true};
       if (RT == 1) {
-        bar.ml[t][row] = make_float2(mine > 0 ? m : -INFINITY, mine > 0 ? sum : 0.f);
+        sync_chains();   // what the chains told within themselves has been read
+        exchange[t].x[half][row] = half == 0 ? m : sum;
         tc::tc_fence_before();
         sync_chains();
         tc::tc_fence_after();
-        const float2 a = bar.ml[0][row], b = bar.ml[1][row];
-        m = fmaxf(a.x, b.x);
+        const float m0 = exchange[0].x[0][row], m1 = exchange[1].x[0][row];
+        const float l0 = exchange[0].x[1][row], l1 = exchange[1].x[1][row];
+        m = fmaxf(m0, m1);
         has[1] = n > 1;
-        f[0] = m == -INFINITY ? 0.f : exp2_approx((a.x - m) * p.scale_log2);
-        f[1] = m == -INFINITY ? 0.f : exp2_approx((b.x - m) * p.scale_log2);
-        sum = a.y * f[0] + b.y * f[1];
-        if (isnan(a.y) || isnan(b.y)) sum = NAN;
+        f[0] = m == -INFINITY ? 0.f : exp2_approx((m0 - m) * p.scale_log2);
+        f[1] = m == -INFINITY ? 0.f : exp2_approx((m1 - m) * p.scale_log2);
+        sum = l0 * f[0] + l1 * f[1];
+        if (isnan(l0) || isnan(l1)) sum = NAN;
       }
       const bool whole = !split && tile + n == u.tiles;
       // nothing seen: the sum is 0 and so is the output
@@ -547,21 +636,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         const int g = r - token * p.group;
         T* to = static_cast<T*>(p.out) + (int64_t(u.b) * p.drafted + token) * p.heads * p.dim + int64_t(u.head * p.group + g) * p.dim;
 #pragma unroll 1
-        for (int x = col0; x < col0 + kCols; x += 32) {
-          uint32_t raw[32];
-          float o[32];
-          tc::tmem_ld32(tmem + lane_base + 256 + (RT == 1 ? 0 : t * 128) + x, raw);
+        for (int x = col0; x < col0 + kCols; x += 16) {
+          uint32_t raw[16];
+          float o[16];
+          tc::tmem_ld16(tmem + lane_base + 256 + (RT == 1 ? 0 : t * 128) + x, raw);
           tc::tmem_wait_ld();
 #pragma unroll
-          for (int y = 0; y < 32; ++y) o[y] = __uint_as_float(raw[y]);
+          for (int y = 0; y < 16; ++y) o[y] = __uint_as_float(raw[y]);
           if (RT == 1) {
 #pragma unroll
-            for (int y = 0; y < 32; ++y) o[y] *= f[0];
+            for (int y = 0; y < 16; ++y) o[y] *= f[0];
             if (has[1]) {
-              tc::tmem_ld32(tmem + lane_base + 256 + 128 + x, raw);
+              tc::tmem_ld16(tmem + lane_base + 256 + 128 + x, raw);
               tc::tmem_wait_ld();
 #pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] = fmaf(__uint_as_float(raw[y]), f[1], o[y]);
+              for (int y = 0; y < 16; ++y) o[y] = fmaf(__uint_as_float(raw[y]), f[1], o[y]);
             }
           }
           if (!there) continue;
@@ -570,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
               if (!(p.mask == nullptr ? d <= token : p.mask[u.b * p.mask_stride + int64_t(token) * p.drafted + d] != 0)) continue;
               const T* v = static_cast<const T*>(p.v) + u.b * p.v_stride[0] + d * p.v_stride[1] + u.head * p.v_stride[2];
 #pragma unroll
-              for (int y = 0; y < 32; ++y) {
+              for (int y = 0; y < 16; ++y) {
                 const float value = x + y < p.dim ? to_float(v[x + y]) : 0.f;
                 if (!isfinite(value)) o[y] += value;
               }
@@ -578,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           }
           if (whole) {
 #pragma unroll
-            for (int y = 0; y < 32; y += 8) {
+            for (int y = 0; y < 16; y += 8) {
               if (x + y < p.dim) {
                 uint4 w;
                 w.x = pack_pair<T>(o[y] * inv, o[y + 1] * inv);
@@ -590,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             }
           } else {
 #pragma unroll
-            for (int y = 0; y < 32; y += 4) *reinterpret_cast<float4*>(part + x + y) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+            for (int y = 0; y < 16; y += 4) *reinterpret_cast<float4*>(part + x + y) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
           }
         }
         if (!whole && there && col0 == 0) {
@@ -599,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         }
       }
       tc::tc_fence_before();
-      if (RT == 1) sync_chains();   // the other chain has read this one's O
+      if (RT == 1) sync_chains();   // the other chain has read this one's O, m and l
       rest -= n;
       tile = 0;
       split = false;
@@ -608,9 +697,271 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 19) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- few rows ------------------------------------------------------------------------------------------
+// Up to 16 rows (plain decoding, small trees of small groups): mma.sync m16n8k16, whose sums are in registers.  Eight warps
+// have 16 tokens of every tile each and go through them on their own; what they have of a unit is joined at its end.
+constexpr int kFewThreads = 384;   // warps 0-7: 16 tokens of every tile each; 8-11: copies
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int DP>
+struct FewConfig {
+  static constexpr int kTileBytes = kTile * DP * 2;
+  static constexpr uint32_t kSlab = kTile * 128;
+  static constexpr int kStages = DP == 128 ? 6 : 10;
+  static constexpr int kJoinBytes = 4 * 16 * DP * 4;   // what four warps leave for four others
+  static constexpr int kBytes = kStages * kTileBytes + kJoinBytes + 2048;
+};
+struct FewBars {
+  uint64_t kv_full[10], kv_empty[10];
+  Share<kFewThreads / 32> share;
+  int failed, strange;
+  float m[8][16], l[8][16];
+};
+static_assert(sizeof(FewBars) <= 2048, "");
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_constant__ TreeParams p) {
+  using C = FewConfig<DP>;
+  constexpr int kKSteps = DP / 16, kDB = DP / 8;
+  extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
+  const uint32_t kv_base = tc::smem_u32(smem);
+  float* join = reinterpret_cast<float*>(smem + C::kStages * C::kTileBytes);
+  FewBars& bar = *reinterpret_cast<FewBars*>(smem + C::kStages * C::kTileBytes + C::kJoinBytes);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int quad = lane >> 2, in_quad = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      tc::mbar_init(&bar.kv_full[s], 128);
+      tc::mbar_init(&bar.kv_empty[s], 8);
+    }
+    bar.failed = bar.strange = 0;
+    tc::fence_mbar_init();
+  }
+  Unit u;
+  int tile, rest;
+  if (!part_of_cta<kFewThreads / 32>(p, bar.share, u, tile, rest)) return;
+  const attn::Waiter waiter{&bar.failed};
+  if (warp >= 8) {
+    bring_tiles<T, DP, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange);
+    return;
+  }
+
+  uint32_t qf[kKSteps][4];
+  int token_of[2];
+  auto queries = [&](const Unit& x) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = quad + 8 * half;
+      const bool there = r < p.rows;
+      const int n = there ? r / p.group : 0, g = there ? r - n * p.group : 0;
+      token_of[half] = there ? n : -1;
+      const T* row = static_cast<const T*>(p.q) + x.b * p.q_stride[0] + n * p.q_stride[1] + int64_t(x.head * p.group + g) * p.q_stride[2];
+#pragma unroll
+      for (int s = 0; s < kKSteps; ++s) {
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh) {
+          const int col = s * 16 + kh * 8 + in_quad * 2;
+          qf[s][kh * 2 + half] = there && col < p.dim ? *reinterpret_cast<const uint32_t*>(row + col) : 0u;
+        }
+      }
+    }
+  };
+  queries(u);
+  const float by = p.negate ? -p.scale_log2 : p.scale_log2;
+  // where this lane's part of an ldmatrix begins: rows of this warp's 16 tokens
+  const int k_row = warp * 16 + (lane & 7) + ((lane >> 4) << 3), v_row = warp * 16 + (lane & 15);
+  int used = 0;
+  bool ok = true, split = tile != 0;   // the unit began in another CTA
+  while (rest > 0) {
+    const int n = min(rest, u.tiles - tile);
+    float o[kDB][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < kDB; ++d) { o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f; }
+    for (int j = 0; j < n && ok; ++j) {
+      const int xk = used + max(2 * j - 1, 0), xv = used + min(2 * j + 2, 2 * n - 1);
+      if (!(ok = waiter.wait(&bar.kv_full[xk % C::kStages], (xk / C::kStages) & 1))) break;
+      const uint32_t k_tile = kv_base + (xk % C::kStages) * C::kTileBytes, v_tile = kv_base + (xv % C::kStages) * C::kTileBytes;
+      // S = Q K^T: two blocks of 8 tokens, two sums each
+      float s2[2][2][4];
+#pragma unroll
+      for (int x = 0; x < 16; ++x) s2[x >> 3][(x >> 2) & 1][x & 3] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < kKSteps; ++ks) {
+        uint32_t kf[4];  // tokens 0..7 and 8..15, channels ks*16 + 0..7 and 8..15
+        ldmatrix4(kf, place_of<DP>(k_tile, C::kSlab, k_row, ks * 2 + ((lane >> 3) & 1)));
+        mma16816<T>(s2[ks & 1][0], qf[ks], kf[0], kf[1]);
+        mma16816<T>(s2[ks & 1][1], qf[ks], kf[2], kf[3]);
+      }
+      __syncwarp();
+      tc::mbar_arrive(&bar.kv_empty[xk % C::kStages], lane == 0);
+      const int first_token = (tile + j) * kTile + warp * 16;
+      float s[2][4];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) s[x >> 2][x & 3] = (s2[0][x >> 2][x & 3] + s2[1][x >> 2][x & 3]) * by;
+      if (first_token + 16 > u.length) {   // drafted tokens, or the end
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int d = first_token + (x >> 2) * 8 + in_quad * 2 + (x & 1) - u.length, token = token_of[(x >> 1) & 1];
+          bool see = d < 0;
+          if (!see && d < p.drafted && token >= 0) {
+            see = p.mask == nullptr ? d <= token : p.mask[u.b * p.mask_stride + int64_t(token) * p.drafted + d] != 0;
+          }
+          if (!see) s[x >> 2][x & 3] = -INFINITY;
+        }
+      }
+      // running maximum and sum of the two rows of this thread's quad
+      uint32_t pa[4];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float top = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float now = fmaxf(m[half], top);
+        const float base = now == -INFINITY ? 0.f : now;   // nothing seen yet: every weight is exp(-inf) = 0
+        const float keep = exp2_approx(m[half] - base);
+        float w[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) w[x] = exp2_approx(s[x >> 1][2 * half + (x & 1)] - base);
+        l[half] = l[half] * keep + ((w[0] + w[1]) + (w[2] + w[3]));   // (of this thread's columns; the quad's are added at the end)
+        pa[half] = pack_pair<T>(w[0], w[1]);       // weights at most 1, rounded to the values' type for the product
+        pa[2 + half] = pack_pair<T>(w[2], w[3]);
+        if (__any_sync(0xffffffffu, now != m[half])) {
+#pragma unroll
+          for (int d = 0; d < kDB; ++d) { o[d][2 * half] *= keep; o[d][2 * half + 1] *= keep; }
+        }
+        m[half] = now;
+      }
+      // O += P V
+      if (!(ok = waiter.wait(&bar.kv_full[xv % C::kStages], (xv / C::kStages) & 1))) break;
+#pragma unroll
+      for (int d = 0; d < kDB; d += 2) {
+        uint32_t vf[4];  // channels d*8.. (tokens 0..7, 8..15), channels (d+1)*8.. (the same)
+        ldmatrix4_trans(vf, place_of<DP>(v_tile, C::kSlab, v_row, d + (lane >> 4)));
+        mma16816<T>(o[d], pa, vf[0], vf[1]);
+        mma16816<T>(o[d + 1], pa, vf[2], vf[3]);
+      }
+      __syncwarp();
+      tc::mbar_arrive(&bar.kv_empty[xv % C::kStages], lane == 0);
+    }
+    used += 2 * n;
+    Unit next = u;
+    if (rest > n) {
+      next_unit(p, next);
+      queries(next);   // on their way while the warps join
+    }
+
+    // the eight warps' sums
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+      if (in_quad == 0) bar.m[warp][quad + 8 * half] = m[half];
+    }
+    auto sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    sync();
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = quad + 8 * half;
+      float top = bar.m[0][r];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) top = fmaxf(top, bar.m[w][r]);
+      const float f = top == -INFINITY ? 0.f : exp2_approx(m[half] - top);
+      m[half] = top;
+#pragma unroll
+      for (int d = 0; d < kDB; ++d) { o[d][2 * half] *= f; o[d][2 * half + 1] *= f; }
+      if (in_quad == 0) bar.l[warp][r] = isnan(l[half]) ? l[half] : l[half] * f;
+    }
+#pragma unroll
+    for (int with = 4; with > 0; with >>= 1) {
+      float2* at = reinterpret_cast<float2*>(join + (warp & (with - 1)) * 16 * DP);
+      if (warp >= with && warp < 2 * with) {
+#pragma unroll
+        for (int x = 0; x < 2 * kDB; ++x) at[x * 32 + lane] = make_float2(o[x >> 1][2 * (x & 1)], o[x >> 1][2 * (x & 1) + 1]);
+      }
+      sync();
+      if (warp < with) {
+#pragma unroll
+        for (int x = 0; x < 2 * kDB; ++x) {
+          const float2 y = at[x * 32 + lane];
+          o[x >> 1][2 * (x & 1)] += y.x;
+          o[x >> 1][2 * (x & 1) + 1] += y.y;
+        }
+      }
+      if (with > 1) sync();
+    }
+    if (warp == 0) {
+      const bool whole = !split && tile + n == u.tiles, strange = *static_cast<volatile int*>(&bar.strange) != 0;
+      const int64_t slot = int64_t(blockIdx.x) * 2 + (split ? 0 : 1);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int r = quad + 8 * half;
+        if (r >= p.rows) continue;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) sum += bar.l[w][r];
+        // nothing seen: the sum is 0 and so is the output
+        const float inv = !ok || u.bad ? NAN : !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+        const int i = r / p.group, g = r - i * p.group;
+        if (strange) {
+          for (int d = max(0, tile * kTile - u.length); d < min(p.drafted, (tile + n) * kTile - u.length); ++d) {
+            if (!(p.mask == nullptr ? d <= i : p.mask[u.b * p.mask_stride + int64_t(i) * p.drafted + d] != 0)) continue;
+            const T* v = static_cast<const T*>(p.v) + u.b * p.v_stride[0] + d * p.v_stride[1] + u.head * p.v_stride[2];
+#pragma unroll
+            for (int x = 0; x < 2 * kDB; ++x) {
+              const int col = (x >> 1) * 8 + in_quad * 2 + (x & 1);
+              const float value = col < p.dim ? to_float(v[col]) : 0.f;
+              if (!isfinite(value)) o[x >> 1][2 * half + (x & 1)] += value;
+            }
+          }
+        }
+        T* to = static_cast<T*>(p.out) + (int64_t(u.b) * p.drafted + i) * p.heads * p.dim + int64_t(u.head * p.group + g) * p.dim;
+        float* part = p.partials + (slot * 16 + r) * DP;
+#pragma unroll
+        for (int d = 0; d < kDB; ++d) {
+          const int col = d * 8 + in_quad * 2;
+          const float2 y = make_float2(o[d][2 * half], o[d][2 * half + 1]);
+          if (!whole) *reinterpret_cast<float2*>(part + col) = y;
+          else if (col < p.dim) *reinterpret_cast<uint32_t*>(to + col) = pack_pair<T>(y.x * inv, y.y * inv);
+        }
+        if (!whole && in_quad == 0) {
+          *reinterpret_cast<float2*>(p.partials + int64_t(p.ctas) * 2 * 16 * DP + (slot * 16 + r) * 2) = make_float2(m[half], inv * sum);
+        }
+      }
+    }
+    sync();   // what the warps told each other has been read
+    rest -= n;
+    tile = 0;
+    split = false;
+    u = next;
   }
 }
 
@@ -665,8 +1016,29 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
   for (int y = 0; y < kOwn; y += 2) *reinterpret_cast<uint32_t*>(to + y) = pack_pair<T>(acc[y] * inv, acc[y + 1] * inv);
 }
 
+constexpr int kFewRows = 16;
 // rows of a block
-int block_rows(int64_t rows) { return rows <= 128 ? 128 : 256; }
+int block_rows(int64_t rows) { return rows <= kFewRows ? kFewRows : rows <= 128 ? 128 : 256; }
+
+// the CTAs of tree_join_kernel for a unit
+int joining_ctas(const TreeParams& p, int rows) { return (std::min(p.rows, rows) + kJoinThreads / 32 - 1) / (kJoinThreads / 32); }
+
+template <typename T, int DP>
+int launch_join(const TreeParams& p, int rows, cudaStream_t stream) {
+  const int per_unit = joining_ctas(p, rows);
+  return launch_beside(&tree_join_kernel<T, DP>, unsigned(p.batch * p.kv_heads * p.row_blocks * per_unit), kJoinThreads, 0, stream, p,
+                       rows, per_unit);
+}
+
+template <typename T, int DP>
+int launch_few(const TreeParams& p, cudaStream_t stream) {
+  constexpr int kBytes = FewConfig<DP>::kBytes;
+  const cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(&tree_few_kernel<T, DP>), kBytes);
+  if (err != cudaSuccess) { record_cuda_error(err); return GDN2_ERR_LAUNCH; }
+  tree_few_kernel<T, DP><<<unsigned(p.ctas), kFewThreads, kBytes, stream>>>(p);
+  const int status = check_launch();
+  return status != GDN2_OK ? status : launch_join<T, DP>(p, kFewRows, stream);
+}
 
 template <typename T, int DP, int RT, int QR>
 int launch_tree_typed(const TreeParams& p, cudaStream_t stream) {
@@ -674,17 +1046,14 @@ int launch_tree_typed(const TreeParams& p, cudaStream_t stream) {
   const void* kernel = reinterpret_cast<const void*>(&tree_kernel<T, DP, RT, QR>);
   const cudaError_t err = ensure_dynamic_smem(kernel, C::kBytes);
   if (err != cudaSuccess) { record_cuda_error(err); return GDN2_ERR_LAUNCH; }
-  const int per_unit = (std::min(p.rows, C::kRows) + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
-  const int64_t joining = int64_t(p.batch) * p.kv_heads * p.row_blocks * per_unit;
-  if (joining > int64_t(0x7fffffff)) return GDN2_ERR_TOO_LARGE;
   tree_kernel<T, DP, RT, QR><<<unsigned(p.ctas), kThreads, C::kBytes, stream>>>(p);
   const int status = check_launch();
-  if (status != GDN2_OK) return status;
-  return launch_beside(&tree_join_kernel<T, DP>, unsigned(joining), kJoinThreads, 0, stream, p, C::kRows, per_unit);
+  return status != GDN2_OK ? status : launch_join<T, DP>(p, C::kRows, stream);
 }
 
 template <typename T>
 int launch_tree_dim(const TreeParams& p, cudaStream_t stream) {
+  if (p.rows <= kFewRows) return p.dim <= 64 ? launch_few<T, 64>(p, stream) : launch_few<T, 128>(p, stream);
   if (p.dim <= 64) {
     return p.rows <= 128 ? launch_tree_typed<T, 64, 1, 128>(p, stream) : launch_tree_typed<T, 64, 2, 128>(p, stream);
   }
@@ -739,11 +1108,21 @@ int launch_tree(const void* q, const void* k, const void* v, const void* k_pages
   p.batch = batch; p.drafted = drafted; p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads;
   p.dim = dim; p.page = page; p.columns = columns;
   p.rows = drafted * p.group;
+  // Whole boxes of tiled copies come out of a page only where it has 8 or 16 rows, or a multiple of 32; pages of other
+  // sizes, and tiles that a sequence ends in, are copied row by row.
+  p.box = page % 32 == 0 ? 32 : page == 16 || page == 8 ? page : 0;
+  if (p.box > 0) {
+    const int64_t page_strides[3] = {int64_t(page) * kv_heads * dim, int64_t(kv_heads) * dim, dim};
+    if (!attn::encode_heads_map(&p.k_map, k_pages, page_strides, pages, page, kv_heads, dim, dtype, p.box) ||
+        !attn::encode_heads_map(&p.v_map, v_pages, page_strides, pages, page, kv_heads, dim, dtype, p.box)) {
+      return GDN2_ERR_LAUNCH;
+    }
+  }
   const int per_block = block_rows(p.rows);
   p.row_blocks = (p.rows + per_block - 1) / per_block;
   const int status = tree_ctas(&p.ctas);
   if (status != GDN2_OK) return status;
-  if (int64_t(batch) * kv_heads * p.row_blocks > int64_t(0x7fffffff)) return GDN2_ERR_TOO_LARGE;
+  if (int64_t(batch) * kv_heads * p.row_blocks > int64_t(0x7fffffff) / joining_ctas(p, per_block)) return GDN2_ERR_TOO_LARGE;
   // the sign goes to the product, and a scale of 0 stays a positive number, so that -inf * scale masks as ever
   p.negate = scale < 0.f;
   p.scale_log2 = fmaxf(fabsf(scale) * attn::kLog2e, 1e-30f);
