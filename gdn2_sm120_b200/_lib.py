@@ -125,6 +125,7 @@ class _PythonWay:
     """Stands in for the native host path and takes no call: the Python wrappers do the same on the same kernels."""
 
     forward = train_forward = train_backward = prologue_forward = prologue_backward = staticmethod(lambda *_: None)
+    rotary = append_tokens = tree_attention = attention_forward = attention_backward = staticmethod(lambda *_: None)
 
 
 _host_module = None

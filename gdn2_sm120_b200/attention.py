@@ -17,7 +17,9 @@ from . import _lib, _validate
 from .varlen import _bounds
 
 
-def _check(q, k, v):
+def _check(q, k, v, bounds, scale):
+    """Bounds and scale as the library takes them, if everything is as it should be."""
+
     if not isinstance(q, torch.Tensor):
         raise TypeError("q must be a torch.Tensor")
     for name, x in (("q", q), ("k", k), ("v", v)):
@@ -29,6 +31,9 @@ def _check(q, k, v):
     if q.shape[2] % k.shape[2]:
         raise ValueError("the number of query heads must be a multiple of that of key heads")
     _lib.require_b200(q.device)
+    if bounds is not None:
+        bounds = _bounds(bounds, q.shape[1])
+    return bounds, _validate.float32_scale(scale, q.shape[3])
 
 
 def _sequences(q, bounds):
@@ -68,7 +73,11 @@ def _forward(q, k, v, bounds, scale, training):
 class _CausalAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bounds, scale):
-        out, statistics = _forward(*(_validate.detached(x) for x in (q, k, v)), bounds, scale, True)
+        done = _native(q, k, v, bounds, scale, True)
+        if done is None:
+            bounds, scale = _check(q, k, v, bounds, scale)
+            done = _forward(*(_validate.detached(x) for x in (q, k, v)), bounds, scale, True)
+        out, statistics = done
         ctx.save_for_backward(q, k, v, out, statistics)
         ctx.bounds, ctx.scale = bounds, scale
         return out
@@ -77,6 +86,11 @@ class _CausalAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
         q, k, v, out, statistics = ctx.saved_tensors
+        if statistics is not None and _lib.KERNEL_EVENTS is None:
+            done = _lib.host().attention_backward(q, k, v, out, statistics, d_out, ctx.bounds, ctx.scale)
+            if done is not None:
+                return (*done, None, None)
+        scale = _validate.float32_scale(ctx.scale, q.shape[3])
         q, k, v = (_validate.detached(x) for x in (q, k, v))
         grads = tuple(torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
         if statistics is None:
@@ -89,16 +103,27 @@ class _CausalAttention(torch.autograd.Function):
         scratch = torch.empty_like(statistics)
         _lib.call("gdn2_attention_backward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                   d_out.data_ptr(), statistics.data_ptr(), scratch.data_ptr(), *(x.data_ptr() for x in grads), strides,
-                  host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], _lib.dtype_code(q.dtype), ctx.scale,
+                  host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], _lib.dtype_code(q.dtype), scale,
                   _lib.stream_ptr(q.device), kernels=3 * _launches(ctx.bounds))
         return (*grads, None, None)
 
 
+def _native(q, k, v, bounds, scale, training):
+    """The call on the native host path, ``(output, statistics)``; None where it is not the plain case."""
+
+    if _lib.KERNEL_EVENTS is not None or not getattr(q, "is_cuda", False):
+        return None
+    return _lib.host().attention_forward(q, k, v, bounds, scale, training)
+
+
 def _attention(q, k, v, bounds, scale):
-    scale = _validate.float32_scale(scale, q.shape[3])
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v)):
         return _CausalAttention.apply(q, k, v, bounds, scale)
-    return _forward(*(_validate.detached(x) for x in (q, k, v)), bounds, scale, False)[0]
+    done = _native(q, k, v, bounds, scale, False)
+    if done is None:
+        bounds, scale = _check(q, k, v, bounds, scale)
+        done = _forward(*(_validate.detached(x) for x in (q, k, v)), bounds, scale, False)
+    return done[0]
 
 
 def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None) -> torch.Tensor:
@@ -108,7 +133,6 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale
     of ``Hkv``; views are fine where their rows of channels are 16-byte aligned.  ``scale`` defaults to ``D ** -0.5``.
     Returns a contiguous tensor like ``q``; differentiable in ``q``, ``k`` and ``v``."""
 
-    _check(q, k, v)
     return _attention(q, k, v, None, scale)
 
 
@@ -127,9 +151,9 @@ def causal_attention_varlen(
 
     if not isinstance(q, torch.Tensor) or q.ndim != 4 or q.shape[0] != 1:
         raise ValueError("packed sequence tensors must have shape [1, total, H, D]")
-    bounds = _bounds(cu_seqlens, q.shape[1])
-    _check(q, k, v)
-    return _attention(q, k, v, bounds, scale)
+    if not isinstance(cu_seqlens, tuple):
+        cu_seqlens = _bounds(cu_seqlens, q.shape[1])
+    return _attention(q, k, v, cu_seqlens, scale)
 
 
 __all__ = ["causal_attention", "causal_attention_varlen"]

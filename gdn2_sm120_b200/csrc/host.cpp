@@ -16,6 +16,8 @@
 
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
+#include <vector>
 
 #include "../../include/gdn2_b200.h"
 
@@ -37,6 +39,13 @@ struct Api {
   decltype(&gdn2_chunk_scratch_bytes) chunk_scratch_bytes;
   decltype(&gdn2_gate_prologue) gate_prologue;
   decltype(&gdn2_gate_prologue_vjp) gate_prologue_vjp;
+  decltype(&gdn2_rotary) rotary;
+  decltype(&gdn2_append_tokens) append_tokens;
+  decltype(&gdn2_tree_workspace_bytes) tree_workspace_bytes;
+  decltype(&gdn2_tree_attention) tree_attention;
+  decltype(&gdn2_attention_stat_rows) attention_stat_rows;
+  decltype(&gdn2_attention_forward) attention_forward;
+  decltype(&gdn2_attention_backward) attention_backward;
 } api;
 PyObject* g_check = nullptr;     // _lib.check(status, name): raises
 PyObject* g_launches = nullptr;  // _lib.LAUNCHES
@@ -521,6 +530,326 @@ PyObject* prologue_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_CATCH
 }
 
+// ---- attention layers ------------------------------------------------------------------------------------
+// a strided CUDA tensor of `dims` dimensions whose innermost one is contiguous
+const at::Tensor* strided(PyObject* o, int64_t dims) {
+  const at::Tensor* t = tensor(o);
+  if (t == nullptr || !t->defined() || t->dim() != dims || !t->is_cuda() || t->layout() != at::kStrided || t->is_neg() ||
+      t->is_conj() || (dims > 0 && t->size(dims - 1) > 1 && t->stride(dims - 1) != 1)) {
+    return nullptr;
+  }
+  return t;
+}
+
+// the same on q's device, contiguous and of one type
+const at::Tensor* dense(PyObject* o, int64_t dims, at::ScalarType type, const at::Tensor& like) {
+  const at::Tensor* t = strided(o, dims);
+  return t != nullptr && t->scalar_type() == type && t->device() == like.device() && t->is_contiguous() ? t : nullptr;
+}
+
+bool wants_grad(std::initializer_list<const at::Tensor*> tensors) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : tensors) {
+    if (t->requires_grad()) return true;
+  }
+  return false;
+}
+
+// batch, token and head stride of a [B, T, H, D] tensor; a dimension of size 1 gets that of a contiguous one
+void head_strides(const at::Tensor& t, int64_t* to) {
+  const int64_t dense[3] = {t.size(1) * t.size(2) * t.size(3), t.size(2) * t.size(3), t.size(3)};
+  for (int i = 0; i < 3; ++i) to[i] = t.size(i) <= 1 ? dense[i] : t.stride(i);
+}
+
+// q, k, v of attention: types, sizes, rows that are 16-byte aligned and have places of their own
+struct Heads {
+  const at::Tensor* t[3];
+  int64_t batch, time, heads, kv_heads, dim;
+  int dtype;
+  int64_t strides[12];
+};
+
+bool aligned_rows(const at::Tensor& t, int64_t* strides) {
+  for (int i = 0; i < 3; ++i) {
+    if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) % 8 != 0)) return false;
+  }
+  head_strides(t, strides);
+  return aligned(t);
+}
+
+bool read_heads(PyObject* const* a, Heads* h) {
+  for (int i = 0; i < 3; ++i) {
+    h->t[i] = strided(a[i], 4);
+    if (h->t[i] == nullptr) return false;
+  }
+  const at::Tensor &q = *h->t[0], &k = *h->t[1], &v = *h->t[2];
+  h->dtype = dtype_code(q.scalar_type());
+  if (h->dtype != GDN2_BF16 && h->dtype != GDN2_FP16) return false;
+  if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() || k.device() != q.device() ||
+      v.device() != q.device() || k.sizes() != v.sizes()) {
+    return false;
+  }
+  h->batch = q.size(0); h->time = q.size(1); h->heads = q.size(2); h->dim = q.size(3); h->kv_heads = k.size(2);
+  if (k.size(0) != h->batch || k.size(1) != h->time || k.size(3) != h->dim) return false;
+  if (h->batch <= 0 || h->time <= 0 || h->heads <= 0 || h->kv_heads <= 0 || h->heads % h->kv_heads != 0) return false;
+  if (h->dim <= 0 || h->dim > GDN2_ATTENTION_MAX_DIM || h->dim % 8 != 0) return false;
+  for (int i = 0; i < 3; ++i) {
+    if (!aligned_rows(*h->t[i], h->strides + 3 * i)) return false;
+  }
+  return b200(q.device().index());
+}
+
+bool read_attention_scale(PyObject* o, int64_t dim, float* scale) {
+  double value = 1.0 / std::sqrt(double(dim));
+  if (o != Py_None) {
+    if (!PyFloat_Check(o)) return false;
+    value = PyFloat_AS_DOUBLE(o);
+  }
+  *scale = static_cast<float>(value);
+  return std::isfinite(value) && std::isfinite(*scale);
+}
+
+// None, or a tuple of cumulative lengths of packed sequences (other forms are the wrapper's)
+bool read_bounds(PyObject* o, const Heads& h, std::vector<int64_t>* bounds) {
+  if (o == Py_None) return true;
+  if (!PyTuple_Check(o) || h.batch != 1) return false;
+  const Py_ssize_t n = PyTuple_GET_SIZE(o);
+  if (n < 2) return false;
+  bounds->resize(size_t(n));
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* x = PyTuple_GET_ITEM(o, i);
+    int overflow = 1;
+    if (!PyLong_Check(x)) return false;
+    (*bounds)[size_t(i)] = PyLong_AsLongLongAndOverflow(x, &overflow);
+    if (overflow != 0 || (i > 0 && (*bounds)[size_t(i)] < (*bounds)[size_t(i - 1)])) return false;
+  }
+  return bounds->front() == 0 && bounds->back() == h.time;
+}
+
+// launches of a pass: one, or one for every GDN2_PACKED_MAX_SEQUENCES packed sequences of which any has a token
+long passes(const std::vector<int64_t>& bounds) {
+  if (bounds.empty()) return 1;
+  long count = 0;
+  const size_t n = bounds.size() - 1, most = GDN2_PACKED_MAX_SEQUENCES;
+  for (size_t i = 0; i < n; i += most) count += bounds[i] < bounds[i + most < n ? i + most : n];
+  return count;
+}
+
+// rotary(q, k, cos, sin, positions, interleaved, inverse) -> (q, k) or None
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  GDN2_TRY
+  if (!g_bound || n != 7) return none();
+  const at::Tensor *q = strided(a[0], 4), *k = strided(a[1], 4);
+  if (q == nullptr || k == nullptr || q->scalar_type() != k->scalar_type() || q->device() != k->device()) return none();
+  const int dtype = dtype_code(q->scalar_type());
+  const int64_t batch = q->size(0), time = q->size(1), dim = q->size(3);
+  if (dtype < 0 || batch <= 0 || time <= 0 || q->size(2) <= 0 || k->size(2) <= 0 || dim <= 0 || dim > 512 || dim % 2 != 0 ||
+      k->size(0) != batch || k->size(1) != time || k->size(3) != dim || wants_grad({q, k}) || !b200(q->device().index())) {
+    return none();
+  }
+  const at::Tensor *cos = dense(a[2], 2, at::kFloat, *q), *sin = dense(a[3], 2, at::kFloat, *q), *positions = nullptr;
+  if (cos == nullptr || sin == nullptr || cos->sizes() != sin->sizes() || cos->size(0) <= 0 || cos->size(1) <= 0 ||
+      2 * cos->size(1) > dim) {
+    return none();
+  }
+  int64_t position_stride = 0;
+  if (a[4] == Py_None) {
+    if (time > cos->size(0)) return none();
+  } else {
+    positions = dense(a[4], 2, at::kLong, *q);
+    if (positions == nullptr || positions->size(0) != batch || positions->size(1) != time) return none();
+    position_stride = time;
+  }
+  at::Tensor q_out, k_out;
+  int status;
+  WithoutGil others;
+  const c10::cuda::CUDAGuard guard(q->device());
+  q_out = at::empty(q->sizes(), q->options());
+  k_out = at::empty(k->sizes(), k->options());
+  int64_t strides[12];
+  const at::Tensor* all[4] = {q, k, &q_out, &k_out};
+  for (int i = 0; i < 4; ++i) head_strides(*all[i], strides + 3 * i);
+  status = api.rotary(q->data_ptr(), k->data_ptr(), q_out.data_ptr(), k_out.data_ptr(), fptr(cos), fptr(sin),
+                      positions == nullptr ? nullptr : static_cast<const int64_t*>(positions->data_ptr()), strides, position_stride,
+                      batch, time, q->size(2), k->size(2), dim, cos->size(1), cos->size(0), a[5] == Py_True, a[6] == Py_True, dtype,
+                      at::cuda::getCurrentCUDAStream().stream());
+  others.end();
+  if (!ok(status, "gdn2_rotary", 1)) return nullptr;
+  PyObject* result = PyTuple_New(2);
+  PyTuple_SET_ITEM(result, 0, wrap(q_out));
+  PyTuple_SET_ITEM(result, 1, wrap(k_out));
+  return result;
+  GDN2_CATCH
+}
+
+struct Extent {
+  uintptr_t lo, hi;
+  explicit Extent(const at::Tensor& t) : lo(reinterpret_cast<uintptr_t>(t.data_ptr())), hi(lo) {
+    if (t.numel() == 0) return;
+    int64_t last = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    hi = lo + uintptr_t(last) * t.element_size();
+  }
+  bool meets(const Extent& o) const { return lo < o.hi && o.lo < hi; }
+};
+
+// k_pages and v_pages as the cache of kv heads of one type; null pages or other layouts are the wrapper's
+bool read_pages(PyObject* const* a, const at::Tensor& like, int64_t kv_heads, int64_t dim, const at::Tensor** pages) {
+  for (int i = 0; i < 2; ++i) {
+    pages[i] = dense(a[i], 4, like.scalar_type(), like);
+    if (pages[i] == nullptr || pages[i]->numel() == 0 || pages[i]->size(2) != kv_heads || pages[i]->size(3) != dim) return false;
+  }
+  return pages[0]->sizes() == pages[1]->sizes();
+}
+
+// append_tokens(k, v, k_pages, v_pages, slots) -> True or None
+PyObject* append_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  GDN2_TRY
+  if (!g_bound || n != 5) return none();
+  const at::Tensor *k = strided(a[0], 3), *v = strided(a[1], 3);
+  if (k == nullptr || v == nullptr || k->sizes() != v->sizes() || k->numel() == 0 || k->scalar_type() != v->scalar_type() ||
+      k->device() != v->device() || dtype_code(k->scalar_type()) < 0 || !b200(k->device().index())) {
+    return none();
+  }
+  const at::Tensor *pages[2], *slots = dense(a[4], 1, at::kLong, *k);
+  if (slots == nullptr || slots->size(0) != k->size(0) || !read_pages(a + 2, *k, k->size(1), k->size(2), pages)) return none();
+  const Extent to[2] = {Extent(*pages[0]), Extent(*pages[1])};
+  if (to[0].meets(to[1])) return none();
+  for (const at::Tensor* x : {k, v, slots}) {
+    if (Extent(*x).meets(to[0]) || Extent(*x).meets(to[1])) return none();
+  }
+  int status;
+  WithoutGil others;
+  const c10::cuda::CUDAGuard guard(k->device());
+  const int64_t strides[4] = {k->stride(0), k->stride(1), v->stride(0), v->stride(1)};
+  status = api.append_tokens(k->data_ptr(), v->data_ptr(), pages[0]->data_ptr(), pages[1]->data_ptr(),
+                             static_cast<const int64_t*>(slots->data_ptr()), strides, k->size(0), pages[0]->size(0), pages[0]->size(1),
+                             k->size(1), k->size(2), dtype_code(k->scalar_type()), at::cuda::getCurrentCUDAStream().stream());
+  others.end();
+  if (!ok(status, "gdn2_append_tokens", 1)) return nullptr;
+  Py_RETURN_TRUE;
+  GDN2_CATCH
+}
+
+// tree_attention(q, k, v, k_pages, v_pages, page_table, lengths, mask, scale) -> output or None
+PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  GDN2_TRY
+  Heads h;
+  float scale;
+  if (!g_bound || n != 9 || !read_heads(a, &h) || !read_attention_scale(a[8], h.dim, &scale) ||
+      wants_grad({h.t[0], h.t[1], h.t[2]})) {
+    return none();
+  }
+  const at::Tensor &q = *h.t[0], *pages[2], *mask = nullptr;
+  const at::Tensor *table = strided(a[5], 2), *lengths = dense(a[6], 1, at::kInt, q);
+  if (!read_pages(a + 3, q, h.kv_heads, h.dim, pages) || !aligned(*pages[0]) || !aligned(*pages[1])) return none();
+  if (table == nullptr || table->scalar_type() != at::kInt || table->device() != q.device() || table->size(0) != h.batch ||
+      table->size(1) <= 0 || lengths == nullptr || lengths->size(0) != h.batch) {
+    return none();
+  }
+  if (a[7] != Py_None) {
+    const at::Tensor* t = tensor(a[7]);
+    mask = t == nullptr ? nullptr : dense(a[7], t->dim() == 2 ? 2 : 3, at::kBool, q);
+    if (mask == nullptr || mask->size(-1) != h.time || mask->size(-2) != h.time || (mask->dim() == 3 && mask->size(0) != h.batch)) {
+      return none();
+    }
+  }
+  at::Tensor out;
+  int status;
+  WithoutGil others;
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int64_t size = api.tree_workspace_bytes(h.time, h.heads, h.kv_heads, h.dim);
+  if (size <= 0) {
+    others.end();
+    return none();
+  }
+  out = at::empty(q.sizes(), q.options());
+  const at::Tensor workspace = bytes(size, q);
+  status = api.tree_attention(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), pages[0]->data_ptr(), pages[1]->data_ptr(),
+                              static_cast<const int*>(table->data_ptr()), static_cast<const int*>(lengths->data_ptr()),
+                              mask == nullptr ? nullptr : mask->data_ptr(), out.data_ptr(), workspace.data_ptr(), h.strides,
+                              h.batch > 1 ? table->stride(0) : table->size(1),
+                              mask == nullptr || mask->dim() == 2 ? 0 : h.time * h.time, h.batch, h.time, h.heads, h.kv_heads, h.dim,
+                              pages[0]->size(0), pages[0]->size(1), table->size(1), h.dtype, scale,
+                              at::cuda::getCurrentCUDAStream().stream());
+  others.end();
+  if (!ok(status, "gdn2_tree_attention", 2)) return nullptr;
+  return wrap(out);
+  GDN2_CATCH
+}
+
+// attention_forward(q, k, v, bounds, scale, training) -> (output, statistics or None) or None
+PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  GDN2_TRY
+  Heads h;
+  float scale;
+  std::vector<int64_t> bounds;
+  if (!g_bound || n != 6 || !read_heads(a, &h) || !read_bounds(a[3], h, &bounds) || !read_attention_scale(a[4], h.dim, &scale) ||
+      wants_grad({h.t[0], h.t[1], h.t[2]})) {
+    return none();
+  }
+  const bool training = a[5] == Py_True;
+  const at::Tensor& q = *h.t[0];
+  const int64_t* host = bounds.empty() ? nullptr : bounds.data();
+  const int64_t n_seq = bounds.empty() ? h.batch : int64_t(bounds.size()) - 1;
+  at::Tensor out, statistics;
+  int status;
+  int64_t rows = 0;
+  WithoutGil others;
+  const c10::cuda::CUDAGuard guard(q.device());
+  if (training && (rows = api.attention_stat_rows(host, n_seq, h.time)) < 0) {
+    others.end();
+    return none();
+  }
+  out = at::empty(q.sizes(), q.options());
+  if (training) statistics = floats({h.heads, rows}, q);
+  status = api.attention_forward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out.data_ptr(),
+                                 training ? fptr(&statistics) : nullptr, h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim,
+                                 h.dtype, scale, at::cuda::getCurrentCUDAStream().stream());
+  others.end();
+  if (!ok(status, "gdn2_attention_forward", passes(bounds))) return nullptr;
+  PyObject* result = PyTuple_New(2);
+  PyTuple_SET_ITEM(result, 0, wrap(out));
+  PyTuple_SET_ITEM(result, 1, training ? wrap(statistics) : Py_NewRef(Py_None));
+  return result;
+  GDN2_CATCH
+}
+
+// attention_backward(q, k, v, output, statistics, d_output, bounds, scale) -> (dq, dk, dv) or None
+PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  GDN2_TRY
+  Heads h;
+  float scale;
+  std::vector<int64_t> bounds;
+  if (!g_bound || n != 8 || !read_heads(a, &h) || !read_bounds(a[6], h, &bounds) || !read_attention_scale(a[7], h.dim, &scale)) {
+    return none();
+  }
+  const at::Tensor& q = *h.t[0];
+  const at::Tensor *out = dense(a[3], 4, q.scalar_type(), q), *statistics = dense(a[4], 2, at::kFloat, q), *d_out = strided(a[5], 4);
+  if (out == nullptr || statistics == nullptr || d_out == nullptr || out->sizes() != q.sizes() || d_out->sizes() != q.sizes() ||
+      d_out->scalar_type() != q.scalar_type() || d_out->device() != q.device() || !aligned_rows(*d_out, h.strides + 9)) {
+    return none();
+  }
+  const int64_t* host = bounds.empty() ? nullptr : bounds.data();
+  const int64_t n_seq = bounds.empty() ? h.batch : int64_t(bounds.size()) - 1;
+  at::Tensor grads[3];
+  int status;
+  WithoutGil others;
+  const c10::cuda::CUDAGuard guard(q.device());
+  for (int i = 0; i < 3; ++i) grads[i] = at::empty(h.t[i]->sizes(), q.options());
+  const at::Tensor scratch = at::empty(statistics->sizes(), statistics->options());
+  status = api.attention_backward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out->data_ptr(), d_out->data_ptr(),
+                                  fptr(statistics), fptr(&scratch), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(),
+                                  h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim, h.dtype, scale,
+                                  at::cuda::getCurrentCUDAStream().stream());
+  others.end();
+  if (!ok(status, "gdn2_attention_backward", 3 * passes(bounds))) return nullptr;
+  PyObject* result = PyTuple_New(3);
+  for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(result, i, wrap(grads[i]));
+  return result;
+  GDN2_CATCH
+}
+
 // bind({entry point: address}, _lib.check, _lib.LAUNCHES, torch.cuda.OutOfMemoryError)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 4 || !PyDict_Check(a[0]) || !PyList_Check(a[2])) {
@@ -549,6 +878,13 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_BIND(chunk_scratch_bytes);
   GDN2_BIND(gate_prologue);
   GDN2_BIND(gate_prologue_vjp);
+  GDN2_BIND(rotary);
+  GDN2_BIND(append_tokens);
+  GDN2_BIND(tree_workspace_bytes);
+  GDN2_BIND(tree_attention);
+  GDN2_BIND(attention_stat_rows);
+  GDN2_BIND(attention_forward);
+  GDN2_BIND(attention_backward);
 #undef GDN2_BIND
   if (missing) {
     PyErr_SetString(PyExc_RuntimeError, "libgdn2_b200.so lacks an entry point");
@@ -568,6 +904,11 @@ PyMethodDef methods[] = {
     {"train_backward", reinterpret_cast<PyCFunction>(train_backward), METH_FASTCALL, nullptr},
     {"prologue_forward", reinterpret_cast<PyCFunction>(prologue_forward), METH_FASTCALL, nullptr},
     {"prologue_backward", reinterpret_cast<PyCFunction>(prologue_backward), METH_FASTCALL, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(rotary), METH_FASTCALL, nullptr},
+    {"append_tokens", reinterpret_cast<PyCFunction>(append_tokens), METH_FASTCALL, nullptr},
+    {"tree_attention", reinterpret_cast<PyCFunction>(tree_attention), METH_FASTCALL, nullptr},
+    {"attention_forward", reinterpret_cast<PyCFunction>(attention_forward), METH_FASTCALL, nullptr},
+    {"attention_backward", reinterpret_cast<PyCFunction>(attention_backward), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native host path of gdn2_sm120_b200.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

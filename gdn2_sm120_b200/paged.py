@@ -52,6 +52,9 @@ def append_tokens(
     token's place, ``page number * page + place in the page``.  A slot that is negative or behind the cache leaves the
     token out.  Two tokens with one slot are not allowed (which of them stays is undefined).  fp16, bf16 or fp32."""
 
+    if _lib.KERNEL_EVENTS is None and getattr(k, "is_cuda", False):
+        if _lib.host().append_tokens(k, v, k_pages, v_pages, slots):
+            return k_pages, v_pages
     if not all(isinstance(x, torch.Tensor) for x in (k, v, slots)):
         raise TypeError("k, v, and slots must be torch.Tensor objects")
     if k.ndim not in (3, 4) or k.shape != v.shape:
@@ -105,6 +108,10 @@ def tree_attention(
     stay on the device: no call waits for it, and a captured graph may be replayed with other contents.  A page number
     outside the cache or a length beyond ``columns`` pages makes the sequence's output NaN.  Inference only."""
 
+    if _lib.KERNEL_EVENTS is None and getattr(q, "is_cuda", False):
+        done = _lib.host().tree_attention(q, k, v, k_pages, v_pages, page_table, lengths, mask, scale)
+        if done is not None:
+            return done
     if not isinstance(q, torch.Tensor):
         raise TypeError("q must be a torch.Tensor")
     for name, x in (("q", q), ("k", k), ("v", v)):

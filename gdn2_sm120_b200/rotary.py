@@ -117,6 +117,15 @@ def _check(q, k, cos, sin, positions, layout):
         if positions.shape not in (q.shape[:2], q.shape[1:2]):
             raise ValueError("positions must have shape [B, T] or [T]")
     _lib.require_b200(q.device)
+    return None if positions is None else positions.to(torch.int64).contiguous()
+
+
+def _native(q, k, cos, sin, positions, layout, inverse):
+    """The call on the native host path; None where it is not the plain case."""
+
+    if _lib.KERNEL_EVENTS is not None or layout not in _LAYOUTS or not getattr(q, "is_cuda", False):
+        return None
+    return _lib.host().rotary(q, k, cos, sin, positions, layout == "interleaved", inverse)
 
 
 def _launch(q, k, q_out, k_out, cos, sin, positions, layout, inverse):
@@ -138,16 +147,22 @@ def _contiguous_like(x):
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, cos, sin, positions, layout):
-        q_out, k_out = _contiguous_like(q), _contiguous_like(k)
-        _launch(q.detach(), k.detach(), q_out, k_out, cos, sin, positions, layout, False)
+        done = _native(q, k, cos, sin, positions, layout, False)
+        if done is None:
+            positions = _check(q, k, cos, sin, positions, layout)
+            done = _contiguous_like(q), _contiguous_like(k)
+            _launch(q.detach(), k.detach(), *done, cos, sin, positions, layout, False)
         ctx.save_for_backward(cos, sin, positions)
         ctx.layout = layout
-        return q_out, k_out
+        return done
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         cos, sin, positions = ctx.saved_tensors
+        done = _native(dq, dk, cos, sin, positions, ctx.layout, True)
+        if done is not None:
+            return (*done, None, None, None, None)
         dq, dk = (x if x.stride(3) == 1 else x.contiguous() for x in (dq, dk))
         q_out, k_out = _contiguous_like(dq), _contiguous_like(dk)
         _launch(dq, dk, q_out, k_out, cos, sin, positions, ctx.layout, True)
@@ -172,13 +187,16 @@ def apply_rotary(
     continued sequences give theirs.  A position outside the tables makes the token's rotated channels NaN.
     Differentiable in ``q`` and ``k``; ``inplace=True`` turns the tensors themselves (no gradient) and returns them."""
 
-    _check(q, k, cos, sin, positions, layout)
-    if positions is not None:
-        positions = positions.to(torch.int64).contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
-        if inplace:
-            raise ValueError("inplace=True has no gradient")
-        return _Rotary.apply(q, k, cos.detach(), sin.detach(), positions, layout)
+    wants_grad = torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k))
+    if not inplace:
+        if wants_grad:
+            return _Rotary.apply(q, k, cos, sin, positions, layout)
+        done = _native(q, k, cos, sin, positions, layout, False)
+        if done is not None:
+            return done
+    positions = _check(q, k, cos, sin, positions, layout)
+    if wants_grad:
+        raise ValueError("inplace=True has no gradient")
     given = q, k
     q, k = q.detach(), k.detach()
     if inplace:
