@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
   const Waiter waiter{&bar.failed};
 
   if (warp >= 16) {
-    give_registers();
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");   // 640 threads of 96 registers = 512 of 104 + 128 of 64
     if (warp == 17) {
       // ---- copies ----------------------------------------------------------------------------------------
       const uint32_t leader = tc::elect_leader();
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
     }
   } else {
     // ---- weights: two threads a row ------------------------------------------------------------------------
-    take_registers();
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     const int b = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & 127;   // two threads a row, 32 columns each
     const uint32_t lane_base = uint32_t(warp & 3) << 21;   // 32 lanes of TMEM, in bits 16 and up
     const uint32_t s_at = tmem + lane_base + 256 + b * 128 + half * 32, dp_at = s_at + 64;

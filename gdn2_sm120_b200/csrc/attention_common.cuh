@@ -87,11 +87,6 @@ struct Waiter {
   }
 };
 
-// Registers move from the warps that copy and issue to those that compute; the sum stays what the CTA was launched with:
-// 640 threads of 96 = 512 of 104 + 128 of 64.
-__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 104;"); }
-__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
-
 // ---- 16-bit products ---------------------------------------------------------------------------------------
 // Tiles of [rows][64] channels in lines of 128 bytes whose 16-byte pieces are permuted by the line (the 128-byte
 // swizzle of the tiled copies); a tile of 128 channels is two of them.  One copy serves both ways of reading it:
@@ -131,90 +126,86 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// One tile of 128 x 128 scores becomes weights.  Two threads have a row, 64 columns each (of chain `id`, 256 threads), so
-// that eight warps and not four hide the latencies of one chain: 3900 clocks a tile with four (1950 with two chains).
-// S is read from TMEM, masked, and P = exp2(S c - m c) in 16 bits lies over the first half of its own 64 columns.  m is the
-// row's reference so far and `sum` this thread's part of its weights; both and O (as it is after all tiles before this one)
-// follow a maximum that has grown by more than 2^kRescale: weights stay below that and sums in 32 bits lose nothing.  Only
-// then, and at the first tile, do the two threads have to tell each other their maxima.
-constexpr float kRescale = 8.f;
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
+// One tile of scores becomes weights, a row a thread: S (128 columns of TMEM at s_at) is read, masked, and overlaid by
+// P = exp2(S c - m c) in 16 bits.  m is the row's reference, a maximum of some tile so far (-inf: nothing but -inf has been
+// seen), `sum` the sum of its weights.  No tile but the first looks for its maximum: where the sum of its weights stays below
+// kGrowth, so does each of them, and nothing overflows or loses digits in 32 bits or in either 16-bit type.  Otherwise m
+// becomes the maximum, sum and O (DP columns at o_at, as it is after all tiles before this one) are scaled down, and the
+// tile's weights are made again.
+constexpr float kGrowth = 32768.f;
+
+// mask(x, s): columns 32 x .. 32 x + 31 in s
+template <typename Mask>
+__device__ __forceinline__ float row_maximum(uint32_t s_at, Mask mask) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    uint32_t s[32];
+    tc::tmem_ld32(s_at + x * 32, s);
+    tc::tmem_wait_ld();
+    mask(x, s);
+    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int y = 0; y < 32; ++y) tops[y & 3] = fmaxf(tops[y & 3], __uint_as_float(s[y]));
+    top = fmaxf(top, fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+  }
+  return top;
 }
-// what the two threads of a row tell each other
-struct Exchange { float x[2][128]; };
 
-struct Half {
-  int id, half, row;       // chain, columns, row
-  int threads;             // of the chain that have rows: all of some warps
-  Exchange* exchange;
-  __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory"); }
-  // the other thread's value
-  __device__ __forceinline__ float other(float mine) const {
-    exchange->x[half][row] = mine;
-    sync();
-    const float r = exchange->x[half ^ 1][row];
-    sync();
-    return r;
-  }
-  __device__ __forceinline__ bool any(bool x) const {   // of the chain
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %3, 0;\n\tbar.red.or.pred p, %1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(r) : "r"(id + 1), "r"(threads), "r"(uint32_t(x)) : "memory");
-    return r != 0;
-  }
-};
-
-template <typename T, int DP, typename Mask>
-__device__ __forceinline__ void soften(const Half& h, uint32_t s_at, uint32_t o_at, float c, bool first, float& m, float2 (&sum)[2],
-                                       Mask mask) {
-  uint32_t s[2][32];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) tc::tmem_ld32(s_at + x * 32, s[x]);
-  tc::tmem_wait_ld();
-  mask(s);
-  float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int x = 0; x < 64; x += 2) {
-    tops[(x >> 1) & 3] = max3(tops[(x >> 1) & 3], __uint_as_float(s[x >> 5][x & 31]), __uint_as_float(s[x >> 5][(x & 31) + 1]));
-  }
-  float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
-  if (first) {
-    m = fmaxf(top, h.other(top));
-  } else if (h.any((top - m) * c > kRescale)) {
-    top = fmaxf(top, h.other(top));
-    const bool grown = (top - m) * c > kRescale;
-    if (__any_sync(0xffffffffu, grown)) {
-      const float f = grown ? exp2_approx((m - top) * c) : 1.f;
-      if (grown) m = top;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) sum[x] = mul2(sum[x], twice(f));
-#pragma unroll
-      for (int x = 0; x < DP / 2; x += 16) {
-        uint32_t o[16];
-        tc::tmem_ld16(o_at + x, o);
-        tc::tmem_wait_ld();
-#pragma unroll
-        for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-        tc::tmem_st16(o_at + x, o);
-      }
-    }
-  }
-  // a row that has seen nothing but -inf so far has weights 0
+template <typename T, typename Mask>
+__device__ __forceinline__ float row_weights(uint32_t s_at, float c, float m, uint32_t (&w)[2][32], Mask mask) {
   const float2 minus = twice(m == -INFINITY ? 0.f : -m * c), by = twice(c);
+  float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+  uint32_t s[2][32];
+  tc::tmem_ld32(s_at, s[0]);
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    uint32_t w[16];
+  for (int x = 0; x < 4; ++x) {
+    tc::tmem_wait_ld();
+    if (x < 3) tc::tmem_ld32(s_at + (x + 1) * 32, s[(x + 1) & 1]);
+    mask(x, s[x & 1]);
 #pragma unroll
     for (int y = 0; y < 16; ++y) {
-      const float2 e = exp2_2(fma2(make_float2(__uint_as_float(s[x][2 * y]), __uint_as_float(s[x][2 * y + 1])), by, minus));
+      const float2 z = fma2(make_float2(__uint_as_float(s[x & 1][2 * y]), __uint_as_float(s[x & 1][2 * y + 1])), by, minus);
+      const float2 e = exp2_2(z);
       sum[y & 1] = add2(sum[y & 1], e);
-      w[y] = pack_pair<T>(e.x, e.y);   // the sum has them as they were, the product rounded to the values' type
+      w[x >> 1][(x & 1) * 16 + y] = pack_pair<T>(e.x, e.y);   // the sum has them as they were, the product rounded
     }
-    tc::tmem_st16(s_at + x * 16, w);
   }
+  return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+}
+
+template <typename T, int DP, typename Mask>
+__device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, float& m, float& sum, Mask mask) {
+  uint32_t w[2][32];
+  float more;
+  bool grown = m == -INFINITY;
+#pragma unroll 1
+  for (bool look = __any_sync(0xffffffffu, grown);;) {
+    if (look) {
+      const float top = fmaxf(m, row_maximum(s_at, mask));
+      const float f = grown && m != -INFINITY ? exp2_approx((m - top) * c) : 1.f;
+      if (grown) m = top;
+      if (__any_sync(0xffffffffu, f != 1.f)) {
+        sum *= f;
+#pragma unroll
+        for (int x = 0; x < DP; x += 16) {
+          uint32_t o[16];
+          tc::tmem_ld16(o_at + x, o);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+          tc::tmem_st16(o_at + x, o);
+        }
+      }
+    }
+    more = row_weights<T>(s_at, c, m, w, mask);
+    grown = more > kGrowth;
+    look = __any_sync(0xffffffffu, grown);
+    if (!look) break;
+  }
+  sum += more;
+  tc::tmem_st32(s_at, w[0]);
+  tc::tmem_st32(s_at + 32, w[1]);
   tc::tmem_wait_st();
 }
 

@@ -19,14 +19,14 @@ namespace attn {
 
 namespace {
 
-constexpr int kThreads = 640;    // warps 0-7, 8-15: the rows of the two tiles; 16: products; 17: copies
+constexpr int kThreads = 384;    // warps 0-3, 4-7: the rows of the two tiles; 8: products; 9: copies; 10, 11: look at values
 
 template <int DP>
 struct FwdConfig {
   static constexpr int kTileBytes = 128 * DP * 2;
   static constexpr int kSlab = 128 * 128;               // 64 channels of 128 rows
   static constexpr int kStages = DP == 128 ? 5 : 8;
-  static constexpr int kBytes = (2 + kStages) * kTileBytes + 512 + 2 * int(sizeof(Exchange));
+  static constexpr int kBytes = (2 + kStages) * kTileBytes + 512;
 };
 
 struct FwdParams {
@@ -56,8 +56,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
   uint8_t* q_tiles = smem;
   uint8_t* kv_tiles = smem + 2 * C::kTileBytes;
   FwdBars& bar = *reinterpret_cast<FwdBars*>(smem + (2 + C::kStages) * C::kTileBytes);
-  Exchange* exchange = reinterpret_cast<Exchange*>(smem + (2 + C::kStages) * C::kTileBytes + 512);
-  static_assert(sizeof(FwdBars) <= 512, "");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -65,7 +63,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       tc::mbar_init(&bar.q_full[t], 1);
       tc::mbar_init(&bar.q_empty[t], 1);
       tc::mbar_init(&bar.s_full[t], 1);
-      tc::mbar_init(&bar.p_ready[t], 8);
+      tc::mbar_init(&bar.p_ready[t], 4);
       tc::mbar_init(&bar.o_full[t], 1);
     }
     tc::mbar_init(&bar.raw, 1);
@@ -77,7 +75,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
     bar.failed = 0;
     tc::fence_mbar_init();
   }
-  if (warp == 16) {
+  if (warp == 8) {
     tc::tmem_alloc(&bar.tmem, 512);
     tc::tmem_relinquish();
   }
@@ -98,10 +96,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
     return tile * 128 < it.len ? tile + 1 : 0;
   };
 
-  // 640 threads of 96 registers = 512 of 104 + 128 of 64
-  if (warp >= 16) {
-    give_registers();
-    if (warp == 17) {
+  if (warp >= 8) {
+    if (warp == 9) {
       // ---- copies ------------------------------------------------------------------------------------------
       const uint32_t leader = tc::elect_leader();
       int filled = 0, loaded[2] = {0, 0}, mended = 0;
@@ -177,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
           for (int i = 0; loaded[t] > 0 && i < 4096 && !tc::mbar_try_wait(&bar.q_full[t], (loaded[t] - 1) & 1); ++i) {}
         }
       }
-    } else if (warp == 16) {
+    } else if (warp == 8) {
       // ---- products ----------------------------------------------------------------------------------------
       const uint32_t leader = tc::elect_leader();
       const uint32_t id_s = tc::idesc(128, 128, Format<T>::code, tc::kMajorK, tc::kMajorK, p.negate);
@@ -225,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
               tc::tc_fence_after();
   #pragma unroll
               for (int ks = 0; ks < 8; ++ks) {
-                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + (ks >> 2) * 64 + (ks & 3) * 8, desc_mn(v_tile, C::kSlab, ks), id_o, j > 0 || ks > 0, leader);
+                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, desc_mn(v_tile, C::kSlab, ks), id_o, j > 0 || ks > 0, leader);
               }
               if (j + 1 == n_t[t]) tc::mma_commit(&bar.o_full[t], leader);
             }
@@ -247,12 +243,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       __syncwarp();
     }
   } else {
-    // ---- weights: two threads a row ------------------------------------------------------------------------
-    take_registers();
-    const int t = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & 127;
+    // ---- weights: a row a thread ---------------------------------------------------------------------------
+    const int t = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lane_base = uint32_t(warp & 3) << 21;   // 32 lanes of TMEM, in bits 16 and up
-    const uint32_t s_at = tmem + lane_base + t * 128 + half * 64, o_at = tmem + lane_base + 256 + t * 128 + half * (DP / 2);
-    const Half h{t, half, row, 256, exchange + t};
+    const uint32_t s_at = tmem + lane_base + t * 128, o_at = tmem + lane_base + 256 + t * 128;
     const float c = p.scale_log2;
     int seen = 0, outs = 0;
     bool ok = true;
@@ -263,20 +257,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       const Item it = item_at(index, &head);
       const int n = key_tiles(it, t);
       if (n == 0) {
-        if (p.lse != nullptr && half == 0) p.lse[head * p.seq.stat_rows + it.stat + (2 * it.tile + t) * 128 + row] = INFINITY;
+        if (p.lse != nullptr) p.lse[head * p.seq.stat_rows + it.stat + (2 * it.tile + t) * 128 + row] = INFINITY;
         continue;
       }
       float m = -INFINITY;
-      float2 sum2[2] = {{0.f, 0.f}, {0.f, 0.f}};
+      float sum = 0.f;
       for (int j = 0; j < n && ok; ++j) {
         if (!(ok = waiter.wait(&bar.s_full[t], seen & 1))) break;
         ++seen;
         tc::tc_fence_after();
-        soften<T, DP>(h, s_at, o_at, c, j == 0, m, sum2, [&](uint32_t (&s)[2][32]) {
+        soften<T, DP>(s_at, o_at, c, m, sum, [&](int x, uint32_t (&s)[32]) {
           if (j + 1 == n) {   // the tile on the diagonal; what lies behind the sequence's end lies behind every row
 #pragma unroll
-            for (int x = 0; x < 64; ++x) {
-              if (x > row - half * 64) s[x >> 5][x & 31] = 0xff800000u;
+            for (int y = 0; y < 32; ++y) {
+              if (x * 32 + y > row) s[y] = 0xff800000u;
             }
           }
         });
@@ -289,33 +283,30 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       tc::tc_fence_after();
       const int i = (2 * it.tile + t) * 128 + row;
       const bool there = i < it.len;
-      float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-      sum += h.other(sum);
       const float inv = ok ? 1.f / sum : NAN;
       T* to = static_cast<T*>(p.out) + ((it.row + i) * p.heads + head) * p.dim;
 #pragma unroll
-      for (int x = 0; x < DP / 2; x += 32) {
+      for (int x = 0; x < DP / 32; ++x) {
         uint32_t o[32];
-        tc::tmem_ld32(o_at + x, o);
+        tc::tmem_ld32(o_at + x * 32, o);
         tc::tmem_wait_ld();
         if (there) {
 #pragma unroll
-          for (int y = 0; y < 32; y += 8) {
-            const int col = half * (DP / 2) + x + y;
-            if (col < p.dim) {
+          for (int y = 0; y < 4; ++y) {
+            if (x * 32 + y * 8 < p.dim) {
               uint4 w;
-              w.x = pack_pair<T>(__uint_as_float(o[y]) * inv, __uint_as_float(o[y + 1]) * inv);
-              w.y = pack_pair<T>(__uint_as_float(o[y + 2]) * inv, __uint_as_float(o[y + 3]) * inv);
-              w.z = pack_pair<T>(__uint_as_float(o[y + 4]) * inv, __uint_as_float(o[y + 5]) * inv);
-              w.w = pack_pair<T>(__uint_as_float(o[y + 6]) * inv, __uint_as_float(o[y + 7]) * inv);
-              *reinterpret_cast<uint4*>(to + col) = w;
+              w.x = pack_pair<T>(__uint_as_float(o[y * 8]) * inv, __uint_as_float(o[y * 8 + 1]) * inv);
+              w.y = pack_pair<T>(__uint_as_float(o[y * 8 + 2]) * inv, __uint_as_float(o[y * 8 + 3]) * inv);
+              w.z = pack_pair<T>(__uint_as_float(o[y * 8 + 4]) * inv, __uint_as_float(o[y * 8 + 5]) * inv);
+              w.w = pack_pair<T>(__uint_as_float(o[y * 8 + 6]) * inv, __uint_as_float(o[y * 8 + 7]) * inv);
+              *reinterpret_cast<uint4*>(to + x * 32 + y * 8) = w;
             }
           }
         }
       }
       tc::tc_fence_before();
       // rows behind the end: a backward gives them weights exp2(0 - inf) = 0
-      if (p.lse != nullptr && half == 0) {
+      if (p.lse != nullptr) {
         p.lse[head * p.seq.stat_rows + it.stat + i] =
             !there ? INFINITY : ok ? m * c + log2f(sum) : NAN;
       }
@@ -323,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 8) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }

@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 
 // ---- tree attention ----------------------------------------------------------------------------------
 constexpr int kTile = 128;     // tokens of a tile
-constexpr int kThreads = 640;  // warps 0-7, 8-15: weights; 16, 17: keys and values; 18: queries; 19: products
+constexpr int kThreads = 512;  // warps 0-3, 4-7: weights; 8-11: keys and values; 12: products; 13: queries
 constexpr int kJoinThreads = 128;
 struct TreeParams {
   const void *q, *k, *v;
@@ -188,7 +188,7 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 }
 
 // both chains
-__device__ __forceinline__ void sync_chains() { asm volatile("bar.sync 3, 512;" ::: "memory"); }
+__device__ __forceinline__ void sync_chains() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // The key of a page number outside the cache: 128 channels of NaN, in either type
 #define GDN2_NAN4 {~0u, ~0u, ~0u, ~0u}
@@ -374,7 +374,7 @@ struct TreeConfig {
   // Queries of two units, so that the copies need not wait between two; those of 256 rows of 128 channels leave no room.
   static constexpr int kQueries = RT == 2 ? 1 : 2;
   static constexpr int kStages = DP == 64 ? 8 : QR == 32 ? 6 : 5;
-  static constexpr int kBytes = RT * kQueries * kQueryBytes + kStages * kTileBytes + 768 + 2 * int(sizeof(attn::Exchange));
+  static constexpr int kBytes = RT * kQueries * kQueryBytes + kStages * kTileBytes + 768 + 2048;
 };
 
 struct TreeBars {
@@ -393,14 +393,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
   const uint32_t q_base = tc::smem_u32(smem), kv_base = q_base + RT * C::kQueries * C::kQueryBytes;
   TreeBars& bar = *reinterpret_cast<TreeBars*>(smem + RT * C::kQueries * C::kQueryBytes + C::kStages * C::kTileBytes);
-  attn::Exchange* exchange = reinterpret_cast<attn::Exchange*>(smem + RT * C::kQueries * C::kQueryBytes + C::kStages * C::kTileBytes + 768);
+  // (m, l) of the rows of two chains
+  float2(*told)[128] = reinterpret_cast<float2(*)[128]>(smem + RT * C::kQueries * C::kQueryBytes + C::kStages * C::kTileBytes + 768);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (tid == 0) {
     for (int t = 0; t < 2; ++t) {
       tc::mbar_init(&bar.s_full[t], 1);
-      tc::mbar_init(&bar.p_ready[t], 8);
+      tc::mbar_init(&bar.p_ready[t], 4);
       tc::mbar_init(&bar.o_full[t], 1);
     }
     for (int x = 0; x < C::kQueries; ++x) {
@@ -409,13 +410,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     }
     tc::mbar_init(&bar.drained, 1);
     for (int s = 0; s < C::kStages; ++s) {
-      tc::mbar_init(&bar.kv_full[s], 64);
+      tc::mbar_init(&bar.kv_full[s], 128);
       tc::mbar_init(&bar.kv_empty[s], 1);
     }
     bar.failed = bar.strange = 0;
     tc::fence_mbar_init();
   }
-  if (warp == 19) {
+  if (warp == 12) {
     tc::tmem_alloc(&bar.tmem, 512);
     tc::tmem_relinquish();
   }
@@ -427,16 +428,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   tc::tc_fence_after();
   const uint32_t tmem = bar.tmem;
   if (idle) {
-    if (warp == 19) tc::tmem_dealloc(tmem, 512);
+    if (warp == 12) tc::tmem_dealloc(tmem, 512);
     return;
   }
   const attn::Waiter waiter{&bar.failed};
   // tiles of 128 rows that a unit has
   auto row_tiles = [&](const Unit& x) { return RT == 2 && p.rows - x.block * C::kRows > 128 ? 2 : 1; };
 
-  if (warp >= 16) {
-    attn::give_registers();
-    if (warp == 19) {
+  // 512 threads of 128 registers = 256 of 168 + 256 of 88
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 12) {
       // ---- products --------------------------------------------------------------------------------------
       const uint32_t leader = tc::elect_leader();
       const uint32_t id_s = tc::idesc(128, 128, Format<T>::code, tc::kMajorK, tc::kMajorK, p.negate);
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         tc::tc_fence_after();
 #pragma unroll
         for (int ks = 0; ks < kTile / 16; ++ks) {
-          attn::mma_ts(tmem + 256 + t * 128, tmem + t * 128 + (ks >> 2) * 64 + (ks & 3) * 8, attn::desc_mn(kv_base + (x % C::kStages) * C::kTileBytes, C::kSlab, ks),
+          attn::mma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, attn::desc_mn(kv_base + (x % C::kStages) * C::kTileBytes, C::kSlab, ks),
                        id_o, !first || ks > 0, leader);
         }
         return true;
@@ -524,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         for (int i = 0; i < 4096 && !tc::mbar_try_wait(&bar.drained, 0); ++i) {}
       }
       __syncwarp();
-    } else if (warp == 18) {
+    } else if (warp == 13) {
       // ---- queries ---------------------------------------------------------------------------------------
       int units = 0;
       while (rest > 0) {
@@ -543,54 +545,47 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         if (rest > 0) next_unit(p, u);
       }
       cp_async_wait_all();
-    } else {
-      bring_tiles<T, DP, C::kStages, 2>(p, u, tile, rest, warp - 16, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange);
+    } else if (warp < 12) {
+      bring_tiles<T, DP, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange);
     }
   } else {
-    // ---- weights: two threads a row ------------------------------------------------------------------------
-    attn::take_registers();
-    const int t = warp >> 3, half = (warp >> 2) & 1, row = tid & 127;
+    // ---- weights: a row a thread ---------------------------------------------------------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    const int t = warp >> 2, row = tid & 127;
     const uint32_t lane_base = uint32_t(warp & 3) << 21;   // 32 lanes of TMEM, in bits 16 and up
-    const uint32_t s_at = tmem + lane_base + t * 128 + half * 64, o_at = tmem + lane_base + 256 + t * 128 + half * (DP / 2);
-    attn::Half h{t, half, row, 0, exchange + t};
+    const uint32_t s_at = tmem + lane_base + t * 128, o_at = tmem + lane_base + 256 + t * 128;
     int seen = 0, outs = 0;
-    bool ok = true, split = false;   // the unit began in another CTA
-    split = tile != 0;
+    bool ok = true, split = tile != 0;   // the unit began in another CTA
     while (rest > 0) {
       const int n = min(rest, u.tiles - tile), chains = row_tiles(u);
       const int local = (RT == 2 ? t * 128 : 0) + row, r = u.block * C::kRows + local;   // row in the block, of all
       const int token = r / p.group;
       const bool there = r < p.rows, any_there = r - lane < p.rows;
       const bool takes_part = RT == 1 || t < chains;
-      // warps without a row have nothing to do but to keep count
-      h.threads = 64 * min(4, (p.rows - u.block * C::kRows - (RT == 2 ? t * 128 : 0) + 31) / 32);
       float m = -INFINITY;
-      float2 sum2[2] = {{0.f, 0.f}, {0.f, 0.f}};
+      float sum = 0.f;
       int mine = 0;
       for (int j = RT == 1 ? t : 0; j < n && takes_part; j += RT == 1 ? 2 : 1) {
         if (!ok || !(ok = waiter.wait(&bar.s_full[t], seen & 1))) break;
         ++seen;
         tc::tc_fence_after();
-        if (any_there) {
-          const int first_token = (tile + j) * kTile + half * 64;
-          attn::soften<T, DP>(h, s_at, o_at, p.scale_log2, mine == 0, m, sum2, [&](uint32_t (&s)[2][32]) {
-            if (first_token + 64 <= u.length) return;
+        if (any_there) {   // warps without a row have nothing to do but to keep count
+          const int first_token = (tile + j) * kTile;
+          attn::soften<T, DP>(s_at, o_at, p.scale_log2, m, sum, [&](int x, uint32_t (&s)[32]) {
+            if (first_token + x * 32 + 32 <= u.length) return;
             // drafted tokens, or the end
             const uint8_t* mask = p.mask == nullptr || !there ? nullptr : p.mask + u.b * p.mask_stride + int64_t(token) * p.drafted;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              uint32_t sees = 0;
+            uint32_t sees = 0;
 #pragma unroll 8
-              for (int y = 0; y < 32; ++y) {
-                const int d = first_token + x * 32 + y - u.length;
-                bool see = d < 0;
-                if (!see && d < p.drafted && there) see = p.mask == nullptr ? d <= token : mask[d] != 0;
-                sees |= uint32_t(see) << y;
-              }
+            for (int y = 0; y < 32; ++y) {
+              const int d = first_token + x * 32 + y - u.length;
+              bool see = d < 0;
+              if (!see && d < p.drafted && there) see = p.mask == nullptr ? d <= token : mask[d] != 0;
+              sees |= uint32_t(see) << y;
+            }
 #pragma unroll
-              for (int y = 0; y < 32; ++y) {
-                if (!((sees >> y) & 1)) s[x][y] = 0xff800000u;
-              }
+            for (int y = 0; y < 32; ++y) {
+              if (!((sees >> y) & 1)) s[y] = 0xff800000u;
             }
           });
         }
@@ -604,21 +599,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         ++outs;
       }
       tc::tc_fence_after();
-      float sum = (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
-      if (any_there) sum += h.other(sum);
-      // the columns of this thread: half of its row's, or where both chains have the row a quarter of the sum of both
-      constexpr int kCols = RT == 1 ? DP / 4 : DP / 2;
-      const int col0 = RT == 1 ? (2 * t + half) * kCols : half * kCols;
+      // the columns of this thread: all of its row's, or where both chains have the row a half of the sum of both
+      constexpr int kCols = RT == 1 ? DP / 2 : DP;
+      const int col0 = RT == 1 ? t * kCols : 0;
       float f[2] = {1.f, 1.f};
       bool has[2] = {true, true};
       if (RT == 1) {
-        sync_chains();   // what the chains told within themselves has been read
-        exchange[t].x[half][row] = half == 0 ? m : sum;
+        told[t][row] = make_float2(m, sum);
         tc::tc_fence_before();
         sync_chains();
         tc::tc_fence_after();
-        const float m0 = exchange[0].x[0][row], m1 = exchange[1].x[0][row];
-        const float l0 = exchange[0].x[1][row], l1 = exchange[1].x[1][row];
+        const float m0 = told[0][row].x, m1 = told[1][row].x, l0 = told[0][row].y, l1 = told[1][row].y;
         m = fmaxf(m0, m1);
         has[1] = n > 1;
         f[0] = m == -INFINITY ? 0.f : exp2_approx((m0 - m) * p.scale_log2);
@@ -697,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == 19) {
+  if (warp == 12) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }
