@@ -14,7 +14,8 @@
 // every time, at the price of forming S and dP twice (seven products in place of five).  The rows that go by alternate
 // between two sets of S and dP: four warps make weights of one (a row a thread) while the tensor cores form the other.
 //
-// TMEM: two sums of 128 columns, two sets of S and dP of 64 each; P and dS (16-bit) overlay theirs.
+// TMEM: keys: two sums of 128 columns, queries: one, and the rows that stay, 64 columns each; two sets of S and dP of 64
+// each; P and dS (16-bit) overlay theirs.
 
 #include "attention_common.cuh"
 
@@ -42,11 +43,12 @@ struct BwdParams {
   int64_t items;
   float scale, scale_log2;   // scale_log2 is positive
   uint32_t negate;
+  bool wide;                 // rows of the gradients are 32-byte aligned
   Sequences seq;
 };
 
 struct BwdBars {
-  uint64_t stay_full, stay_empty, acc_full, acc_empty, raw, drained;
+  uint64_t stay_full, stay_empty, in_tmem, acc_full, acc_empty, raw, drained;
   uint64_t s_full[2], ds_ready[2], go_full[6], go_empty[6];
   uint32_t tmem;
   int failed;
@@ -87,7 +89,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
 
   if (threadIdx.x == 0) {
     tc::mbar_init(&bar.stay_full, 1);
-    tc::mbar_init(&bar.stay_empty, 1);
+    tc::mbar_init(&bar.stay_empty, kKeys ? 1 : 16);
+    tc::mbar_init(&bar.in_tmem, 16);
     tc::mbar_init(&bar.acc_full, 1);
     tc::mbar_init(&bar.acc_empty, 16);
     tc::mbar_init(&bar.raw, 1);
@@ -195,16 +198,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
         const uint32_t xs = go_base + (x % C::kStages) * 2 * C::kGoBytes, ys = xs + C::kGoBytes;
         const uint32_t s_at = tmem + 256 + b * 128, dp_at = s_at + 64;
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) mma_ss(s_at, desc_k(x_base, C::kStaySlab, ks), desc_k(xs, C::kGoSlab, ks), id_s, ks > 0, leader);
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          if (kKeys) mma_ss(s_at, desc_k(x_base, C::kStaySlab, ks), desc_k(xs, C::kGoSlab, ks), id_s, ks > 0, leader);
+          else mma_ts(s_at, tmem + 128 + ks * 8, desc_k(xs, C::kGoSlab, ks), id_s, ks > 0, leader);
+        }
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) mma_ss(dp_at, desc_k(y_base, C::kStaySlab, ks), desc_k(ys, C::kGoSlab, ks), id_dp, ks > 0, leader);
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          if (kKeys) mma_ss(dp_at, desc_k(y_base, C::kStaySlab, ks), desc_k(ys, C::kGoSlab, ks), id_dp, ks > 0, leader);
+          else mma_ts(dp_at, tmem + 192 + ks * 8, desc_k(ys, C::kGoSlab, ks), id_dp, ks > 0, leader);
+        }
         tc::mma_commit(&bar.s_full[b], leader);
         return true;
       };
       for (int turn = 0; turn < p.turns && ok; ++turn) {
         BwdItem w;
         if (!bwd_item<kKeys>(p, turn, &w)) continue;
-        ok = waiter.wait(&bar.stay_full, stayed & 1);
+        ok = waiter.wait(kKeys ? &bar.stay_full : &bar.in_tmem, stayed & 1);
         if (ok) ok = both(0, used);
         if (ok && w.steps > 1) ok = both(1, used + 1);
         for (int i = 0; i < w.steps && ok; ++i) {
@@ -220,11 +229,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
             for (int ks = 0; ks < kStep / 16; ++ks) mma_ts(tmem, p_at + (ks >> 1) * 32 + (ks & 1) * 8, desc_mn(ys, C::kGoSlab, ks), id_acc, i > 0 || ks > 0, leader);
           }
 #pragma unroll
-          for (int ks = 0; ks < kStep / 16; ++ks) mma_ts(tmem + 128, ds_at + (ks >> 1) * 32 + (ks & 1) * 8, desc_mn(xs, C::kGoSlab, ks), id_acc, i > 0 || ks > 0, leader);
+          for (int ks = 0; ks < kStep / 16; ++ks) mma_ts(kKeys ? tmem + 128 : tmem, ds_at + (ks >> 1) * 32 + (ks & 1) * 8, desc_mn(xs, C::kGoSlab, ks), id_acc, i > 0 || ks > 0, leader);
           tc::mma_commit(&bar.go_empty[x % C::kStages], leader);
           if (i + 1 == w.steps) {
             tc::mma_commit(&bar.acc_full, leader);
-            tc::mma_commit(&bar.stay_empty, leader);
+            if (kKeys) tc::mma_commit(&bar.stay_empty, leader);
           }
           if (i + 2 < w.steps) ok = both(b, x + 2);
         }
@@ -243,13 +252,42 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
     const int b = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & 127;   // two threads a row, 32 columns each
     const uint32_t lane_base = uint32_t(warp & 3) << 21;   // 32 lanes of TMEM, in bits 16 and up
     const uint32_t s_at = tmem + lane_base + 256 + b * 128 + half * 32, dp_at = s_at + 64;
-    int used = 0, seen = 0, outs = 0;
+    int used = 0, seen = 0, outs = 0, stayed = 0;
     bool ok = true;
+    // Queries: a product whose first operand comes from TMEM reads a third of the shared memory (16 KiB of the rows that go
+    // by, and not 32 KiB of those that stay), which is what bounds it.  A thread brings half a row of q and of do there.
+    auto into_tmem = [&]() {
+      if (ok) ok = waiter.wait(&bar.stay_full, stayed & 1);
+      ++stayed;
+      tc::tc_fence_after();
+      constexpr int kWords = DP / 4;   // of half a row
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+#pragma unroll
+        for (int x = 0; x < kWords; x += 16) {
+          uint32_t w[16];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int piece = (half * kWords + x) / 4 + y;
+            const uint4 v = *reinterpret_cast<const uint4*>(stay + which * C::kStayBytes + (piece >> 3) * C::kStaySlab + row * 128 +
+                                                            ((piece ^ row) & 7) * 16);
+            w[4 * y] = v.x; w[4 * y + 1] = v.y; w[4 * y + 2] = v.z; w[4 * y + 3] = v.w;
+          }
+          tc::tmem_st16(tmem + lane_base + 128 + which * 64 + half * kWords + x, w);
+        }
+      }
+      tc::tmem_wait_st();
+      tc::tc_fence_before();
+      __syncwarp();
+      tc::mbar_arrive(&bar.stay_empty, lane == 0);
+      tc::mbar_arrive(&bar.in_tmem, lane == 0);
+    };
     for (int turn = 0; turn < p.turns; ++turn) {
       BwdItem w;
       if (!bwd_item<kKeys>(p, turn, &w)) continue;
       float lse = 0.f, delta = 0.f;
       if (!kKeys) {
+        if (stayed == outs) into_tmem();
         const int64_t at = w.head * p.seq.stat_rows + w.at.stat + w.tile * 128 + row;
         lse = p.lse[at];
         delta = p.delta[at];
@@ -297,33 +335,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
       if (ok) ok = waiter.wait(&bar.acc_full, outs & 1);
       ++outs;
       tc::tc_fence_after();
+      if (!kKeys) {   // the next item's, ahead of this one's stores
+        BwdItem next;
+        for (int later = turn + 1; later < p.turns; ++later) {
+          if (bwd_item<kKeys>(p, later, &next)) {
+            into_tmem();
+            break;
+          }
+        }
+      }
       // keys: eight warps have dv, the others dk, a thread half of a row's channels; queries: a quarter of dq's
       const int i = w.tile * 128 + row;
       const bool there = i < w.at.len;
       const float by = !ok ? NAN : kKeys && b == 0 ? 1.f : p.scale;
       const int64_t out_row = ((w.at.row + i) * (kKeys ? p.kv_heads : p.heads) + w.head) * p.dim;
       T* to = static_cast<T*>(kKeys ? (b == 0 ? p.dv : p.dk) : p.dq) + out_row;
-      const uint32_t acc = tmem + lane_base + (kKeys ? b * 128 : 128);
+      const uint32_t acc = tmem + lane_base + (kKeys ? b * 128 : 0);
       constexpr int kCols = kKeys ? DP / 2 : DP / 4;
       const int col0 = kKeys ? half * kCols : (2 * b + half) * kCols;
 #pragma unroll
       for (int x = 0; x < kCols; x += 16) {
-        uint32_t o[16];
-        tc::tmem_ld16(acc + col0 + x, o);
+        uint32_t raw[16];
+        float o[16];
+        tc::tmem_ld16(acc + col0 + x, raw);
         tc::tmem_wait_ld();
-        if (there) {
 #pragma unroll
-          for (int y = 0; y < 16; y += 8) {
-            if (col0 + x + y < p.dim) {
-              uint4 v;
-              v.x = pack_pair<T>(__uint_as_float(o[y]) * by, __uint_as_float(o[y + 1]) * by);
-              v.y = pack_pair<T>(__uint_as_float(o[y + 2]) * by, __uint_as_float(o[y + 3]) * by);
-              v.z = pack_pair<T>(__uint_as_float(o[y + 4]) * by, __uint_as_float(o[y + 5]) * by);
-              v.w = pack_pair<T>(__uint_as_float(o[y + 6]) * by, __uint_as_float(o[y + 7]) * by);
-              *reinterpret_cast<uint4*>(to + col0 + x + y) = v;
-            }
-          }
-        }
+        for (int y = 0; y < 16; ++y) o[y] = __uint_as_float(raw[y]);
+        if (there) store_row16<T>(to + col0 + x, o, by, p.dim - col0 - x, p.wide);
       }
       tc::tc_fence_before();
       __syncwarp();
@@ -424,6 +462,7 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.dim = dim;
   p.scale = scale;
   p.negate = scale < 0.f;
+  p.wide = wide_rows(dq, dim) && wide_rows(dk, dim) && wide_rows(dv, dim);
   p.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
   return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {
     DeltaParams d{out, d_out, {strides[9], strides[10], strides[11]}, delta, heads, dim, p.seq};

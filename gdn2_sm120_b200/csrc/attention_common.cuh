@@ -209,6 +209,26 @@ __device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, fl
   tc::tmem_wait_st();
 }
 
+// 16 channels of a row, scaled and rounded.  Every lane of a warp has a row of its own, and an instruction takes as long as
+// it has rows: 32 bytes each where rows are aligned to that (`wide`: 16 channels at a time), 16 otherwise.
+template <typename T>
+__device__ __forceinline__ void store_row16(T* to, const float (&x)[16], float by, int channels, bool wide) {
+  uint32_t w[8];
+#pragma unroll
+  for (int y = 0; y < 8; ++y) w[y] = pack_pair<T>(x[2 * y] * by, x[2 * y + 1] * by);
+  if (wide) {
+    if (channels > 0) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                   "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                   : "memory");
+    }
+    return;
+  }
+  if (channels > 0) *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (channels > 8) *reinterpret_cast<uint4*>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+}
+inline bool wide_rows(const void* base, int dim) { return dim % 16 == 0 && (reinterpret_cast<uintptr_t>(base) & 31) == 0; }
+
 // [batch][rows][heads][dim] with any strides that are multiples of 16 bytes, in boxes of 64 channels x box_rows rows
 // of one head.  Channels from dim on and rows behind a batch entry's last one arrive as zeros.
 inline bool encode_heads_map(CUtensorMap* tm, const void* base, const int64_t* strides, int64_t batch, int64_t rows,

@@ -37,6 +37,7 @@ struct FwdParams {
   int64_t items;
   float scale_log2;    // positive
   uint32_t negate;     // the scale is negative: Q counts with its sign changed
+  bool wide;           // rows of the output are 32-byte aligned
   Sequences seq;
 };
 
@@ -286,23 +287,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       const float inv = ok ? 1.f / sum : NAN;
       T* to = static_cast<T*>(p.out) + ((it.row + i) * p.heads + head) * p.dim;
 #pragma unroll
-      for (int x = 0; x < DP / 32; ++x) {
-        uint32_t o[32];
-        tc::tmem_ld32(o_at + x * 32, o);
+      for (int x = 0; x < DP; x += 16) {
+        uint32_t raw[16];
+        float o[16];
+        tc::tmem_ld16(o_at + x, raw);
         tc::tmem_wait_ld();
-        if (there) {
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            if (x * 32 + y * 8 < p.dim) {
-              uint4 w;
-              w.x = pack_pair<T>(__uint_as_float(o[y * 8]) * inv, __uint_as_float(o[y * 8 + 1]) * inv);
-              w.y = pack_pair<T>(__uint_as_float(o[y * 8 + 2]) * inv, __uint_as_float(o[y * 8 + 3]) * inv);
-              w.z = pack_pair<T>(__uint_as_float(o[y * 8 + 4]) * inv, __uint_as_float(o[y * 8 + 5]) * inv);
-              w.w = pack_pair<T>(__uint_as_float(o[y * 8 + 6]) * inv, __uint_as_float(o[y * 8 + 7]) * inv);
-              *reinterpret_cast<uint4*>(to + x * 32 + y * 8) = w;
-            }
-          }
-        }
+        for (int y = 0; y < 16; ++y) o[y] = __uint_as_float(raw[y]);
+        if (there) store_row16<T>(to + x, o, inv, p.dim - x, p.wide);
       }
       tc::tc_fence_before();
       // rows behind the end: a backward gives them weights exp2(0 - inf) = 0
@@ -352,6 +344,7 @@ int launch_attention_forward(const void* q, const void* k, const void* v, void* 
   p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.dim = dim;
   // the sign goes to the product, and a scale of 0 stays a positive number, so that -inf * scale masks as ever
   p.negate = scale < 0.f;
+  p.wide = wide_rows(out, dim);
   p.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
   return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {
     p.items = int64_t(p.seq.tiles) * heads;

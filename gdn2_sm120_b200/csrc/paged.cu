@@ -80,6 +80,7 @@ struct TreeParams {
   CUtensorMap k_map, v_map;
   float scale_log2;                          // positive
   uint32_t negate;                           // the scale is negative: Q counts with its sign changed
+  bool wide;                                 // rows of the output are 32-byte aligned
 };
 
 // A sequence's cached tokens and then its drafted ones, in tiles; kRows rows of one key head
@@ -657,17 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             }
           }
           if (whole) {
-#pragma unroll
-            for (int y = 0; y < 16; y += 8) {
-              if (x + y < p.dim) {
-                uint4 w;
-                w.x = pack_pair<T>(o[y] * inv, o[y + 1] * inv);
-                w.y = pack_pair<T>(o[y + 2] * inv, o[y + 3] * inv);
-                w.z = pack_pair<T>(o[y + 4] * inv, o[y + 5] * inv);
-                w.w = pack_pair<T>(o[y + 6] * inv, o[y + 7] * inv);
-                *reinterpret_cast<uint4*>(to + x + y) = w;
-              }
-            }
+            attn::store_row16<T>(to + x, o, inv, p.dim - x, p.wide);
           } else {
 #pragma unroll
             for (int y = 0; y < 16; y += 4) *reinterpret_cast<float4*>(part + x + y) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
@@ -1116,6 +1107,7 @@ int launch_tree(const void* q, const void* k, const void* v, const void* k_pages
   if (int64_t(batch) * kv_heads * p.row_blocks > int64_t(0x7fffffff) / joining_ctas(p, per_block)) return GDN2_ERR_TOO_LARGE;
   // the sign goes to the product, and a scale of 0 stays a positive number, so that -inf * scale masks as ever
   p.negate = scale < 0.f;
+  p.wide = attn::wide_rows(out, dim);
   p.scale_log2 = fmaxf(fabsf(scale) * attn::kLog2e, 1e-30f);
   return dtype == GDN2_BF16 ? launch_tree_dim<__nv_bfloat16>(p, stream) : launch_tree_dim<__half>(p, stream);
 }
