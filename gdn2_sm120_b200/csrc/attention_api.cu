@@ -54,9 +54,9 @@ int check_sequences(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t 
       if (bounds[i] < 0 || bounds[i + 1] < bounds[i] || bounds[i + 1] > time) return GDN2_ERR_BAD_RANGE;
     }
   }
-  // tiles of 256 rows are numbered with 31 bits
+  // pieces of 64 rows are numbered with 31 bits
   const int64_t stat = attn::attention_stat_rows(bounds, n_seq, time);
-  return stat / 128 > kMost / heads ? GDN2_ERR_TOO_LARGE : GDN2_OK;
+  return stat / 64 > kMost / heads ? GDN2_ERR_TOO_LARGE : GDN2_OK;
 }
 
 }  // namespace

@@ -28,17 +28,17 @@ constexpr int kThreads = 640;    // warps 0-7: even steps; 8-15: odd ones; 16: p
 constexpr int kStep = 64;        // rows of a step
 
 template <int DP>
-struct BwdConfig {
+struct QueryConfig {
   static constexpr int kStayBytes = 128 * DP * 2, kStaySlab = 128 * 128;
   static constexpr int kGoBytes = kStep * DP * 2, kGoSlab = kStep * 128;
   static constexpr int kStages = DP == 128 ? 4 : 6;
-  static constexpr int kBytes = 2 * kStayBytes + kStages * (2 * kGoBytes + 2 * kStep * 4) + 512;
+  static constexpr int kBytes = 2 * kStayBytes + kStages * 2 * kGoBytes + 512;
 };
 
 struct BwdParams {
-  CUtensorMap q_stay, do_stay, k_stay, v_stay, q_go, do_go, k_go, v_go;
+  CUtensorMap q_tile, do_tile, k_tile, v_tile, k_step, v_step;   // 128 rows, 64 rows
   void *dq, *dk, *dv;
-  const float *lse, *delta;
+  const float *lse, *delta;  // -(m + log2 l) in powers of two, -delta
   int heads, kv_heads, group, dim, turns;
   int64_t items;
   float scale, scale_log2;   // scale_log2 is positive
@@ -47,7 +47,7 @@ struct BwdParams {
   Sequences seq;
 };
 
-struct BwdBars {
+struct QueryBars {
   uint64_t stay_full, stay_empty, in_tmem, acc_full, acc_empty, raw, drained;
   uint64_t s_full[2], ds_ready[2], go_full[6], go_empty[6];
   uint32_t tmem;
@@ -57,7 +57,7 @@ struct BwdBars {
 struct BwdItem {
   Item at;
   int head, tile;       // of queries, or of keys; 128-row tile in the sequence
-  int first, per_head, steps;  // first 64-row step, steps of a query head, of all
+  int first, per_head, steps;  // keys: first 128-row step, steps of a query head, of all; queries: 64-row steps
 };
 
 template <bool kKeys>
@@ -70,26 +70,24 @@ __device__ __forceinline__ bool bwd_item(const BwdParams& p, int turn, BwdItem* 
   w->at = find_item(p.seq, u >> 1, !kKeys);
   w->tile = 2 * w->at.tile + (kKeys ? u & 1 : 1 - (u & 1));
   if (w->tile * 128 >= w->at.len) return false;
-  const int all = (w->at.len + kStep - 1) / kStep;
-  w->first = kKeys ? 2 * w->tile : 0;
-  w->per_head = kKeys ? all - w->first : min(2 * w->tile + 2, all);
+  w->first = kKeys ? w->tile : 0;
+  w->per_head = kKeys ? (w->at.len + 127) / 128 - w->tile : min(2 * w->tile + 2, (w->at.len + kStep - 1) / kStep);
   w->steps = kKeys ? w->per_head * p.group : w->per_head;
   return true;
 }
 
-template <typename T, int DP, bool kKeys>
-__global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const __grid_constant__ BwdParams p) {
-  using C = BwdConfig<DP>;
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __grid_constant__ BwdParams p) {
+  using C = QueryConfig<DP>;
   extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
   uint8_t* stay = smem;
   uint8_t* go = smem + 2 * C::kStayBytes;
-  float* stats = reinterpret_cast<float*>(go + C::kStages * 2 * C::kGoBytes);   // [stage][lse, delta][64]
-  BwdBars& bar = *reinterpret_cast<BwdBars*>(stats + C::kStages * 2 * kStep);
+  QueryBars& bar = *reinterpret_cast<QueryBars*>(go + C::kStages * 2 * C::kGoBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     tc::mbar_init(&bar.stay_full, 1);
-    tc::mbar_init(&bar.stay_empty, kKeys ? 1 : 16);
+    tc::mbar_init(&bar.stay_empty, 16);
     tc::mbar_init(&bar.in_tmem, 16);
     tc::mbar_init(&bar.acc_full, 1);
     tc::mbar_init(&bar.acc_empty, 16);
@@ -125,16 +123,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
       bool ok = true;
       for (int turn = 0; turn < p.turns && ok; ++turn) {
         BwdItem w;
-        if (!bwd_item<kKeys>(p, turn, &w)) continue;
-        const int kv_head = kKeys ? w.head : w.head / p.group;
+        if (!bwd_item<false>(p, turn, &w)) continue;
+        const int kv_head = w.head / p.group;
         if (stayed > 0) ok = waiter.wait(&bar.stay_empty, (stayed - 1) & 1);
         if (!ok) break;
         tc::mbar_arrive_expect_tx(&bar.stay_full, 2 * C::kStayBytes, leader);
 #pragma unroll
         for (int slab = 0; slab < DP / 64; ++slab) {
           const int row = w.at.row0 + w.tile * 128;
-          tc::tma_load_4d(stay + slab * C::kStaySlab, kKeys ? &p.k_stay : &p.q_stay, slab * 64, w.head, row, w.at.batch, &bar.stay_full, leader);
-          tc::tma_load_4d(stay + C::kStayBytes + slab * C::kStaySlab, kKeys ? &p.v_stay : &p.do_stay, slab * 64, w.head, row, w.at.batch,
+          tc::tma_load_4d(stay + slab * C::kStaySlab, &p.q_tile, slab * 64, w.head, row, w.at.batch, &bar.stay_full, leader);
+          tc::tma_load_4d(stay + C::kStayBytes + slab * C::kStaySlab, &p.do_tile, slab * 64, w.head, row, w.at.batch,
                           &bar.stay_full, leader);
         }
         ++stayed;
@@ -142,24 +140,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
           const int s = filled % C::kStages;
           if (filled >= C::kStages) ok = waiter.wait(&bar.go_empty[s], (filled / C::kStages - 1) & 1);
           if (!ok) break;
-          const int g = i / w.per_head, at = (w.first + i - g * w.per_head) * kStep;
-          const int head = kKeys ? w.head * p.group + g : kv_head;
+          const int at = i * kStep;
           uint8_t* to = go + s * 2 * C::kGoBytes;
           // rows of the next sequence would meet weights of 0, but 0 * inf and 0 * NaN are not 0
           const int valid = w.at.len - at;
           const bool mend = p.seq.packed && valid < kStep;
           uint64_t* full = mend ? &bar.raw : &bar.go_full[s];
-          tc::mbar_arrive_expect_tx(full, 2 * C::kGoBytes + (kKeys ? 2 * kStep * 4 : 0), leader);
+          tc::mbar_arrive_expect_tx(full, 2 * C::kGoBytes, leader);
 #pragma unroll
           for (int slab = 0; slab < DP / 64; ++slab) {
-            tc::tma_load_4d(to + slab * C::kGoSlab, kKeys ? &p.q_go : &p.k_go, slab * 64, head, w.at.row0 + at, w.at.batch, full, leader);
-            tc::tma_load_4d(to + C::kGoBytes + slab * C::kGoSlab, kKeys ? &p.do_go : &p.v_go, slab * 64, head, w.at.row0 + at, w.at.batch,
+            tc::tma_load_4d(to + slab * C::kGoSlab, &p.k_step, slab * 64, kv_head, w.at.row0 + at, w.at.batch, full, leader);
+            tc::tma_load_4d(to + C::kGoBytes + slab * C::kGoSlab, &p.v_step, slab * 64, kv_head, w.at.row0 + at, w.at.batch,
                             full, leader);
-          }
-          if (kKeys) {
-            const int64_t from = head * p.seq.stat_rows + w.at.stat + at;
-            tc::bulk_g2s(stats + s * 2 * kStep, p.lse + from, kStep * 4, full, leader);
-            tc::bulk_g2s(stats + s * 2 * kStep + kStep, p.delta + from, kStep * 4, full, leader);
           }
           if (mend) {
             ok = waiter.wait(&bar.raw, mended & 1);
@@ -189,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
       const uint32_t id_s = tc::idesc(128, kStep, Format<T>::code, tc::kMajorK, tc::kMajorK, p.negate);
       const uint32_t id_dp = tc::idesc(128, kStep, Format<T>::code, tc::kMajorK, tc::kMajorK);
       const uint32_t id_acc = tc::idesc(128, DP, Format<T>::code, tc::kMajorK, tc::kMajorMN);
-      const uint32_t x_base = tc::smem_u32(stay), y_base = x_base + C::kStayBytes, go_base = tc::smem_u32(go);
+      const uint32_t go_base = tc::smem_u32(go);
       int used = 0, stayed = 0, ready[2] = {0, 0};
       bool ok = true;
       auto both = [&](int b, int x) {   // S and dP of the step in stage x
@@ -198,22 +190,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
         const uint32_t xs = go_base + (x % C::kStages) * 2 * C::kGoBytes, ys = xs + C::kGoBytes;
         const uint32_t s_at = tmem + 256 + b * 128, dp_at = s_at + 64;
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          if (kKeys) mma_ss(s_at, desc_k(x_base, C::kStaySlab, ks), desc_k(xs, C::kGoSlab, ks), id_s, ks > 0, leader);
-          else mma_ts(s_at, tmem + 128 + ks * 8, desc_k(xs, C::kGoSlab, ks), id_s, ks > 0, leader);
-        }
+        for (int ks = 0; ks < DP / 16; ++ks) mma_ts(s_at, tmem + 128 + ks * 8, desc_k(xs, C::kGoSlab, ks), id_s, ks > 0, leader);
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          if (kKeys) mma_ss(dp_at, desc_k(y_base, C::kStaySlab, ks), desc_k(ys, C::kGoSlab, ks), id_dp, ks > 0, leader);
-          else mma_ts(dp_at, tmem + 192 + ks * 8, desc_k(ys, C::kGoSlab, ks), id_dp, ks > 0, leader);
-        }
+        for (int ks = 0; ks < DP / 16; ++ks) mma_ts(dp_at, tmem + 192 + ks * 8, desc_k(ys, C::kGoSlab, ks), id_dp, ks > 0, leader);
         tc::mma_commit(&bar.s_full[b], leader);
         return true;
       };
       for (int turn = 0; turn < p.turns && ok; ++turn) {
         BwdItem w;
-        if (!bwd_item<kKeys>(p, turn, &w)) continue;
-        ok = waiter.wait(kKeys ? &bar.stay_full : &bar.in_tmem, stayed & 1);
+        if (!bwd_item<false>(p, turn, &w)) continue;
+        ok = waiter.wait(&bar.in_tmem, stayed & 1);
         if (ok) ok = both(0, used);
         if (ok && w.steps > 1) ok = both(1, used + 1);
         for (int i = 0; i < w.steps && ok; ++i) {
@@ -222,19 +208,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
           if (!(ok = waiter.wait(&bar.ds_ready[b], ready[b] & 1))) break;
           ++ready[b];
           tc::tc_fence_after();
-          const uint32_t xs = go_base + (x % C::kStages) * 2 * C::kGoBytes, ys = xs + C::kGoBytes;
-          const uint32_t p_at = tmem + 256 + b * 128, ds_at = p_at + 64;
-          if (kKeys) {
+          const uint32_t xs = go_base + (x % C::kStages) * 2 * C::kGoBytes, ds_at = tmem + 256 + b * 128 + 64;
 #pragma unroll
-            for (int ks = 0; ks < kStep / 16; ++ks) mma_ts(tmem, p_at + (ks >> 1) * 32 + (ks & 1) * 8, desc_mn(ys, C::kGoSlab, ks), id_acc, i > 0 || ks > 0, leader);
-          }
-#pragma unroll
-          for (int ks = 0; ks < kStep / 16; ++ks) mma_ts(kKeys ? tmem + 128 : tmem, ds_at + (ks >> 1) * 32 + (ks & 1) * 8, desc_mn(xs, C::kGoSlab, ks), id_acc, i > 0 || ks > 0, leader);
+          for (int ks = 0; ks < kStep / 16; ++ks) mma_ts(tmem, ds_at + (ks >> 1) * 32 + (ks & 1) * 8, desc_mn(xs, C::kGoSlab, ks), id_acc, i > 0 || ks > 0, leader);
           tc::mma_commit(&bar.go_empty[x % C::kStages], leader);
-          if (i + 1 == w.steps) {
-            tc::mma_commit(&bar.acc_full, leader);
-            if (kKeys) tc::mma_commit(&bar.stay_empty, leader);
-          }
+          if (i + 1 == w.steps) tc::mma_commit(&bar.acc_full, leader);
           if (i + 2 < w.steps) ok = both(b, x + 2);
         }
         used += w.steps;
@@ -252,9 +230,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
     const int b = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & 127;   // two threads a row, 32 columns each
     const uint32_t lane_base = uint32_t(warp & 3) << 21;   // 32 lanes of TMEM, in bits 16 and up
     const uint32_t s_at = tmem + lane_base + 256 + b * 128 + half * 32, dp_at = s_at + 64;
-    int used = 0, seen = 0, outs = 0, stayed = 0;
+    int seen = 0, outs = 0, stayed = 0, all[2] = {0, 0};   // steps of this set, items, items in TMEM, steps of both sets
     bool ok = true;
-    // Queries: a product whose first operand comes from TMEM reads a third of the shared memory (16 KiB of the rows that go
+    // A product whose first operand comes from TMEM reads a third of the shared memory (16 KiB of the rows that go
     // by, and not 32 KiB of those that stay), which is what bounds it.  A thread brings half a row of q and of do there.
     auto into_tmem = [&]() {
       if (ok) ok = waiter.wait(&bar.stay_full, stayed & 1);
@@ -284,80 +262,370 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
     };
     for (int turn = 0; turn < p.turns; ++turn) {
       BwdItem w;
-      if (!bwd_item<kKeys>(p, turn, &w)) continue;
-      float lse = 0.f, delta = 0.f;
-      if (!kKeys) {
-        if (stayed == outs) into_tmem();
-        const int64_t at = w.head * p.seq.stat_rows + w.at.stat + w.tile * 128 + row;
-        lse = p.lse[at];
-        delta = p.delta[at];
-      }
+      if (!bwd_item<false>(p, turn, &w)) continue;
+      if (stayed == outs) into_tmem();
+      const int64_t stat = w.head * p.seq.stat_rows + w.at.stat + w.tile * 128 + row;
+      const float2 minus_lse = twice(p.lse[stat]), minus_delta = twice(p.delta[stat]), by_scale = twice(p.scale_log2);
       for (int i = b; i < w.steps && ok; i += 2) {
         if (!(ok = waiter.wait(&bar.s_full[b], seen & 1))) break;
         ++seen;
         tc::tc_fence_after();
-        const int g = i / w.per_head, at = (w.first + i - g * w.per_head) * kStep;
-        // queries see keys up to themselves: of the rows that go by, x from `from` on (keys), up to `from` (queries)
-        const int from = w.tile * 128 + row - at;
-        const bool diagonal = kKeys ? at < w.tile * 128 + 128 : at + kStep > w.tile * 128;
-        const float* st = stats + ((used + i) % C::kStages) * 2 * kStep;
-        uint32_t s[32], dp[32], pw[16], dsw[16];
+        // a query sees keys up to itself: of those that go by the first to `last`
+        const int last = w.tile * 128 + row - i * kStep;
+        const bool diagonal = (i + 1) * kStep > w.tile * 128;
+        uint32_t s[32], dp[32], dsw[16];
         tc::tmem_ld32(s_at, s);
         tc::tmem_ld32(dp_at, dp);
         tc::tmem_wait_ld();
 #pragma unroll
         for (int y = 0; y < 32; y += 2) {
           const int x = half * 32 + y;
-          float2 l = twice(lse), d = twice(delta);
-          if (kKeys) {
-            l = *reinterpret_cast<const float2*>(st + x);
-            d = *reinterpret_cast<const float2*>(st + kStep + x);
-          }
-          const float2 sc = fma2(make_float2(__uint_as_float(s[y]), __uint_as_float(s[y + 1])), twice(p.scale_log2), minus2(make_float2(0.f, 0.f), l));
-          float2 e = exp2_2(sc);
-          float2 ds = mul2(e, minus2(make_float2(__uint_as_float(dp[y]), __uint_as_float(dp[y + 1])), d));
+          const float2 z = fma2(make_float2(__uint_as_float(s[y]), __uint_as_float(s[y + 1])), by_scale, minus_lse);
+          const float2 e = exp2_2(z);
+          float2 ds = mul2(e, add2(make_float2(__uint_as_float(dp[y]), __uint_as_float(dp[y + 1])), minus_delta));
           if (diagonal) {
-            if (kKeys ? x < from : x > from) { e.x = 0.f; ds.x = 0.f; }
-            if (kKeys ? x + 1 < from : x + 1 > from) { e.y = 0.f; ds.y = 0.f; }
+            if (x > last) ds.x = 0.f;
+            if (x + 1 > last) ds.y = 0.f;
           }
-          // both are rounded to the inputs' type for their products, the sums are in 32 bits
-          if (kKeys) pw[y / 2] = pack_pair<T>(e.x, e.y);
-          dsw[y / 2] = pack_pair<T>(ds.x, ds.y);
+          dsw[y / 2] = pack_pair<T>(ds.x, ds.y);   // rounded to the inputs' type for its product, whose sums are in 32 bits
         }
-        if (kKeys) tc::tmem_st16(s_at, pw);
         tc::tmem_st16(dp_at, dsw);
         tc::tmem_wait_st();
         tc::tc_fence_before();
         __syncwarp();
         tc::mbar_arrive(&bar.ds_ready[b], lane == 0);
       }
-      used += w.steps;
+      // When the last S has arrived nobody reads this item's q and do any more: the next item's take their place, and its
+      // first products begin, ahead of this one's stores.
+      const int last_set = (w.steps - 1) & 1;
+      all[0] += (w.steps + 1) / 2;
+      all[1] += w.steps / 2;
+      if (ok) ok = waiter.wait(&bar.s_full[last_set], (all[last_set] - 1) & 1);
+      BwdItem next;
+      for (int later = turn + 1; later < p.turns; ++later) {
+        if (bwd_item<false>(p, later, &next)) {
+          into_tmem();
+          break;
+        }
+      }
       if (ok) ok = waiter.wait(&bar.acc_full, outs & 1);
       ++outs;
       tc::tc_fence_after();
-      if (!kKeys) {   // the next item's, ahead of this one's stores
-        BwdItem next;
-        for (int later = turn + 1; later < p.turns; ++later) {
-          if (bwd_item<kKeys>(p, later, &next)) {
-            into_tmem();
-            break;
-          }
-        }
-      }
-      // keys: eight warps have dv, the others dk, a thread half of a row's channels; queries: a quarter of dq's
+      // a thread has a quarter of its row's channels
       const int i = w.tile * 128 + row;
       const bool there = i < w.at.len;
-      const float by = !ok ? NAN : kKeys && b == 0 ? 1.f : p.scale;
-      const int64_t out_row = ((w.at.row + i) * (kKeys ? p.kv_heads : p.heads) + w.head) * p.dim;
-      T* to = static_cast<T*>(kKeys ? (b == 0 ? p.dv : p.dk) : p.dq) + out_row;
-      const uint32_t acc = tmem + lane_base + (kKeys ? b * 128 : 0);
-      constexpr int kCols = kKeys ? DP / 2 : DP / 4;
-      const int col0 = kKeys ? half * kCols : (2 * b + half) * kCols;
+      const float by = ok ? p.scale : NAN;
+      T* to = static_cast<T*>(p.dq) + ((w.at.row + i) * p.heads + w.head) * p.dim;
+      constexpr int kCols = DP / 4;
+      const int col0 = (2 * b + half) * kCols;
 #pragma unroll
       for (int x = 0; x < kCols; x += 16) {
         uint32_t raw[16];
         float o[16];
-        tc::tmem_ld16(acc + col0 + x, raw);
+        tc::tmem_ld16(tmem + lane_base + col0 + x, raw);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int y = 0; y < 16; ++y) o[y] = __uint_as_float(raw[y]);
+        if (there) store_row16<T>(to + col0 + x, o, by, p.dim - col0 - x, p.wide);
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      tc::mbar_arrive(&bar.acc_empty, lane == 0);
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 16) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 512);
+  }
+  outlast_others();   // the key kernel
+}
+
+// Keys: K and V of 128 keys stay; q and do of all queries that see them go by, 128 at a time, for every head of the group.
+// One set of S^T and dP^T (128 columns each; the two sums have the rest of TMEM), in two phases that overlap the products:
+//
+//   products   dv += P^T do, S^T(i + 1) | dk += dS^T q, dP^T(i + 1) | ...
+//   threads    dS(i) from dP^T(i)       | P(i + 1) from S^T(i + 1)  | ...
+//
+// P and dS (16-bit) overlay S^T and dP^T.  Sixteen warps, a quarter of a row a thread: its weights stay in registers from the
+// first phase to the second.
+template <int DP>
+struct KeyConfig {
+  static constexpr int kTileBytes = 128 * DP * 2, kSlab = 128 * 128;
+  static constexpr int kStages = DP == 128 ? 4 : 8;       // tiles of q and of do by turns
+  static constexpr int kStats = kStages / 2;              // steps whose statistics are there
+  static constexpr int kBytes = (2 + kStages) * kTileBytes + kStats * 2 * 128 * 4 + 512;
+};
+
+struct KeyBars {
+  uint64_t stay_full, stay_empty, acc_full, acc_empty, raw, drained;
+  uint64_t s_full, dp_full, p_ready, ds_ready, go_full[8], go_empty[8];
+  uint32_t tmem;
+  int failed;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __grid_constant__ BwdParams p) {
+  using C = KeyConfig<DP>;
+  extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
+  uint8_t* go = smem + 2 * C::kTileBytes;
+  float* stats = reinterpret_cast<float*>(go + C::kStages * C::kTileBytes);   // [step by turns][-lse, -delta][128]
+  KeyBars& bar = *reinterpret_cast<KeyBars*>(stats + C::kStats * 2 * 128);
+  static_assert(sizeof(KeyBars) <= 512, "");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    tc::mbar_init(&bar.stay_full, 1);
+    tc::mbar_init(&bar.stay_empty, 1);
+    tc::mbar_init(&bar.acc_full, 1);
+    tc::mbar_init(&bar.acc_empty, 16);
+    tc::mbar_init(&bar.raw, 1);
+    tc::mbar_init(&bar.drained, 1);
+    tc::mbar_init(&bar.s_full, 1);
+    tc::mbar_init(&bar.dp_full, 1);
+    tc::mbar_init(&bar.p_ready, 16);
+    tc::mbar_init(&bar.ds_ready, 16);
+    for (int s = 0; s < C::kStages; ++s) {
+      tc::mbar_init(&bar.go_full[s], 1);
+      tc::mbar_init(&bar.go_empty[s], 1);
+    }
+    bar.failed = 0;
+    tc::fence_mbar_init();
+  }
+  if (warp == 16) {
+    tc::tmem_alloc(&bar.tmem, 512);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = bar.tmem;
+  const Waiter waiter{&bar.failed};
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // delta
+  let_others_begin();
+
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");   // 640 threads of 96 registers = 512 of 104 + 128 of 64
+    if (warp == 17) {
+      // ---- copies ----------------------------------------------------------------------------------------
+      tc::fence_async_all();   // delta was written by threads, and is read by bulk copies
+      const uint32_t leader = tc::elect_leader();
+      int filled = 0, stayed = 0, mended = 0;
+      bool ok = true;
+      for (int turn = 0; turn < p.turns && ok; ++turn) {
+        BwdItem w;
+        if (!bwd_item<true>(p, turn, &w)) continue;
+        if (stayed > 0 && !(ok = waiter.wait(&bar.stay_empty, (stayed - 1) & 1))) break;
+        tc::mbar_arrive_expect_tx(&bar.stay_full, 2 * C::kTileBytes, leader);
+#pragma unroll
+        for (int slab = 0; slab < DP / 64; ++slab) {
+          const int row = w.at.row0 + w.tile * 128;
+          tc::tma_load_4d(smem + slab * C::kSlab, &p.k_tile, slab * 64, w.head, row, w.at.batch, &bar.stay_full, leader);
+          tc::tma_load_4d(smem + C::kTileBytes + slab * C::kSlab, &p.v_tile, slab * 64, w.head, row, w.at.batch, &bar.stay_full, leader);
+        }
+        ++stayed;
+        for (int i = 0; i < 2 * w.steps && ok; ++i) {   // q and do by turns
+          const int s = filled % C::kStages, step = i >> 1;
+          if (filled >= C::kStages && !(ok = waiter.wait(&bar.go_empty[s], (filled / C::kStages - 1) & 1))) break;
+          const int g = step / w.per_head, at = (w.first + step - g * w.per_head) * 128;
+          const int head = w.head * p.group + g;
+          uint8_t* to = go + s * C::kTileBytes;
+          // rows of the next sequence would meet weights of 0, but 0 * inf and 0 * NaN are not 0
+          const int valid = w.at.len - at;
+          const bool mend = p.seq.packed && valid < 128, queries = (i & 1) == 0;
+          uint64_t* full = mend ? &bar.raw : &bar.go_full[s];
+          tc::mbar_arrive_expect_tx(full, C::kTileBytes + (queries ? 2 * 128 * 4 : 0), leader);
+#pragma unroll
+          for (int slab = 0; slab < DP / 64; ++slab) {
+            tc::tma_load_4d(to + slab * C::kSlab, queries ? &p.q_tile : &p.do_tile, slab * 64, head, w.at.row0 + at, w.at.batch, full, leader);
+          }
+          if (queries) {
+            const int64_t from = head * p.seq.stat_rows + w.at.stat + at;
+            float* st = stats + (filled >> 1) % C::kStats * 2 * 128;
+            tc::bulk_g2s(st, p.lse + from, 128 * 4, full, leader);
+            tc::bulk_g2s(st + 128, p.delta + from, 128 * 4, full, leader);
+          }
+          if (mend) {
+            ok = waiter.wait(&bar.raw, mended & 1);
+            ++mended;
+#pragma unroll
+            for (int slab = 0; slab < DP / 64; ++slab) {
+              uint4* lines = reinterpret_cast<uint4*>(to + slab * C::kSlab);
+              for (int x = valid * 8 + lane; x < 128 * 8; x += 32) lines[x] = make_uint4(0, 0, 0, 0);
+            }
+            tc::fence_async_smem();
+            __syncwarp();
+            tc::mbar_arrive(&bar.go_full[s], leader);
+          }
+          ++filled;
+        }
+      }
+      if (!ok) {  // copies under way end before the CTA does
+        for (int back = 1; back <= C::kStages && back <= filled; ++back) {
+          const int x = filled - back;
+          for (int i = 0; i < 4096 && !tc::mbar_try_wait(&bar.go_full[x % C::kStages], (x / C::kStages) & 1); ++i) {}
+        }
+        for (int i = 0; stayed > 0 && i < 4096 && !tc::mbar_try_wait(&bar.stay_full, (stayed - 1) & 1); ++i) {}
+      }
+    } else if (warp == 16) {
+      // ---- products --------------------------------------------------------------------------------------
+      const uint32_t leader = tc::elect_leader();
+      const uint32_t id_s = tc::idesc(128, 128, Format<T>::code, tc::kMajorK, tc::kMajorK, p.negate);
+      const uint32_t id_dp = tc::idesc(128, 128, Format<T>::code, tc::kMajorK, tc::kMajorK);
+      const uint32_t id_acc = tc::idesc(128, DP, Format<T>::code, tc::kMajorK, tc::kMajorMN);
+      const uint32_t k_base = tc::smem_u32(smem), v_base = k_base + C::kTileBytes, go_base = tc::smem_u32(go);
+      int used = 0, stayed = 0, steps = 0;   // tiles, items, steps
+      bool ok = true;
+      auto full = [&](int x) { return waiter.wait(&bar.go_full[x % C::kStages], (x / C::kStages) & 1); };
+      auto scores = [&](int x) {   // S^T from the queries in stage x
+        if (!full(x)) return false;
+        tc::tc_fence_after();
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          mma_ss(tmem + 256, desc_k(k_base, C::kSlab, ks), desc_k(go_base + (x % C::kStages) * C::kTileBytes, C::kSlab, ks), id_s, ks > 0, leader);
+        }
+        tc::mma_commit(&bar.s_full, leader);
+        return true;
+      };
+      auto slopes = [&](int x) {   // dP^T
+        if (!full(x)) return false;
+        tc::tc_fence_after();
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          mma_ss(tmem + 384, desc_k(v_base, C::kSlab, ks), desc_k(go_base + (x % C::kStages) * C::kTileBytes, C::kSlab, ks), id_dp, ks > 0, leader);
+        }
+        tc::mma_commit(&bar.dp_full, leader);
+        return true;
+      };
+      for (int turn = 0; turn < p.turns && ok; ++turn) {
+        BwdItem w;
+        if (!bwd_item<true>(p, turn, &w)) continue;
+        if (!(ok = waiter.wait(&bar.stay_full, stayed & 1))) break;
+        if (!(ok = scores(used)) || !(ok = slopes(used + 1))) break;
+        for (int i = 0; i < w.steps && ok; ++i) {
+          const int x = used + 2 * i;
+          const bool more = i + 1 < w.steps;
+          if (i == 0 && stayed > 0 && !(ok = waiter.wait(&bar.acc_empty, (stayed - 1) & 1))) break;
+          if (!(ok = waiter.wait(&bar.p_ready, steps & 1))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {   // the 16-bit numbers of a quarter of the queries are 32 columns apart
+            mma_ts(tmem, tmem + 256 + (ks >> 1) * 32 + (ks & 1) * 8, desc_mn(go_base + ((x + 1) % C::kStages) * C::kTileBytes, C::kSlab, ks),
+                   id_acc, i > 0 || ks > 0, leader);
+          }
+          tc::mma_commit(&bar.go_empty[(x + 1) % C::kStages], leader);
+          if (more && !(ok = scores(x + 2))) break;
+          if (!(ok = waiter.wait(&bar.ds_ready, steps & 1))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            mma_ts(tmem + 128, tmem + 384 + (ks >> 1) * 32 + (ks & 1) * 8, desc_mn(go_base + (x % C::kStages) * C::kTileBytes, C::kSlab, ks),
+                   id_acc, i > 0 || ks > 0, leader);
+          }
+          tc::mma_commit(&bar.go_empty[x % C::kStages], leader);
+          if (more && !(ok = slopes(x + 3))) break;
+          ++steps;
+        }
+        tc::mma_commit(&bar.acc_full, leader);
+        tc::mma_commit(&bar.stay_empty, leader);
+        used += 2 * w.steps;
+        ++stayed;
+      }
+      if (!ok) {  // products under way end before the CTA does
+        tc::mma_commit(&bar.drained, leader);
+        for (int i = 0; i < 4096 && !tc::mbar_try_wait(&bar.drained, 0); ++i) {}
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---- weights: four threads a row -----------------------------------------------------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int part = warp >> 2, row = threadIdx.x & 127;   // 32 of a step's queries, key
+    const uint32_t lane_base = uint32_t(warp & 3) << 21;   // 32 lanes of TMEM, in bits 16 and up
+    const uint32_t s_at = tmem + lane_base + 256 + part * 32, dp_at = s_at + 128;
+    const float2 by_scale = twice(p.scale_log2);
+    int steps = 0, outs = 0;
+    bool ok = true;
+    for (int turn = 0; turn < p.turns; ++turn) {
+      BwdItem w;
+      if (!bwd_item<true>(p, turn, &w)) continue;
+      int in_head = 0;
+      for (int i = 0; i < w.steps && ok; ++i, ++steps) {
+        const float* st = stats + steps % C::kStats * 2 * 128 + part * 32;
+        // queries see keys up to themselves; a head's first step is the one on the diagonal
+        const bool diagonal = in_head == 0;
+        const int from = row - part * 32;
+        if (++in_head == w.per_head) in_head = 0;
+        if (!(ok = waiter.wait(&bar.s_full, steps & 1))) break;
+        tc::tc_fence_after();
+        uint32_t s[32], w16[16];
+        float2 e[16];
+        tc::tmem_ld32(s_at, s);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int y = 0; y < 16; y += 2) {
+          const float4 l = *reinterpret_cast<const float4*>(st + 2 * y);
+          const float2 a = fma2(make_float2(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1])), by_scale, make_float2(l.x, l.y));
+          const float2 b = fma2(make_float2(__uint_as_float(s[2 * y + 2]), __uint_as_float(s[2 * y + 3])), by_scale, make_float2(l.z, l.w));
+          e[y] = exp2_2(a);
+          e[y + 1] = (y & 2) != 0 ? exp2_fma(b) : exp2_2(b);
+        }
+        if (diagonal) {
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            if (2 * y < from) e[y].x = 0.f;
+            if (2 * y + 1 < from) e[y].y = 0.f;
+          }
+        }
+        // rounded to the inputs' type for their product, whose sums are in 32 bits
+#pragma unroll
+        for (int y = 0; y < 16; ++y) w16[y] = pack_pair<T>(e[y].x, e[y].y);
+        tc::tmem_st16(s_at, w16);
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        __syncwarp();
+        tc::mbar_arrive(&bar.p_ready, lane == 0);
+
+        if (!(ok = waiter.wait(&bar.dp_full, steps & 1))) break;
+        tc::tc_fence_after();
+        tc::tmem_ld32(dp_at, s);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int y = 0; y < 16; y += 2) {
+          const float4 d = *reinterpret_cast<const float4*>(st + 128 + 2 * y);
+          e[y] = mul2(e[y], add2(make_float2(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1])), make_float2(d.x, d.y)));
+          e[y + 1] = mul2(e[y + 1], add2(make_float2(__uint_as_float(s[2 * y + 2]), __uint_as_float(s[2 * y + 3])), make_float2(d.z, d.w)));
+        }
+        if (diagonal) {   // 0 times what is not finite
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            if (2 * y < from) e[y].x = 0.f;
+            if (2 * y + 1 < from) e[y].y = 0.f;
+          }
+        }
+#pragma unroll
+        for (int y = 0; y < 16; ++y) w16[y] = pack_pair<T>(e[y].x, e[y].y);
+        tc::tmem_st16(dp_at, w16);
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        __syncwarp();
+        tc::mbar_arrive(&bar.ds_ready, lane == 0);
+      }
+      if (ok) ok = waiter.wait(&bar.acc_full, outs & 1);
+      ++outs;
+      tc::tc_fence_after();
+      // a thread has half of its row of dv or of dk
+      const int i = w.tile * 128 + row;
+      const bool there = i < w.at.len;
+      const float by = !ok ? NAN : part < 2 ? 1.f : p.scale;
+      T* to = static_cast<T*>(part < 2 ? p.dv : p.dk) + ((w.at.row + i) * p.kv_heads + w.head) * p.dim;
+      const int col0 = (part & 1) * (DP / 2);
+#pragma unroll
+      for (int x = 0; x < DP / 2; x += 16) {
+        uint32_t raw[16];
+        float o[16];
+        tc::tmem_ld16(tmem + lane_base + (part >> 1) * 128 + col0 + x, raw);
         tc::tmem_wait_ld();
 #pragma unroll
         for (int y = 0; y < 16; ++y) o[y] = __uint_as_float(raw[y]);
@@ -376,7 +644,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
   }
 }
 
-// delta_i = do_i . o_i in 32 bits, 0 for the rows behind a sequence's end: a CTA has 256 rows of a head, half a warp a row
+// -delta_i = -do_i . o_i in 32 bits, 0 for the rows behind a sequence's end: a CTA has 64 rows of a head, half a warp a row
+constexpr int kDeltaRows = 64;
 struct DeltaParams {
   const void *out, *d_out;
   int64_t do_stride[3];
@@ -387,56 +656,64 @@ struct DeltaParams {
 
 template <typename T>
 __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ DeltaParams p) {
-  const int t = int(blockIdx.x) / p.heads, head = int(blockIdx.x) - t * p.heads;
-  const Item it = find_item(p.seq, t, false);
+  let_others_begin();
+  const int unit = int(blockIdx.x) / p.heads, head = int(blockIdx.x) - unit * p.heads;
+  const Item it = find_item(p.seq, unit / (kTileRows / kDeltaRows), false);
+  const int first = it.tile * kTileRows + unit % (kTileRows / kDeltaRows) * kDeltaRows;
   const int part = threadIdx.x & 15, group = threadIdx.x >> 4;
-  float* to = p.delta + head * p.seq.stat_rows + it.stat + it.tile * kTileRows;
-#pragma unroll 4
-  for (int r = group; r < kTileRows; r += 16) {
-    const int i = it.tile * kTileRows + r;
-    float sum = 0.f;
-    if (i < it.len && part * 8 < p.dim) {
-      const T* o = static_cast<const T*>(p.out) + ((it.row + i) * p.heads + head) * p.dim;
-      const T* d = static_cast<const T*>(p.d_out) + it.batch * p.do_stride[0] + int64_t(it.row0 + i) * p.do_stride[1] + head * p.do_stride[2];
-      const uint4 a = *reinterpret_cast<const uint4*>(o + part * 8), b = *reinterpret_cast<const uint4*>(d + part * 8);
-      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+  constexpr int kEach = kDeltaRows / 16;
+  uint4 a[kEach], b[kEach];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 x = unpack2<T>(aw[j]), y = unpack2<T>(bw[j]);
-        sum = fmaf(x.x, y.x, sum);
-        sum = fmaf(x.y, y.y, sum);
-      }
+  for (int x = 0; x < kEach; ++x) {
+    const int i = first + x * 16 + group;
+    a[x] = b[x] = make_uint4(0, 0, 0, 0);
+    if (i < it.len && part * 8 < p.dim) {
+      a[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + ((it.row + i) * p.heads + head) * p.dim + part * 8);
+      b[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.d_out) + it.batch * p.do_stride[0] + int64_t(it.row0 + i) * p.do_stride[1] +
+                                             head * p.do_stride[2] + part * 8);
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < kEach; ++x) {
+    const uint32_t aw[4] = {a[x].x, a[x].y, a[x].z, a[x].w}, bw[4] = {b[x].x, b[x].y, b[x].z, b[x].w};
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 u = unpack2<T>(aw[j]), v = unpack2<T>(bw[j]);
+      sum = fmaf(u.x, v.x, sum);
+      sum = fmaf(u.y, v.y, sum);
     }
 #pragma unroll
     for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (part == 0) to[r] = sum;
+    if (part == 0) p.delta[head * p.seq.stat_rows + it.stat + first + x * 16 + group] = -sum;
   }
 }
 
-template <typename T, int DP, bool kKeys>
-int launch_half(const BwdParams& base, cudaStream_t stream) {
-  using C = BwdConfig<DP>;
-  const void* kernel = reinterpret_cast<const void*>(&attention_backward_kernel<T, DP, kKeys>);
-  const cudaError_t err = ensure_dynamic_smem(kernel, C::kBytes);
+// One after the other, but a kernel begins on the SMs that the one before it has left: the key kernel waits for delta, and
+// nobody's results are read by the query kernel, which begins after that wait.
+template <typename Kernel>
+int launch_half(Kernel kernel, int bytes, const BwdParams& base, int64_t items, cudaStream_t stream) {
+  const cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), bytes);
   if (err != cudaSuccess) { record_cuda_error(err); return GDN2_ERR_LAUNCH; }
   int sms = 0;
   const int status = multiprocessors(&sms);
   if (status != GDN2_OK) return status;
   BwdParams p = base;
-  p.items = int64_t(p.seq.tiles) * 2 * (kKeys ? p.kv_heads : p.heads);
+  p.items = items;
   const int64_t grid = p.items < sms ? p.items : sms;
   p.turns = int((p.items + grid - 1) / grid);
-  attention_backward_kernel<T, DP, kKeys><<<unsigned(grid), kThreads, C::kBytes, stream>>>(p);
-  return check_launch();
+  return launch_beside(kernel, unsigned(grid), kThreads, bytes, stream, p);
 }
 
 template <typename T, int DP>
 int launch_typed(const BwdParams& p, const DeltaParams& d, cudaStream_t stream) {
-  attention_delta_kernel<T><<<unsigned(p.seq.tiles * p.heads), 256, 0, stream>>>(d);
+  attention_delta_kernel<T><<<unsigned(p.seq.tiles * (kTileRows / kDeltaRows) * p.heads), 256, 0, stream>>>(d);
   int status = check_launch();
   if (status != GDN2_OK) return status;
-  status = launch_half<T, DP, true>(p, stream);
-  return status != GDN2_OK ? status : launch_half<T, DP, false>(p, stream);
+  const int64_t tiles = int64_t(p.seq.tiles) * 2;
+  status = launch_half(&attention_keys_kernel<T, DP>, KeyConfig<DP>::kBytes, p, tiles * p.kv_heads, stream);
+  if (status != GDN2_OK) return status;
+  return launch_half(&attention_queries_kernel<T, DP>, QueryConfig<DP>::kBytes, p, tiles * p.heads, stream);
 }
 
 }  // namespace
@@ -450,10 +727,9 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   BwdParams p;
   const int64_t batch = bounds != nullptr ? 1 : n_seq;
   struct { CUtensorMap* map; const void* base; const int64_t* strides; int heads, rows; } maps[] = {
-      {&p.q_stay, q, strides, heads, 128},         {&p.k_stay, k, strides + 3, kv_heads, 128},
-      {&p.v_stay, v, strides + 6, kv_heads, 128},  {&p.do_stay, d_out, strides + 9, heads, 128},
-      {&p.q_go, q, strides, heads, kStep},         {&p.k_go, k, strides + 3, kv_heads, kStep},
-      {&p.v_go, v, strides + 6, kv_heads, kStep},  {&p.do_go, d_out, strides + 9, heads, kStep}};
+      {&p.q_tile, q, strides, heads, 128},         {&p.k_tile, k, strides + 3, kv_heads, 128},
+      {&p.v_tile, v, strides + 6, kv_heads, 128},  {&p.do_tile, d_out, strides + 9, heads, 128},
+      {&p.k_step, k, strides + 3, kv_heads, kStep}, {&p.v_step, v, strides + 6, kv_heads, kStep}};
   for (const auto& m : maps) {
     if (!encode_heads_map(m.map, m.base, m.strides, batch, time, m.heads, dim, dtype, m.rows)) return GDN2_ERR_LAUNCH;
   }

@@ -126,6 +126,27 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// 2^x of two numbers, none above 127, on the FMA units, which are idle where the special-function unit is what bounds a
+// phase.  Adding 1.5 * 2^23 rounds x to n, whose low bits are then those of the sum; f = x - n is in [-1/2, 1/2], where 2^f is
+// 1 + f p(f) with the cubic p that interpolates (2^f - 1) / f at the four Chebyshev nodes (relative error 7e-6, a weight's
+// rounding is 2^-9 or 2^-12); 2^n is made of its exponent.  Below -126.5 the result is 0; NaN stays NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  x.x = max_nan(x.x, -127.f);
+  x.y = max_nan(x.y, -127.f);
+  const float2 t = add2(x, twice(12582912.f));
+  const float2 f = minus2(x, add2(t, twice(-12582912.f)));
+  float2 r = fma2(f, twice(0.009656711f), twice(0.055838283f));
+  r = fma2(f, r, twice(0.2402253f));
+  r = fma2(f, r, twice(0.69313675f));
+  r = fma2(f, r, twice(1.f));
+  return mul2(r, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
+}
+
 // One tile of scores becomes weights, a row a thread: S (128 columns of TMEM at s_at) is read, masked, and overlaid by
 // P = exp2(S c - m c) in 16 bits.  m is the row's reference, a maximum of some tile so far (-inf: nothing but -inf has been
 // seen), `sum` the sum of its weights.  No tile but the first looks for its maximum: where the sum of its weights stays below

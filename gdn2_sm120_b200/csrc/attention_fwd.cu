@@ -32,7 +32,7 @@ struct FwdConfig {
 struct FwdParams {
   CUtensorMap q, k, v;
   void* out;
-  float* lse;          // [heads][stat rows] in powers of two, or null
+  float* lse;          // [heads][stat rows]: -(m + log2 l) in powers of two, or null
   int heads, kv_heads, group, dim, turns;
   int64_t items;
   float scale_log2;    // positive
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       const Item it = item_at(index, &head);
       const int n = key_tiles(it, t);
       if (n == 0) {
-        if (p.lse != nullptr) p.lse[head * p.seq.stat_rows + it.stat + (2 * it.tile + t) * 128 + row] = INFINITY;
+        if (p.lse != nullptr) p.lse[head * p.seq.stat_rows + it.stat + (2 * it.tile + t) * 128 + row] = -INFINITY;
         continue;
       }
       float m = -INFINITY;
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       // rows behind the end: a backward gives them weights exp2(0 - inf) = 0
       if (p.lse != nullptr) {
         p.lse[head * p.seq.stat_rows + it.stat + i] =
-            !there ? INFINITY : ok ? m * c + log2f(sum) : NAN;
+            !there ? -INFINITY : ok ? -(m * c + log2f(sum)) : NAN;
       }
     }
   }
