@@ -74,7 +74,7 @@ int gdn2_rotary(const void* q, const void* k, void* q_out, void* k_out, const fl
   if (batch <= 0 || time <= 0 || q_heads <= 0 || k_heads <= 0 || table <= 0) return GDN2_ERR_BAD_SHAPE;
   if (dim <= 0 || dim > 512 || dim % 2 != 0 || pairs <= 0 || 2 * pairs > dim) return GDN2_ERR_BAD_SHAPE;
   if (dtype != GDN2_BF16 && dtype != GDN2_FP16 && dtype != GDN2_FP32) return GDN2_ERR_BAD_DTYPE;
-  if (batch > kMost || time > kMost || q_heads > 65535 || k_heads > 65535) return GDN2_ERR_TOO_LARGE;
+  if (batch > kMost || time > kMost || batch * time > kMost || q_heads > 65535 || k_heads > 65535) return GDN2_ERR_TOO_LARGE;
   const void* need[] = {q, k, q_out, k_out};
   for (const void* p : need) {
     if (!aligned(p, uintptr_t(element_size(dtype)))) return GDN2_ERR_ALIGNMENT;

@@ -19,7 +19,7 @@ namespace attn {
 
 namespace {
 
-constexpr int kThreads = 384;    // warps 0-3, 4-7: the rows of the two tiles; 8: products; 9: copies; 10, 11: look at values
+constexpr int kThreads = 384;    // warps 0-3, 4-7: the rows of the two tiles; 8: products; 9: copies
 
 template <int DP>
 struct FwdConfig {
@@ -31,6 +31,8 @@ struct FwdConfig {
 
 struct FwdParams {
   CUtensorMap q, k, v;
+  const void *queries, *keys, *values;
+  int64_t strides[9];  // batch, token and head of each, in elements
   void* out;
   float* lse;          // [heads][stat rows]: -(m + log2 l) in powers of two, or null
   int heads, kv_heads, group, dim, turns;
@@ -49,6 +51,31 @@ struct FwdBars {
   uint32_t tmem;
   int failed;
 };
+
+// In the tile on the diagonal a row meets values that it does not see, with weights of 0; but 0 * inf and 0 * NaN are not 0.
+// A row that came out infinite or NaN looks whether such a value is behind it, and if so is made again without the tensor
+// cores, from the reference m and the sum that the scores alone have given.
+template <typename T>
+__device__ __noinline__ void row_again(const FwdParams& p, int64_t row0, int batch, int len, int head, int i, float m, float sum, T* to) {
+  const int kv_head = head / p.group;
+  const T* q = static_cast<const T*>(p.queries) + batch * p.strides[0] + (row0 + i) * p.strides[1] + head * p.strides[2];
+  const T* k = static_cast<const T*>(p.keys) + batch * p.strides[3] + row0 * p.strides[4] + kv_head * p.strides[5];
+  const T* v = static_cast<const T*>(p.values) + batch * p.strides[6] + row0 * p.strides[7] + kv_head * p.strides[8];
+  bool behind = false;
+  for (int j = i + 1; j < min(len, (i / 128 + 1) * 128) && !behind; ++j) {
+    for (int x = 0; x < p.dim; ++x) behind = behind || !isfinite(to_float(v[j * p.strides[7] + x]));
+  }
+  if (!behind) return;
+  float o[128];
+  for (int x = 0; x < p.dim; ++x) o[x] = 0.f;
+  for (int j = 0; j <= i; ++j) {
+    float s = 0.f;
+    for (int x = 0; x < p.dim; ++x) s = fmaf(to_float(q[x]), to_float(k[j * p.strides[4] + x]), s);
+    const float w = exp2_approx(((p.negate ? -s : s) - m) * p.scale_log2);
+    for (int x = 0; x < p.dim; ++x) o[x] = fmaf(w, to_float(v[j * p.strides[7] + x]), o[x]);
+  }
+  for (int x = 0; x < p.dim; ++x) to[x] = from_float<T>(o[x] / sum);
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __grid_constant__ FwdParams p) {
@@ -286,6 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       const bool there = i < it.len;
       const float inv = ok ? 1.f / sum : NAN;
       T* to = static_cast<T*>(p.out) + ((it.row + i) * p.heads + head) * p.dim;
+      float strange = 0.f;   // NaN if a channel is infinite or NaN
 #pragma unroll
       for (int x = 0; x < DP; x += 16) {
         uint32_t raw[16];
@@ -293,9 +321,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
         tc::tmem_ld16(o_at + x, raw);
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int y = 0; y < 16; ++y) o[y] = __uint_as_float(raw[y]);
+        for (int y = 0; y < 16; ++y) {
+          o[y] = __uint_as_float(raw[y]);
+          strange = fmaf(o[y], 0.f, strange);
+        }
         if (there) store_row16<T>(to + x, o, inv, p.dim - x, p.wide);
       }
+      if (strange != 0.f && there && ok && isfinite(sum)) row_again<T>(p, it.row0, it.batch, it.len, head, i, m, sum, to);
       tc::tc_fence_before();
       // rows behind the end: a backward gives them weights exp2(0 - inf) = 0
       if (p.lse != nullptr) {
@@ -340,6 +372,8 @@ int launch_attention_forward(const void* q, const void* k, const void* v, void* 
       !encode_heads_map(&p.v, v, strides + 6, batch, time, kv_heads, dim, dtype, 128)) {
     return GDN2_ERR_LAUNCH;
   }
+  p.queries = q; p.keys = k; p.values = v;
+  for (int i = 0; i < 9; ++i) p.strides[i] = strides[i];
   p.out = out; p.lse = lse;
   p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.dim = dim;
   // the sign goes to the product, and a scale of 0 stays a positive number, so that -inf * scale masks as ever

@@ -156,6 +156,31 @@ def test_packed_sequences_do_not_see_each_other(what):
             assert torch.equal(a[:, 100:165], b[:, 100:165])
 
 
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("time,at", [(300, 0), (300, 129), (300, 255), (300, 299), (70, 33), (600, 260)])
+def test_later_tokens_may_hold_anything(what, time, at):
+    """A token that is not finite reaches itself and the later ones, and no earlier one."""
+
+    q, k, v, _ = _inputs((1, time), 2, 1, 72, FP16, seed=at)
+    want = exact.attention(*(x[0].transpose(0, 1) for x in (q, k, v)), exact.causal(time, DEV), 72 ** -0.5)["o"]
+    for which in range(3):
+        inputs = [x.clone() for x in (q, k, v)]
+        inputs[which][0, at, :, 5] = what
+        out = causal_attention(*inputs)
+        exact.check("earlier", out[0, :at], *(x[:, :at] for x in want))
+        if which == 0:      # a query is its own
+            exact.check("later", out[0, at + 1:], *(x[:, at + 1:] for x in want))
+            assert torch.isnan(out[:, at]).all()
+        elif which == 1 and math.isnan(what):
+            assert torch.isnan(out[:, at:]).all()
+        elif which == 2:
+            assert not torch.isfinite(out[:, at:, :, 5]).any()
+            others = [c for c in range(72) if c != 5]
+            exact.check("other channels", out[0][..., others], *(x[..., others] for x in want))
+            if math.isnan(what):
+                assert torch.isnan(out[:, at:, :, 5]).all()
+
+
 def test_the_same_bits_every_time_alone_and_in_a_batch():
     q, k, v, do = _inputs((3, 333), 4, 2, 128, BF16, seed=6)
     first = _run(q, k, v, do)
