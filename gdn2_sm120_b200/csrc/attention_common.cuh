@@ -135,6 +135,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
   x.x = max_nan(x.x, -127.f);
   x.y = max_nan(x.y, -127.f);
@@ -249,6 +254,96 @@ __device__ __forceinline__ void store_row16(T* to, const float (&x)[16], float b
   if (channels > 8) *reinterpret_cast<uint4*>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 inline bool wide_rows(const void* base, int dim) { return dim % 16 == 0 && (reinterpret_cast<uintptr_t>(base) & 31) == 0; }
+
+// The same with two threads a row, 64 columns each (S at s_at, P over the first half of them, DP / 2 columns of O at o_at):
+// the latencies of a chain, and not its instructions, are what the tensor cores wait for.  All 256 threads of a chain look
+// again together.  A quarter of the weights is made on the FMA units; there a score that is 127 powers of two above the
+// reference counts as 127, and the row looks again.  8 x 4096 tokens, 16 heads (and one prompt of 16381, 8 heads): one thread
+// a row 517 us (472), two 476 (450), with the FMA units' quarter 474 (427).
+struct Pair {
+  int chain, half, row;
+  float (*told)[128];      // [half][row], what the two tell each other
+  __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, 256;" ::"r"(chain + 1) : "memory"); }
+  __device__ __forceinline__ float other(float mine) const {
+    told[half][row] = mine;
+    sync();
+    const float r = told[half ^ 1][row];
+    sync();
+    return r;
+  }
+  __device__ __forceinline__ bool any(bool x) const {   // of the chain
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %2, 0;\n\tbar.red.or.pred p, %1, 256, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(r) : "r"(chain + 1), "r"(uint32_t(x)) : "memory");
+    return r != 0;
+  }
+};
+
+template <typename T, int DP, typename Mask>
+__device__ __forceinline__ void soften_half(const Pair& pair, uint32_t s_at, uint32_t o_at, float c, bool first, float& m, float& sum,
+                                            Mask mask) {
+  uint32_t w[2][16];
+  float more = 0.f;
+#pragma unroll 1
+  for (bool look = first;;) {
+    if (look) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint32_t s[32];
+        tc::tmem_ld32(s_at + x * 32, s);
+        tc::tmem_wait_ld();
+        mask(x, s);
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int y = 0; y < 32; ++y) tops[y & 3] = fmaxf(tops[y & 3], __uint_as_float(s[y]));
+        top = fmaxf(top, fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+      }
+      top = fmaxf(top, pair.other(top));
+      if (first) {
+        m = top == -INFINITY ? 0.f : top;   // (any reference will do for a row that has seen nothing but -inf)
+      } else {
+        const float f = top > m ? exp2_approx((m - top) * c) : 1.f;
+        m = fmaxf(m, top);
+        sum *= f;
+#pragma unroll
+        for (int x = 0; x < DP / 2; x += 16) {
+          uint32_t o[16];
+          tc::tmem_ld16(o_at + x, o);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+          tc::tmem_st16(o_at + x, o);
+        }
+      }
+    }
+    const float2 minus = twice(-m * c), by = twice(c);
+    float2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};
+    uint32_t s[2][32];
+    tc::tmem_ld32(s_at, s[0]);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      tc::tmem_wait_ld();
+      if (x == 0) tc::tmem_ld32(s_at + 32, s[1]);
+      mask(x, s[x]);
+#pragma unroll
+      for (int y = 0; y < 16; ++y) {
+        const float2 z = fma2(make_float2(__uint_as_float(s[x][2 * y]), __uint_as_float(s[x][2 * y + 1])), by, minus);
+        const float2 e = (y & 3) == 3 ? exp2_fma(make_float2(min_nan(z.x, 127.f), min_nan(z.y, 127.f))) : exp2_2(z);
+        sums[y & 1] = add2(sums[y & 1], e);
+        w[x][y] = pack_pair<T>(e.x, e.y);   // the sum has them as they were, the product rounded
+      }
+    }
+    more = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+    if (look) break;    // no weight is above 1
+    look = pair.any(more > kGrowth);
+    if (!look) break;
+  }
+  sum += more;
+  tc::tmem_st16(s_at, w[0]);
+  tc::tmem_st16(s_at + 16, w[1]);
+  tc::tmem_wait_st();
+}
 
 // [batch][rows][heads][dim] with any strides that are multiples of 16 bytes, in boxes of 64 channels x box_rows rows
 // of one head.  Channels from dim on and rows behind a batch entry's last one arrive as zeros.

@@ -19,14 +19,14 @@ namespace attn {
 
 namespace {
 
-constexpr int kThreads = 384;    // warps 0-3, 4-7: the rows of the two tiles; 8: products; 9: copies
+constexpr int kThreads = 576;    // warps 0-7, 8-15: the rows of the two tiles; 16: products; 17: copies
 
 template <int DP>
 struct FwdConfig {
   static constexpr int kTileBytes = 128 * DP * 2;
   static constexpr int kSlab = 128 * 128;               // 64 channels of 128 rows
   static constexpr int kStages = DP == 128 ? 5 : 8;
-  static constexpr int kBytes = (2 + kStages) * kTileBytes + 512;
+  static constexpr int kBytes = (2 + kStages) * kTileBytes + 512 + 2 * 2 * 128 * 4;
 };
 
 struct FwdParams {
@@ -56,25 +56,26 @@ struct FwdBars {
 // A row that came out infinite or NaN looks whether such a value is behind it, and if so is made again without the tensor
 // cores, from the reference m and the sum that the scores alone have given.
 template <typename T>
-__device__ __noinline__ void row_again(const FwdParams& p, int64_t row0, int batch, int len, int head, int i, float m, float sum, T* to) {
+__device__ __noinline__ void row_again(const FwdParams& p, int64_t row0, int batch, int len, int head, int i, float m, float sum, T* to,
+                                       int first, int last) {
   const int kv_head = head / p.group;
   const T* q = static_cast<const T*>(p.queries) + batch * p.strides[0] + (row0 + i) * p.strides[1] + head * p.strides[2];
   const T* k = static_cast<const T*>(p.keys) + batch * p.strides[3] + row0 * p.strides[4] + kv_head * p.strides[5];
   const T* v = static_cast<const T*>(p.values) + batch * p.strides[6] + row0 * p.strides[7] + kv_head * p.strides[8];
   bool behind = false;
   for (int j = i + 1; j < min(len, (i / 128 + 1) * 128) && !behind; ++j) {
-    for (int x = 0; x < p.dim; ++x) behind = behind || !isfinite(to_float(v[j * p.strides[7] + x]));
+    for (int x = first; x < last; ++x) behind = behind || !isfinite(to_float(v[j * p.strides[7] + x]));
   }
   if (!behind) return;
-  float o[128];
-  for (int x = 0; x < p.dim; ++x) o[x] = 0.f;
+  float o[64];
+  for (int x = first; x < last; ++x) o[x - first] = 0.f;
   for (int j = 0; j <= i; ++j) {
     float s = 0.f;
     for (int x = 0; x < p.dim; ++x) s = fmaf(to_float(q[x]), to_float(k[j * p.strides[4] + x]), s);
     const float w = exp2_approx(((p.negate ? -s : s) - m) * p.scale_log2);
-    for (int x = 0; x < p.dim; ++x) o[x] = fmaf(w, to_float(v[j * p.strides[7] + x]), o[x]);
+    for (int x = first; x < last; ++x) o[x - first] = fmaf(w, to_float(v[j * p.strides[7] + x]), o[x - first]);
   }
-  for (int x = 0; x < p.dim; ++x) to[x] = from_float<T>(o[x] / sum);
+  for (int x = first; x < last; ++x) to[x] = from_float<T>(o[x - first] / sum);
 }
 
 template <typename T, int DP>
@@ -84,6 +85,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
   uint8_t* q_tiles = smem;
   uint8_t* kv_tiles = smem + 2 * C::kTileBytes;
   FwdBars& bar = *reinterpret_cast<FwdBars*>(smem + (2 + C::kStages) * C::kTileBytes);
+  float(*told)[2][128] = reinterpret_cast<float(*)[2][128]>(smem + (2 + C::kStages) * C::kTileBytes + 512);
+  static_assert(sizeof(FwdBars) <= 512, "");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -91,7 +94,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       tc::mbar_init(&bar.q_full[t], 1);
       tc::mbar_init(&bar.q_empty[t], 1);
       tc::mbar_init(&bar.s_full[t], 1);
-      tc::mbar_init(&bar.p_ready[t], 4);
+      tc::mbar_init(&bar.p_ready[t], 8);
       tc::mbar_init(&bar.o_full[t], 1);
     }
     tc::mbar_init(&bar.raw, 1);
@@ -103,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
     bar.failed = 0;
     tc::fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == 16) {
     tc::tmem_alloc(&bar.tmem, 512);
     tc::tmem_relinquish();
   }
@@ -124,8 +127,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
     return tile * 128 < it.len ? tile + 1 : 0;
   };
 
-  if (warp >= 8) {
-    if (warp == 9) {
+  if (warp >= 16) {
+    if (warp == 17) {
       // ---- copies ------------------------------------------------------------------------------------------
       const uint32_t leader = tc::elect_leader();
       int filled = 0, loaded[2] = {0, 0}, mended = 0;
@@ -201,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
           for (int i = 0; loaded[t] > 0 && i < 4096 && !tc::mbar_try_wait(&bar.q_full[t], (loaded[t] - 1) & 1); ++i) {}
         }
       }
-    } else if (warp == 8) {
+    } else if (warp == 16) {
       // ---- products ----------------------------------------------------------------------------------------
       const uint32_t leader = tc::elect_leader();
       const uint32_t id_s = tc::idesc(128, 128, Format<T>::code, tc::kMajorK, tc::kMajorK, p.negate);
@@ -249,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
               tc::tc_fence_after();
   #pragma unroll
               for (int ks = 0; ks < 8; ++ks) {
-                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, desc_mn(v_tile, C::kSlab, ks), id_o, j > 0 || ks > 0, leader);
+                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + (ks >> 2) * 64 + (ks & 3) * 8, desc_mn(v_tile, C::kSlab, ks), id_o, j > 0 || ks > 0, leader);
               }
               if (j + 1 == n_t[t]) tc::mma_commit(&bar.o_full[t], leader);
             }
@@ -272,9 +275,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
     }
   } else {
     // ---- weights: a row a thread ---------------------------------------------------------------------------
-    const int t = warp >> 2, row = threadIdx.x & 127;
+    const int t = warp >> 3, half = (warp >> 2) & 1, row = threadIdx.x & 127;
     const uint32_t lane_base = uint32_t(warp & 3) << 21;   // 32 lanes of TMEM, in bits 16 and up
-    const uint32_t s_at = tmem + lane_base + t * 128, o_at = tmem + lane_base + 256 + t * 128;
+    const uint32_t s_at = tmem + lane_base + t * 128 + half * 64, o_at = tmem + lane_base + 256 + t * 128 + half * (DP / 2);
+    const Pair pair{t, half, row, told[t]};
     const float c = p.scale_log2;
     int seen = 0, outs = 0;
     bool ok = true;
@@ -285,20 +289,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       const Item it = item_at(index, &head);
       const int n = key_tiles(it, t);
       if (n == 0) {
-        if (p.lse != nullptr) p.lse[head * p.seq.stat_rows + it.stat + (2 * it.tile + t) * 128 + row] = -INFINITY;
+        if (p.lse != nullptr && half == 0) p.lse[head * p.seq.stat_rows + it.stat + (2 * it.tile + t) * 128 + row] = -INFINITY;
         continue;
       }
-      float m = -INFINITY;
+      float m = 0.f;
       float sum = 0.f;
       for (int j = 0; j < n && ok; ++j) {
         if (!(ok = waiter.wait(&bar.s_full[t], seen & 1))) break;
         ++seen;
         tc::tc_fence_after();
-        soften<T, DP>(s_at, o_at, c, m, sum, [&](int x, uint32_t (&s)[32]) {
+        soften_half<T, DP>(pair, s_at, o_at, c, j == 0, m, sum, [&](int x, uint32_t (&s)[32]) {
           if (j + 1 == n) {   // the tile on the diagonal; what lies behind the sequence's end lies behind every row
 #pragma unroll
             for (int y = 0; y < 32; ++y) {
-              if (x * 32 + y > row) s[y] = 0xff800000u;
+              if (half * 64 + x * 32 + y > row) s[y] = 0xff800000u;
             }
           }
         });
@@ -309,13 +313,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       if (ok) ok = waiter.wait(&bar.o_full[t], outs & 1);
       ++outs;
       tc::tc_fence_after();
-      const int i = (2 * it.tile + t) * 128 + row;
+      sum += pair.other(sum);
+      const int i = (2 * it.tile + t) * 128 + row, col0 = half * (DP / 2);
       const bool there = i < it.len;
       const float inv = ok ? 1.f / sum : NAN;
       T* to = static_cast<T*>(p.out) + ((it.row + i) * p.heads + head) * p.dim;
       float strange = 0.f;   // NaN if a channel is infinite or NaN
 #pragma unroll
-      for (int x = 0; x < DP; x += 16) {
+      for (int x = 0; x < DP / 2; x += 16) {
         uint32_t raw[16];
         float o[16];
         tc::tmem_ld16(o_at + x, raw);
@@ -325,12 +330,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
           o[y] = __uint_as_float(raw[y]);
           strange = fmaf(o[y], 0.f, strange);
         }
-        if (there) store_row16<T>(to + x, o, inv, p.dim - x, p.wide);
+        if (there) store_row16<T>(to + col0 + x, o, inv, p.dim - col0 - x, p.wide);
       }
-      if (strange != 0.f && there && ok && isfinite(sum)) row_again<T>(p, it.row0, it.batch, it.len, head, i, m, sum, to);
+      if (strange != 0.f && there && ok && isfinite(sum)) row_again<T>(p, it.row0, it.batch, it.len, head, i, m, sum, to, col0, min(p.dim, col0 + DP / 2));
       tc::tc_fence_before();
       // rows behind the end: a backward gives them weights exp2(0 - inf) = 0
-      if (p.lse != nullptr) {
+      if (p.lse != nullptr && half == 0) {
         p.lse[head * p.seq.stat_rows + it.stat + i] =
             !there ? -INFINITY : ok ? -(m * c + log2f(sum)) : NAN;
       }
@@ -338,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }
