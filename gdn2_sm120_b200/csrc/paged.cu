@@ -20,10 +20,13 @@
 //                 whose part begins or ends inside a sequence leaves (O, m, l) in the workspace; tree_join_kernel joins
 //                 these in the order of the tiles: the same inputs give the same bits.
 //
-// A CTA: two chains of four warps turn scores into weights, a row a thread.  Up to 128 rows both work on the same rows,
-// on every other tile, and their (O, m, l) are joined at the end; above, each has 128 rows and all tiles.  Four warps
-// bring in rows with 16-byte asynchronous copies, since pages of any size make no box for a tiled copy; one issues the
-// products.  TMEM: S0 S1 O0 O1, 128 columns each, P over S.
+// A CTA of tree_kernel: two chains of four warps turn scores into weights, a row a thread.  Up to 128 rows both work on the
+// same rows, on every other tile, and their (O, m, l) are joined at the end; above, each has 128 rows and all tiles.  Four
+// warps bring in keys and values, in boxes of a tiled copy where the pages allow it and row by row with 16-byte asynchronous
+// copies elsewhere; one brings queries, one issues the products.  TMEM: S0 S1 O0 O1, 128 columns each, P over S.  48 drafted
+// tokens of 8 sequences over up to 16000 cached ones, 4 heads a group (192 rows): 110 us, 3.3 TB/s; what bounds it is a chain's
+// round trip between the tensor cores and its warps (the copies left out, 108 us of 142 remained; the weights left out, 116).
+// tree_few_kernel has up to 16 rows (below).
 
 #include <algorithm>
 
@@ -46,6 +49,7 @@ struct AppendParams {
   int per_head, per_token;                   // packs of a head, of a token
 };
 
+// 16411 tokens of 8 heads of 128, keys and values (121 MB both ways, half of it in L2): 18 us, 6.5 TB/s.
 template <typename P>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
   const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -364,18 +368,15 @@ __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int til
   }
 }
 
-// RT: tiles of 128 rows that a CTA has, 1 or 2; QR: rows of queries that a tile has in shared memory.  Where that is 32
-// the product reads on behind them: what its other rows are nobody looks at.
-template <int DP, int RT, int QR>
+template <int DP, int RT>   // RT: tiles of 128 rows that a CTA has, 1 or 2
 struct TreeConfig {
   static constexpr int kTileBytes = kTile * DP * 2;
   static constexpr int kSlab = kTile * 128;                    // 64 channels of 128 rows
   static constexpr int kRows = 128 * RT;
-  static constexpr int kQuerySlab = QR * 128, kQueryBytes = QR * DP * 2;
   // Queries of two units, so that the copies need not wait between two; those of 256 rows of 128 channels leave no room.
   static constexpr int kQueries = RT == 2 ? 1 : 2;
-  static constexpr int kStages = DP == 64 ? 8 : QR == 32 ? 6 : 5;
-  static constexpr int kBytes = RT * kQueries * kQueryBytes + kStages * kTileBytes + 768 + 2048;
+  static constexpr int kStages = DP == 64 ? 8 : 5;
+  static constexpr int kBytes = RT * kQueries * kTileBytes + kStages * kTileBytes + 768 + 2048;
 };
 
 struct TreeBars {
@@ -388,14 +389,14 @@ struct TreeBars {
 };
 static_assert(sizeof(TreeBars) <= 768, "");
 
-template <typename T, int DP, int RT, int QR>
+template <typename T, int DP, int RT>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ TreeParams p) {
-  using C = TreeConfig<DP, RT, QR>;
+  using C = TreeConfig<DP, RT>;
   extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
-  const uint32_t q_base = tc::smem_u32(smem), kv_base = q_base + RT * C::kQueries * C::kQueryBytes;
-  TreeBars& bar = *reinterpret_cast<TreeBars*>(smem + RT * C::kQueries * C::kQueryBytes + C::kStages * C::kTileBytes);
+  const uint32_t q_base = tc::smem_u32(smem), kv_base = q_base + RT * C::kQueries * C::kTileBytes;
+  TreeBars& bar = *reinterpret_cast<TreeBars*>(smem + RT * C::kQueries * C::kTileBytes + C::kStages * C::kTileBytes);
   // (m, l) of the rows of two chains
-  float2(*told)[128] = reinterpret_cast<float2(*)[128]>(smem + RT * C::kQueries * C::kQueryBytes + C::kStages * C::kTileBytes + 768);
+  float2(*told)[128] = reinterpret_cast<float2(*)[128]>(smem + RT * C::kQueries * C::kTileBytes + C::kStages * C::kTileBytes + 768);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -454,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       auto scores = [&](int t, int x) {   // S_t from the keys in stage x
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) {
-          attn::mma_ss(tmem + t * 128, attn::desc_k(q_base + (RT == 2 ? t : queries) * C::kQueryBytes, C::kQuerySlab, ks),
+          attn::mma_ss(tmem + t * 128, attn::desc_k(q_base + (RT == 2 ? t : queries) * C::kTileBytes, C::kSlab, ks),
                        attn::desc_k(kv_base + (x % C::kStages) * C::kTileBytes, C::kSlab, ks), id_s, ks > 0, leader);
         }
         tc::mma_commit(&bar.s_full[t], leader);
@@ -534,11 +535,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         const int n = min(rest, u.tiles - tile), place = units % C::kQueries;
         if (units >= C::kQueries && !waiter.wait(&bar.q_empty[place], (units / C::kQueries - 1) & 1)) break;
         ++units;
-        for (int x = 0; x < RT * QR; x += 32) {
+        for (int x = 0; x < RT * 128; x += 32) {
           const int r = u.block * C::kRows + x + lane;
           const int i = r / p.group, g = r - i * p.group;
           const T* at = static_cast<const T*>(p.q) + u.b * p.q_stride[0] + i * p.q_stride[1] + int64_t(u.head * p.group + g) * p.q_stride[2];
-          copy_rows<DP>(q_base + (RT == 2 ? (x / QR) * C::kQueryBytes : place * C::kQueryBytes), C::kQuerySlab, x % QR, p.dim, r < p.rows ? at : nullptr);
+          copy_rows<DP>(q_base + (RT == 2 ? x / 128 : place) * C::kTileBytes, C::kSlab, x % 128, p.dim, r < p.rows ? at : nullptr);
         }
         cp_async_arrive(&bar.q_full[place]);
         rest -= n;
@@ -686,8 +687,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------
-// Up to 16 rows (plain decoding, small trees of small groups): mma.sync m16n8k16, whose sums are in registers.  Eight warps
-// have 16 tokens of every tile each and go through them on their own; what they have of a unit is joined at its end.
+// Up to 16 rows (plain decoding, small trees of small groups): mma.sync m16n8k16, whose sums are in registers: no product has
+// more rows than there are, and no score goes through TMEM to a few lanes.  Eight warps have 16 tokens of every tile each and
+// go through them on their own; what they have of a unit is joined at its end.  Decoding 64 sequences of up to 8192 tokens,
+// 8 key heads: 217 us, 6.25 TB/s of the copy rate's 6.53.  (Copies by the computing warps themselves: 248 us.)
 constexpr int kFewThreads = 384;   // warps 0-7: 16 tokens of every tile each; 8-11: copies
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
@@ -998,6 +1001,8 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
   for (int y = 0; y < kOwn; y += 2) *reinterpret_cast<uint32_t*>(to + y) = pack_pair<T>(acc[y] * inv, acc[y + 1] * inv);
 }
 
+// Where tree_few_kernel is taken: all the rows that one of its products has.  4 drafted tokens, 4 heads a group (16 rows): 4
+// sequences of 500 tokens 19 us, with tree_kernel 28; 32 of 8192 142 us, 146.
 constexpr int kFewRows = 16;
 // rows of a block
 int block_rows(int64_t rows) { return rows <= kFewRows ? kFewRows : rows <= 128 ? 128 : 256; }
@@ -1022,13 +1027,13 @@ int launch_few(const TreeParams& p, cudaStream_t stream) {
   return status != GDN2_OK ? status : launch_join<T, DP>(p, kFewRows, stream);
 }
 
-template <typename T, int DP, int RT, int QR>
+template <typename T, int DP, int RT>
 int launch_tree_typed(const TreeParams& p, cudaStream_t stream) {
-  using C = TreeConfig<DP, RT, QR>;
-  const void* kernel = reinterpret_cast<const void*>(&tree_kernel<T, DP, RT, QR>);
+  using C = TreeConfig<DP, RT>;
+  const void* kernel = reinterpret_cast<const void*>(&tree_kernel<T, DP, RT>);
   const cudaError_t err = ensure_dynamic_smem(kernel, C::kBytes);
   if (err != cudaSuccess) { record_cuda_error(err); return GDN2_ERR_LAUNCH; }
-  tree_kernel<T, DP, RT, QR><<<unsigned(p.ctas), kThreads, C::kBytes, stream>>>(p);
+  tree_kernel<T, DP, RT><<<unsigned(p.ctas), kThreads, C::kBytes, stream>>>(p);
   const int status = check_launch();
   return status != GDN2_OK ? status : launch_join<T, DP>(p, C::kRows, stream);
 }
@@ -1036,11 +1041,8 @@ int launch_tree_typed(const TreeParams& p, cudaStream_t stream) {
 template <typename T>
 int launch_tree_dim(const TreeParams& p, cudaStream_t stream) {
   if (p.rows <= kFewRows) return p.dim <= 64 ? launch_few<T, 64>(p, stream) : launch_few<T, 128>(p, stream);
-  if (p.dim <= 64) {
-    return p.rows <= 128 ? launch_tree_typed<T, 64, 1, 128>(p, stream) : launch_tree_typed<T, 64, 2, 128>(p, stream);
-  }
-  return p.rows <= 32 ? launch_tree_typed<T, 128, 1, 32>(p, stream)
-                      : p.rows <= 128 ? launch_tree_typed<T, 128, 1, 128>(p, stream) : launch_tree_typed<T, 128, 2, 128>(p, stream);
+  if (p.dim <= 64) return p.rows <= 128 ? launch_tree_typed<T, 64, 1>(p, stream) : launch_tree_typed<T, 64, 2>(p, stream);
+  return p.rows <= 128 ? launch_tree_typed<T, 128, 1>(p, stream) : launch_tree_typed<T, 128, 2>(p, stream);
 }
 
 }  // namespace
@@ -1091,7 +1093,8 @@ int launch_tree(const void* q, const void* k, const void* v, const void* k_pages
   p.dim = dim; p.page = page; p.columns = columns;
   p.rows = drafted * p.group;
   // Whole boxes of tiled copies come out of a page only where it has 8 or 16 rows, or a multiple of 32; pages of other
-  // sizes, and tiles that a sequence ends in, are copied row by row.
+  // sizes, and tiles that a sequence ends in, are copied row by row.  Decoding as above, pages of 64: 238 us with boxes,
+  // 254 row by row; of 16 238 and 240.
   p.box = page % 32 == 0 ? 32 : page == 16 || page == 8 ? page : 0;
   if (p.box > 0) {
     const int64_t page_strides[3] = {int64_t(page) * kv_heads * dim, int64_t(kv_heads) * dim, dim};
