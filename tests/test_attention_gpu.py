@@ -109,6 +109,20 @@ def test_maxima_that_move_far(rising):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("height", [20.0, 60.0, 400.0])
+def test_single_scores_far_above_all_others(dtype, height):
+    """Weights against the reference of earlier tiles would leave the 16-bit types' range, or the 32-bit one's."""
+
+    time, dim = 520, 64
+    q, k, v, do = _inputs((1, time), 2, 1, dim, dtype, seed=11)
+    q[..., 0], k[..., 0] = 4.0, 0.0
+    for at, share in ((3, 0.25), (140, 0.5), (300, 0.75), (301, 0.75), (511, 1.0)):
+        k[0, at, 0, 0] = height * share / 4.0
+    got = _run(q, k, v, do, scale=1.0)
+    _check_sequence([x[0] for x in got], q[0], k[0], v[0], do[0], 1.0, f"height {height}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_views_of_one_projection_and_gradients_of_views(dtype):
     batch, time, heads, kv_heads, dim = 2, 150, 4, 2, 64
     gen = torch.Generator(device=DEV).manual_seed(1)
@@ -230,6 +244,30 @@ def test_another_stream_and_a_captured_graph():
     q.mul_(0.5)
     graph.replay()
     assert torch.equal(out, causal_attention(q, k, v))
+
+
+def test_a_captured_training_step():
+    q, k, v, do = _inputs((1, 400), 4, 2, 64, BF16, seed=13)
+    bounds = (0, 150, 151, 400)
+    _run(q, k, v, do, bounds)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):      # autograd's own first step
+        torch.autograd.grad(causal_attention_varlen(*leaves, bounds), leaves, do)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = causal_attention_varlen(*leaves, bounds)
+        grads = torch.autograd.grad(out, leaves, do)
+    for seed in (14, 15):
+        new = _inputs((1, 400), 4, 2, 64, BF16, seed=seed)
+        with torch.no_grad():
+            for x, y in zip((*leaves, do), new):
+                x.copy_(y)
+        graph.replay()
+        want = _run(*new[:3], new[3], bounds)
+        assert all(torch.equal(a, b) for a, b in zip((out.detach(), *grads), want))
 
 
 def test_no_tokens():

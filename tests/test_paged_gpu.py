@@ -86,6 +86,23 @@ def test_trees_over_a_cache(dtype, lengths, page, drafted, heads, kv_heads, dim)
     assert torch.equal(plain, tree_attention(q, k, v, *cache, chain))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("drafted,heads", [(2, 4), (20, 4), (40, 16)])
+@pytest.mark.parametrize("height", [20.0, 400.0])
+def test_single_scores_far_above_all_others(dtype, drafted, heads, height):
+    """In the cache and among the drafts, in tiles of either chain: 4, 40 and 320 rows of a key head."""
+
+    cache = _cache((900,), 16, 2, 64, dtype)
+    q, k, v = _fresh(1, drafted, heads, 2, 64, dtype)
+    q[..., 0], k[..., 0] = 4.0, 0.0
+    cache[0][..., 0] = 0.0
+    for at, share in ((100, 0.25), (200, 0.4), (513, 0.6), (890, 0.8)):
+        cache[0][cache[2][0, at // 16].long(), at % 16, :, 0] = height * share / 4.0
+    k[:, drafted - 1, :, 0] = height / 4.0
+    mask = _tree(1, drafted)
+    _check(tree_attention(q, k, v, *cache, mask, scale=1.0), q, k, v, cache, mask, 1.0)
+
+
 def test_many_sequences_and_a_long_one():
     lengths = [(37 * i) % 200 for i in range(300)] + [30011]
     cache = _cache(lengths, 16, 1, 64, BF16)
