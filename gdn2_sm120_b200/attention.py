@@ -100,11 +100,15 @@ class _CausalAttention(torch.autograd.Function):
             d_out = d_out.clone(memory_format=torch.contiguous_format)
         host, n_seq, rows = _sequences(q, ctx.bounds)
         strides = _lib.int64s(*(s for x in (q, k, v, d_out) for s in _validate.head_strides(x)))
-        scratch = torch.empty_like(statistics)
+        with torch.cuda.device(q.device):
+            size = _lib.lib().gdn2_attention_backward_bytes(host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3])
+        if size < 0:
+            _lib.check(int(size), "gdn2_attention_backward_bytes")
+        scratch = torch.empty(size, device=q.device, dtype=torch.uint8)
         _lib.call("gdn2_attention_backward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                   d_out.data_ptr(), statistics.data_ptr(), scratch.data_ptr(), *(x.data_ptr() for x in grads), strides,
                   host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], _lib.dtype_code(q.dtype), scale,
-                  _lib.stream_ptr(q.device), kernels=3 * _launches(ctx.bounds))
+                  _lib.stream_ptr(q.device), kernels=(3 + (size > 4 * statistics.numel() + 15)) * _launches(ctx.bounds))
         return (*grads, None, None)
 
 

@@ -18,7 +18,8 @@ namespace attn {
 int64_t attention_stat_rows(const int64_t*, int64_t, int64_t);
 int launch_attention_forward(const void*, const void*, const void*, void*, float*, const int64_t*, const int64_t*, int64_t,
                              int64_t, int, int, int, int, float, cudaStream_t);
-int launch_attention_backward(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*,
+int64_t attention_backward_bytes(const int64_t*, int64_t, int64_t, int, int, int);
+int launch_attention_backward(const void*, const void*, const void*, const void*, const void*, const float*, void*, void*,
                               void*, void*, const int64_t*, const int64_t*, int64_t, int64_t, int, int, int, int, float,
                               cudaStream_t);
 }  // namespace attn
@@ -155,8 +156,15 @@ int gdn2_attention_forward(const void* q, const void* k, const void* v, void* ou
                                         int(dim), dtype, scale, static_cast<cudaStream_t>(stream));
 }
 
+int64_t gdn2_attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads,
+                                      int64_t dim) {
+  int status = check_heads(heads, kv_heads, dim);
+  if (status == GDN2_OK) status = check_sequences(bounds, n_seq, time, heads);
+  return status != GDN2_OK ? status : attn::attention_backward_bytes(bounds, n_seq, time, int(heads), int(kv_heads), int(dim));
+}
+
 int gdn2_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out,
-                            const float* statistics, float* scratch, void* dq, void* dk, void* dv, const int64_t* strides,
+                            const float* statistics, void* scratch, void* dq, void* dk, void* dv, const int64_t* strides,
                             const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads, int64_t dim,
                             int dtype, float scale, void* stream) {
   if (!q || !k || !v || !out || !d_out || !statistics || !scratch || !dq || !dk || !dv || !strides) {

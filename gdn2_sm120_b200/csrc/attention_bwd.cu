@@ -14,6 +14,8 @@
 //
 // Training 4 x 2048 tokens, 16 heads of 128 channels, 4 heads a group: delta 12 us, keys 129, queries 116, forward 85.
 
+#include <algorithm>
+
 #include "attention_common.cuh"
 
 namespace gdn2 {
@@ -40,6 +42,9 @@ struct BwdParams {
   CUtensorMap q_tile, do_tile, k_tile, v_tile, k_step, v_step;   // 128 rows, 64 rows
   void *dq, *dk, *dv;
   const float *lse, *delta;  // -(m + log2 l) in powers of two, -delta
+  float* partials;           // dk and dv of the parts of an item, [part][dk, dv][row][kv head][dim]
+  int64_t partial_rows;      // rows * kv heads
+  int parts;                 // of an item of the key kernel
   int heads, kv_heads, group, dim, turns;
   int64_t items;
   float scale, scale_log2;   // scale_log2 is positive
@@ -58,23 +63,29 @@ struct QueryBars {
 struct BwdItem {
   Item at;
   int head, tile;       // of queries, or of keys; 128-row tile in the sequence
-  int first, per_head, steps;  // keys: first 128-row step, steps of a query head, of all; queries: 64-row steps
+  int first, per_head, steps;  // keys: first 128-row step, steps of a query head, of this part; queries: 64-row steps
+  int part, begin;             // keys: which part, its first step of the item's
 };
+
+// the first step of a part of an item of the key kernel
+__device__ __forceinline__ int part_begin(int steps, int part, int parts) { return int(int64_t(steps) * part / parts); }
 
 template <bool kKeys>
 __device__ __forceinline__ bool bwd_item(const BwdParams& p, int turn, BwdItem* w) {
   const int64_t index = item_of_turn(turn);
   if (index >= p.items) return false;
-  const int heads = kKeys ? p.kv_heads : p.heads;
-  const int u = int(index / heads);
-  w->head = int(index - int64_t(u) * heads);
+  const int parts = kKeys ? p.parts : 1, heads = (kKeys ? p.kv_heads : p.heads) * parts;
+  const int u = int(index / heads), in_tile = int(index - int64_t(u) * heads);
+  w->head = in_tile / parts;
+  w->part = in_tile - w->head * parts;
   w->at = find_item(p.seq, u >> 1, !kKeys);
   w->tile = 2 * w->at.tile + (kKeys ? u & 1 : 1 - (u & 1));
   if (w->tile * 128 >= w->at.len) return false;
   w->first = kKeys ? w->tile : 0;
   w->per_head = kKeys ? (w->at.len + 127) / 128 - w->tile : min(2 * w->tile + 2, (w->at.len + kStep - 1) / kStep);
-  w->steps = kKeys ? w->per_head * p.group : w->per_head;
-  return true;
+  w->begin = kKeys ? part_begin(w->per_head * p.group, w->part, parts) : 0;
+  w->steps = kKeys ? part_begin(w->per_head * p.group, w->part + 1, parts) - w->begin : w->per_head;
+  return w->steps > 0;
 }
 
 template <typename T, int DP>
@@ -430,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
         }
         ++stayed;
         for (int i = 0; i < 2 * w.steps && ok; ++i) {   // q and do by turns
-          const int s = filled % C::kStages, step = i >> 1;
+          const int s = filled % C::kStages, step = w.begin + (i >> 1);
           if (filled >= C::kStages && !(ok = waiter.wait(&bar.go_empty[s], (filled / C::kStages - 1) & 1))) break;
           const int g = step / w.per_head, at = (w.first + step - g * w.per_head) * 128;
           const int head = w.head * p.group + g;
@@ -554,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
     for (int turn = 0; turn < p.turns; ++turn) {
       BwdItem w;
       if (!bwd_item<true>(p, turn, &w)) continue;
-      int in_head = 0;
+      int in_head = w.begin % w.per_head;
       for (int i = 0; i < w.steps && ok; ++i, ++steps) {
         const float* st = stats + steps % C::kStats * 2 * 128 + part * 32;
         // queries see keys up to themselves; a head's first step is the one on the diagonal
@@ -623,7 +634,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
       const int i = w.tile * 128 + row;
       const bool there = i < w.at.len;
       const float by = !ok ? NAN : part < 2 ? 1.f : p.scale;
-      T* to = static_cast<T*>(part < 2 ? p.dv : p.dk) + ((w.at.row + i) * p.kv_heads + w.head) * p.dim;
+      const int64_t out_row = (w.at.row + i) * p.kv_heads + w.head;
+      T* to = static_cast<T*>(part < 2 ? p.dv : p.dk) + out_row * p.dim;
+      float* partial = p.partials + ((2 * w.part + (part < 2)) * p.partial_rows + out_row) * p.dim;
       const int col0 = (part & 1) * (DP / 2);
 #pragma unroll
       for (int x = 0; x < DP / 2; x += 16) {
@@ -633,7 +646,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
         tc::tmem_wait_ld();
 #pragma unroll
         for (int y = 0; y < 16; ++y) o[y] = __uint_as_float(raw[y]);
-        if (there) store_row16<T>(to + col0 + x, o, by, p.dim - col0 - x, p.wide);
+        if (!there) continue;
+        if (p.parts == 1) {
+          store_row16<T>(to + col0 + x, o, by, p.dim - col0 - x, p.wide);
+        } else {
+#pragma unroll
+          for (int y = 0; y < 16; y += 4) {
+            if (col0 + x + y < p.dim) *reinterpret_cast<float4*>(partial + col0 + x + y) = make_float4(o[y] * by, o[y + 1] * by, o[y + 2] * by, o[y + 3] * by);
+          }
+        }
       }
       tc::tc_fence_before();
       __syncwarp();
@@ -693,6 +714,31 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
   }
 }
 
+// Where single items of the keys would take longer than all the rest (key_parts), each is cut into parts that sum over some
+// of its steps (heads and queries) and leave their sums in 32 bits; these are added up here in the order of the parts, four
+// channels a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) attention_parts_kernel(const __grid_constant__ BwdParams p) {
+  const int pieces = p.dim / 4;
+  const int64_t x = int64_t(blockIdx.y) * blockDim.x + threadIdx.x;   // (row of the tile, kv head, piece)
+  const Item it = find_item(p.seq, int(blockIdx.x) >> 1, false);
+  const int tile = 2 * it.tile + (int(blockIdx.x) & 1);
+  const int i = tile * 128 + int(x / (p.kv_heads * pieces));
+  if (i >= it.len || x >= int64_t(128) * p.kv_heads * pieces) return;
+  const int64_t at = ((it.row + tile * 128) * p.kv_heads * pieces + x) * 4;
+  const int steps = ((it.len + 127) / 128 - tile) * p.group;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {   // dk, dv
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int part = 0; part < p.parts; ++part) {
+      if (part_begin(steps, part, p.parts) == part_begin(steps, part + 1, p.parts)) continue;
+      const float4 y = *reinterpret_cast<const float4*>(p.partials + (2 * part + which) * p.partial_rows * p.dim + at);
+      sum.x += y.x; sum.y += y.y; sum.z += y.z; sum.w += y.w;
+    }
+    *reinterpret_cast<uint2*>(static_cast<T*>(which ? p.dv : p.dk) + at) = make_uint2(pack_pair<T>(sum.x, sum.y), pack_pair<T>(sum.z, sum.w));
+  }
+}
+
 // One after the other, but a kernel begins on the SMs that the one before it has left: the key kernel waits for delta, and
 // nobody's results are read by the query kernel, which begins after that wait.
 template <typename Kernel>
@@ -715,17 +761,49 @@ int launch_typed(const BwdParams& p, const DeltaParams& d, cudaStream_t stream) 
   int status = check_launch();
   if (status != GDN2_OK) return status;
   const int64_t tiles = int64_t(p.seq.tiles) * 2;
-  status = launch_half(&attention_keys_kernel<T, DP>, KeyConfig<DP>::kBytes, p, tiles * p.kv_heads, stream);
+  status = launch_half(&attention_keys_kernel<T, DP>, KeyConfig<DP>::kBytes, p, tiles * p.kv_heads * p.parts, stream);
   if (status != GDN2_OK) return status;
-  return launch_half(&attention_queries_kernel<T, DP>, QueryConfig<DP>::kBytes, p, tiles * p.heads, stream);
+  status = launch_half(&attention_queries_kernel<T, DP>, QueryConfig<DP>::kBytes, p, tiles * p.heads, stream);
+  if (status != GDN2_OK || p.parts == 1) return status;
+  const int64_t threads = int64_t(128) * p.kv_heads * (p.dim / 4);
+  attention_parts_kernel<T><<<dim3(unsigned(tiles), unsigned((threads + 255) / 256)), 256, 0, stream>>>(p);
+  return check_launch();
 }
 
 }  // namespace
 
+// Parts of the key kernel's items.  The first tile of the longest sequence has the most steps, and the other SMs have the
+// rest of the keys and then the queries, about as many steps again, to do meanwhile: parts as many as bring it down to an
+// SM's share of both.  16 heads; whole items / parts: 1 x 2048 tokens, 2 key heads (128 steps, a share of 29) 259 / 134 us;
+// packed 700, 1200, 300 tokens, 2 key heads (80, 18) 173 / 128; 2 x 2048, 4 key heads (64, 118) 178 / 188; below sixteen
+// steps, 1 x 1000 tokens, 8 heads (8, 4) 122 / 126.
+static int key_parts(const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, int sms) {
+  const int group = heads / kv_heads;
+  int64_t longest = 0, all = 0;
+  for (int64_t i = 0; i < (bounds != nullptr ? n_seq : 1); ++i) {
+    const int64_t tiles = ((bounds != nullptr ? bounds[i + 1] - bounds[i] : time) + 127) / 128;
+    longest = std::max(longest, tiles * group);
+    all += tiles * (tiles + 1) / 2 * heads;
+  }
+  if (bounds == nullptr) all *= n_seq;
+  const int64_t share = std::max<int64_t>(1, 2 * all / sms);
+  return longest < 16 ? 1 : int(std::max<int64_t>(1, longest / share));
+}
+
+// delta, then the parts' sums
+int64_t attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, int dim) {
+  int sms = 0;
+  const int status = multiprocessors(&sms);
+  if (status != GDN2_OK) return status;
+  const int64_t delta = (stat_rows(bounds, n_seq, time) * heads * 4 + 15) / 16 * 16;
+  const int parts = key_parts(bounds, n_seq, time, heads, kv_heads, sms);
+  return delta + (parts == 1 ? 0 : int64_t(parts) * 2 * (bounds != nullptr ? time : n_seq * time) * kv_heads * dim * 4);
+}
+
 int64_t attention_stat_rows(const int64_t* bounds, int64_t n_seq, int64_t time) { return stat_rows(bounds, n_seq, time); }
 
 int launch_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out,
-                              const float* lse, float* delta, void* dq, void* dk, void* dv, const int64_t* strides,
+                              const float* lse, void* scratch, void* dq, void* dk, void* dv, const int64_t* strides,
                               const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, int dim,
                               int dtype, float scale, cudaStream_t stream) {
   BwdParams p;
@@ -738,7 +816,14 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
     if (!encode_heads_map(m.map, m.base, m.strides, batch, time, m.heads, dim, dtype, m.rows)) return GDN2_ERR_LAUNCH;
   }
   p.dq = dq; p.dk = dk; p.dv = dv;
+  float* delta = static_cast<float*>(scratch);
   p.lse = lse; p.delta = delta;
+  int sms = 0;
+  const int status = multiprocessors(&sms);
+  if (status != GDN2_OK) return status;
+  p.parts = key_parts(bounds, n_seq, time, heads, kv_heads, sms);
+  p.partials = delta + (stat_rows(bounds, n_seq, time) * heads + 3) / 4 * 4;
+  p.partial_rows = batch * time * kv_heads;
   p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.dim = dim;
   p.scale = scale;
   p.negate = scale < 0.f;

@@ -45,6 +45,7 @@ struct Api {
   decltype(&gdn2_tree_attention) tree_attention;
   decltype(&gdn2_attention_stat_rows) attention_stat_rows;
   decltype(&gdn2_attention_forward) attention_forward;
+  decltype(&gdn2_attention_backward_bytes) attention_backward_bytes;
   decltype(&gdn2_attention_backward) attention_backward;
 } api;
 PyObject* g_check = nullptr;     // _lib.check(status, name): raises
@@ -836,14 +837,20 @@ PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int status;
   WithoutGil others;
   const c10::cuda::CUDAGuard guard(q.device());
+  const int64_t size = api.attention_backward_bytes(host, n_seq, h.time, h.heads, h.kv_heads, h.dim);
+  if (size < 0) {
+    others.end();
+    return none();
+  }
   for (int i = 0; i < 3; ++i) grads[i] = at::empty(h.t[i]->sizes(), q.options());
-  const at::Tensor scratch = at::empty(statistics->sizes(), statistics->options());
+  const at::Tensor scratch = bytes(size, q);
   status = api.attention_backward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out->data_ptr(), d_out->data_ptr(),
-                                  fptr(statistics), fptr(&scratch), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(),
+                                  fptr(statistics), scratch.data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(),
                                   h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim, h.dtype, scale,
                                   at::cuda::getCurrentCUDAStream().stream());
   others.end();
-  if (!ok(status, "gdn2_attention_backward", 3 * passes(bounds))) return nullptr;
+  const bool parts = size > 4 * statistics->numel() + 15;   // sums of several CTAs are added up
+  if (!ok(status, "gdn2_attention_backward", (parts ? 4 : 3) * passes(bounds))) return nullptr;
   PyObject* result = PyTuple_New(3);
   for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(result, i, wrap(grads[i]));
   return result;
@@ -884,6 +891,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_BIND(tree_attention);
   GDN2_BIND(attention_stat_rows);
   GDN2_BIND(attention_forward);
+  GDN2_BIND(attention_backward_bytes);
   GDN2_BIND(attention_backward);
 #undef GDN2_BIND
   if (missing) {

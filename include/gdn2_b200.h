@@ -494,12 +494,15 @@ int gdn2_attention_forward(const void* q, const void* k, const void* v, void* ou
                            void* stream);
 
 /*
- * Its gradients.  out and statistics are the forward's; dq, dk, dv contiguous; scratch has the size of
- * statistics.  strides: batch, token and head of q, k, v, d_out.  No atomics: the same inputs give the same
- * bits.
+ * Its gradients.  out and statistics are the forward's; dq, dk, dv contiguous; scratch has
+ * gdn2_attention_backward_bytes (a negative status if the sizes are wrong; the device is the current one)
+ * and is dead when the call's kernels have run.  strides: batch, token and head of q, k, v, d_out.  No
+ * atomics: the same inputs give the same bits.
  */
+int64_t gdn2_attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads,
+                                      int64_t kv_heads, int64_t dim);
 int gdn2_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out,
-                            const float* statistics, float* scratch, void* dq, void* dk, void* dv,
+                            const float* statistics, void* scratch, void* dq, void* dk, void* dv,
                             const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time,
                             int64_t heads, int64_t kv_heads, int64_t dim, int dtype, float scale,
                             void* stream);

@@ -72,6 +72,23 @@ def test_packed_forward_and_gradients(dtype, lengths, heads, kv_heads, dim):
                             f"rows {lo} to {hi}")
 
 
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim", [((700,), 8, 1, 64), ((1300,), 6, 2, 40), ((600, 30, 1, 513), 12, 1, 128)])
+def test_key_gradients_summed_by_several_ctas(lengths, heads, kv_heads, dim):
+    """Few sequences and key heads, large groups: the sums of a key's gradients are cut into parts."""
+
+    bounds = [0]
+    for n in lengths:
+        bounds.append(bounds[-1] + n)
+    q, k, v, do = _inputs((1, bounds[-1]), heads, kv_heads, dim, BF16, seed=17)
+    got = _run(q, k, v, do, bounds)
+    for lo, hi in zip(bounds, bounds[1:]):
+        part = slice(lo, hi)
+        _check_sequence([x[0, part] for x in got], q[0, part], k[0, part], v[0, part], do[0, part], dim ** -0.5, f"rows {lo} to {hi}")
+    assert all(torch.equal(a, b) for a, b in zip(got, _run(q, k, v, do, bounds)))
+    if len(lengths) == 1:
+        assert all(torch.equal(a, b) for a, b in zip(got, _run(q, k, v, do)))
+
+
 def test_more_sequences_than_a_launch_holds():
     lengths = [(7 * i) % 61 for i in range(600)]
     bounds = [0]
