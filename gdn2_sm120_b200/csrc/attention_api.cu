@@ -120,7 +120,8 @@ int gdn2_tree_attention(const void* q, const void* k, const void* v, const void*
   if (status != GDN2_OK) return status;
   if (batch <= 0 || drafted <= 0 || pages <= 0 || page <= 0 || columns < 0) return GDN2_ERR_BAD_SHAPE;
   if (!valid_seq_dtype(dtype)) return GDN2_ERR_BAD_DTYPE;
-  if (batch > kMost || drafted > kMost / heads || pages > kMost || page > kMost || columns > kMost / page - 64 / page - 1) {
+  // a sequence's tokens, cached and drafted, are numbered with 31 bits
+  if (batch > kMost || drafted > kMost / 2 / heads || pages > kMost || page > kMost || columns > (kMost / 2 - 128) / page) {
     return GDN2_ERR_TOO_LARGE;
   }
   if ((status = check_strides(strides, 9)) != GDN2_OK) return status;
