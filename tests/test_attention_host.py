@@ -95,3 +95,17 @@ def test_entry_points_check_their_arguments():
     assert tree(table=None) == -1 and tree(drafted=0) == -2 and tree(dim=12) == -2 and tree(workspace=at + 4) == -5
     assert tree(page=2 ** 20, columns=2 ** 12) == -9
     assert handle.gdn2_tree_workspace_bytes(1, 3, 2, 64) == -2
+
+
+def test_tree_attention_refuses_more_tokens_than_31_bits_number():
+    handle, buffer = _lib.lib(), (ctypes.c_char * 4096)()
+    at = (ctypes.addressof(buffer) + 63) // 64 * 64
+    strides = _lib.int64s(*([64] * 9))
+
+    def tree(drafted, columns):
+        return handle.gdn2_tree_attention(at, at, at, at, at, at, at, None, at, at, strides, 1, 0, 1, drafted, 2, 1, 64, 1, 16, columns, 0,
+                                          1.0, None)
+
+    # each side alone would fit an int, both together would not
+    assert tree(drafted=2 ** 29, columns=2 ** 26) == -9
+    assert tree(drafted=1, columns=2 ** 26) == -9 and tree(drafted=2 ** 30, columns=1) == -9
