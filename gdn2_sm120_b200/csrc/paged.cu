@@ -954,7 +954,6 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
 template <typename T, int DP>
 __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ TreeParams p, int block_rows, int ctas_of_unit) {
   __shared__ int64_t scan[kJoinThreads / 32];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int unit = int(blockIdx.x) / ctas_of_unit;
   const int block = unit % p.row_blocks, head = unit / p.row_blocks % p.kv_heads, b = unit / p.row_blocks / p.kv_heads;
   int64_t total = 0, from = 0, before;
@@ -968,6 +967,8 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
   read_length(p, u);
   const int64_t t0 = from + (int64_t(head) * p.row_blocks + block) * u.tiles, t1 = t0 + u.tiles;
   const int64_t ctas = sharing(p, total), c0 = ((t0 + 1) * ctas - 1) / total, c1 = (t1 * ctas - 1) / total;
+  // Until here only lengths were read, which stood before the other kernel began; the parts are there when it has ended
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (c0 == c1) return;   // one CTA had it all
   const int lane = threadIdx.x & 31;
   const int local = (int(blockIdx.x) - unit * ctas_of_unit) * (kJoinThreads / 32) + int(threadIdx.x >> 5);
