@@ -9,7 +9,7 @@
 //
 // Bound by HBM: every value is read and written once, 20 KiB each way for a token of 40 heads of 128, against 512 B of
 // angles, which the heads of a token share.  A thread keeps the angles of its pairs in registers and goes from head to
-// head; q and k are one launch.
+// head, but where there are few tokens; q and k are one launch.
 
 #include <algorithm>
 
@@ -24,6 +24,10 @@ namespace {
 // 144 us, 5 136, 10 132.
 constexpr int kHeadsInTurn = 10;
 constexpr int64_t kManyUnits = int64_t(148) * 2048 * kHeadsInTurn;
+// Up to here a call takes as long as one thread does: every unit (two packs of channels of a head) has a thread of its own,
+// and is fetched while the position and then the angles are looked up.  40 heads of 128 in a replayed graph, with this and
+// with the loop over heads: 64 tokens 2.3 and 2.7 us, 256 3.15 and 3.45, 512 4.15 and 4.0, 1500 8.1 and 7.2.
+constexpr int64_t kFewUnits = int64_t(148) * 768;
 
 struct RotaryParams {
   const void* x[2];
@@ -44,6 +48,31 @@ struct RotaryParams {
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
 template <typename T, int V>
+__device__ __forceinline__ void turn(Pack<T, V>& lo, Pack<T, V>& hi, const float* c, const float* s, bool interleaved) {
+  float a[2 * V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) { a[j] = to_float(lo.v[j]); a[V + j] = to_float(hi.v[j]); }
+  if (interleaved) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float u = a[2 * j], w = a[2 * j + 1];
+      a[2 * j] = u * c[j] - w * s[j];
+      a[2 * j + 1] = w * c[j] + u * s[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float u = a[j], w = a[V + j];
+      a[j] = u * c[j] - w * s[j];
+      a[V + j] = w * c[j] + u * s[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) { lo.v[j] = from_float<T>(a[j]); hi.v[j] = from_float<T>(a[V + j]); }
+}
+
+// kFew: blockIdx.y counts the heads that a CTA begins with, and a thread has one unit
+template <typename T, int V, bool kFew>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   using P = Pack<T, V>;
   const uint32_t per_token = uint32_t(p.units * p.heads_at_once);
@@ -51,18 +80,18 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   const uint32_t token = blockIdx.x * p.tokens_at_once + slot;
   if (token >= uint32_t(p.tokens)) return;
   const uint32_t at = threadIdx.x - slot * per_token;
-  const int first_head = int(at / uint32_t(p.units)), unit = int(at - uint32_t(first_head) * uint32_t(p.units));
+  const int in_pass = int(at / uint32_t(p.units)), unit = int(at - uint32_t(in_pass) * uint32_t(p.units));
+  const int first_head = kFew ? in_pass + int(blockIdx.y) * p.heads_at_once : in_pass;
   const int64_t b = token / uint32_t(p.time), t = token - uint32_t(b) * uint32_t(p.time);
 
   // a unit is two packs of a head: those of V pairs, or 2 V channels that pass
   const bool turns = unit < p.units_turned;
   if (!turns && !p.copy_rest) return;
-  int c0, c1;
+  const int i = unit * V;
+  const int c0 = !turns ? 2 * p.pairs + 2 * V * (unit - p.units_turned) : p.interleaved ? 2 * i : i;
+  const int c1 = !turns || p.interleaved ? c0 + V : i + p.pairs;
   float c[V], s[V];
-  if (turns) {
-    const int i = unit * V;
-    c0 = p.interleaved ? 2 * i : i;
-    c1 = p.interleaved ? 2 * i + V : i + p.pairs;
+  auto angles = [&] {
     const int64_t pos = p.positions != nullptr ? p.positions[b * p.position_stride + t] : t;
     if (pos >= 0 && pos < p.table) {
       const Pack<float, V> pc = *reinterpret_cast<const Pack<float, V>*>(p.cos + pos * p.pairs + i);
@@ -73,49 +102,34 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
 #pragma unroll
       for (int j = 0; j < V; ++j) c[j] = s[j] = __int_as_float(0x7fffffff);
     }
-  } else {
-    c0 = 2 * p.pairs + 2 * V * (unit - p.units_turned);
-    c1 = c0 + V;
-  }
+  };
   // the token's rows of q, then those of k as heads behind them
   const int heads = p.heads[0] + p.heads[1];
   const T *x0[2];
   T *y0[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    x0[i] = static_cast<const T*>(p.x[i]) + b * p.x_stride[i][0] + t * p.x_stride[i][1] - i * p.heads[0] * p.x_stride[i][2];
-    y0[i] = static_cast<T*>(p.y[i]) + b * p.y_stride[i][0] + t * p.y_stride[i][1] - i * p.heads[0] * p.y_stride[i][2];
+  for (int x = 0; x < 2; ++x) {
+    x0[x] = static_cast<const T*>(p.x[x]) + b * p.x_stride[x][0] + t * p.x_stride[x][1] - x * p.heads[0] * p.x_stride[x][2];
+    y0[x] = static_cast<T*>(p.y[x]) + b * p.y_stride[x][0] + t * p.y_stride[x][1] - x * p.heads[0] * p.y_stride[x][2];
   }
+  if (!kFew && turns) angles();
   for (int h = first_head; h < heads; h += p.heads_at_once) {
     const bool of_k = h >= p.heads[0];
     const T* x = (of_k ? x0[1] : x0[0]) + h * (of_k ? p.x_stride[1][2] : p.x_stride[0][2]);
     T* y = (of_k ? y0[1] : y0[0]) + h * (of_k ? p.y_stride[1][2] : p.y_stride[0][2]);
     P lo = *reinterpret_cast<const P*>(x + c0), hi = *reinterpret_cast<const P*>(x + c1);
-    if (turns) {
-      float a[2 * V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) { a[j] = to_float(lo.v[j]); a[V + j] = to_float(hi.v[j]); }
-      if (p.interleaved) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float u = a[2 * j], w = a[2 * j + 1];
-          a[2 * j] = u * c[j] - w * s[j];
-          a[2 * j + 1] = w * c[j] + u * s[j];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float u = a[j], w = a[V + j];
-          a[j] = u * c[j] - w * s[j];
-          a[V + j] = w * c[j] + u * s[j];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) { lo.v[j] = from_float<T>(a[j]); hi.v[j] = from_float<T>(a[V + j]); }
-    }
+    if (kFew && turns) angles();
+    if (turns) turn(lo, hi, c, s, p.interleaved);
     *reinterpret_cast<P*>(y + c0) = lo;
     *reinterpret_cast<P*>(y + c1) = hi;
+    if (kFew) return;
   }
+}
+
+template <typename T, int V>
+void launch_width(const RotaryParams& p, unsigned blocks, int passes, int threads, cudaStream_t stream) {
+  if (passes > 0) rotary_kernel<T, V, true><<<dim3(blocks, unsigned(passes)), threads, 0, stream>>>(p);
+  else rotary_kernel<T, V, false><<<blocks, threads, 0, stream>>>(p);
 }
 
 template <typename T>
@@ -134,10 +148,11 @@ int launch_typed(const RotaryParams& base, int dim, int vec, cudaStream_t stream
   const int threads = p.units * p.heads_at_once * p.tokens_at_once;
   const int64_t blocks = (p.tokens + p.tokens_at_once - 1) / p.tokens_at_once;
   if (blocks <= 0 || blocks > int64_t(0x7fffffff)) return GDN2_ERR_TOO_LARGE;
+  const int apart = p.tokens * heads * p.units <= kFewUnits ? (heads + p.heads_at_once - 1) / p.heads_at_once : 0;
   constexpr int kWide = 16 / int(sizeof(T));
-  if (vec == kWide) rotary_kernel<T, kWide><<<unsigned(blocks), threads, 0, stream>>>(p);
-  else if (vec == 4) rotary_kernel<T, 4><<<unsigned(blocks), threads, 0, stream>>>(p);
-  else rotary_kernel<T, 1><<<unsigned(blocks), threads, 0, stream>>>(p);
+  if (vec == kWide) launch_width<T, kWide>(p, unsigned(blocks), apart, threads, stream);
+  else if (vec == 4) launch_width<T, 4>(p, unsigned(blocks), apart, threads, stream);
+  else launch_width<T, 1>(p, unsigned(blocks), apart, threads, stream);
   return check_launch();
 }
 

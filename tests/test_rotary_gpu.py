@@ -192,3 +192,28 @@ def test_other_refusals():
     args["q"].requires_grad_(True)
     with pytest.raises(ValueError, match="gradient"):
         apply_rotary(**args, inplace=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("batch,time,heads,kv_heads,dim,rotated", [
+    # 8 channels at a time (fp32: 4), 4 and 1; the last thread's heads, a block's last token and a call's last block are not full
+    (3, 201, 20, 5, 128, 64), (1, 1501, 11, 2, 40, 24), (1, 6007, 3, 2, 10, 6),
+    # every thread takes ten heads
+    (1, 9001, 37, 6, 128, 128),
+    # at the border of one unit a thread: 37 tokens of 12 heads of 256 units are 113664, 38 are more
+    (1, 37, 11, 1, 512, 2), (1, 38, 11, 1, 512, 2),
+])
+def test_many_tokens(dtype, layout, batch, time, heads, kv_heads, dim, rotated):
+    table = 300
+    cos, sin = rotary_tables(table, rotated)
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    at = torch.randint(0, table, (batch, time), generator=gen, device=DEV)
+    at[-1, -1] = table   # a position outside
+    q, k = _inputs(batch, time, heads, kv_heads, dim, dtype)
+    for got, x in zip(apply_rotary(q, k, cos, sin, at, layout=layout), (q, k)):
+        assert got[-1, -1, :, :rotated].isnan().all() and torch.equal(got[-1, -1, :, rotated:], x[-1, -1, :, rotated:])
+        want, bound = _turned(x, cos, sin, at.clamp(max=table - 1), layout)
+        inside = torch.ones(batch, time, dtype=torch.bool, device=DEV)
+        inside[-1, -1] = False
+        assert ((got.double() - want).abs() <= bound)[inside].all()
