@@ -152,12 +152,36 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
   return mul2(r, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
 }
 
+// What a row's weights are made against: exp2((s - shift) c - scaled), for a score m that is the maximum of some tile so far.
+// A nearby reference (|m c| below kNear) is fl(m c): that weights stand against m c rounded, by a factor of up to 2^(2^-14),
+// is the same for all of a row's weights, sums and outputs.  Farther away the rounding of m c would itself be powers of two
+// (16 at 2^28), so there the difference s - m comes first, which is 0 for m and negative for what is below it: no weight
+// passes 1, however large the scores.
+constexpr float kNear = 1024.f;
+struct Reference { float shift, scaled; };
+__device__ __forceinline__ Reference reference(float m, float c) {
+  const float scaled = m * c;
+  const bool near = fabsf(scaled) < kNear;
+  return {near || m == -INFINITY ? 0.f : m, near ? scaled : 0.f};   // (-inf: nothing but weights of 0 so far, any will do)
+}
+// the exponent that takes what was made against the reference of `from` to that of `to`
+__device__ __forceinline__ float between(float from, float to, float c) {
+  const Reference a = reference(from, c), b = reference(to, c);
+  return fmaf(a.shift - b.shift, c, a.scaled - b.scaled);
+}
+// What a chain, a warp or a CTA has, made against m, to the reference of top >= m; 0 where it has nothing
+__device__ __forceinline__ float factor_to(float m, float top, float c) { return m == -INFINITY ? 0.f : exp2_approx(between(m, top, c)); }
+__device__ __forceinline__ void take_shift(uint32_t (&s)[32], float shift) {
+#pragma unroll
+  for (int y = 0; y < 32; ++y) s[y] = __float_as_uint(__uint_as_float(s[y]) - shift);
+}
+
 // One tile of scores becomes weights, a row a thread: S (128 columns of TMEM at s_at) is read, masked, and overlaid by
-// P = exp2(S c - m c) in 16 bits.  m is the row's reference, a maximum of some tile so far (-inf: nothing but -inf has been
-// seen), `sum` the sum of its weights.  No tile but the first looks for its maximum: where the sum of its weights stays below
+// P in 16 bits, made against the reference of m, a maximum of some tile so far (-inf: nothing but -inf has been seen); `sum` is
+// the sum of the row's weights.  No tile but the first looks for its maximum: where the sum of its weights stays below
 // kGrowth, so does each of them, and nothing overflows or loses digits in 32 bits or in either 16-bit type.  Otherwise m
 // becomes the maximum, sum and O (DP columns at o_at, as it is after all tiles before this one) are scaled down, and the
-// tile's weights are made again.
+// tile's weights are made again, none of them above 1: a tile looks once at most.
 constexpr float kGrowth = 32768.f;
 
 // mask(x, s): columns 32 x .. 32 x + 31 in s
@@ -178,9 +202,10 @@ __device__ __forceinline__ float row_maximum(uint32_t s_at, Mask mask) {
   return top;
 }
 
-template <typename T, typename Mask>
+template <typename T, bool kFar, typename Mask>
 __device__ __forceinline__ float row_weights(uint32_t s_at, float c, float m, uint32_t (&w)[2][32], Mask mask) {
-  const float2 minus = twice(m == -INFINITY ? 0.f : -m * c), by = twice(c);
+  const Reference ref = reference(m, c);
+  const float2 minus = twice(kFar ? -ref.scaled : m == -INFINITY ? 0.f : -m * c), by = twice(c);
   float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
   uint32_t s[2][32];
   tc::tmem_ld32(s_at, s[0]);
@@ -189,6 +214,7 @@ __device__ __forceinline__ float row_weights(uint32_t s_at, float c, float m, ui
     tc::tmem_wait_ld();
     if (x < 3) tc::tmem_ld32(s_at + (x + 1) * 32, s[(x + 1) & 1]);
     mask(x, s[x & 1]);
+    if (kFar) take_shift(s[x & 1], ref.shift);
 #pragma unroll
     for (int y = 0; y < 16; ++y) {
       const float2 z = fma2(make_float2(__uint_as_float(s[x & 1][2 * y]), __uint_as_float(s[x & 1][2 * y + 1])), by, minus);
@@ -200,17 +226,18 @@ __device__ __forceinline__ float row_weights(uint32_t s_at, float c, float m, ui
   return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
 }
 
+// `far` says whether the reference of a row of the warp is; m is -inf, and `far` false, where there has been no tile
 template <typename T, int DP, typename Mask>
-__device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, float& m, float& sum, Mask mask) {
+__device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, float& m, float& sum, bool& far, Mask mask) {
   uint32_t w[2][32];
   float more;
-  bool grown = m == -INFINITY;
 #pragma unroll 1
-  for (bool look = __any_sync(0xffffffffu, grown);;) {
+  for (bool look = __any_sync(0xffffffffu, m == -INFINITY);;) {
     if (look) {
       const float top = fmaxf(m, row_maximum(s_at, mask));
-      const float f = grown && m != -INFINITY ? exp2_approx((m - top) * c) : 1.f;
-      if (grown) m = top;
+      const float f = top > m && m != -INFINITY ? exp2_approx(between(m, top, c)) : 1.f;
+      m = top;
+      far = __any_sync(0xffffffffu, reference(m, c).shift != 0.f);
       if (__any_sync(0xffffffffu, f != 1.f)) {
         sum *= f;
 #pragma unroll
@@ -224,9 +251,9 @@ __device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, fl
         }
       }
     }
-    more = row_weights<T>(s_at, c, m, w, mask);
-    grown = more > kGrowth;
-    look = __any_sync(0xffffffffu, grown);
+    more = far ? row_weights<T, true>(s_at, c, m, w, mask) : row_weights<T, false>(s_at, c, m, w, mask);
+    if (look) break;
+    look = __any_sync(0xffffffffu, more > kGrowth);
     if (!look) break;
   }
   sum += more;

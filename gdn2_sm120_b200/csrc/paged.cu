@@ -566,6 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       const bool takes_part = RT == 1 || t < chains;
       float m = -INFINITY;
       float sum = 0.f;
+      bool far = false;
       int mine = 0;
       for (int j = RT == 1 ? t : 0; j < n && takes_part; j += RT == 1 ? 2 : 1) {
         if (!ok || !(ok = waiter.wait(&bar.s_full[t], seen & 1))) break;
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         tc::tc_fence_after();
         if (any_there) {   // warps without a row have nothing to do but to keep count
           const int first_token = (tile + j) * kTile;
-          attn::soften<T, DP>(s_at, o_at, p.scale_log2, m, sum, [&](int x, uint32_t (&s)[32]) {
+          attn::soften<T, DP>(s_at, o_at, p.scale_log2, m, sum, far, [&](int x, uint32_t (&s)[32]) {
             if (first_token + x * 32 + 32 <= u.length) return;
             // drafted tokens, or the end
             const uint8_t* mask = p.mask == nullptr || !there ? nullptr : p.mask + u.b * p.mask_stride + int64_t(token) * p.drafted;
@@ -614,8 +615,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         const float m0 = told[0][row].x, m1 = told[1][row].x, l0 = told[0][row].y, l1 = told[1][row].y;
         m = fmaxf(m0, m1);
         has[1] = n > 1;
-        f[0] = m == -INFINITY ? 0.f : exp2_approx((m0 - m) * p.scale_log2);
-        f[1] = m == -INFINITY ? 0.f : exp2_approx((m1 - m) * p.scale_log2);
+        f[0] = attn::factor_to(m0, m, p.scale_log2);
+        f[1] = attn::factor_to(m1, m, p.scale_log2);
         sum = l0 * f[0] + l1 * f[1];
         if (isnan(l0) || isnan(l1)) sum = NAN;
       }
@@ -667,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         }
         if (!whole && there && col0 == 0) {
           float* ml = p.partials + int64_t(p.ctas) * 2 * C::kRows * DP + (slot * C::kRows + local) * 2;
-          *reinterpret_cast<float2*>(ml) = make_float2(m == -INFINITY ? m : m * p.scale_log2, inv * sum);
+          *reinterpret_cast<float2*>(ml) = make_float2(m, inv * sum);
         }
       }
       tc::tc_fence_before();
@@ -761,6 +762,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
   }
 
   uint32_t qf[kKSteps][4];
+  const uint32_t sign = p.negate ? 0x80008000u : 0u;   // the scale's goes to the queries
   int token_of[2];
   auto queries = [&](const Unit& x) {
 #pragma unroll
@@ -775,13 +777,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
 #pragma unroll
         for (int kh = 0; kh < 2; ++kh) {
           const int col = s * 16 + kh * 8 + in_quad * 2;
-          qf[s][kh * 2 + half] = there && col < p.dim ? *reinterpret_cast<const uint32_t*>(row + col) : 0u;
+          qf[s][kh * 2 + half] = (there && col < p.dim ? *reinterpret_cast<const uint32_t*>(row + col) : 0u) ^ sign;
         }
       }
     }
   };
   queries(u);
-  const float by = p.negate ? -p.scale_log2 : p.scale_log2;
+  const float c = p.scale_log2;
   // where this lane's part of an ldmatrix begins: rows of this warp's 16 tokens
   const int k_row = warp * 16 + (lane & 7) + ((lane >> 4) << 3), v_row = warp * 16 + (lane & 15);
   int used = 0;
@@ -811,7 +813,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       const int first_token = (tile + j) * kTile + warp * 16;
       float s[2][4];
 #pragma unroll
-      for (int x = 0; x < 8; ++x) s[x >> 2][x & 3] = (s2[0][x >> 2][x & 3] + s2[1][x >> 2][x & 3]) * by;
+      for (int x = 0; x < 8; ++x) s[x >> 2][x & 3] = s2[0][x >> 2][x & 3] + s2[1][x >> 2][x & 3];
       if (first_token + 16 > u.length) {   // drafted tokens, or the end
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
@@ -830,20 +832,20 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
         float top = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float now = fmaxf(m[half], top);
-        const float base = now == -INFINITY ? 0.f : now;   // nothing seen yet: every weight is exp(-inf) = 0
-        const float keep = exp2_approx(m[half] - base);
-        float w[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) w[x] = exp2_approx(s[x >> 1][2 * half + (x & 1)] - base);
-        l[half] = l[half] * keep + ((w[0] + w[1]) + (w[2] + w[3]));   // (of this thread's columns; the quad's are added at the end)
-        pa[half] = pack_pair<T>(w[0], w[1]);       // weights at most 1, rounded to the values' type for the product
-        pa[2 + half] = pack_pair<T>(w[2], w[3]);
-        if (__any_sync(0xffffffffu, now != m[half])) {
+        if (__any_sync(0xffffffffu, top > m[half])) {
+          const float now = fmaxf(m[half], top), keep = attn::factor_to(m[half], now, c);
+          l[half] *= keep;
 #pragma unroll
           for (int d = 0; d < kDB; ++d) { o[d][2 * half] *= keep; o[d][2 * half + 1] *= keep; }
+          m[half] = now;
         }
-        m[half] = now;
+        const attn::Reference ref = attn::reference(m[half], c);
+        float w[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) w[x] = exp2_approx(fmaf(s[x >> 1][2 * half + (x & 1)] - ref.shift, c, -ref.scaled));
+        l[half] += (w[0] + w[1]) + (w[2] + w[3]);   // (of this thread's columns; the quad's are added at the end)
+        pa[half] = pack_pair<T>(w[0], w[1]);       // weights at most 1, rounded to the values' type for the product
+        pa[2 + half] = pack_pair<T>(w[2], w[3]);
       }
       // O += P V
       if (!(ok = waiter.wait(&bar.kv_full[xv % C::kStages], (xv / C::kStages) & 1))) break;
@@ -879,7 +881,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       float top = bar.m[0][r];
 #pragma unroll
       for (int w = 1; w < 8; ++w) top = fmaxf(top, bar.m[w][r]);
-      const float f = top == -INFINITY ? 0.f : exp2_approx(m[half] - top);
+      const float f = attn::factor_to(m[half], top, c);
       m[half] = top;
 #pragma unroll
       for (int d = 0; d < kDB; ++d) { o[d][2 * half] *= f; o[d][2 * half + 1] *= f; }
@@ -977,23 +979,33 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
   const float* all_ml = p.partials + int64_t(p.ctas) * 2 * block_rows * DP;
   // the part of CTA i: its last unit where the unit began there, its first one otherwise
   auto row_of = [&](int64_t i) { return (i * 2 + (i == c0 ? 1 : 0)) * block_rows + local; };
-  float top = -INFINITY;
-  for (int64_t i = c0 + lane; i <= c1; i += 32) top = fmaxf(top, all_ml[row_of(i) * 2]);
+  // a part a lane: the first 32 parts' m and l stay
+  const float2 none = make_float2(-INFINITY, 0.f);
+  auto part_ml = [&](int64_t i) { return i <= c1 ? *reinterpret_cast<const float2*>(all_ml + row_of(i) * 2) : none; };
+  const float2 ml0 = part_ml(c0 + lane);
+  float top = ml0.x;
+  for (int64_t i = c0 + 32 + lane; i <= c1; i += 32) top = fmaxf(top, part_ml(i).x);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   constexpr int kOwn = DP / 32;
   float sum = 0.f, acc[kOwn];
 #pragma unroll
   for (int y = 0; y < kOwn; ++y) acc[y] = 0.f;
-#pragma unroll 4
-  for (int64_t i = c0; i <= c1; ++i) {
-    const float2 ml = *reinterpret_cast<const float2*>(all_ml + row_of(i) * 2);
-    const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
+  for (int64_t i0 = c0; i0 <= c1; i0 += 32) {
+    const float2 ml = i0 == c0 ? ml0 : part_ml(i0 + lane);
+    const float f = attn::factor_to(ml.x, top, p.scale_log2);
     sum += isnan(ml.y) ? ml.y : ml.y * f;
-    const float* o = p.partials + row_of(i) * DP + lane * kOwn;
+    const int count = int(c1 - i0 < 32 ? c1 - i0 + 1 : 32);
+#pragma unroll 4
+    for (int j = 0; j < count; ++j) {
+      const float by = __shfl_sync(0xffffffffu, f, j);
+      const float* o = p.partials + row_of(i0 + j) * DP + lane * kOwn;
 #pragma unroll
-    for (int y = 0; y < kOwn; ++y) acc[y] = fmaf(o[y], f, acc[y]);
+      for (int y = 0; y < kOwn; ++y) acc[y] = fmaf(o[y], by, acc[y]);
+    }
   }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int n = r / p.group, g = r - n * p.group, d = lane * kOwn;
   if (d >= p.dim) return;
