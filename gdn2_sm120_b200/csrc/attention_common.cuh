@@ -171,9 +171,19 @@ __device__ __forceinline__ float between(float from, float to, float c) {
 }
 // What a chain, a warp or a CTA has, made against m, to the reference of top >= m; 0 where it has nothing
 __device__ __forceinline__ float factor_to(float m, float top, float c) { return m == -INFINITY ? 0.f : exp2_approx(between(m, top, c)); }
-__device__ __forceinline__ void take_shift(uint32_t (&s)[32], float shift) {
+// s - shift for kColumns scores of a row a thread, where they are in TMEM
+template <int kColumns>
+__device__ __forceinline__ void take_shift(uint32_t s_at, float shift) {
+#pragma unroll 1
+  for (int x = 0; x < kColumns; x += 32) {
+    uint32_t s[32];
+    tc::tmem_ld32(s_at + x, s);
+    tc::tmem_wait_ld();
 #pragma unroll
-  for (int y = 0; y < 32; ++y) s[y] = __float_as_uint(__uint_as_float(s[y]) - shift);
+    for (int y = 0; y < 32; ++y) s[y] = __float_as_uint(__uint_as_float(s[y]) - shift);
+    tc::tmem_st32(s_at + x, s);
+  }
+  tc::tmem_wait_st();
 }
 
 // One tile of scores becomes weights, a row a thread: S (128 columns of TMEM at s_at) is read, masked, and overlaid by
@@ -181,7 +191,8 @@ __device__ __forceinline__ void take_shift(uint32_t (&s)[32], float shift) {
 // the sum of the row's weights.  No tile but the first looks for its maximum: where the sum of its weights stays below
 // kGrowth, so does each of them, and nothing overflows or loses digits in 32 bits or in either 16-bit type.  Otherwise m
 // becomes the maximum, sum and O (DP columns at o_at, as it is after all tiles before this one) are scaled down, and the
-// tile's weights are made again, none of them above 1: a tile looks once at most.
+// tile's weights are made again, none of them above 1: a tile looks once at most.  Rows whose reference is far look at every
+// tile, and then the shift is taken off where the scores are.
 constexpr float kGrowth = 32768.f;
 
 // mask(x, s): columns 32 x .. 32 x + 31 in s
@@ -202,10 +213,9 @@ __device__ __forceinline__ float row_maximum(uint32_t s_at, Mask mask) {
   return top;
 }
 
-template <typename T, bool kFar, typename Mask>
-__device__ __forceinline__ float row_weights(uint32_t s_at, float c, float m, uint32_t (&w)[2][32], Mask mask) {
-  const Reference ref = reference(m, c);
-  const float2 minus = twice(kFar ? -ref.scaled : m == -INFINITY ? 0.f : -m * c), by = twice(c);
+template <typename T, typename Mask>
+__device__ __forceinline__ float row_weights(uint32_t s_at, float c, float scaled, uint32_t (&w)[2][32], Mask mask) {
+  const float2 minus = twice(-scaled), by = twice(c);
   float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
   uint32_t s[2][32];
   tc::tmem_ld32(s_at, s[0]);
@@ -214,7 +224,6 @@ __device__ __forceinline__ float row_weights(uint32_t s_at, float c, float m, ui
     tc::tmem_wait_ld();
     if (x < 3) tc::tmem_ld32(s_at + (x + 1) * 32, s[(x + 1) & 1]);
     mask(x, s[x & 1]);
-    if (kFar) take_shift(s[x & 1], ref.shift);
 #pragma unroll
     for (int y = 0; y < 16; ++y) {
       const float2 z = fma2(make_float2(__uint_as_float(s[x & 1][2 * y]), __uint_as_float(s[x & 1][2 * y + 1])), by, minus);
@@ -232,12 +241,11 @@ __device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, fl
   uint32_t w[2][32];
   float more;
 #pragma unroll 1
-  for (bool look = __any_sync(0xffffffffu, m == -INFINITY);;) {
+  for (bool look = far || __any_sync(0xffffffffu, m == -INFINITY);;) {
     if (look) {
       const float top = fmaxf(m, row_maximum(s_at, mask));
       const float f = top > m && m != -INFINITY ? exp2_approx(between(m, top, c)) : 1.f;
       m = top;
-      far = __any_sync(0xffffffffu, reference(m, c).shift != 0.f);
       if (__any_sync(0xffffffffu, f != 1.f)) {
         sum *= f;
 #pragma unroll
@@ -250,8 +258,11 @@ __device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, fl
           tc::tmem_st16(o_at + x, o);
         }
       }
+      const float shift = reference(m, c).shift;
+      far = __any_sync(0xffffffffu, shift != 0.f);
+      if (far) take_shift<128>(s_at, shift);
     }
-    more = far ? row_weights<T, true>(s_at, c, m, w, mask) : row_weights<T, false>(s_at, c, m, w, mask);
+    more = row_weights<T>(s_at, c, reference(m, c).scaled, w, mask);
     if (look) break;
     look = __any_sync(0xffffffffu, more > kGrowth);
     if (!look) break;
@@ -291,10 +302,11 @@ struct Pair {
   int chain, half, row;
   float (*told)[128];      // [half][row], what the two tell each other
   __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, 256;" ::"r"(chain + 1) : "memory"); }
+  __device__ __forceinline__ void tell(float mine) const { told[half][row] = mine; sync(); }
+  __device__ __forceinline__ float heard() const { return told[half ^ 1][row]; }   // a barrier later the next may be told
   __device__ __forceinline__ float other(float mine) const {
-    told[half][row] = mine;
-    sync();
-    const float r = told[half ^ 1][row];
+    tell(mine);
+    const float r = heard();
     sync();
     return r;
   }
@@ -306,13 +318,14 @@ struct Pair {
   }
 };
 
+// `far` says whether the reference of a row of the chain is; false before the first tile
 template <typename T, int DP, typename Mask>
 __device__ __forceinline__ void soften_half(const Pair& pair, uint32_t s_at, uint32_t o_at, float c, bool first, float& m, float& sum,
-                                            Mask mask) {
+                                            bool& far, Mask mask) {
   uint32_t w[2][16];
   float more = 0.f;
 #pragma unroll 1
-  for (bool look = first;;) {
+  for (bool look = first || far;;) {
     if (look) {
       float top = -INFINITY;
 #pragma unroll
@@ -326,12 +339,14 @@ __device__ __forceinline__ void soften_half(const Pair& pair, uint32_t s_at, uin
         for (int y = 0; y < 32; ++y) tops[y & 3] = fmaxf(tops[y & 3], __uint_as_float(s[y]));
         top = fmaxf(top, fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
       }
-      top = fmaxf(top, pair.other(top));
-      if (first) {
-        m = top == -INFINITY ? 0.f : top;   // (any reference will do for a row that has seen nothing but -inf)
-      } else {
-        const float f = top > m ? exp2_approx((m - top) * c) : 1.f;
-        m = fmaxf(m, top);
+      pair.tell(top);
+      top = fmaxf(top, pair.heard());
+      const float before = m;
+      m = first ? (top == -INFINITY ? 0.f : top) : fmaxf(m, top);   // (any will do for a row that has seen nothing but -inf)
+      const float shift = reference(m, c).shift;
+      far = pair.any(shift != 0.f);       // and all have heard
+      if (!first) {
+        const float f = m > before ? exp2_approx(between(before, m, c)) : 1.f;
         sum *= f;
 #pragma unroll
         for (int x = 0; x < DP / 2; x += 16) {
@@ -343,8 +358,9 @@ __device__ __forceinline__ void soften_half(const Pair& pair, uint32_t s_at, uin
           tc::tmem_st16(o_at + x, o);
         }
       }
+      if (far) take_shift<64>(s_at, shift);
     }
-    const float2 minus = twice(-m * c), by = twice(c);
+    const float2 minus = twice(-reference(m, c).scaled), by = twice(c);
     float2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};
     uint32_t s[2][32];
     tc::tmem_ld32(s_at, s[0]);
@@ -362,7 +378,7 @@ __device__ __forceinline__ void soften_half(const Pair& pair, uint32_t s_at, uin
       }
     }
     more = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
-    if (look) break;    // no weight is above 1
+    if (look) break;    // no weight is above 1 (2^(2^-14) against a nearby reference)
     look = pair.any(more > kGrowth);
     if (!look) break;
   }

@@ -78,7 +78,8 @@ __device__ __noinline__ void row_again(const FwdParams& p, int64_t row0, int bat
   for (int j = 0; j <= i; ++j) {
     float s = 0.f;
     for (int x = 0; x < p.dim; ++x) s = fmaf(to_float(q[x]), to_float(k[j * p.strides[4] + x]), s);
-    const float w = exp2_approx(((p.negate ? -s : s) - m) * p.scale_log2);
+    const Reference ref = reference(m, p.scale_log2);
+    const float w = exp2_approx(fmaf((p.negate ? -s : s) - ref.shift, p.scale_log2, -ref.scaled));
     for (int x = first; x < last; ++x) o[x - first] = fmaf(w, to_float(v[j * p.strides[7] + x]), o[x - first]);
   }
   for (int x = first; x < last; ++x) to[x] = from_float<T>(o[x - first] / sum);
@@ -300,11 +301,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       }
       float m = 0.f;
       float sum = 0.f;
+      bool far = false;
       for (int j = 0; j < n && ok; ++j) {
         if (!(ok = waiter.wait(&bar.s_full[t], seen & 1))) break;
         ++seen;
         tc::tc_fence_after();
-        soften_half<T, DP>(pair, s_at, o_at, c, j == 0, m, sum, [&](int x, uint32_t (&s)[32]) {
+        soften_half<T, DP>(pair, s_at, o_at, c, j == 0, m, sum, far, [&](int x, uint32_t (&s)[32]) {
           if (j + 1 == n) {   // the tile on the diagonal; what lies behind the sequence's end lies behind every row
 #pragma unroll
             for (int y = 0; y < 32; ++y) {
@@ -342,8 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       tc::tc_fence_before();
       // rows behind the end: a backward gives them weights exp2(0 - inf) = 0
       if (p.lse != nullptr && half == 0) {
-        p.lse[head * p.seq.stat_rows + it.stat + i] =
-            !there ? -INFINITY : ok ? -(m * c + log2f(sum)) : NAN;
+        const Reference ref = reference(m, c);
+        p.lse[head * p.seq.stat_rows + it.stat + i] = !there ? -INFINITY : ok ? -fmaf(ref.shift, c, ref.scaled + log2f(sum)) : NAN;
       }
     }
   }

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import attention_bounds as exact
+from gdn2_sm120_b200.attention import causal_attention, causal_attention_varlen
 from gdn2_sm120_b200.paged import tree_attention
 
 pytestmark = pytest.mark.gpu
@@ -73,3 +74,19 @@ def test_trees(dtype, exponent, scale, way, drafted, heads, cached):
     seen = torch.cat([torch.ones(drafted, cached, device=DEV, dtype=torch.bool), exact.causal(drafted, DEV)], 1)
     want = exact.attention(*(x[0].transpose(0, 1) for x in (q, k, v)), seen, scale)
     exact.check("tree", out[0], *want["o"])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("exponent,scale", HEIGHTS)
+@pytest.mark.parametrize("way", ["high", "low", "mixed"])
+@pytest.mark.parametrize("lengths,dim", [((700,), 64), ((1, 130, 520), 128)])
+def test_causal(dtype, exponent, scale, way, lengths, dim):
+    heads, kv_heads, total = 4, 2, sum(lengths)
+    bounds = [sum(lengths[:i]) for i in range(len(lengths) + 1)]
+    q, v = _normal((1, total, heads, dim), dtype, 4), _normal((1, total, kv_heads, dim), dtype, 5)
+    k = torch.empty_like(v)
+    _scores(q, k, exponent, *_keys(total, way))
+    out = causal_attention(q, k, v, scale=scale) if len(lengths) == 1 else causal_attention_varlen(q, k, v, bounds, scale=scale)
+    for lo, hi in zip(bounds, bounds[1:]):
+        want = exact.attention(*(x[0, lo:hi].transpose(0, 1) for x in (q, k, v)), exact.causal(hi - lo, DEV), scale)
+        exact.check(f"rows {lo} to {hi}", out[0, lo:hi], *want["o"])
