@@ -62,7 +62,7 @@ def _forward(q, k, v, bounds, scale, training):
         each = _lib.lib().gdn2_attention_stat_rows(host, n_seq, rows)
         if each < 0:
             _lib.check(int(each), "gdn2_attention_stat_rows")
-        statistics = torch.empty((q.shape[2], each), device=q.device, dtype=torch.float32)
+        statistics = torch.empty((2, q.shape[2], each), device=q.device, dtype=torch.float32)
     strides = _lib.int64s(*(s for x in (q, k, v) for s in _validate.head_strides(x)))
     _lib.call("gdn2_attention_forward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
               _lib.ptr(statistics), strides, host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3],
@@ -108,7 +108,7 @@ class _CausalAttention(torch.autograd.Function):
         _lib.call("gdn2_attention_backward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                   d_out.data_ptr(), statistics.data_ptr(), scratch.data_ptr(), *(x.data_ptr() for x in grads), strides,
                   host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], _lib.dtype_code(q.dtype), scale,
-                  _lib.stream_ptr(q.device), kernels=(3 + (size > 4 * statistics.numel() + 15)) * _launches(ctx.bounds))
+                  _lib.stream_ptr(q.device), kernels=(3 + (size > 2 * statistics.numel() + 15)) * _launches(ctx.bounds))
         return (*grads, None, None)
 
 

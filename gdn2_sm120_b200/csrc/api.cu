@@ -181,7 +181,7 @@ using namespace gdn2;
 
 extern "C" {
 
-int gdn2_version(void) { return 200; /* 0.2.0: row-major WY tiles, scratch kinds */ }
+int gdn2_version(void) { return 201; /* 0.2.1: causal attention leaves two statistics a row */ }
 
 const char* gdn2_status_string(int status) {
   switch (status) {

@@ -42,6 +42,7 @@ struct BwdParams {
   CUtensorMap q_tile, do_tile, k_tile, v_tile, k_step, v_step;   // 128 rows, 64 rows
   void *dq, *dk, *dv;
   const float *lse, *delta;  // -(m + log2 l) in powers of two, -delta
+  const float* shifts;       // references that are far away, where lse says so
   float* partials;           // dk and dv of the parts of an item, [part][dk, dv][row][kv head][dim]
   int64_t partial_rows;      // rows * kv heads
   int parts;                 // of an item of the key kernel
@@ -66,6 +67,38 @@ struct BwdItem {
   int first, per_head, steps;  // keys: first 128-row step, steps of a query head, of this part; queries: 64-row steps
   int part, begin;             // keys: which part, its first step of the item's
 };
+
+// The weight of a score s of a query whose statistic is l and whose reference, if that is far away, is *shift.  Scores are
+// formed anew, so that one may lie above the forward's maximum by an ulp, which is powers of two for large ones: no weight is
+// above 1.
+__device__ __forceinline__ float far_weight(uint32_t s, float l, const float* shift, float c) {
+  const float x = __uint_as_float(s);
+  return exp2_approx(l > kFarFrom ? min_nan(fmaf(x - *shift, c, l - kFarMark), 0.f) : fmaf(x, c, l));
+}
+
+// dS of half a row of the query kernel whose warp has a row with such a reference, formed and left over dP: the row sees its
+// columns up to `last`
+template <typename T>
+__device__ __noinline__ void far_slopes(uint32_t s_at, uint32_t dp_at, float l, const float* shift, float minus_delta, float c, int last) {
+  uint32_t w[16];
+#pragma unroll
+  for (int x = 0; x < 32; x += 16) {
+    uint32_t s[16], dp[16];
+    tc::tmem_ld16(s_at + x, s);
+    tc::tmem_ld16(dp_at + x, dp);
+    tc::tmem_wait_ld();
+#pragma unroll
+    for (int y = 0; y < 16; y += 2) {
+      float ds[2];
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        ds[z] = x + y + z > last ? 0.f : far_weight(s[y + z], l, shift, c) * (__uint_as_float(dp[y + z]) + minus_delta);
+      }
+      w[(x + y) / 2] = pack_pair<T>(ds[0], ds[1]);
+    }
+  }
+  tc::tmem_st16(dp_at, w);
+}
 
 // the first step of a part of an item of the key kernel
 __device__ __forceinline__ int part_begin(int steps, int part, int parts) { return int(int64_t(steps) * part / parts); }
@@ -277,7 +310,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
       if (!bwd_item<false>(p, turn, &w)) continue;
       if (stayed == outs) into_tmem();
       const int64_t stat = w.head * p.seq.stat_rows + w.at.stat + w.tile * 128 + row;
-      const float2 minus_lse = twice(p.lse[stat]), minus_delta = twice(p.delta[stat]), by_scale = twice(p.scale_log2);
+      const float lse = p.lse[stat];
+      const bool far = __any_sync(0xffffffffu, lse > kFarFrom);
+      const float2 minus_lse = twice(lse), minus_delta = twice(p.delta[stat]), by_scale = twice(p.scale_log2);
       for (int i = b; i < w.steps && ok; i += 2) {
         if (!(ok = waiter.wait(&bar.s_full[b], seen & 1))) break;
         ++seen;
@@ -301,7 +336,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
           }
           dsw[y / 2] = pack_pair<T>(ds.x, ds.y);   // rounded to the inputs' type for its product, whose sums are in 32 bits
         }
-        tc::tmem_st16(dp_at, dsw);
+        if (far) far_slopes<T>(s_at, dp_at, lse, p.shifts + stat, minus_delta.x, p.scale_log2, diagonal ? last - half * 32 : 32);
+        else tc::tmem_st16(dp_at, dsw);
         tc::tmem_wait_st();
         tc::tc_fence_before();
         __syncwarp();
@@ -570,13 +606,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
         const float* st = stats + steps % C::kStats * 2 * 128 + part * 32;
         // queries see keys up to themselves; a head's first step is the one on the diagonal
         const bool diagonal = in_head == 0;
-        const int from = row - part * 32;
+        const int from = row - part * 32, query = (w.first + in_head) * 128 + part * 32;
         if (++in_head == w.per_head) in_head = 0;
         if (!(ok = waiter.wait(&bar.s_full, steps & 1))) break;
         tc::tc_fence_after();
         uint32_t s[32], w16[16];
         float2 e[16];
         tc::tmem_ld32(s_at, s);
+        const bool far = __any_sync(0xffffffffu, st[lane] > kFarFrom);
         tc::tmem_wait_ld();
 #pragma unroll
         for (int y = 0; y < 16; y += 2) {
@@ -585,6 +622,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
           const float2 b = fma2(make_float2(__uint_as_float(s[2 * y + 2]), __uint_as_float(s[2 * y + 3])), by_scale, make_float2(l.z, l.w));
           e[y] = exp2_2(a);
           e[y + 1] = (y & 2) != 0 ? exp2_fma(b) : exp2_2(b);
+        }
+        if (__builtin_expect(far, 0)) {   // once more, from the scores where they still are
+          const float* shifts = p.shifts + (w.head * p.group + (w.begin + i) / w.per_head) * p.seq.stat_rows + w.at.stat + query;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            uint32_t again[16];
+            tc::tmem_ld16(s_at + x * 16, again);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int y = 0; y < 16; ++y) {
+              const float weight = far_weight(again[y], st[x * 16 + y], shifts + x * 16 + y, p.scale_log2);
+              if ((y & 1) == 0) e[x * 8 + y / 2].x = weight; else e[x * 8 + y / 2].y = weight;
+            }
+          }
         }
         if (diagonal) {
 #pragma unroll
@@ -818,6 +869,7 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   p.dq = dq; p.dk = dk; p.dv = dv;
   float* delta = static_cast<float*>(scratch);
   p.lse = lse; p.delta = delta;
+  p.shifts = lse + stat_rows(bounds, n_seq, time) * heads;
   int sms = 0;
   const int status = multiprocessors(&sms);
   if (status != GDN2_OK) return status;

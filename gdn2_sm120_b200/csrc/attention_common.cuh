@@ -164,6 +164,10 @@ __device__ __forceinline__ Reference reference(float m, float c) {
   const bool near = fabsf(scaled) < kNear;
   return {near || m == -INFINITY ? 0.f : m, near ? scaled : 0.f};   // (-inf: nothing but weights of 0 so far, any will do)
 }
+// A row's statistic for the backward is -(r + log2 l) for a nearby reference r, rounded once; for one that is far away it is
+// kFarMark - log2 l, above kFarFrom, and the reference itself is its second number.  (A nearby one with l as large as sums get
+// stays within 1024 + 64.)
+constexpr float kFarMark = 2048.f, kFarFrom = 1536.f;
 // the exponent that takes what was made against the reference of `from` to that of `to`
 __device__ __forceinline__ float between(float from, float to, float c) {
   const Reference a = reference(from, c), b = reference(to, c);
@@ -173,7 +177,7 @@ __device__ __forceinline__ float between(float from, float to, float c) {
 __device__ __forceinline__ float factor_to(float m, float top, float c) { return m == -INFINITY ? 0.f : exp2_approx(between(m, top, c)); }
 // s - shift for kColumns scores of a row a thread, where they are in TMEM
 template <int kColumns>
-__device__ __forceinline__ void take_shift(uint32_t s_at, float shift) {
+__device__ __noinline__ void take_shift(uint32_t s_at, float shift) {
 #pragma unroll 1
   for (int x = 0; x < kColumns; x += 32) {
     uint32_t s[32];
@@ -235,13 +239,13 @@ __device__ __forceinline__ float row_weights(uint32_t s_at, float c, float scale
   return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
 }
 
-// `far` says whether the reference of a row of the warp is; m is -inf, and `far` false, where there has been no tile
+// m is -inf where there has been no tile
 template <typename T, int DP, typename Mask>
-__device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, float& m, float& sum, bool& far, Mask mask) {
+__device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, float& m, float& sum, Mask mask) {
   uint32_t w[2][32];
   float more;
 #pragma unroll 1
-  for (bool look = far || __any_sync(0xffffffffu, m == -INFINITY);;) {
+  for (bool look = __any_sync(0xffffffffu, !(fabsf(m * c) < kNear));;) {   // (-inf is not near)
     if (look) {
       const float top = fmaxf(m, row_maximum(s_at, mask));
       const float f = top > m && m != -INFINITY ? exp2_approx(between(m, top, c)) : 1.f;
@@ -259,8 +263,7 @@ __device__ __forceinline__ void soften(uint32_t s_at, uint32_t o_at, float c, fl
         }
       }
       const float shift = reference(m, c).shift;
-      far = __any_sync(0xffffffffu, shift != 0.f);
-      if (far) take_shift<128>(s_at, shift);
+      if (__any_sync(0xffffffffu, shift != 0.f)) take_shift<128>(s_at, shift);
     }
     more = row_weights<T>(s_at, c, reference(m, c).scaled, w, mask);
     if (look) break;
@@ -358,7 +361,7 @@ __device__ __forceinline__ void soften_half(const Pair& pair, uint32_t s_at, uin
           tc::tmem_st16(o_at + x, o);
         }
       }
-      if (far) take_shift<64>(s_at, shift);
+      if (__builtin_expect(far, 0)) take_shift<64>(s_at, shift);
     }
     const float2 minus = twice(-reference(m, c).scaled), by = twice(c);
     float2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};

@@ -40,7 +40,7 @@ struct FwdParams {
   const void *queries, *keys, *values;
   int64_t strides[9];  // batch, token and head of each, in elements
   void* out;
-  float* lse;          // [heads][stat rows]: -(m + log2 l) in powers of two, or null
+  float* lse;          // [heads][stat rows]: -(m + log2 l) in powers of two, then far references; or null
   int heads, kv_heads, group, dim, turns;
   int64_t items;
   float scale_log2;    // positive
@@ -345,7 +345,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       // rows behind the end: a backward gives them weights exp2(0 - inf) = 0
       if (p.lse != nullptr && half == 0) {
         const Reference ref = reference(m, c);
-        p.lse[head * p.seq.stat_rows + it.stat + i] = !there ? -INFINITY : ok ? -fmaf(ref.shift, c, ref.scaled + log2f(sum)) : NAN;
+        const int64_t at = head * p.seq.stat_rows + it.stat + i;
+        const float lse = ref.shift != 0.f ? kFarMark - log2f(sum) : -(ref.scaled + log2f(sum));
+        p.lse[at] = !there ? -INFINITY : ok ? lse : NAN;
+        if (there && lse > kFarFrom) p.lse[p.heads * p.seq.stat_rows + at] = ref.shift;
       }
     }
   }

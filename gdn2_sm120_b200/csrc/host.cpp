@@ -803,7 +803,7 @@ PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return none();
   }
   out = at::empty(q.sizes(), q.options());
-  if (training) statistics = floats({h.heads, rows}, q);
+  if (training) statistics = floats({2, h.heads, rows}, q);
   status = api.attention_forward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out.data_ptr(),
                                  training ? fptr(&statistics) : nullptr, h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim,
                                  h.dtype, scale, at::cuda::getCurrentCUDAStream().stream());
@@ -826,7 +826,7 @@ PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return none();
   }
   const at::Tensor& q = *h.t[0];
-  const at::Tensor *out = dense(a[3], 4, q.scalar_type(), q), *statistics = dense(a[4], 2, at::kFloat, q), *d_out = strided(a[5], 4);
+  const at::Tensor *out = dense(a[3], 4, q.scalar_type(), q), *statistics = dense(a[4], 3, at::kFloat, q), *d_out = strided(a[5], 4);
   if (out == nullptr || statistics == nullptr || d_out == nullptr || out->sizes() != q.sizes() || d_out->sizes() != q.sizes() ||
       d_out->scalar_type() != q.scalar_type() || d_out->device() != q.device() || !aligned_rows(*d_out, h.strides + 9)) {
     return none();
@@ -849,7 +849,7 @@ PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                   h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim, h.dtype, scale,
                                   at::cuda::getCurrentCUDAStream().stream());
   others.end();
-  const bool parts = size > 4 * statistics->numel() + 15;   // sums of several CTAs are added up
+  const bool parts = size > 2 * statistics->numel() + 15;   // sums of several CTAs are added up
   if (!ok(status, "gdn2_attention_backward", (parts ? 4 : 3) * passes(bounds))) return nullptr;
   PyObject* result = PyTuple_New(3);
   for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(result, i, wrap(grads[i]));

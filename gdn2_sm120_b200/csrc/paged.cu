@@ -566,7 +566,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       const bool takes_part = RT == 1 || t < chains;
       float m = -INFINITY;
       float sum = 0.f;
-      bool far = false;
       int mine = 0;
       for (int j = RT == 1 ? t : 0; j < n && takes_part; j += RT == 1 ? 2 : 1) {
         if (!ok || !(ok = waiter.wait(&bar.s_full[t], seen & 1))) break;
@@ -574,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         tc::tc_fence_after();
         if (any_there) {   // warps without a row have nothing to do but to keep count
           const int first_token = (tile + j) * kTile;
-          attn::soften<T, DP>(s_at, o_at, p.scale_log2, m, sum, far, [&](int x, uint32_t (&s)[32]) {
+          attn::soften<T, DP>(s_at, o_at, p.scale_log2, m, sum, [&](int x, uint32_t (&s)[32]) {
             if (first_token + x * 32 + 32 <= u.length) return;
             // drafted tokens, or the end
             const uint8_t* mask = p.mask == nullptr || !there ? nullptr : p.mask + u.b * p.mask_stride + int64_t(token) * p.drafted;

@@ -483,7 +483,7 @@ int gdn2_tree_attention(const void* q, const void* k, const void* v, const void*
 /*
  * Causal attention over whole sequences: n_seq of `time` tokens each (bounds NULL), or n_seq packed ones
  * that are rows bounds[i] .. bounds[i + 1] of [1, time, H, D] tensors (host array of n_seq + 1).
- * out [.., heads, dim] is contiguous.  `statistics` (NULL for inference): heads * gdn2_attention_stat_rows
+ * out [.., heads, dim] is contiguous.  `statistics` (NULL for inference): 2 * heads * gdn2_attention_stat_rows
  * floats that a backward needs.  Rows of `out` that belong to no sequence are not written.
  * strides: batch, token and head of q, k, v.
  */

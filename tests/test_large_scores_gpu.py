@@ -90,3 +90,27 @@ def test_causal(dtype, exponent, scale, way, lengths, dim):
     for lo, hi in zip(bounds, bounds[1:]):
         want = exact.attention(*(x[0, lo:hi].transpose(0, 1) for x in (q, k, v)), exact.causal(hi - lo, DEV), scale)
         exact.check(f"rows {lo} to {hi}", out[0, lo:hi], *want["o"])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("exponent,scale", HEIGHTS)
+@pytest.mark.parametrize("way", ["high", "low", "mixed"])
+@pytest.mark.parametrize("lengths,heads,dim", [((700,), 4, 64), ((1, 130, 520), 4, 128), ((1100,), 12, 64)])
+def test_causal_gradients(dtype, exponent, scale, way, lengths, heads, dim):
+    """dq and dk are sums of keys and queries of up to 2^15: small cotangents keep them in fp16's range.  The last lengths have
+    the sums over the keys cut into parts."""
+
+    kv_heads, total = 2, sum(lengths)
+    bounds = [sum(lengths[:i]) for i in range(len(lengths) + 1)]
+    q, v = _normal((1, total, heads, dim), dtype, 4), _normal((1, total, kv_heads, dim), dtype, 5)
+    do = _normal(q.shape, dtype, 6, 2.0 ** -14)
+    k = torch.empty_like(v)
+    _scores(q, k, exponent, *_keys(total, way))
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    out = causal_attention(q, k, v, scale=scale) if len(lengths) == 1 else causal_attention_varlen(q, k, v, bounds, scale=scale)
+    grads = torch.autograd.grad(out, leaves, do)
+    for lo, hi in zip(bounds, bounds[1:]):
+        want = exact.attention(*(x.detach()[0, lo:hi].transpose(0, 1) for x in leaves), exact.causal(hi - lo, DEV), scale,
+                               do[0, lo:hi].transpose(0, 1))
+        for name, x in zip(("o", "dq", "dk", "dv"), (out.detach(), *grads)):
+            exact.check(f"{name}, rows {lo} to {hi}", x[0, lo:hi], *want[name])
