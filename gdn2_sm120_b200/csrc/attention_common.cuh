@@ -120,6 +120,38 @@ template <typename T> struct Format;
 template <> struct Format<__nv_bfloat16> { static constexpr uint32_t code = tc::kFmtBF16, exponent = 0x7f80u; };
 template <> struct Format<__half> { static constexpr uint32_t code = tc::kFmtF16, exponent = 0x7c00u; };
 
+// Where 8 channels of a row are in a tile: a slab has 64 channels, in lines of 128 bytes whose 16-byte pieces are permuted by
+// the line.
+template <int DP>
+__device__ __forceinline__ uint32_t place_of(uint32_t base, uint32_t slab, int row, int piece) {
+  return base + uint32_t(piece >> 3) * slab + uint32_t(row) * 128u + ((uint32_t(piece ^ row) & 7u) << 4);
+}
+
+// An infinite or NaN value must reach the rows that see it and no others, but in the product it would meet every row of a
+// tile (0 * NaN): it leaves the tile, and is added to those rows at the end.  Rows first .. last - 1, by the warp that copied
+// them; found(row) is called by threads that found one.
+template <typename T, int DP, typename Found>
+__device__ __forceinline__ void sift(uint32_t base, uint32_t slab, int first, int last, Found found) {
+  constexpr int kPieces = DP / 8, kAtOnce = 32 / kPieces;
+  const int lane = threadIdx.x & 31, piece = lane % kPieces, sub = lane / kPieces;
+  __syncwarp();
+  for (int r = first + sub; r < last; r += kAtOnce) {
+    const uint32_t at = place_of<DP>(base, slab, r, piece);
+    uint32_t w[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if ((w[j] & Format<T>::exponent) == Format<T>::exponent) { w[j] &= 0xffff0000u; any = true; }
+      if (((w[j] >> 16) & Format<T>::exponent) == Format<T>::exponent) { w[j] &= 0xffffu; any = true; }
+    }
+    if (any) {
+      asm volatile("st.shared.v4.b32 [%4], {%0, %1, %2, %3};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(at) : "memory");
+      found(r);
+    }
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   const typename Pair<T>::type v = Pair<T>::make(lo, hi);

@@ -32,13 +32,14 @@ struct FwdConfig {
   static constexpr int kTileBytes = 128 * DP * 2;
   static constexpr int kSlab = 128 * 128;               // 64 channels of 128 rows
   static constexpr int kStages = DP == 128 ? 5 : 8;
-  static constexpr int kBytes = (2 + kStages) * kTileBytes + 512 + 2 * 2 * 128 * 4;
+  static constexpr int kBarBytes = 1024;
+  static constexpr int kBytes = (2 + kStages) * kTileBytes + kBarBytes + 2 * 2 * 128 * 4;
 };
 
 struct FwdParams {
   CUtensorMap q, k, v;
-  const void *queries, *keys, *values;
-  int64_t strides[9];  // batch, token and head of each, in elements
+  const void* values;
+  int64_t strides[3];  // of the values: batch, token and head, in elements
   void* out;
   float* lse;          // [heads][stat rows]: -(m + log2 l) in powers of two, then far references; or null
   int heads, kv_heads, group, dim, turns;
@@ -54,74 +55,60 @@ struct FwdBars {
   uint64_t raw;        // a tile that is mended before the products may read it
   uint64_t drained;
   uint64_t kv_full[8], kv_empty[8];
+};
+struct FwdMarks {
+  uint32_t again[32];      // items to be done once more, a bit a turn modulo 1024 (another one of that bit is done for nothing)
+  uint32_t strange[4][8];  // rows of an item's two diagonal tiles with values that are not finite, of the last four such items
   uint32_t tmem;
   int failed;
 };
 
 // In the tile on the diagonal a row meets values that it does not see, with weights of 0; but 0 * inf and 0 * NaN are not 0.
-// A row that came out infinite or NaN looks whether such a value is behind it, and if so is made again without the tensor
-// cores, from the reference m and the sum that the scores alone have given.
+// Nothing is looked for in advance: where a row comes out infinite or NaN, its item is marked, and the CTA goes through its
+// marked items once more when it has done them all.  Then values that are not finite leave the tiles on the diagonals, and
+// are added here to the rows that see them: `to` is a row's output, the last of the rows `seen` of these tiles; strange[] has
+// a bit for every row of the two tiles from v on that held such a value.
 template <typename T>
-__device__ __noinline__ void row_again(const FwdParams& p, int64_t row0, int batch, int len, int head, int i, float m, float sum, T* to,
-                                       int first, int last) {
-  const int kv_head = head / p.group;
-  const T* q = static_cast<const T*>(p.queries) + batch * p.strides[0] + (row0 + i) * p.strides[1] + head * p.strides[2];
-  const T* k = static_cast<const T*>(p.keys) + batch * p.strides[3] + row0 * p.strides[4] + kv_head * p.strides[5];
-  const T* v = static_cast<const T*>(p.values) + batch * p.strides[6] + row0 * p.strides[7] + kv_head * p.strides[8];
-  bool behind = false;
-  for (int j = i + 1; j < min(len, (i / 128 + 1) * 128) && !behind; ++j) {
-    for (int x = first; x < last; ++x) behind = behind || !isfinite(to_float(v[j * p.strides[7] + x]));
+__device__ __noinline__ void add_strange(const T* v, int64_t stride, const uint32_t* strange, int seen, T* to, int channels) {
+  for (int j = 0; j <= seen; ++j) {
+    if (((strange[j >> 5] >> (j & 31)) & 1) == 0) continue;
+    for (int x = 0; x < channels; x += 8) {
+      uint4 raw = *reinterpret_cast<const uint4*>(v + j * stride + x);
+      const T* value = reinterpret_cast<const T*>(&raw);
+      for (int y = 0; y < 8; ++y) {
+        if (!isfinite(to_float(value[y]))) to[x + y] = from_float<T>(to_float(to[x + y]) + to_float(value[y]));
+      }
+    }
   }
-  if (!behind) return;
-  float o[64];
-  for (int x = first; x < last; ++x) o[x - first] = 0.f;
-  for (int j = 0; j <= i; ++j) {
-    float s = 0.f;
-    for (int x = 0; x < p.dim; ++x) s = fmaf(to_float(q[x]), to_float(k[j * p.strides[4] + x]), s);
-    const Reference ref = reference(m, p.scale_log2);
-    const float w = exp2_approx(fmaf((p.negate ? -s : s) - ref.shift, p.scale_log2, -ref.scaled));
-    for (int x = first; x < last; ++x) o[x - first] = fmaf(w, to_float(v[j * p.strides[7] + x]), o[x - first]);
-  }
-  for (int x = first; x < last; ++x) to[x] = from_float<T>(o[x - first] / sum);
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __grid_constant__ FwdParams p) {
+template <int kStages>
+__device__ __forceinline__ void init_bars(FwdBars& bar) {
+  for (int t = 0; t < 2; ++t) {
+    tc::mbar_init(&bar.q_full[t], 1);
+    tc::mbar_init(&bar.q_empty[t], 1);
+    tc::mbar_init(&bar.s_full[t], 1);
+    tc::mbar_init(&bar.p_ready[t], 8);
+    tc::mbar_init(&bar.o_full[t], 1);
+  }
+  tc::mbar_init(&bar.raw, 1);
+  tc::mbar_init(&bar.drained, 1);
+  for (int s = 0; s < kStages; ++s) {
+    tc::mbar_init(&bar.kv_full[s], 1);
+    tc::mbar_init(&bar.kv_empty[s], 1);
+  }
+  tc::fence_mbar_init();
+}
+
+// All items of the CTA, or the marked ones once more
+template <typename T, int DP, bool kAgain>
+__device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem, FwdBars& bar, FwdMarks& marks, float (*told)[2][128],
+                                              uint32_t tmem) {
   using C = FwdConfig<DP>;
-  extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
   uint8_t* q_tiles = smem;
   uint8_t* kv_tiles = smem + 2 * C::kTileBytes;
-  FwdBars& bar = *reinterpret_cast<FwdBars*>(smem + (2 + C::kStages) * C::kTileBytes);
-  float(*told)[2][128] = reinterpret_cast<float(*)[2][128]>(smem + (2 + C::kStages) * C::kTileBytes + 512);
-  static_assert(sizeof(FwdBars) <= 512, "");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  if (threadIdx.x == 0) {
-    for (int t = 0; t < 2; ++t) {
-      tc::mbar_init(&bar.q_full[t], 1);
-      tc::mbar_init(&bar.q_empty[t], 1);
-      tc::mbar_init(&bar.s_full[t], 1);
-      tc::mbar_init(&bar.p_ready[t], 8);
-      tc::mbar_init(&bar.o_full[t], 1);
-    }
-    tc::mbar_init(&bar.raw, 1);
-    tc::mbar_init(&bar.drained, 1);
-    for (int s = 0; s < C::kStages; ++s) {
-      tc::mbar_init(&bar.kv_full[s], 1);
-      tc::mbar_init(&bar.kv_empty[s], 1);
-    }
-    bar.failed = 0;
-    tc::fence_mbar_init();
-  }
-  if (warp == 16) {
-    tc::tmem_alloc(&bar.tmem, 512);
-    tc::tmem_relinquish();
-  }
-  tc::tc_fence_before();
-  __syncthreads();
-  tc::tc_fence_after();
-  const uint32_t tmem = bar.tmem;
-  const Waiter waiter{&bar.failed};
+  const Waiter waiter{&marks.failed};
 
   // an item's head, rows and numbers of key tiles
   auto item_at = [&](int64_t index, int* head) {
@@ -134,11 +121,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
     return tile * 128 < it.len ? tile + 1 : 0;
   };
 
+  auto marked = [&](int turn) { return ((marks.again[(turn >> 5) & 31] >> (turn & 31)) & 1) != 0; };
+
   if (warp >= 16) {
     if (warp == 17) {
       // ---- copies ------------------------------------------------------------------------------------------
       const uint32_t leader = tc::elect_leader();
-      int filled = 0, loaded[2] = {0, 0}, mended = 0;
+      int filled = 0, loaded[2] = {0, 0}, mended = 0, redone = 0;
       bool ok = true;
       auto load = [&](const CUtensorMap* map, uint8_t* to, int head, int row, int batch, uint64_t* full) {
         tc::mbar_arrive_expect_tx(full, C::kTileBytes, leader);
@@ -149,7 +138,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       };
       for (int turn = 0; turn < p.turns && ok; ++turn) {
         const int64_t index = item_of_turn(turn);
-        if (index >= p.items) continue;
+        if (index >= p.items || (kAgain && !marked(turn))) continue;
+        redone += kAgain;
         int head;
         const Item it = item_at(index, &head);
         const int kv_head = head / p.group;
@@ -183,7 +173,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
           if (!ok) break;
           uint8_t* to = kv_tiles + s * C::kTileBytes;
           const int valid = it.len - j * 128;   // rows of the sequence
-          if (p.seq.packed && valid < 128) {
+          const bool diagonal = kAgain && j >= 2 * it.tile;   // of one of the two tiles of queries
+          if (diagonal || (p.seq.packed && valid < 128)) {
             // rows of the next sequence: their weights are 0, but 0 * inf and 0 * NaN are not
             load(&p.v, to, kv_head, it.row0 + j * 128, it.batch, &bar.raw);
             ok = waiter.wait(&bar.raw, mended & 1);
@@ -192,6 +183,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
             for (int slab = 0; slab < DP / 64; ++slab) {
               uint4* lines = reinterpret_cast<uint4*>(to + slab * C::kSlab);
               for (int x = valid * 8 + lane; x < 128 * 8; x += 32) lines[x] = make_uint4(0, 0, 0, 0);
+            }
+            if (diagonal) {
+              // (when an item's queries could be loaded, nobody reads the rows of the one three before it any more)
+              uint32_t* strange = marks.strange[redone & 3];
+              if (j == 2 * it.tile && lane < 8) strange[lane] = 0;
+              sift<T, DP>(tc::smem_u32(to), C::kSlab, 0, min(valid, 128),
+                          [&](int row) { atomicOr(&strange[(j - 2 * it.tile) * 4 + (row >> 5)], 1u << (row & 31)); });
             }
             tc::fence_async_smem();
             __syncwarp();
@@ -229,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       };
       for (int turn = 0; turn < p.turns && ok; ++turn) {
         const int64_t index = item_of_turn(turn);
-        if (index >= p.items) continue;
+        if (index >= p.items || (kAgain && !marked(turn))) continue;
         int head;
         const Item it = item_at(index, &head);
         const int n_t[2] = {key_tiles(it, 0), key_tiles(it, 1)};
@@ -287,11 +285,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
     const uint32_t s_at = tmem + lane_base + t * 128 + half * 64, o_at = tmem + lane_base + 256 + t * 128 + half * (DP / 2);
     const Pair pair{t, half, row, told[t]};
     const float c = p.scale_log2;
-    int seen = 0, outs = 0;
+    int seen = 0, outs = 0, redone = 0;
     bool ok = true;
     for (int turn = 0; turn < p.turns; ++turn) {
       const int64_t index = item_of_turn(turn);
-      if (index >= p.items) continue;
+      if (index >= p.items || (kAgain && !marked(turn))) continue;
+      redone += kAgain;
       int head;
       const Item it = item_at(index, &head);
       const int n = key_tiles(it, t);
@@ -340,7 +339,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
         }
         if (there) store_row16<T>(to + col0 + x, o, inv, p.dim - col0 - x, p.wide);
       }
-      if (strange != 0.f && there && ok && isfinite(sum)) row_again<T>(p, it.row0, it.batch, it.len, head, i, m, sum, to, col0, min(p.dim, col0 + DP / 2));
+      if (!kAgain) {
+        if (strange != 0.f && there && ok && isfinite(sum)) atomicOr(&marks.again[(turn >> 5) & 31], 1u << (turn & 31));
+      } else if (there && ok && col0 < p.dim) {
+        const T* v = static_cast<const T*>(p.values) + it.batch * p.strides[0] + (it.row0 + int64_t(it.tile) * kTileRows) * p.strides[1] +
+                     head / p.group * p.strides[2] + col0;
+        add_strange<T>(v, p.strides[1], marks.strange[redone & 3], t * 128 + row, to + col0, min(p.dim - col0, DP / 2));
+      }
       tc::tc_fence_before();
       // rows behind the end: a backward gives them weights exp2(0 - inf) = 0
       if (p.lse != nullptr && half == 0) {
@@ -352,12 +357,45 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
       }
     }
   }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __grid_constant__ FwdParams p) {
+  using C = FwdConfig<DP>;
+  extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
+  FwdBars* bars = reinterpret_cast<FwdBars*>(smem + (2 + C::kStages) * C::kTileBytes);
+  FwdMarks& marks = *reinterpret_cast<FwdMarks*>(bars + 2);
+  float(*told)[2][128] = reinterpret_cast<float(*)[2][128]>(smem + (2 + C::kStages) * C::kTileBytes + C::kBarBytes);
+  static_assert(2 * sizeof(FwdBars) + sizeof(FwdMarks) <= C::kBarBytes, "");
+  const int warp = threadIdx.x >> 5;
+
+  if (threadIdx.x == 0) {
+    init_bars<C::kStages>(bars[0]);
+    marks.failed = 0;
+  }
+  if (threadIdx.x < 32) marks.again[threadIdx.x] = 0;
+  if (warp == 16) {
+    tc::tmem_alloc(&marks.tmem, 512);
+    tc::tmem_relinquish();
+  }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  tc::tc_fence_after();
+  const uint32_t tmem = marks.tmem;
+  forward_items<T, DP, false>(p, smem, bars[0], marks, told, tmem);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  // (a CTA in which a wait ran out leaves it at that)
+  if (__any_sync(0xffffffffu, marks.again[threadIdx.x & 31] != 0) && marks.failed == 0) {
+    if (threadIdx.x == 0) init_bars<C::kStages>(bars[1]);
+    __syncthreads();
+    forward_items<T, DP, true>(p, smem, bars[1], marks, told, tmem);
+    tc::tc_fence_before();
+    __syncthreads();
     tc::tc_fence_after();
-    tc::tmem_dealloc(tmem, 512);
   }
+  if (warp == 16) tc::tmem_dealloc(tmem, 512);
 }
 
 template <typename T, int DP>
@@ -388,8 +426,8 @@ int launch_attention_forward(const void* q, const void* k, const void* v, void* 
       !encode_heads_map(&p.v, v, strides + 6, batch, time, kv_heads, dim, dtype, 128)) {
     return GDN2_ERR_LAUNCH;
   }
-  p.queries = q; p.keys = k; p.values = v;
-  for (int i = 0; i < 9; ++i) p.strides[i] = strides[i];
+  p.values = v;
+  for (int i = 0; i < 3; ++i) p.strides[i] = strides[6 + i];
   p.out = out; p.lse = lse;
   p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.dim = dim;
   // the sign goes to the product, and a scale of 0 stays a positive number, so that -inf * scale masks as ever

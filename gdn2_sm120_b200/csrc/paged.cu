@@ -36,6 +36,7 @@ namespace gdn2 {
 
 using attn::Format;
 using attn::pack_pair;
+using attn::place_of;
 
 namespace {
 
@@ -202,11 +203,7 @@ __device__ const uint4 g_nan_row[16] = {GDN2_NAN4, GDN2_NAN4, GDN2_NAN4, GDN2_NA
 #undef GDN2_NAN4
 
 // A warp copies 32 rows of DP channels, half of it or a quarter a row at a time: `at` is where row `first + lane` is, null
-// for zeros.  In shared memory a slab has 64 channels, in lines of 128 bytes whose 16-byte pieces are permuted by the line.
-template <int DP>
-__device__ __forceinline__ uint32_t place_of(uint32_t base, uint32_t slab, int row, int piece) {
-  return base + uint32_t(piece >> 3) * slab + uint32_t(row) * 128u + ((uint32_t(piece ^ row) & 7u) << 4);
-}
+// for zeros.
 template <int DP>
 __device__ __forceinline__ void copy_rows(uint32_t base, uint32_t slab, int first, int dim, const void* at) {
   constexpr int kPieces = DP / 8, kAtOnce = 32 / kPieces;
@@ -228,33 +225,6 @@ __device__ __forceinline__ void copy_rows(uint32_t base, uint32_t slab, int firs
                  reinterpret_cast<const uint8_t*>(there ? row[x] : anything) + piece * 16, there);
     }
   }
-}
-
-// An infinite or NaN value of a drafted token must reach the rows that see it and no others, but in the product it would
-// meet every row (0 * NaN): it leaves the tile, and is added to those rows at the end.  Rows first .. last - 1, by the warp
-// that copied them; true for a thread that found one.
-template <typename T, int DP>
-__device__ __forceinline__ bool sift(uint32_t base, uint32_t slab, int first, int last) {
-  constexpr int kPieces = DP / 8, kAtOnce = 32 / kPieces;
-  const int lane = threadIdx.x & 31, piece = lane % kPieces, sub = lane / kPieces;
-  bool found = false;
-  __syncwarp();
-  for (int r = first + sub; r < last; r += kAtOnce) {
-    const uint32_t at = place_of<DP>(base, slab, r, piece);
-    uint32_t w[4];
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-    bool any = false;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if ((w[j] & Format<T>::exponent) == Format<T>::exponent) { w[j] &= 0xffff0000u; any = true; }
-      if (((w[j] >> 16) & Format<T>::exponent) == Format<T>::exponent) { w[j] &= 0xffffu; any = true; }
-    }
-    if (any) {
-      asm volatile("st.shared.v4.b32 [%4], {%0, %1, %2, %3};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(at) : "memory");
-      found = true;
-    }
-  }
-  return found;
 }
 
 // a tiled copy into shared memory that is given by its address there
@@ -334,7 +304,8 @@ __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int til
     }
     if (!keys && t0 + kMine > u.length) {
       cp_async_wait_all();
-      if (sift<T, DP>(base, kSlab, mine + max(0, u.length - t0), mine + kMine)) *static_cast<volatile int*>(strange) = 1;
+      // a drafted token's values that are not finite are added to the rows that see them
+      attn::sift<T, DP>(base, kSlab, mine + max(0, u.length - t0), mine + kMine, [&](int) { *static_cast<volatile int*>(strange) = 1; });
       tc::mbar_arrive(&full[s]);
     } else {
       cp_async_arrive(&full[s]);
