@@ -1,6 +1,8 @@
 // extern "C" entry points of the operators of an attention layer: argument validation + kernel launches.
 // No allocation, no synchronisation, no exceptions cross this boundary.
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace gdn2 {
@@ -15,6 +17,8 @@ int launch_tree(const void*, const void*, const void*, const void*, const void*,
                 void*, void*, const int64_t*, int64_t, int64_t, int, int, int, int, int, int64_t, int, int, int, float,
                 cudaStream_t);
 namespace attn {
+static std::atomic<uint32_t> g_wait_polls{GDN2_ATTENTION_WAIT_POLLS};
+uint32_t wait_polls() { return g_wait_polls.load(std::memory_order_relaxed); }
 int64_t attention_stat_rows(const int64_t*, int64_t, int64_t);
 int launch_attention_forward(const void*, const void*, const void*, void*, float*, const int64_t*, const int64_t*, int64_t,
                              int64_t, int, int, int, int, float, cudaStream_t);
@@ -183,6 +187,12 @@ int gdn2_attention_backward(const void* q, const void* k, const void* v, const v
   return attn::launch_attention_backward(q, k, v, out, d_out, statistics, scratch, dq, dk, dv, strides, bounds, n_seq, time,
                                          int(heads), int(kv_heads), int(dim), dtype, scale,
                                          static_cast<cudaStream_t>(stream));
+}
+
+int gdn2_debug_wait_limit(int64_t polls) {
+  if (polls > GDN2_ATTENTION_WAIT_POLLS) return GDN2_ERR_TOO_LARGE;
+  attn::g_wait_polls.store(polls < 0 ? GDN2_ATTENTION_WAIT_POLLS : uint32_t(polls), std::memory_order_relaxed);
+  return GDN2_OK;
 }
 
 }  // extern "C"

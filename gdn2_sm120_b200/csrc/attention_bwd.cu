@@ -50,6 +50,7 @@ struct BwdParams {
   int64_t items;
   float scale, scale_log2;   // scale_log2 is positive
   uint32_t negate;
+  uint32_t polls;            // of a wait
   bool wide;                 // rows of the gradients are 32-byte aligned
   Sequences seq;
 };
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = bar.tmem;
-  const Waiter waiter{&bar.failed};
+  const Waiter waiter{&bar.failed, p.polls};
 
   if (warp >= 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");   // 640 threads of 96 registers = 512 of 104 + 128 of 64
@@ -219,6 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
           for (int i = 0; i < 4096 && !tc::mbar_try_wait(&bar.go_full[x % C::kStages], (x / C::kStages) & 1); ++i) {}
         }
         for (int i = 0; stayed > 0 && i < 4096 && !tc::mbar_try_wait(&bar.stay_full, (stayed - 1) & 1); ++i) {}
+        for (int i = 0; mended > 0 && i < 4096 && !tc::mbar_try_wait(&bar.raw, (mended - 1) & 1); ++i) {}
       }
     } else if (warp == 16) {
       // ---- products --------------------------------------------------------------------------------------
@@ -302,8 +304,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
       tc::tmem_wait_st();
       tc::tc_fence_before();
       __syncwarp();
-      tc::mbar_arrive(&bar.stay_empty, lane == 0);
-      tc::mbar_arrive(&bar.in_tmem, lane == 0);
+      tc::mbar_arrive(&bar.stay_empty, lane == 0 && ok);
+      tc::mbar_arrive(&bar.in_tmem, lane == 0 && ok);
     };
     for (int turn = 0; turn < p.turns; ++turn) {
       BwdItem w;
@@ -356,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
           break;
         }
       }
-      if (ok) ok = waiter.wait(&bar.acc_full, outs & 1);
+      if (ok) ok = waiter.wait(&bar.acc_full, outs & 1) && waiter.nobody_failed();
       ++outs;
       tc::tc_fence_after();
       // a thread has a quarter of its row's channels
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
       }
       tc::tc_fence_before();
       __syncwarp();
-      tc::mbar_arrive(&bar.acc_empty, lane == 0);
+      tc::mbar_arrive(&bar.acc_empty, lane == 0 && ok);
     }
   }
   tc::tc_fence_before();
@@ -452,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = bar.tmem;
-  const Waiter waiter{&bar.failed};
+  const Waiter waiter{&bar.failed, p.polls};
   asm volatile("griddepcontrol.wait;" ::: "memory");   // delta
   let_others_begin();
 
@@ -518,6 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
           for (int i = 0; i < 4096 && !tc::mbar_try_wait(&bar.go_full[x % C::kStages], (x / C::kStages) & 1); ++i) {}
         }
         for (int i = 0; stayed > 0 && i < 4096 && !tc::mbar_try_wait(&bar.stay_full, (stayed - 1) & 1); ++i) {}
+        for (int i = 0; mended > 0 && i < 4096 && !tc::mbar_try_wait(&bar.raw, (mended - 1) & 1); ++i) {}
       }
     } else if (warp == 16) {
       // ---- products --------------------------------------------------------------------------------------
@@ -578,6 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
           if (more && !(ok = slopes(x + 3))) break;
           ++steps;
         }
+        if (!ok) break;   // dk and dv lack a product, and are not reported
         tc::mma_commit(&bar.acc_full, leader);
         tc::mma_commit(&bar.stay_empty, leader);
         used += 2 * w.steps;
@@ -678,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
         __syncwarp();
         tc::mbar_arrive(&bar.ds_ready, lane == 0);
       }
-      if (ok) ok = waiter.wait(&bar.acc_full, outs & 1);
+      if (ok) ok = waiter.wait(&bar.acc_full, outs & 1) && waiter.nobody_failed();
       ++outs;
       tc::tc_fence_after();
       // a thread has half of its row of dv or of dk
@@ -709,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
       }
       tc::tc_fence_before();
       __syncwarp();
-      tc::mbar_arrive(&bar.acc_empty, lane == 0);
+      tc::mbar_arrive(&bar.acc_empty, lane == 0 && ok);
     }
   }
   tc::tc_fence_before();
@@ -879,6 +883,7 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.dim = dim;
   p.scale = scale;
   p.negate = scale < 0.f;
+  p.polls = wait_polls();
   p.wide = wide_rows(dq, dim) && wide_rows(dk, dim) && wide_rows(dv, dim);
   p.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
   return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {

@@ -69,18 +69,25 @@ __device__ __forceinline__ int64_t item_of_turn(int turn) {
   return turn * n + ((turn & 1) ? n - 1 - c : c);
 }
 
-// Waits of a CTA are bounded: whoever waits in vain says so, and all others stop waiting too.
+// How often a wait polls; a test may have fewer.
+uint32_t wait_polls();
+
+// Waits of a CTA are bounded: whoever waits in vain says so, and all others stop waiting too.  A poll takes up to 4 us.  What
+// is made of data that others waited for is right only where nobody has failed by then: whoever stores results looks at
+// that behind the last barrier between them.
 struct Waiter {
   volatile int* failed;
+  uint32_t polls;
   // by whole warps, whose lanes agree on what came of it
   __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) const {
-    return __all_sync(0xffffffffu, tc::mbar_try_wait(bar, parity) || wait_on(bar, parity));
+    return __all_sync(0xffffffffu, tc::mbar_test(bar, parity) || wait_on(bar, parity));
   }
+  __device__ __forceinline__ bool nobody_failed() const { return __all_sync(0xffffffffu, *failed == 0); }   // by whole warps
   __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity) const {
 #pragma unroll 1
-    for (uint32_t i = 0; i < (1u << 20); ++i) {
+    for (uint32_t i = 0; i < polls; ++i) {
       if (tc::mbar_try_wait(bar, parity)) return true;
-      if ((i & 63) == 63 && *failed) return false;
+      if (*failed) return false;
     }
     *failed = 1;
     return false;

@@ -46,6 +46,7 @@ struct FwdParams {
   int64_t items;
   float scale_log2;    // positive
   uint32_t negate;     // the scale is negative: Q counts with its sign changed
+  uint32_t polls;      // of a wait
   bool wide;           // rows of the output are 32-byte aligned
   Sequences seq;
 };
@@ -108,7 +109,7 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
   uint8_t* q_tiles = smem;
   uint8_t* kv_tiles = smem + 2 * C::kTileBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Waiter waiter{&marks.failed};
+  const Waiter waiter{&marks.failed, p.polls};
 
   // an item's head, rows and numbers of key tiles
   auto item_at = [&](int64_t index, int* head) {
@@ -208,6 +209,7 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
         for (int t = 0; t < 2; ++t) {
           for (int i = 0; loaded[t] > 0 && i < 4096 && !tc::mbar_try_wait(&bar.q_full[t], (loaded[t] - 1) & 1); ++i) {}
         }
+        for (int i = 0; mended > 0 && i < 4096 && !tc::mbar_try_wait(&bar.raw, (mended - 1) & 1); ++i) {}
       }
     } else if (warp == 16) {
       // ---- products ----------------------------------------------------------------------------------------
@@ -286,7 +288,6 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
     const Pair pair{t, half, row, told[t]};
     const float c = p.scale_log2;
     int seen = 0, outs = 0, redone = 0;
-    bool ok = true;
     for (int turn = 0; turn < p.turns; ++turn) {
       const int64_t index = item_of_turn(turn);
       if (index >= p.items || (kAgain && !marked(turn))) continue;
@@ -301,8 +302,10 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
       float m = 0.f;
       float sum = 0.f;
       bool far = false;
-      for (int j = 0; j < n && ok; ++j) {
-        if (!(ok = waiter.wait(&bar.s_full[t], seen & 1))) break;
+      // The warps of a chain meet in barriers: one that waited in vain goes on as the others do, and what came of all waits is
+      // asked behind the last of them.
+      for (int j = 0; j < n; ++j) {
+        waiter.wait(&bar.s_full[t], seen & 1);
         ++seen;
         tc::tc_fence_after();
         soften_half<T, DP>(pair, s_at, o_at, c, j == 0, m, sum, far, [&](int x, uint32_t (&s)[32]) {
@@ -317,10 +320,11 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
         __syncwarp();
         tc::mbar_arrive(&bar.p_ready[t], lane == 0);
       }
-      if (ok) ok = waiter.wait(&bar.o_full[t], outs & 1);
+      waiter.wait(&bar.o_full[t], outs & 1);
       ++outs;
       tc::tc_fence_after();
       sum += pair.other(sum);
+      const bool ok = waiter.nobody_failed();
       const int i = (2 * it.tile + t) * 128 + row, col0 = half * (DP / 2);
       const bool there = i < it.len;
       const float inv = ok ? 1.f / sum : NAN;
@@ -432,6 +436,7 @@ int launch_attention_forward(const void* q, const void* k, const void* v, void* 
   p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.dim = dim;
   // the sign goes to the product, and a scale of 0 stays a positive number, so that -inf * scale masks as ever
   p.negate = scale < 0.f;
+  p.polls = wait_polls();
   p.wide = wide_rows(out, dim);
   p.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
   return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {

@@ -85,6 +85,7 @@ struct TreeParams {
   CUtensorMap k_map, v_map;
   float scale_log2;                          // positive
   uint32_t negate;                           // the scale is negative: Q counts with its sign changed
+  uint32_t polls;                            // of a wait
   bool wide;                                 // rows of the output are 32-byte aligned
 };
 
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     if (warp == 12) tc::tmem_dealloc(tmem, 512);
     return;
   }
-  const attn::Waiter waiter{&bar.failed};
+  const attn::Waiter waiter{&bar.failed, p.polls};
   // tiles of 128 rows that a unit has
   auto row_tiles = [&](const Unit& x) { return RT == 2 && p.rows - x.block * C::kRows > 128 ? 2 : 1; };
 
@@ -590,6 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         sum = l0 * f[0] + l1 * f[1];
         if (isnan(l0) || isnan(l1)) sum = NAN;
       }
+      ok = ok && waiter.nobody_failed();
       const bool whole = !split && tile + n == u.tiles;
       // nothing seen: the sum is 0 and so is the output
       const float inv = !ok || u.bad ? NAN : !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
@@ -725,7 +727,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
   Unit u;
   int tile, rest;
   if (!part_of_cta<kFewThreads / 32>(p, bar.share, u, tile, rest)) return;
-  const attn::Waiter waiter{&bar.failed};
+  const attn::Waiter waiter{&bar.failed, p.polls};
   if (warp >= 8) {
     bring_tiles<T, DP, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange);
     return;
@@ -878,6 +880,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
     if (warp == 0) {
       const bool whole = !split && tile + n == u.tiles, strange = *static_cast<volatile int*>(&bar.strange) != 0;
       const int64_t slot = int64_t(blockIdx.x) * 2 + (split ? 0 : 1);
+      ok = ok && waiter.nobody_failed();   // none of the eight
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int r = quad + 8 * half;
@@ -1093,6 +1096,7 @@ int launch_tree(const void* q, const void* k, const void* v, const void* k_pages
   if (int64_t(batch) * kv_heads * p.row_blocks > int64_t(0x7fffffff) / joining_ctas(p, per_block)) return GDN2_ERR_TOO_LARGE;
   // the sign goes to the product, and a scale of 0 stays a positive number, so that -inf * scale masks as ever
   p.negate = scale < 0.f;
+  p.polls = attn::wait_polls();
   p.wide = attn::wide_rows(out, dim);
   p.scale_log2 = fmaxf(fabsf(scale) * attn::kLog2e, 1e-30f);
   return dtype == GDN2_BF16 ? launch_tree_dim<__nv_bfloat16>(p, stream) : launch_tree_dim<__half>(p, stream);

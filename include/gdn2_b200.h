@@ -507,6 +507,13 @@ int gdn2_attention_backward(const void* q, const void* k, const void* v, const v
                             int64_t heads, int64_t kv_heads, int64_t dim, int dtype, float scale,
                             void* stream);
 
+/*
+ * Test aid: how often a wait inside the attention kernels of later calls polls (0: it looks once; negative: as usual).
+ * A CTA in which a wait runs out ends by itself and leaves NaN in place of what it has not finished.  For the process.
+ */
+#define GDN2_ATTENTION_WAIT_POLLS (1 << 20)
+int gdn2_debug_wait_limit(int64_t polls);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif
