@@ -162,6 +162,77 @@ def spans_overlap(left: tuple[int, int], right: tuple[int, int]) -> bool:
     return left[0] < right[1] and right[0] < left[1]
 
 
+def _sums_to(terms, target, tries=20000):
+    """Whether ``target`` is a sum of ``stride * y`` with ``lo <= y <= hi`` for ``(stride, lo, hi)`` in ``terms``.  Largest
+    strides first, every choice bounded by what the smaller ones can still make up for: a try or two a stride in layouts
+    that nest.  True where that many tries do not tell."""
+
+    terms.sort(reverse=True)
+    reach = [(0, 0)]                        # least and most of the terms behind
+    for stride, lo, hi in terms[:0:-1]:
+        reach.append((reach[-1][0] + stride * lo, reach[-1][1] + stride * hi))
+    reach.reverse()
+    open_ends = [(0, target)]
+    while open_ends:
+        i, target = open_ends.pop()
+        if i == len(terms):
+            if target == 0:
+                return True
+            continue
+        (stride, lo, hi), (least, most) = terms[i], reach[i]
+        for y in range(max(lo, -((most - target) // stride)), min(hi, (target - least) // stride) + 1):
+            open_ends.append((i + 1, target - stride * y))
+            tries -= 1
+        if tries < 0:
+            return True
+    return False
+
+
+def _places(tensor: torch.Tensor):
+    """First byte, byte behind the last, and ``(bytes, size)`` of the dimensions that have more than one place."""
+
+    size = tensor.element_size()
+    lo, dims = tensor.data_ptr(), [(s * size, n) for s, n in zip(tensor.stride(), tensor.shape) if n != 1]
+    return lo, lo + sum((n - 1) * s for s, n in dims) + size if tensor.numel() else lo, dims
+
+
+def share_elements(left: torch.Tensor, right: torch.Tensor) -> bool:
+    """True when two strided tensors have a byte in common (slices of one projection have none, though their extents meet)."""
+
+    lo, end, dims = _places(left)
+    other_lo, other_end, other_dims = _places(right)
+    if not spans_overlap((lo, end), (other_lo, other_end)):
+        return False
+    ranges = {1: [1 - right.element_size(), left.element_size() - 1]}
+    for s, n in dims:
+        if s:
+            ranges.setdefault(s, [0, 0])[1] += n - 1
+    for s, n in other_dims:
+        if s:
+            ranges.setdefault(s, [0, 0])[0] -= n - 1
+    return _sums_to([(s, lo, hi) for s, (lo, hi) in ranges.items()], other_lo - lo)
+
+
+def shares_with_itself(tensor: torch.Tensor) -> bool:
+    """True when two elements of a strided tensor share a place."""
+
+    if tensor.is_contiguous() or tensor.numel() == 0:
+        return False
+    dims = sorted(_places(tensor)[2])
+    behind, nests = tensor.element_size(), True
+    for s, n in dims:
+        nests = nests and s >= behind       # every stride passes all that the smaller ones reach
+        behind += (n - 1) * s
+    if nests:
+        return False
+    reach = 0
+    for i, (s, n) in enumerate(dims):       # the largest stride in which two places differ
+        if s == 0 or any(_sums_to([(t, 1 - m, m - 1) for t, m in dims[:i]], s * y) for y in range(1, min(n - 1, reach // s) + 1)):
+            return True
+        reach += (n - 1) * s
+    return False
+
+
 def detached(tensor):
     """Storage-sharing view without an autograd edge (``None`` passes through)."""
 

@@ -13,7 +13,7 @@ import math
 
 import torch
 
-from . import _lib
+from . import _lib, _validate
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _LAYOUTS = ("half", "interleaved")
@@ -185,7 +185,8 @@ def apply_rotary(
     contiguous.  ``cos`` and ``sin`` are those of ``rotary_tables``, twice their second size channels turn.
     ``positions`` (int32 or int64, ``[B, T]`` or ``[T]``) defaults to a token's number in its sequence; packed and
     continued sequences give theirs.  A position outside the tables makes the token's rotated channels NaN.
-    Differentiable in ``q`` and ``k``; ``inplace=True`` turns the tensors themselves (no gradient) and returns them."""
+    Differentiable in ``q`` and ``k``; ``inplace=True`` turns the tensors themselves (no gradient) and returns them: slices of
+    one projection are fine, tensors that share an element are refused."""
 
     wants_grad = torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k))
     if not inplace:
@@ -200,8 +201,11 @@ def apply_rotary(
     given = q, k
     q, k = q.detach(), k.detach()
     if inplace:
-        if any(s == 0 and n > 1 for x in (q, k) for s, n in zip(x.stride(), x.shape)):
+        if _validate.shares_with_itself(q) or _validate.shares_with_itself(k) or _validate.share_elements(q, k):
             raise ValueError("inplace=True needs tensors whose elements have places of their own")
+        read = [_validate.byte_span(x) for x in (cos, sin, positions) if x is not None]
+        if any(_validate.spans_overlap(_validate.extent(x), span) for x in (q, k) for span in read):
+            raise ValueError("inplace=True needs cos, sin, and positions that do not lie in q or k")
         q_out, k_out = q, k
     else:
         q_out, k_out = _contiguous_like(q), _contiguous_like(k)

@@ -217,3 +217,30 @@ def test_many_tokens(dtype, layout, batch, time, heads, kv_heads, dim, rotated):
         inside = torch.ones(batch, time, dtype=torch.bool, device=DEV)
         inside[-1, -1] = False
         assert ((got.double() - want).abs() <= bound)[inside].all()
+
+
+def test_in_place_refuses_tensors_that_share_elements():
+    cos, sin = rotary_tables(8, 64)
+    fused = torch.randn(2, 8, 6 * 64, device=DEV).bfloat16()
+    q, k = fused[..., :4 * 64].unflatten(-1, (4, 64)), fused[..., 4 * 64:].unflatten(-1, (2, 64))
+    before = fused.clone()
+    for a, b in (
+        (q, q), (k, k), (q, q[:, :, 3:]),                                             # the same, or one with a part of it
+        (q, fused[..., 3 * 64 + 62:5 * 64 + 62].unflatten(-1, (2, 64))),              # two channels in common
+        (fused.as_strided((2, 8, 5, 64), (6 * 64 * 8, 6 * 64, 62, 1)), k[:1].expand(2, -1, -1, -1).clone()),
+        (q.contiguous(), k[:, :1].expand(-1, 8, -1, -1)),
+    ):
+        with pytest.raises(ValueError, match="places of their own"):
+            apply_rotary(a, b, cos, sin, inplace=True)
+    with pytest.raises(ValueError, match="do not lie in"):
+        whole = torch.randn(2, 8, 4, 64, device=DEV)
+        apply_rotary(whole, whole[:, :, :2].clone(), whole.view(-1)[:256].view(8, 32), sin, inplace=True)
+    assert torch.equal(fused, before)
+    want = apply_rotary(q, k, cos, sin)
+    assert apply_rotary(q, k, cos, sin, inplace=True)[0] is q
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    # heads of q and k by turns, and halves of a batch
+    pairs = torch.randn(2, 8, 3, 2, 64, device=DEV)
+    want = apply_rotary(pairs[..., 0, :], pairs[..., 1, :], cos, sin)
+    apply_rotary(pairs[..., 0, :], pairs[..., 1, :], cos, sin, inplace=True)
+    assert torch.equal(pairs[..., 0, :], want[0]) and torch.equal(pairs[..., 1, :], want[1])
