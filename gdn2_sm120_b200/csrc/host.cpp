@@ -728,6 +728,9 @@ PyObject* append_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
                              k->size(1), k->size(2), dtype_code(k->scalar_type()), at::cuda::getCurrentCUDAStream().stream());
   others.end();
   if (!ok(status, "gdn2_append_tokens", 1)) return nullptr;
+  for (const at::Tensor* x : pages) {   // a backward that has saved them must not use them any more
+    if (!x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+  }
   Py_RETURN_TRUE;
   GDN2_CATCH
 }

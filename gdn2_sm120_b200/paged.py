@@ -83,6 +83,7 @@ def append_tokens(
     _lib.call("gdn2_append_tokens", k.device, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
               slots.data_ptr(), strides, k.shape[0], k_pages.shape[0], k_pages.shape[1], heads, dim,
               _lib.dtype_code(k.dtype), _lib.stream_ptr(k.device))
+    torch.autograd.graph.increment_version((k_pages, v_pages))     # a backward that has saved them must not use them any more
     return k_pages, v_pages
 
 

@@ -210,7 +210,10 @@ def apply_rotary(
     else:
         q_out, k_out = _contiguous_like(q), _contiguous_like(k)
     _launch(q, k, q_out, k_out, cos, sin, positions, layout, False)
-    return given if inplace else (q_out, k_out)
+    if not inplace:
+        return q_out, k_out
+    torch.autograd.graph.increment_version(given)     # a backward that has saved them must not use them any more
+    return given
 
 
 __all__ = ["apply_rotary", "rotary_tables"]

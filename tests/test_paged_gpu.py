@@ -335,3 +335,26 @@ def test_append_refusals():
     ):
         with pytest.raises(error):
             append_tokens(*args)
+
+
+@pytest.mark.parametrize("batched", [False, True])
+def test_append_is_seen_by_autograd(batched):
+    """A cache that a backward has saved and that is written to afterwards gives an error, and no wrong gradient."""
+
+    k, v = (torch.randn(1, 4, 2, 64, device=DEV) for _ in range(2))
+    slots = torch.arange(4, device=DEV)[None]
+    if not batched:
+        k, v, slots = k[0], v[0], slots[0]
+    pages = [torch.zeros(3, 16, 2, 64, device=DEV) for _ in range(2)]
+    weight = torch.ones(64, device=DEV, requires_grad=True)
+    products = [(x * weight).sum() for x in pages]
+    append_tokens(k, v, *pages, slots)
+    assert all(x._version > 0 for x in pages)
+    for product in products:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.backward()
+    with torch.inference_mode():      # tensors without a version
+        cache = [x.clone() for x in pages]
+        append_tokens(k, v, *cache, slots + 5)
+    append_tokens(k, v, *cache, slots + 9)
+    assert torch.equal(cache[0].view(-1, 2, 64)[9:13], k.view(-1, 2, 64))

@@ -244,3 +244,23 @@ def test_in_place_refuses_tensors_that_share_elements():
     want = apply_rotary(pairs[..., 0, :], pairs[..., 1, :], cos, sin)
     apply_rotary(pairs[..., 0, :], pairs[..., 1, :], cos, sin, inplace=True)
     assert torch.equal(pairs[..., 0, :], want[0]) and torch.equal(pairs[..., 1, :], want[1])
+
+
+def test_in_place_is_seen_by_autograd():
+    """A tensor that a backward has saved and that is turned afterwards gives an error, and no wrong gradient."""
+
+    cos, sin = rotary_tables(8, 64)
+    q, k = _inputs(2, 8, 4, 2, 64, torch.float32)
+    weight = torch.ones(64, device=DEV, requires_grad=True)
+    product = (k * weight).sum()
+    versions = q._version, k._version
+    apply_rotary(q, k, cos, sin, inplace=True)
+    assert q._version > versions[0] and k._version > versions[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    with torch.inference_mode():      # tensors without a version
+        a, b = q.clone(), k.clone()
+        want = apply_rotary(a, b, cos, sin)
+        apply_rotary(a, b, cos, sin, inplace=True)
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+    apply_rotary(a, b, cos, sin, inplace=True)
