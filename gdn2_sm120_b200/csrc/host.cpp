@@ -714,6 +714,7 @@ PyObject* append_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   const at::Tensor *pages[2], *slots = dense(a[4], 1, at::kLong, *k);
   if (slots == nullptr || slots->size(0) != k->size(0) || !read_pages(a + 2, *k, k->size(1), k->size(2), pages)) return none();
+  if (wants_grad({k, v, pages[0], pages[1]})) return none();
   const Extent to[2] = {Extent(*pages[0]), Extent(*pages[1])};
   if (to[0].meets(to[1])) return none();
   for (const at::Tensor* x : {k, v, slots}) {

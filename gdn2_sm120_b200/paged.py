@@ -50,7 +50,8 @@ def append_tokens(
 
     ``k`` and ``v`` are ``[N, Hkv, D]`` or ``[B, T, Hkv, D]``; ``slots`` (int64, ``[N]`` or ``[B, T]``) names each
     token's place, ``page number * page + place in the page``.  A slot that is negative or behind the cache leaves the
-    token out.  Two tokens with one slot are not allowed (which of them stays is undefined).  fp16, bf16 or fp32."""
+    token out.  Two tokens with one slot are not allowed (which of them stays is undefined).  fp16, bf16 or fp32.  Inference
+    only."""
 
     if _lib.KERNEL_EVENTS is None and getattr(k, "is_cuda", False):
         if _lib.host().append_tokens(k, v, k_pages, v_pages, slots):
@@ -69,6 +70,8 @@ def append_tokens(
         raise TypeError("slots must use torch.int64")
     heads, dim = k.shape[-2:]
     _check_pages(k_pages, v_pages, k.dtype, k.device, heads, dim)
+    if torch.is_grad_enabled() and any(x.requires_grad for x in (k, v, k_pages, v_pages)):
+        raise RuntimeError("append_tokens has no gradient: call it under torch.no_grad() or with detached inputs")
     _lib.require_b200(k.device)
     spans = [_validate.byte_span(x) for x in (k_pages, v_pages)]
     if _validate.spans_overlap(*spans) or any(

@@ -358,3 +358,20 @@ def test_append_is_seen_by_autograd(batched):
         append_tokens(k, v, *cache, slots + 5)
     append_tokens(k, v, *cache, slots + 9)
     assert torch.equal(cache[0].view(-1, 2, 64)[9:13], k.view(-1, 2, 64))
+
+
+@pytest.mark.parametrize("batched", [False, True])
+@pytest.mark.parametrize("which", range(4))
+def test_append_refuses_to_drop_a_gradient(which, batched):
+    k, v = (torch.randn(1, 4, 2, 64, device=DEV) for _ in range(2))
+    slots = torch.arange(4, device=DEV)[None]
+    if not batched:
+        k, v, slots = k[0], v[0], slots[0]
+    args = [k, v, *(torch.zeros(3, 16, 2, 64, device=DEV) for _ in range(2))]
+    args[which].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        append_tokens(*args, slots)
+    assert not args[2].any()
+    with torch.no_grad():
+        append_tokens(*args, slots)
+    assert torch.equal(args[2].view(-1, 2, 64)[:4], k.view(-1, 2, 64))
