@@ -121,6 +121,7 @@ def _native(q, k, v, bounds, scale, training):
 
 
 def _attention(q, k, v, bounds, scale):
+    _validate.refuse_tangents("causal attention", q, k, v)
     if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v)):
         return _CausalAttention.apply(q, k, v, bounds, scale)
     done = _native(q, k, v, bounds, scale, False)

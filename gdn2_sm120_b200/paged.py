@@ -53,6 +53,7 @@ def append_tokens(
     token out.  Two tokens with one slot are not allowed (which of them stays is undefined).  fp16, bf16 or fp32.  Inference
     only."""
 
+    _validate.refuse_tangents("append_tokens", k, v, k_pages, v_pages)
     if _lib.KERNEL_EVENTS is None and getattr(k, "is_cuda", False):
         if _lib.host().append_tokens(k, v, k_pages, v_pages, slots):
             return k_pages, v_pages
@@ -112,6 +113,7 @@ def tree_attention(
     stay on the device: no call waits for it, and a captured graph may be replayed with other contents.  A page number
     outside the cache or a length beyond ``columns`` pages makes the sequence's output NaN.  Inference only."""
 
+    _validate.refuse_tangents("tree_attention", q, k, v, k_pages, v_pages)
     if _lib.KERNEL_EVENTS is None and getattr(q, "is_cuda", False):
         done = _lib.host().tree_attention(q, k, v, k_pages, v_pages, page_table, lengths, mask, scale)
         if done is not None:

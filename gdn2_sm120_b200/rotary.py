@@ -188,6 +188,7 @@ def apply_rotary(
     Differentiable in ``q`` and ``k``; ``inplace=True`` turns the tensors themselves (no gradient) and returns them: slices of
     one projection are fine, tensors that share an element are refused."""
 
+    _validate.refuse_tangents("apply_rotary", q, k, cos, sin)
     wants_grad = torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k))
     if not inplace:
         if wants_grad:

@@ -109,3 +109,27 @@ def test_tree_attention_refuses_more_tokens_than_31_bits_number():
     # each side alone would fit an int, both together would not
     assert tree(drafted=2 ** 29, columns=2 ** 26) == -9
     assert tree(drafted=1, columns=2 ** 26) == -9 and tree(drafted=2 ** 30, columns=1) == -9
+
+
+def test_forward_mode_tangents_are_refused():
+    """They would be dropped in silence: no kernel has a forward-mode derivative."""
+
+    from torch.autograd import forward_ad
+
+    q, k = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16), torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16)
+    cos, sin = rotary_tables(4, 64, device="cpu")
+    pages = torch.zeros(2, 16, 1, 64, dtype=torch.bfloat16)
+    table, lengths = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    calls = (lambda x: causal_attention(q, x, k), lambda x: causal_attention_varlen(q, k, x, (0, 4)), lambda x: apply_rotary(q, x, cos, sin),
+             lambda x: apply_rotary(q, x, cos, sin, inplace=True), lambda x: append_tokens(x, k, pages, pages.clone(), torch.zeros(1, 4).long()),
+             lambda x: tree_attention(q, x, k, pages, pages.clone(), table, lengths))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(k.clone(), torch.ones_like(k))
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(dual)
+            with pytest.raises(ValueError, match="CUDA"):      # no tangent: the usual refusal of this test's tensors
+                call(k)
+    for call in calls:
+        with pytest.raises(ValueError, match="CUDA"):
+            call(k)
