@@ -375,3 +375,16 @@ def test_append_refuses_to_drop_a_gradient(which, batched):
     with torch.no_grad():
         append_tokens(*args, slots)
     assert torch.equal(args[2].view(-1, 2, 64)[:4], k.view(-1, 2, 64))
+
+
+@pytest.mark.parametrize("drafted,heads", [(2, 8), (20, 4), (40, 16)])
+@pytest.mark.parametrize("scale", [-0.3, -1.5, 0.0, -1e-30])
+def test_signs_and_zeros_of_the_scale(drafted, heads, scale):
+    """8, 40 and 320 rows of a key head, over a cache that several CTAs share."""
+
+    cache = _cache((2500, 90), 16, 2, 64, BF16)
+    q, k, v = _fresh(2, drafted, heads, 2, 64, BF16)
+    mask = _tree(2, drafted)
+    out = tree_attention(q, k, v, *cache, mask, scale=scale)
+    _check(out, q, k, v, cache, mask, scale or 1e-300)      # (_check takes a scale of 0 for none; 1e-300 weighs all alike, too)
+    assert torch.equal(out, tree_attention(-q, k, v, *cache, mask, scale=-scale))
