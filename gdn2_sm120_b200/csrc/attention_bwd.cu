@@ -885,7 +885,7 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   p.negate = scale < 0.f;
   p.polls = wait_polls();
   p.wide = wide_rows(dq, dim) && wide_rows(dk, dim) && wide_rows(dv, dim);
-  p.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
+  p.scale_log2 = positive_scale(scale);
   return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {
     DeltaParams d{out, d_out, {strides[9], strides[10], strides[11]}, delta, heads, dim, p.seq};
     if (dtype == GDN2_BF16) {

@@ -4,6 +4,9 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <limits>
 
 #include "chunk_common.cuh"
 #include "tc05.cuh"
@@ -12,6 +15,11 @@ namespace gdn2 {
 namespace attn {
 
 constexpr float kLog2e = 1.4426950408889634f;
+// The scale of scores in powers of two: its sign goes to a product.  One of 0 becomes the smallest positive number, so that
+// -inf * scale masks as ever (no score makes more than 2^-21 of it), and the largest ones stay finite.
+inline float positive_scale(float scale) {
+  return fminf(fmaxf(fabsf(scale) * kLog2e, std::numeric_limits<float>::denorm_min()), FLT_MAX);
+}
 constexpr int kTileRows = 256;   // query rows of a work item of the forward: two tiles of 128
 constexpr int kMaxSequences = GDN2_PACKED_MAX_SEQUENCES;   // in a launch, whose parameters hold their table
 

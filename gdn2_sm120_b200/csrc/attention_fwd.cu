@@ -434,11 +434,10 @@ int launch_attention_forward(const void* q, const void* k, const void* v, void* 
   for (int i = 0; i < 3; ++i) p.strides[i] = strides[6 + i];
   p.out = out; p.lse = lse;
   p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.dim = dim;
-  // the sign goes to the product, and a scale of 0 stays a positive number, so that -inf * scale masks as ever
   p.negate = scale < 0.f;
   p.polls = wait_polls();
   p.wide = wide_rows(out, dim);
-  p.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
+  p.scale_log2 = positive_scale(scale);
   return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {
     p.items = int64_t(p.seq.tiles) * heads;
     if (dtype == GDN2_BF16) return dim <= 64 ? launch_typed<__nv_bfloat16, 64>(p, stream) : launch_typed<__nv_bfloat16, 128>(p, stream);

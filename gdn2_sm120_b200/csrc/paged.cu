@@ -1094,11 +1094,10 @@ int launch_tree(const void* q, const void* k, const void* v, const void* k_pages
   const int status = tree_ctas(&p.ctas);
   if (status != GDN2_OK) return status;
   if (int64_t(batch) * kv_heads * p.row_blocks > int64_t(0x7fffffff) / joining_ctas(p, per_block)) return GDN2_ERR_TOO_LARGE;
-  // the sign goes to the product, and a scale of 0 stays a positive number, so that -inf * scale masks as ever
   p.negate = scale < 0.f;
   p.polls = attn::wait_polls();
   p.wide = attn::wide_rows(out, dim);
-  p.scale_log2 = fmaxf(fabsf(scale) * attn::kLog2e, 1e-30f);
+  p.scale_log2 = attn::positive_scale(scale);
   return dtype == GDN2_BF16 ? launch_tree_dim<__nv_bfloat16>(p, stream) : launch_tree_dim<__half>(p, stream);
 }
 

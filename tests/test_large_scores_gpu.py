@@ -114,3 +114,29 @@ def test_causal_gradients(dtype, exponent, scale, way, lengths, heads, dim):
                                do[0, lo:hi].transpose(0, 1))
         for name, x in zip(("o", "dq", "dk", "dv"), (out.detach(), *grads)):
             exact.check(f"{name}, rows {lo} to {hi}", x[0, lo:hi], *want[name])
+
+
+@pytest.mark.parametrize("scale,size", [(0.0, 2.0 ** 127), (2.0 ** -130, 2.0 ** 127), (-2.0 ** -126, 2.0 ** 126), (3e38, 0.0), (-3e38, 0.0),
+                                        (2.0 ** 127, 2.0 ** -126)])
+@pytest.mark.parametrize("drafted,heads", [(2, 8), (20, 4), (40, 16)])
+def test_scales_of_any_size(scale, size, drafted, heads):
+    """Scores of up to some units from products and scales at the ends of the 32-bit range, and a scale of 0."""
+
+    kv_heads, dim, cached = 2, 64, 300
+    total = cached + drafted
+    q, v = _normal((1, total, heads, dim), BF16, 1), _normal((1, total, kv_heads, dim), BF16, 2)
+    k = torch.zeros_like(v)
+    q.zero_()
+    steps = torch.randint(-4, 5, (total,), generator=torch.Generator(device=DEV).manual_seed(7), device=DEV) / 4.0
+    if size:
+        exponent = round(torch.log2(torch.tensor(size)).item())
+        q[..., 0] = 2.0 ** (exponent // 2)
+        k[..., 0] = (steps * 2.0 ** (exponent - exponent // 2))[:, None].to(BF16)
+    want = exact.attention(*(x[0].transpose(0, 1) for x in (q, k, v)), exact.causal(total, DEV), scale)["o"]
+    exact.check("causal", causal_attention(q, k, v, scale=scale)[0], *want)
+    pages = [torch.zeros(19, 16, kv_heads, dim, device=DEV, dtype=BF16) for _ in range(2)]
+    for to, x in zip(pages, (k, v)):
+        to.view(-1, kv_heads, dim)[:cached] = x[0, :cached]
+    out = tree_attention(*(x[:, cached:].contiguous() for x in (q, k, v)), *pages, torch.arange(19, device=DEV, dtype=torch.int32)[None],
+                         torch.tensor([cached], device=DEV, dtype=torch.int32), scale=scale)
+    exact.check("tree", out[0], *(x[:, cached:] for x in want))
