@@ -3,10 +3,15 @@
 ``causal_attention``          a batch of equally long sequences
 ``causal_attention_varlen``   sequences of any lengths packed along time, as in ``chunk_gdn2_varlen``
 
-Both are differentiable and run on the tensor cores (csrc/attention_fwd.cu, csrc/attention_bwd.cu): scores, weights and
-sums are in 32 bits, weights are rounded to the inputs' type for their product with the values.  ``Hq`` query heads share
-``Hkv`` key and value heads in groups of ``Hq / Hkv`` consecutive ones; the gradients of a shared head are summed in 32
-bits before they are rounded.
+Both are differentiable and run on the tensor cores (csrc/attention_fwd.cu, csrc/attention_bwd.cu): scores, statistics and
+sums are in 32 bits.  What goes into a product is rounded to the inputs' type, which is what the tensor cores take: the
+weights P for their product with the values (exponentials are good to 2^-17), and in the backward P and the slopes dS = P (dP -
+delta); delta_i = do_i . o_i is taken from the output as it was returned.  ``Hq`` query heads share ``Hkv`` key and value
+heads in groups of ``Hq / Hkv`` consecutive ones; the gradients of a shared head are summed in 32 bits before they are rounded.
+
+An output depends on what its row sees and on nothing else, whatever the tensors hold elsewhere.  Gradients do where q, k and the
+cotangent are finite.  A key that is not also reaches dq, in its channel, of the rows before it in its tile of 128 tokens; a query
+that is not reaches dk, and a cotangent dv, of the keys behind it in its tile.
 """
 
 from __future__ import annotations

@@ -12,6 +12,10 @@
 // error in the 2-norm is that of its own rounding and of one of these, 1.4 times a rounding of the exact gradient, and up to
 // 1.8 times in sequences of a few tokens, where the output's rounding in delta counts as much.
 //
+// P and dS are 0 by selection where a row does not see a key.  In the tiles on the diagonal their products meet those rows of k,
+// q and do all the same, and 0 * inf and 0 * NaN are not 0: a key that is not finite reaches dq, in its channel, of the rows
+// before it in its tile, a query dk and a cotangent dv of the keys behind it there.  (Another sequence's rows never.)
+//
 // Training 4 x 2048 tokens, 16 heads of 128 channels, 4 heads a group: delta 12 us, keys 129, queries 116, forward 85.
 
 #include <algorithm>

@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+import attention_bounds as exact
 from gdn2_sm120_b200.attention import causal_attention, causal_attention_varlen
 
 pytestmark = pytest.mark.gpu
@@ -95,3 +96,48 @@ def test_inf_and_minus_inf_that_a_row_sees_both():
     v[0, 10, 0, 3], v[0, 200, 0, 3], v[0, 290, 0, 3] = math.inf, math.inf, -math.inf
     out = causal_attention(q, k, v)[0, :, :, 3]
     assert torch.isfinite(out[:10]).all() and torch.isposinf(out[10:290]).all() and torch.isnan(out[290:]).all()
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("which", ["q", "k", "v", "do"])
+@pytest.mark.parametrize("time,at", [(700, 300), (700, 0), (700, 383), (130, 129)])
+def test_gradients_of_rows_that_do_not_see_it(which, value, time, at):
+    """A value that is not finite makes the gradients of what it is part of not finite: its own row, the rows that see it and
+    the keys that those see.  Beyond that, a key reaches dq, in its channel, of the rows before it in its tile of 128 tokens; a
+    query reaches dk, and a cotangent dv, of the keys behind it in its tile.  Everything else is as it was: to the bit where
+    no score is infinite (one that is lets the rows of its tile look for their maxima more often, which rounds differently)."""
+
+    channel, head, kv_head = 5, 1, 0
+    q, k, v = _inputs(1, time, 4, 2, 64, BF16, seed=3)
+    do = _inputs(1, time, 4, 2, 64, BF16, seed=4)[0]
+    tensors = dict(q=q, k=k, v=v, do=do)
+
+    def run():
+        leaves = [tensors[x].detach().requires_grad_(True) for x in "qkv"]
+        out = causal_attention(*leaves)
+        return dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, tensors["do"])))
+
+    clean = run()
+    tensors[which] = tensors[which].clone()
+    tensors[which][0, at, head if which in ("q", "do") else kv_head, channel] = value
+    got = run()
+    tile = slice(at // 128 * 128, at // 128 * 128 + 128)
+    may = {x: torch.zeros_like(y, dtype=torch.bool) for x, y in clean.items()}
+    if which in ("q", "do"):       # row `at` of head 1, and what it sees
+        may["dq"][0, at, head] = True
+        may["dk"][0, :at + 1, kv_head] = may["dv"][0, :at + 1, kv_head] = True
+        may["dk" if which == "q" else "dv"][0, tile, kv_head, channel] = True
+    else:                           # every row from `at` on of the heads 0 and 1, and what those see
+        may["dq"][0, at:, :2] = True
+        may["dk"][0, :, kv_head] = may["dv"][0, :, kv_head] = True
+        if which == "k":
+            may["dq"][0, tile, :2, channel] = True
+    want = exact.attention(*(x[0].transpose(0, 1) for x in (q, k, v)), exact.causal(time, DEV), 64 ** -0.5, do[0].transpose(0, 1))
+    for x in clean:
+        untouched = ~may[x]
+        if math.isnan(value) or which in ("v", "do"):
+            assert torch.equal(got[x][untouched], clean[x][untouched]), x
+        off, bound = (got[x][0].double() - want[x][0].transpose(0, 1)).abs(), want[x][1].transpose(0, 1)
+        assert (off <= bound)[untouched[0]].all(), x
+    if math.isnan(value):           # (a score of -inf, or values alone, leave the weights that dv is made of finite)
+        assert torch.isnan(got["dk" if which == "v" else "dv"][0, at, kv_head, channel])
