@@ -42,7 +42,11 @@ def rotary_tables(
                   times as slowly, the fastest as before
     ``"yarn"``    a pair that turns ``r`` times in ``trained`` positions keeps its speed from ``r = fast`` on, is slowed
                   ``factor`` times up to ``r = slow``, and lies linearly between the two in between; cosines and sines
-                  are multiplied by ``1 + 0.1 ln(factor)``, which sharpens the softmax
+                  are multiplied by ``1 + 0.1 ln(factor)``, which sharpens the softmax.  Linearly in ``r``, that is, as the
+                  method is defined; there are models whose tables are linear in the pair's number ``i`` between the pairs
+                  that turn ``fast`` and ``slow`` times.  Both agree at the ends but not in between (128 channels, base 10000,
+                  4096 positions, factor 8: pair 33 turns 0.46 times as fast here as there), so a model needs the tables that
+                  it was trained with
     """
 
     if isinstance(positions, bool) or not isinstance(positions, int) or positions <= 0:

@@ -264,3 +264,19 @@ def test_in_place_is_seen_by_autograd():
         apply_rotary(a, b, cos, sin, inplace=True)
         assert torch.equal(a, want[0]) and torch.equal(b, want[1])
     apply_rotary(a, b, cos, sin, inplace=True)
+
+
+def test_the_ramp_of_yarn_is_linear_in_a_pairs_turns():
+    rotated, base, trained, factor, fast, slow = 128, 10000.0, 4096, 8.0, 32.0, 1.0
+    cos, sin = rotary_tables(2, rotated, base=base, scaling="yarn", factor=factor, trained=trained, fast=fast, slow=slow)
+    got = torch.atan2(sin[1].double(), cos[1].double()).cpu()            # an angle of at most 1: that of position 1
+    between = 0
+    for i in range(rotated // 2):
+        speed = base ** (-2.0 * i / rotated)
+        turns = trained * speed / (2.0 * math.pi)
+        share = min(1.0, max(0.0, (turns - slow) / (fast - slow)))
+        between += 0.0 < share < 1.0
+        want = share * speed + (1.0 - share) * speed / factor
+        # cosine and sine rounded to 32 bits, relative to the amplitude
+        assert abs(got[i] - want) <= 2.0 ** -23 * (1.0 + want), i
+    assert between > 20
