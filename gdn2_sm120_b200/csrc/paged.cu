@@ -241,10 +241,12 @@ __device__ __forceinline__ void tma_load_page(uint32_t to, const CUtensorMap* ma
 
 // The keys and values of all tiles of a CTA, brought in by kWarps warps that share the rows of every tile, in the order K0,
 // K1 V0, K2 V1, ... of a unit, into kStages places by turns.  full[] counts all their threads, empty[] says that a place has
-// been used.
+// been used.  *strange says that a drafted token had a value that is not finite, strange_rows (may be null) which: a bit for
+// every token modulo kStrangeRows.
+constexpr int kStrangeRows = 2048;
 template <typename T, int DP, int kStages, int kWarps>
 __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int tile, int rest, int warp, uint32_t kv_base, uint64_t* full,
-                                            uint64_t* empty, const attn::Waiter& waiter, int* strange) {
+                                            uint64_t* empty, const attn::Waiter& waiter, int* strange, uint32_t* strange_rows) {
   constexpr int kTileBytes = kTile * DP * 2;
   constexpr uint32_t kSlab = kTile * 128;
   constexpr int kMine = kTile / kWarps, kParts = kMine / 32;
@@ -306,7 +308,11 @@ __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int til
     if (!keys && t0 + kMine > u.length) {
       cp_async_wait_all();
       // a drafted token's values that are not finite are added to the rows that see them
-      attn::sift<T, DP>(base, kSlab, mine + max(0, u.length - t0), mine + kMine, [&](int) { *static_cast<volatile int*>(strange) = 1; });
+      attn::sift<T, DP>(base, kSlab, mine + max(0, u.length - t0), mine + kMine, [&](int row) {
+        *static_cast<volatile int*>(strange) = 1;
+        const int d = tile * kTile + row - u.length;
+        if (strange_rows != nullptr) atomicOr(&strange_rows[d % kStrangeRows >> 5], 1u << (d & 31));
+      });
       tc::mbar_arrive(&full[s]);
     } else {
       cp_async_arrive(&full[s]);
@@ -358,6 +364,7 @@ struct TreeBars {
   uint32_t tmem;
   int failed;
   int strange;          // a drafted value was infinite or NaN
+  uint32_t strange_rows[kStrangeRows / 32];
 };
 static_assert(sizeof(TreeBars) <= 768, "");
 
@@ -390,6 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     bar.failed = bar.strange = 0;
     tc::fence_mbar_init();
   }
+  if (tid < kStrangeRows / 32) bar.strange_rows[tid] = 0;
   if (warp == 12) {
     tc::tmem_alloc(&bar.tmem, 512);
     tc::tmem_relinquish();
@@ -520,7 +528,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       }
       cp_async_wait_all();
     } else if (warp < 12) {
-      bring_tiles<T, DP, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange);
+      bring_tiles<T, DP, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange,
+                                              bar.strange_rows);
     }
   } else {
     // ---- weights: a row a thread ---------------------------------------------------------------------------
@@ -621,13 +630,31 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           }
           if (!there) continue;
           if (strange) {
-            for (int d = max(0, tile * kTile - u.length); d < min(p.drafted, (tile + n) * kTile - u.length); ++d) {
-              if (!(p.mask == nullptr ? d <= token : p.mask[u.b * p.mask_stride + int64_t(token) * p.drafted + d] != 0)) continue;
-              const T* v = static_cast<const T*>(p.v) + u.b * p.v_stride[0] + d * p.v_stride[1] + u.head * p.v_stride[2];
+            // of the drafted tokens in this CTA's tiles of the unit those that had such a value in some unit
+            const int first = max(0, tile * kTile - u.length);
+            const int last = min(p.mask == nullptr ? token + 1 : p.drafted, (tile + n) * kTile - u.length);
+            bool done = false;          // all channels are NaN
+            for (int d0 = first & ~31; d0 < last && !done; d0 += 32) {
+              for (uint32_t bits = bar.strange_rows[d0 % kStrangeRows >> 5]; bits != 0 && !done; bits &= bits - 1) {
+                const int d = d0 + __ffs(bits) - 1;
+                if (d < first || d >= last) continue;
+                if (p.mask != nullptr && p.mask[u.b * p.mask_stride + int64_t(token) * p.drafted + d] == 0) continue;
+                const T* v = static_cast<const T*>(p.v) + u.b * p.v_stride[0] + d * p.v_stride[1] + u.head * p.v_stride[2] + x;
 #pragma unroll
-              for (int y = 0; y < 16; ++y) {
-                const float value = x + y < p.dim ? to_float(v[x + y]) : 0.f;
-                if (!isfinite(value)) o[y] += value;
+                for (int y = 0; y < 16; y += 8) {
+                  if (x + y >= p.dim) continue;
+                  const uint4 raw = *reinterpret_cast<const uint4*>(v + y);
+                  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                  for (int z = 0; z < 4; ++z) {
+                    const float2 value = unpack2<T>(w[z]);
+                    if (!isfinite(value.x)) o[y + 2 * z] += value.x;
+                    if (!isfinite(value.y)) o[y + 2 * z + 1] += value.y;
+                  }
+                }
+                done = true;
+#pragma unroll
+                for (int y = 0; y < 16; ++y) done = done && isnan(o[y]);
               }
             }
           }
@@ -729,7 +756,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
   if (!part_of_cta<kFewThreads / 32>(p, bar.share, u, tile, rest)) return;
   const attn::Waiter waiter{&bar.failed, p.polls};
   if (warp >= 8) {
-    bring_tiles<T, DP, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange);
+    bring_tiles<T, DP, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange, nullptr);
     return;
   }
 

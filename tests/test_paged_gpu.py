@@ -388,3 +388,27 @@ def test_signs_and_zeros_of_the_scale(drafted, heads, scale):
     out = tree_attention(q, k, v, *cache, mask, scale=scale)
     _check(out, q, k, v, cache, mask, scale or 1e-300)      # (_check takes a scale of 0 for none; 1e-300 weighs all alike, too)
     assert torch.equal(out, tree_attention(-q, k, v, *cache, mask, scale=-scale))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("drafted,heads,cached", [(9, 4, 40), (200, 4, (130, 1000)), (2500, 2, (60, 700)), (4300, 2, (0,))])
+def test_drafts_that_are_not_finite_in_long_chains(dtype, drafted, heads, cached):
+    """Values that are not finite reach the channels and rows that see them, and not one bit of anything else, in chains of more
+    tokens than are told apart at once, too."""
+
+    cached = (cached,) if isinstance(cached, int) else cached
+    cache = _cache(cached, 16, 2, 64, dtype)
+    q, k, v = _fresh(len(cached), drafted, heads, 2, 64, dtype)
+    clean = tree_attention(q, k, v, *cache)
+    reached = torch.zeros_like(clean, dtype=torch.bool)
+    nan = torch.zeros_like(reached)
+    group = heads // 2
+    for b, token, head, channel, what in ((0, drafted - 1, 0, 3, math.nan), (0, drafted // 2, 1, 40, math.inf), (len(cached) - 1, 5, 0, 63, -math.inf),
+                                          (0, drafted // 2 + 1, 1, 40, -math.inf), (0, drafted // 3, 1, 8, math.nan)):
+        v[b, token, head, channel] = what
+        at = (b, slice(token, drafted), slice(head * group, (head + 1) * group), channel)
+        nan[at] |= reached[at] | math.isnan(what)
+        reached[at] = True
+    out = tree_attention(q, k, v, *cache)
+    assert torch.equal(out[~reached], clean[~reached])
+    assert torch.isnan(out[nan]).all() and torch.isinf(out[reached & ~nan]).all()
