@@ -71,15 +71,33 @@ struct FwdMarks {
 // a bit for every row of the two tiles from v on that held such a value.
 template <typename T>
 __device__ __noinline__ void add_strange(const T* v, int64_t stride, const uint32_t* strange, int seen, T* to, int channels) {
-  for (int j = 0; j <= seen; ++j) {
-    if (((strange[j >> 5] >> (j & 31)) & 1) == 0) continue;
-    for (int x = 0; x < channels; x += 8) {
-      uint4 raw = *reinterpret_cast<const uint4*>(v + j * stride + x);
-      const T* value = reinterpret_cast<const T*>(&raw);
-      for (int y = 0; y < 8; ++y) {
-        if (!isfinite(to_float(value[y]))) to[x + y] = from_float<T>(to_float(to[x + y]) + to_float(value[y]));
+#pragma unroll 1
+  for (int x = 0; x < channels; x += 8) {
+    uint4 out = *reinterpret_cast<const uint4*>(to + x);
+    uint32_t(&w)[4] = reinterpret_cast<uint32_t(&)[4]>(out);
+    float o[8];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) { const float2 u = unpack2<T>(w[y]); o[2 * y] = u.x; o[2 * y + 1] = u.y; }
+    bool done = false;      // all of them are NaN
+    for (int j0 = 0; j0 <= seen; j0 += 32) {
+      uint32_t bits = strange[j0 >> 5];
+      if (seen - j0 < 31) bits &= (2u << (seen - j0)) - 1u;
+      for (; bits != 0 && !done; bits &= bits - 1) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(v + (j0 + __ffs(bits) - 1) * stride + x);
+        const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
+        done = true;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float2 u = unpack2<T>(r[y]);
+          if (!isfinite(u.x)) o[2 * y] += u.x;
+          if (!isfinite(u.y)) o[2 * y + 1] += u.y;
+          done = done && isnan(o[2 * y]) && isnan(o[2 * y + 1]);
+        }
       }
     }
+#pragma unroll
+    for (int y = 0; y < 4; ++y) w[y] = pack_pair<T>(o[2 * y], o[2 * y + 1]);
+    *reinterpret_cast<uint4*>(to + x) = out;
   }
 }
 
