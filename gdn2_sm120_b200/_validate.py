@@ -234,13 +234,38 @@ def shares_with_itself(tensor: torch.Tensor) -> bool:
     return False
 
 
-def refuse_tangents(what: str, *tensors) -> None:
-    """Raise where a tensor is a dual one of forward-mode differentiation, whose tangent the kernels would drop."""
+def heads_in_place(q: torch.Tensor, k: torch.Tensor, read) -> None:
+    """Raise where two ``[B, T, H, D]`` tensors of one type, which a call writes to, share elements, or overlap what it reads
+    (contiguous tensors)."""
 
-    # (outside a dual level, where this is all there is, the call costs 0.1 us)
-    if getattr(forward_ad, "_current_level", 0) >= 0:
-        if any(isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
-            raise RuntimeError(f"{what} has no forward-mode derivative: call it with the primal tensors")
+    size, a, b = q.element_size(), q.data_ptr(), k.data_ptr()
+    q_stride, k_stride = q.stride(), k.stride()
+    batch, time, heads, dim = q.shape
+    first, second = (heads, k.shape[2]) if a <= b else (k.shape[2], heads)
+    span = abs(a - b) // size + second * dim
+    reach = span + (time - 1) * q_stride[1]
+    if (q_stride[2:] == (dim, 1) == k_stride[2:] and span >= (first + second) * dim
+            and (time == 1 or span <= q_stride[1] == k_stride[1]) and (batch == 1 or reach <= q_stride[0] == k_stride[0])):
+        # slices of one projection: a token's heads of both lie behind one another, then comes the next token
+        spans = [(min(a, b), min(a, b) + (reach + (batch - 1) * q_stride[0]) * size)]
+    else:
+        spans = [byte_span(x) if x.is_contiguous() else extent(x) for x in (q, k)]
+        if shares_with_itself(q) or shares_with_itself(k) or (spans_overlap(*spans) and share_elements(q, k)):
+            raise ValueError("inplace=True needs tensors whose elements have places of their own")
+    for x in read:
+        if x is not None:
+            lo, end = byte_span(x)
+            for from_, to in spans:
+                if lo < to and from_ < end:
+                    raise ValueError("inplace=True needs cos, sin, and positions that do not lie in q or k")
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """Raise where a tensor is a dual one of forward-mode differentiation, whose tangent the kernels would drop.  To be called
+    where ``forward_ad._current_level`` is not negative: asking for that costs a small call nothing."""
+
+    if any(isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative: call it with the primal tensors")
 
 
 def detached(tensor):

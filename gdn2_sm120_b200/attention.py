@@ -17,6 +17,7 @@ that is not reaches dk, and a cotangent dv, of the keys behind it in its tile.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, _validate
 from .varlen import _bounds
@@ -126,7 +127,8 @@ def _native(q, k, v, bounds, scale, training):
 
 
 def _attention(q, k, v, bounds, scale):
-    _validate.refuse_tangents("causal attention", q, k, v)
+    if forward_ad._current_level >= 0:
+        _validate.refuse_tangents("causal attention", q, k, v)
     if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v)):
         return _CausalAttention.apply(q, k, v, bounds, scale)
     done = _native(q, k, v, bounds, scale, False)

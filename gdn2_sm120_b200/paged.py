@@ -15,6 +15,7 @@ A step of speculative decoding: ``tree_attention`` with the drafts' keys and val
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, _validate
 
@@ -53,7 +54,8 @@ def append_tokens(
     token out.  Two tokens with one slot are not allowed (which of them stays is undefined).  fp16, bf16 or fp32.  Inference
     only."""
 
-    _validate.refuse_tangents("append_tokens", k, v, k_pages, v_pages)
+    if forward_ad._current_level >= 0:
+        _validate.refuse_tangents("append_tokens", k, v, k_pages, v_pages)
     if _lib.KERNEL_EVENTS is None and getattr(k, "is_cuda", False):
         if _lib.host().append_tokens(k, v, k_pages, v_pages, slots):
             return k_pages, v_pages
@@ -71,7 +73,7 @@ def append_tokens(
         raise TypeError("slots must use torch.int64")
     heads, dim = k.shape[-2:]
     _check_pages(k_pages, v_pages, k.dtype, k.device, heads, dim)
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (k, v, k_pages, v_pages)):
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise RuntimeError("append_tokens has no gradient: call it under torch.no_grad() or with detached inputs")
     _lib.require_b200(k.device)
     spans = [_validate.byte_span(x) for x in (k_pages, v_pages)]
@@ -113,7 +115,8 @@ def tree_attention(
     stay on the device: no call waits for it, and a captured graph may be replayed with other contents.  A page number
     outside the cache or a length beyond ``columns`` pages makes the sequence's output NaN.  Inference only."""
 
-    _validate.refuse_tangents("tree_attention", q, k, v, k_pages, v_pages)
+    if forward_ad._current_level >= 0:
+        _validate.refuse_tangents("tree_attention", q, k, v, k_pages, v_pages)
     if _lib.KERNEL_EVENTS is None and getattr(q, "is_cuda", False):
         done = _lib.host().tree_attention(q, k, v, k_pages, v_pages, page_table, lengths, mask, scale)
         if done is not None:

@@ -12,6 +12,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, _validate
 
@@ -192,7 +193,8 @@ def apply_rotary(
     Differentiable in ``q`` and ``k``; ``inplace=True`` turns the tensors themselves (no gradient) and returns them: slices of
     one projection are fine, tensors that share an element are refused."""
 
-    _validate.refuse_tangents("apply_rotary", q, k, cos, sin)
+    if forward_ad._current_level >= 0:
+        _validate.refuse_tangents("apply_rotary", q, k, cos, sin)
     wants_grad = torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k))
     if not inplace:
         if wants_grad:
@@ -206,11 +208,7 @@ def apply_rotary(
     given = q, k
     q, k = q.detach(), k.detach()
     if inplace:
-        if _validate.shares_with_itself(q) or _validate.shares_with_itself(k) or _validate.share_elements(q, k):
-            raise ValueError("inplace=True needs tensors whose elements have places of their own")
-        read = [_validate.byte_span(x) for x in (cos, sin, positions) if x is not None]
-        if any(_validate.spans_overlap(_validate.extent(x), span) for x in (q, k) for span in read):
-            raise ValueError("inplace=True needs cos, sin, and positions that do not lie in q or k")
+        _validate.heads_in_place(q, k, (cos, sin, positions))
         q_out, k_out = q, k
     else:
         q_out, k_out = _contiguous_like(q), _contiguous_like(k)

@@ -56,3 +56,37 @@ def test_slices_of_one_projection():
                                                 ((2, 2), (3, 2), False), ((3, 3), (3, 2), False), ((3, 4), (3, 2), True), ((3, 4, 2), (8, 2, 1), False)])
 def test_one_tensor(size, stride, shared):
     assert _validate.shares_with_itself(torch.zeros(100).as_strided(size, stride)) == shared
+
+
+def test_heads_in_place_against_all_addresses():
+    """What is refused of random pairs of [B, T, H, D] views is what shares an element."""
+
+    rng = random.Random(1)
+    base = torch.zeros(3000, dtype=torch.int16)
+    apart = torch.zeros(4)
+    seen = {True: 0, False: 0}
+    for _ in range(4000):
+        batch, time, dim = rng.choice([1, 2, 3]), rng.choice([1, 2, 4]), rng.choice([1, 2, 4])
+        heads = [rng.choice([1, 2, 3]) for _ in range(2)]
+        if rng.random() < 0.7:       # slices of one projection, cut at places that need not be right
+            row = max(1, rng.choice([sum(heads) * dim, sum(heads) * dim + rng.randrange(-3, 8)]))
+            strides = [(rng.choice([time * row, time * row + 3, max(1, time * row - 2)]), row, dim, 1)] * 2
+            at = [0, rng.choice([heads[0] * dim, heads[0] * dim + rng.randrange(-2, 3)])]
+        else:
+            strides = [tuple(rng.choice([0, 1, 2, 4, 8, 16, 48]) for _ in range(4)) for _ in range(2)]
+            at = [0, rng.randrange(200)]
+        if rng.random() < 0.5:
+            at.reverse()
+        views = [base.as_strided((batch, time, h, dim), s, max(0, x)) for h, s, x in zip(heads, strides, at)]
+        places = [_bytes(x) for x in views]
+        want = len(set(places[0] + places[1])) < len(places[0]) + len(places[1])
+        if want:
+            with pytest.raises(ValueError, match="places of their own"):
+                _validate.heads_in_place(*views, (apart, apart, None))
+        else:
+            _validate.heads_in_place(*views, (apart, apart, None))
+            inside = base[views[1].storage_offset():views[1].storage_offset() + 1]
+            with pytest.raises(ValueError, match="do not lie in"):
+                _validate.heads_in_place(*views, (apart, inside, None))
+        seen[want] += 1
+    assert min(seen.values()) > 500
