@@ -422,6 +422,40 @@ struct KeyBars {
   int failed;
 };
 
+// A thread's share of a step in which a query's reference is far away: P and dS as below, with weights as in far_weight; the
+// key sees its queries from `from` on.  False where a wait ran out.
+template <typename T>
+__device__ __noinline__ bool far_step(KeyBars& bar, const Waiter& waiter, uint32_t parity, uint32_t s_at, uint32_t dp_at, const float* st,
+                                      const float* shifts, float c, int from) {
+  float e[32];
+  uint32_t w[16], x[32];
+  tc::tmem_ld32(s_at, x);
+  tc::tmem_wait_ld();
+#pragma unroll
+  for (int y = 0; y < 32; ++y) e[y] = y < from ? 0.f : far_weight(x[y], st[y], shifts + y, c);
+#pragma unroll
+  for (int y = 0; y < 16; ++y) w[y] = pack_pair<T>(e[2 * y], e[2 * y + 1]);
+  tc::tmem_st16(s_at, w);
+  tc::tmem_wait_st();
+  tc::tc_fence_before();
+  __syncwarp();
+  tc::mbar_arrive(&bar.p_ready, (threadIdx.x & 31) == 0);
+  if (!waiter.wait(&bar.dp_full, parity)) return false;
+  tc::tc_fence_after();
+  tc::tmem_ld32(dp_at, x);
+  tc::tmem_wait_ld();
+#pragma unroll
+  for (int y = 0; y < 32; ++y) e[y] = y < from ? 0.f : e[y] * (__uint_as_float(x[y]) + st[128 + y]);
+#pragma unroll
+  for (int y = 0; y < 16; ++y) w[y] = pack_pair<T>(e[2 * y], e[2 * y + 1]);
+  tc::tmem_st16(dp_at, w);
+  tc::tmem_wait_st();
+  tc::tc_fence_before();
+  __syncwarp();
+  tc::mbar_arrive(&bar.ds_ready, (threadIdx.x & 31) == 0);
+  return true;
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __grid_constant__ BwdParams p) {
   using C = KeyConfig<DP>;
@@ -623,6 +657,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
         tc::tmem_ld32(s_at, s);
         const bool far = __any_sync(0xffffffffu, st[lane] > kFarFrom);
         tc::tmem_wait_ld();
+        if (far) {
+          const float* shifts = p.shifts + (w.head * p.group + (w.begin + i) / w.per_head) * p.seq.stat_rows + w.at.stat + query;
+          if (!(ok = far_step<T>(bar, waiter, steps & 1, s_at, dp_at, st, shifts, p.scale_log2, diagonal ? from : 0))) break;
+          continue;
+        }
 #pragma unroll
         for (int y = 0; y < 16; y += 2) {
           const float4 l = *reinterpret_cast<const float4*>(st + 2 * y);
@@ -630,20 +669,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
           const float2 b = fma2(make_float2(__uint_as_float(s[2 * y + 2]), __uint_as_float(s[2 * y + 3])), by_scale, make_float2(l.z, l.w));
           e[y] = exp2_2(a);
           e[y + 1] = (y & 2) != 0 ? exp2_fma(b) : exp2_2(b);
-        }
-        if (__builtin_expect(far, 0)) {   // once more, from the scores where they still are
-          const float* shifts = p.shifts + (w.head * p.group + (w.begin + i) / w.per_head) * p.seq.stat_rows + w.at.stat + query;
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            uint32_t again[16];
-            tc::tmem_ld16(s_at + x * 16, again);
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int y = 0; y < 16; ++y) {
-              const float weight = far_weight(again[y], st[x * 16 + y], shifts + x * 16 + y, p.scale_log2);
-              if ((y & 1) == 0) e[x * 8 + y / 2].x = weight; else e[x * 8 + y / 2].y = weight;
-            }
-          }
         }
         if (diagonal) {
 #pragma unroll
