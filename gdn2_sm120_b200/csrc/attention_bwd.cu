@@ -16,7 +16,7 @@
 // q and do all the same, and 0 * inf and 0 * NaN are not 0: a key that is not finite reaches dq, in its channel, of the rows
 // before it in its tile, a query dk and a cotangent dv of the keys behind it there.  (Another sequence's rows never.)
 //
-// Training 4 x 2048 tokens, 16 heads of 128 channels, 4 heads a group: delta 12 us, keys 129, queries 116, forward 85.
+// Training 4 x 2048 tokens, 16 heads of 128 channels, 4 heads a group, each kernel by itself: delta 11 us, keys 121, queries 120, forward 73.
 
 #include <algorithm>
 

@@ -346,7 +346,8 @@ inline bool wide_rows(const void* base, int dim) { return dim % 16 == 0 && (rein
 // The same with two threads a row, 64 columns each (S at s_at, P over the first half of them, DP / 2 columns of O at o_at):
 // the latencies of a chain, and not its instructions, are what the tensor cores wait for.  All 256 threads of a chain look
 // again together.  A quarter of the weights is made on the FMA units; there a score that is 127 powers of two above the
-// reference counts as 127, and the row looks again.  8 x 4096 tokens, 16 heads (and one prompt of 16381, 8 heads): one thread
+// reference counts as 127, and the row looks again.  (A reference that moves only where weights grow, and exponentials by a
+// polynomial on the FMA units, have been published for other kernels of attention.)  8 x 4096 tokens, 16 heads (and one prompt of 16381, 8 heads): one thread
 // a row 517 us (472), two 476 (450), with the FMA units' quarter 474 (427).
 struct Pair {
   int chain, half, row;

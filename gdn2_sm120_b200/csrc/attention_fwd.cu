@@ -8,10 +8,10 @@
 // its two products, the shared memory that they read as long (64 KiB for S, 32 for P V, 64 arrive for both tiles), and the
 // special-function unit 1024 for its exponentials, less a quarter on the FMA units.
 //
-// 8 prompts of 4096 tokens, 16 heads of 128 channels, 4 heads a group: 468 us alone, 1.17 PFLOP/s (72 % of the measured
-// 1.63); one of 16381 tokens, 8 heads 423 us, 1.30.  Back to back under the power cap 560 and 495 us.  The products by
-// themselves, with nobody waiting for anybody, take 376 us of the 468: what bounds it is the tensor cores' own rate with
-// operands from shared memory, then the round trip of a chain.
+// 8 prompts of 4096 tokens, 16 heads of 128 channels, 4 heads a group: 461 to 474 us alone (by the machine), 1.17 PFLOP/s (72 %
+// of the measured 1.63); one of 16381 tokens, 8 heads 424 us, 1.30.  Back to back under the power cap 550 to 565 and 505 us.
+// The products by themselves, with nobody waiting for anybody, take 376 us of them: what bounds it is the tensor cores' own rate
+// with operands from shared memory, then the round trip of a chain.
 //
 // TMEM (512 columns): S0 S1 O0 O1, 128 each; P (16-bit) overlays the first 32 of its half's 64 columns of S and is the A
 // operand of P V from there.  Products are issued in an order that needs no further waits: S_t(j+1) after O_t += P_t(j) V, so

@@ -24,8 +24,9 @@
 // same rows, on every other tile, and their (O, m, l) are joined at the end; above, each has 128 rows and all tiles.  Four
 // warps bring in keys and values, in boxes of a tiled copy where the pages allow it and row by row with 16-byte asynchronous
 // copies elsewhere; one brings queries, one issues the products.  TMEM: S0 S1 O0 O1, 128 columns each, P over S.  48 drafted
-// tokens of 8 sequences over up to 16000 cached ones, 4 heads a group (192 rows): 110 us, 3.3 TB/s; what bounds it is a chain's
-// round trip between the tensor cores and its warps (the copies left out, 108 us of 142 remained; the weights left out, 116).
+// tokens of 8 sequences over up to 16000 cached ones, 4 heads a group (192 rows): 106 us, 3.4 TB/s (a call in a loop, with the
+// join of the parts, 128 to 132); what bounds it is a chain's round trip between the tensor cores and its warps (of an older form
+// that took 142 us, 108 remained without the copies, 116 without the weights).
 // tree_few_kernel has up to 16 rows (below).
 
 #include <algorithm>
@@ -690,7 +691,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 // Up to 16 rows (plain decoding, small trees of small groups): mma.sync m16n8k16, whose sums are in registers: no product has
 // more rows than there are, and no score goes through TMEM to a few lanes.  Eight warps have 16 tokens of every tile each and
 // go through them on their own; what they have of a unit is joined at its end.  Decoding 64 sequences of up to 8192 tokens,
-// 8 key heads: 217 us, 6.25 TB/s of the copy rate's 6.53.  (Copies by the computing warps themselves: 248 us.)
+// 8 key heads: 210 us, 6.45 TB/s of the copy rate's 6.53 (a call in a loop, with the join of the parts, 217 to 227).  (Copies
+// by the computing warps themselves: 31 us more.)
 constexpr int kFewThreads = 384;   // warps 0-7: 16 tokens of every tile each; 8-11: copies
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
@@ -1106,8 +1108,8 @@ int launch_tree(const void* q, const void* k, const void* v, const void* k_pages
   p.dim = dim; p.page = page; p.columns = columns;
   p.rows = drafted * p.group;
   // Whole boxes of tiled copies come out of a page only where it has 8 or 16 rows, or a multiple of 32; pages of other
-  // sizes, and tiles that a sequence ends in, are copied row by row.  Decoding as above, pages of 64: 238 us with boxes,
-  // 254 row by row; of 16 238 and 240.
+  // sizes, and tiles that a sequence ends in, are copied row by row.  Calls in a loop, decoding as above, pages of 64: 220
+  // us with boxes, 242 row by row; of 16 225 and 249.  Trees of 48 drafts as above, pages of 64: 124 and 126; of 16 124 and 128.
   p.box = page % 32 == 0 ? 32 : page == 16 || page == 8 ? page : 0;
   if (p.box > 0) {
     const int64_t page_strides[3] = {int64_t(page) * kv_heads * dim, int64_t(kv_heads) * dim, dim};
