@@ -9,8 +9,8 @@
 // five).
 //
 // p and ds are rounded to the inputs' type for their products, which is as near as a 16-bit operand comes: a gradient's
-// error in the 2-norm is that of its own rounding and of one of these, 1.4 times a rounding of the exact gradient, and up to
-// 1.8 times in sequences of a few tokens, where the output's rounding in delta counts as much.
+// error in the 2-norm is that of its own rounding and of one of these, 1.4 times a rounding of the exact gradient, 1.5 with
+// the output's rounding in delta, and up to 1.8 in sequences of a few tokens, where that counts as much.
 //
 // P and dS are 0 by selection where a row does not see a key.  In the tiles on the diagonal their products meet those rows of k,
 // q and do all the same, and 0 * inf and 0 * NaN are not 0: a key that is not finite reaches dq, in its channel, of the rows
