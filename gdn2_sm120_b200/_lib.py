@@ -73,6 +73,9 @@ _PROTOTYPES: dict[str, list] = {
     "gdn2_attention_forward": [_P] * 7 + [_I64] * 5 + [_INT, _F32, _P],
     "gdn2_attention_backward_bytes": [_P] + [_I64] * 5,
     "gdn2_attention_backward": [_P] * 12 + [_I64] * 5 + [_INT, _F32, _P],
+    "gdn2_window_attention_forward": [_P] * 7 + [_I64] * 7 + [_INT, _F32, _P],
+    "gdn2_window_attention_backward_bytes": [_P] + [_I64] * 7,
+    "gdn2_window_attention_backward": [_P] * 12 + [_I64] * 7 + [_INT, _F32, _P],
     "gdn2_debug_wait_limit": [_I64],
     "gdn2_profile_enable": [_INT],
     "gdn2_profile_chunk_kernels": [_P] * 4,
@@ -80,7 +83,8 @@ _PROTOTYPES: dict[str, list] = {
 _RESTYPES = {"gdn2_status_string": ctypes.c_char_p, "gdn2_last_cuda_error": ctypes.c_char_p,
              "gdn2_chunk_workspace_bytes": ctypes.c_int64, "gdn2_chunk_scratch_bytes": ctypes.c_int64,
              "gdn2_tensor_maps_encoded": ctypes.c_int64, "gdn2_tree_workspace_bytes": ctypes.c_int64,
-             "gdn2_attention_stat_rows": ctypes.c_int64, "gdn2_attention_backward_bytes": ctypes.c_int64}
+             "gdn2_attention_stat_rows": ctypes.c_int64, "gdn2_attention_backward_bytes": ctypes.c_int64,
+             "gdn2_window_attention_backward_bytes": ctypes.c_int64}
 
 
 def library_path() -> pathlib.Path:

@@ -58,7 +58,13 @@ def _launches(bounds) -> int:
     return sum(bounds[i] < bounds[min(i + 256, len(bounds) - 1)] for i in range(0, len(bounds) - 1, 256))
 
 
-def _forward(q, k, v, bounds, scale, training):
+def _entry(name, window):
+    """The entry point ``name`` of attention without a window or with one, and what says so."""
+
+    return f"gdn2_{name}" if window == (0, 0) else f"gdn2_window_{name}", () if window == (0, 0) else window
+
+
+def _forward(q, k, v, bounds, scale, window, training):
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     if q.shape[1] == 0:
         return out, None
@@ -70,22 +76,23 @@ def _forward(q, k, v, bounds, scale, training):
             _lib.check(int(each), "gdn2_attention_stat_rows")
         statistics = torch.empty((2, q.shape[2], each), device=q.device, dtype=torch.float32)
     strides = _lib.int64s(*(s for x in (q, k, v) for s in _validate.head_strides(x)))
-    _lib.call("gdn2_attention_forward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-              _lib.ptr(statistics), strides, host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3],
+    name, more = _entry("attention_forward", window)
+    _lib.call(name, q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+              _lib.ptr(statistics), strides, host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], *more,
               _lib.dtype_code(q.dtype), scale, _lib.stream_ptr(q.device), kernels=_launches(bounds))
     return out, statistics
 
 
 class _CausalAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, bounds, scale):
-        done = _native(q, k, v, bounds, scale, True)
+    def forward(ctx, q, k, v, bounds, scale, window):
+        done = _native(q, k, v, bounds, scale, window, True)
         if done is None:
             bounds, scale = _check(q, k, v, bounds, scale)
-            done = _forward(*(_validate.detached(x) for x in (q, k, v)), bounds, scale, True)
+            done = _forward(*(_validate.detached(x) for x in (q, k, v)), bounds, scale, window, True)
         out, statistics = done
         ctx.save_for_backward(q, k, v, out, statistics)
-        ctx.bounds, ctx.scale = bounds, scale
+        ctx.bounds, ctx.scale, ctx.window = bounds, scale, window
         return out
 
     @staticmethod
@@ -93,49 +100,58 @@ class _CausalAttention(torch.autograd.Function):
     def backward(ctx, d_out):
         q, k, v, out, statistics = ctx.saved_tensors
         if statistics is not None and _lib.KERNEL_EVENTS is None:
-            done = _lib.host().attention_backward(q, k, v, out, statistics, d_out, ctx.bounds, ctx.scale)
+            done = _lib.host().attention_backward(q, k, v, out, statistics, d_out, ctx.bounds, ctx.scale, *ctx.window)
             if done is not None:
-                return (*done, None, None)
+                return (*done, None, None, None)
         scale = _validate.float32_scale(ctx.scale, q.shape[3])
         q, k, v = (_validate.detached(x) for x in (q, k, v))
         grads = tuple(torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
         if statistics is None:
-            return (*grads, None, None)
+            return (*grads, None, None, None)
         if d_out.stride(3) != 1 or d_out.data_ptr() % 16 or any(
                 n > 1 and (s <= 0 or s % 8) for n, s in zip(d_out.shape[:3], d_out.stride())):
             d_out = d_out.clone(memory_format=torch.contiguous_format)
         host, n_seq, rows = _sequences(q, ctx.bounds)
         strides = _lib.int64s(*(s for x in (q, k, v, d_out) for s in _validate.head_strides(x)))
+        name, more = _entry("attention_backward", ctx.window)
         with torch.cuda.device(q.device):
-            size = _lib.lib().gdn2_attention_backward_bytes(host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3])
+            size = getattr(_lib.lib(), name + "_bytes")(host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], *more)
         if size < 0:
-            _lib.check(int(size), "gdn2_attention_backward_bytes")
+            _lib.check(int(size), name + "_bytes")
         scratch = torch.empty(size, device=q.device, dtype=torch.uint8)
-        _lib.call("gdn2_attention_backward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+        _lib.call(name, q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                   d_out.data_ptr(), statistics.data_ptr(), scratch.data_ptr(), *(x.data_ptr() for x in grads), strides,
-                  host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], _lib.dtype_code(q.dtype), scale,
+                  host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], *more, _lib.dtype_code(q.dtype), scale,
                   _lib.stream_ptr(q.device), kernels=(3 + (size > 2 * statistics.numel() + 15)) * _launches(ctx.bounds))
-        return (*grads, None, None)
+        return (*grads, None, None, None)
 
 
-def _native(q, k, v, bounds, scale, training):
+def _native(q, k, v, bounds, scale, window, training):
     """The call on the native host path, ``(output, statistics)``; None where it is not the plain case."""
 
     if _lib.KERNEL_EVENTS is not None or not getattr(q, "is_cuda", False):
         return None
-    return _lib.host().attention_forward(q, k, v, bounds, scale, training)
+    return _lib.host().attention_forward(q, k, v, bounds, scale, *window, training)
 
 
-def _attention(q, k, v, bounds, scale):
+def _attention(q, k, v, bounds, scale, window=(0, 0)):
     if forward_ad._current_level >= 0:
         _validate.refuse_tangents("causal attention", q, k, v)
     if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v)):
-        return _CausalAttention.apply(q, k, v, bounds, scale)
-    done = _native(q, k, v, bounds, scale, False)
+        return _CausalAttention.apply(q, k, v, bounds, scale, window)
+    done = _native(q, k, v, bounds, scale, window, False)
     if done is None:
         bounds, scale = _check(q, k, v, bounds, scale)
-        done = _forward(*(_validate.detached(x) for x in (q, k, v)), bounds, scale, False)
+        done = _forward(*(_validate.detached(x) for x in (q, k, v)), bounds, scale, window, False)
     return done[0]
+
+
+def _packed_bounds(q, cu_seqlens):
+    """Cumulative lengths of packed sequences as a tuple."""
+
+    if not isinstance(q, torch.Tensor) or q.ndim != 4 or q.shape[0] != 1:
+        raise ValueError("packed sequence tensors must have shape [1, total, H, D]")
+    return cu_seqlens if isinstance(cu_seqlens, tuple) else _bounds(cu_seqlens, q.shape[1])
 
 
 def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None) -> torch.Tensor:
@@ -161,11 +177,7 @@ def causal_attention_varlen(
     Tensors are ``[1, total, H, D]``; ``cu_seqlens`` holds ``N + 1`` cumulative lengths (tensor or sequence of ints, read
     on the host).  No token sees one of another sequence, whatever stands there."""
 
-    if not isinstance(q, torch.Tensor) or q.ndim != 4 or q.shape[0] != 1:
-        raise ValueError("packed sequence tensors must have shape [1, total, H, D]")
-    if not isinstance(cu_seqlens, tuple):
-        cu_seqlens = _bounds(cu_seqlens, q.shape[1])
-    return _attention(q, k, v, cu_seqlens, scale)
+    return _attention(q, k, v, _packed_bounds(q, cu_seqlens), scale)
 
 
 __all__ = ["causal_attention", "causal_attention_varlen"]

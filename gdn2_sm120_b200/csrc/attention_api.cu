@@ -21,11 +21,11 @@ static std::atomic<uint32_t> g_wait_polls{GDN2_ATTENTION_WAIT_POLLS};
 uint32_t wait_polls() { return g_wait_polls.load(std::memory_order_relaxed); }
 int64_t attention_stat_rows(const int64_t*, int64_t, int64_t);
 int launch_attention_forward(const void*, const void*, const void*, void*, float*, const int64_t*, const int64_t*, int64_t,
-                             int64_t, int, int, int, int, float, cudaStream_t);
-int64_t attention_backward_bytes(const int64_t*, int64_t, int64_t, int, int, int);
+                             int64_t, int, int, int, int, float, int64_t, int64_t, cudaStream_t);
+int64_t attention_backward_bytes(const int64_t*, int64_t, int64_t, int, int, int, int64_t, int64_t);
 int launch_attention_backward(const void*, const void*, const void*, const void*, const void*, const float*, void*, void*,
                               void*, void*, const int64_t*, const int64_t*, int64_t, int64_t, int, int, int, int, float,
-                              cudaStream_t);
+                              int64_t, int64_t, cudaStream_t);
 }  // namespace attn
 
 namespace {
@@ -62,6 +62,52 @@ int check_sequences(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t 
   // pieces of 64 rows are numbered with 31 bits
   const int64_t stat = attn::attention_stat_rows(bounds, n_seq, time);
   return stat / 64 > kMost / heads ? GDN2_ERR_TOO_LARGE : GDN2_OK;
+}
+
+// Causal attention, with a window of 0 for none
+int attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics, const int64_t* strides,
+                      const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads, int64_t dim,
+                      int64_t window, int64_t sinks, int dtype, float scale, void* stream) {
+  if (!q || !k || !v || !out || !strides) return GDN2_ERR_NULL_POINTER;
+  int status = check_heads(heads, kv_heads, dim);
+  if (status != GDN2_OK) return status;
+  if (!valid_seq_dtype(dtype)) return GDN2_ERR_BAD_DTYPE;
+  if ((status = check_sequences(bounds, n_seq, time, heads)) != GDN2_OK) return status;
+  if ((status = check_strides(strides, 9)) != GDN2_OK) return status;
+  const void* need16[] = {q, k, v, out, statistics};
+  for (const void* p : need16) {
+    if (!aligned(p, 16)) return GDN2_ERR_ALIGNMENT;
+  }
+  return attn::launch_attention_forward(q, k, v, out, statistics, strides, bounds, n_seq, time, int(heads), int(kv_heads),
+                                        int(dim), dtype, scale, window, sinks, static_cast<cudaStream_t>(stream));
+}
+
+int64_t attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads,
+                                 int64_t dim, int64_t window, int64_t sinks) {
+  int status = check_heads(heads, kv_heads, dim);
+  if (status == GDN2_OK) status = check_sequences(bounds, n_seq, time, heads);
+  return status != GDN2_OK ? status : attn::attention_backward_bytes(bounds, n_seq, time, int(heads), int(kv_heads), int(dim), window, sinks);
+}
+
+int attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out, const float* statistics,
+                       void* scratch, void* dq, void* dk, void* dv, const int64_t* strides, const int64_t* bounds, int64_t n_seq,
+                       int64_t time, int64_t heads, int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks, int dtype,
+                       float scale, void* stream) {
+  if (!q || !k || !v || !out || !d_out || !statistics || !scratch || !dq || !dk || !dv || !strides) {
+    return GDN2_ERR_NULL_POINTER;
+  }
+  int status = check_heads(heads, kv_heads, dim);
+  if (status != GDN2_OK) return status;
+  if (!valid_seq_dtype(dtype)) return GDN2_ERR_BAD_DTYPE;
+  if ((status = check_sequences(bounds, n_seq, time, heads)) != GDN2_OK) return status;
+  if ((status = check_strides(strides, 12)) != GDN2_OK) return status;
+  const void* need16[] = {q, k, v, out, d_out, statistics, scratch, dq, dk, dv};
+  for (const void* p : need16) {
+    if (!aligned(p, 16)) return GDN2_ERR_ALIGNMENT;
+  }
+  return attn::launch_attention_backward(q, k, v, out, d_out, statistics, scratch, dq, dk, dv, strides, bounds, n_seq, time,
+                                         int(heads), int(kv_heads), int(dim), dtype, scale, window, sinks,
+                                         static_cast<cudaStream_t>(stream));
 }
 
 }  // namespace
@@ -147,46 +193,44 @@ int64_t gdn2_attention_stat_rows(const int64_t* bounds, int64_t n_seq, int64_t t
 int gdn2_attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics,
                            const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads,
                            int64_t kv_heads, int64_t dim, int dtype, float scale, void* stream) {
-  if (!q || !k || !v || !out || !strides) return GDN2_ERR_NULL_POINTER;
-  int status = check_heads(heads, kv_heads, dim);
-  if (status != GDN2_OK) return status;
-  if (!valid_seq_dtype(dtype)) return GDN2_ERR_BAD_DTYPE;
-  if ((status = check_sequences(bounds, n_seq, time, heads)) != GDN2_OK) return status;
-  if ((status = check_strides(strides, 9)) != GDN2_OK) return status;
-  const void* need16[] = {q, k, v, out, statistics};
-  for (const void* p : need16) {
-    if (!aligned(p, 16)) return GDN2_ERR_ALIGNMENT;
-  }
-  return attn::launch_attention_forward(q, k, v, out, statistics, strides, bounds, n_seq, time, int(heads), int(kv_heads),
-                                        int(dim), dtype, scale, static_cast<cudaStream_t>(stream));
+  return attention_forward(q, k, v, out, statistics, strides, bounds, n_seq, time, heads, kv_heads, dim, 0, 0, dtype, scale, stream);
 }
 
 int64_t gdn2_attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads,
                                       int64_t dim) {
-  int status = check_heads(heads, kv_heads, dim);
-  if (status == GDN2_OK) status = check_sequences(bounds, n_seq, time, heads);
-  return status != GDN2_OK ? status : attn::attention_backward_bytes(bounds, n_seq, time, int(heads), int(kv_heads), int(dim));
+  return attention_backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, 0, 0);
 }
 
 int gdn2_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out,
                             const float* statistics, void* scratch, void* dq, void* dk, void* dv, const int64_t* strides,
                             const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads, int64_t dim,
                             int dtype, float scale, void* stream) {
-  if (!q || !k || !v || !out || !d_out || !statistics || !scratch || !dq || !dk || !dv || !strides) {
-    return GDN2_ERR_NULL_POINTER;
-  }
-  int status = check_heads(heads, kv_heads, dim);
-  if (status != GDN2_OK) return status;
-  if (!valid_seq_dtype(dtype)) return GDN2_ERR_BAD_DTYPE;
-  if ((status = check_sequences(bounds, n_seq, time, heads)) != GDN2_OK) return status;
-  if ((status = check_strides(strides, 12)) != GDN2_OK) return status;
-  const void* need16[] = {q, k, v, out, d_out, statistics, scratch, dq, dk, dv};
-  for (const void* p : need16) {
-    if (!aligned(p, 16)) return GDN2_ERR_ALIGNMENT;
-  }
-  return attn::launch_attention_backward(q, k, v, out, d_out, statistics, scratch, dq, dk, dv, strides, bounds, n_seq, time,
-                                         int(heads), int(kv_heads), int(dim), dtype, scale,
-                                         static_cast<cudaStream_t>(stream));
+  return attention_backward(q, k, v, out, d_out, statistics, scratch, dq, dk, dv, strides, bounds, n_seq, time, heads, kv_heads, dim,
+                            0, 0, dtype, scale, stream);
+}
+
+int gdn2_window_attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics,
+                                  const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads,
+                                  int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks, int dtype, float scale,
+                                  void* stream) {
+  if (window <= 0 || sinks < 0) return GDN2_ERR_BAD_RANGE;
+  return attention_forward(q, k, v, out, statistics, strides, bounds, n_seq, time, heads, kv_heads, dim, window, sinks, dtype, scale,
+                           stream);
+}
+
+int64_t gdn2_window_attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads,
+                                             int64_t dim, int64_t window, int64_t sinks) {
+  if (window <= 0 || sinks < 0) return GDN2_ERR_BAD_RANGE;
+  return attention_backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, window, sinks);
+}
+
+int gdn2_window_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out,
+                                   const float* statistics, void* scratch, void* dq, void* dk, void* dv, const int64_t* strides,
+                                   const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads,
+                                   int64_t dim, int64_t window, int64_t sinks, int dtype, float scale, void* stream) {
+  if (window <= 0 || sinks < 0) return GDN2_ERR_BAD_RANGE;
+  return attention_backward(q, k, v, out, d_out, statistics, scratch, dq, dk, dv, strides, bounds, n_seq, time, heads, kv_heads, dim,
+                            window, sinks, dtype, scale, stream);
 }
 
 int gdn2_debug_wait_limit(int64_t polls) {

@@ -50,6 +50,13 @@ struct BwdParams {
   float* partials;           // dk and dv of the parts of an item, [part][dk, dv][row][kv head][dim]
   int64_t partial_rows;      // rows * kv heads
   int parts;                 // of an item of the key kernel
+  // With a window: the sums of keys that are sinks go on where those of others have ended, over all later queries.  Their
+  // tiles are items of their own, `sink_tiles` of every sequence, in `sink_parts` parts, [part][dk, dv][sequence, row][kv
+  // head][dim] behind the others'.
+  int sink_tiles, sink_parts;
+  float* sink_partials;
+  int64_t sink_items;
+  Span span;
   int heads, kv_heads, group, dim, turns;
   int64_t items;
   float scale, scale_log2;   // scale_log2 is positive
@@ -71,6 +78,10 @@ struct BwdItem {
   int head, tile;       // of queries, or of keys; 128-row tile in the sequence
   int first, per_head, steps;  // keys: first 128-row step, steps of a query head, of this part; queries: 64-row steps
   int part, begin;             // keys: which part, its first step of the item's
+  int sinks;                   // queries, with a window: steps over sinks ahead of those from `first` on; keys: the sinks' sequence or -1
+  // queries: the first key of a step
+  template <bool kWindow>
+  __device__ __forceinline__ int key_of(int step) const { return kStep * (!kWindow || step < sinks ? step : first + step - sinks); }
 };
 
 // The weight of a score s of a query whose statistic is l and whose reference, if that is far away, is *shift.  Scores are
@@ -82,9 +93,9 @@ __device__ __forceinline__ float far_weight(uint32_t s, float l, const float* sh
 }
 
 // dS of half a row of the query kernel whose warp has a row with such a reference, formed and left over dP: the row sees its
-// columns up to `last`
+// columns that have a bit
 template <typename T>
-__device__ __noinline__ void far_slopes(uint32_t s_at, uint32_t dp_at, float l, const float* shift, float minus_delta, float c, int last) {
+__device__ __noinline__ void far_slopes(uint32_t s_at, uint32_t dp_at, float l, const float* shift, float minus_delta, float c, uint32_t sees) {
   uint32_t w[16];
 #pragma unroll
   for (int x = 0; x < 32; x += 16) {
@@ -97,7 +108,7 @@ __device__ __noinline__ void far_slopes(uint32_t s_at, uint32_t dp_at, float l, 
       float ds[2];
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
-        ds[z] = x + y + z > last ? 0.f : far_weight(s[y + z], l, shift, c) * (__uint_as_float(dp[y + z]) + minus_delta);
+        ds[z] = ((sees >> (x + y + z)) & 1) == 0 ? 0.f : far_weight(s[y + z], l, shift, c) * (__uint_as_float(dp[y + z]) + minus_delta);
       }
       w[(x + y) / 2] = pack_pair<T>(ds[0], ds[1]);
     }
@@ -108,10 +119,36 @@ __device__ __noinline__ void far_slopes(uint32_t s_at, uint32_t dp_at, float l, 
 // the first step of a part of an item of the key kernel
 __device__ __forceinline__ int part_begin(int steps, int part, int parts) { return int(int64_t(steps) * part / parts); }
 
-template <bool kKeys>
+// tiles of 128 queries that see some key of a tile of 128, of which no key is a sink: all from the tile's own on, as many as
+// the window reaches
+__device__ __forceinline__ int seeing_tiles(int len, int tile, int window) {
+  return min((len + 127) / 128 - tile, (126 + window) / 128 + 1);
+}
+
+template <bool kKeys, bool kWindow>
 __device__ __forceinline__ bool bwd_item(const BwdParams& p, int turn, BwdItem* w) {
-  const int64_t index = item_of_turn(turn);
+  int64_t index = item_of_turn(turn);
   if (index >= p.items) return false;
+  w->sinks = -1;
+  if (kKeys && kWindow) {
+    if (index < p.sink_items) {
+      const int part = int(index % p.sink_parts);
+      index /= p.sink_parts;
+      w->head = int(index % p.kv_heads);
+      index /= p.kv_heads;
+      w->tile = int(index % p.sink_tiles);
+      w->sinks = int(index / p.sink_tiles);
+      w->at = find_sequence(p.seq, w->sinks);
+      if (w->tile * 128 >= w->at.len) return false;
+      w->first = w->tile;
+      w->per_head = (w->at.len + 127) / 128 - w->tile;
+      w->part = part;
+      w->begin = part_begin(w->per_head * p.group, part, p.sink_parts);
+      w->steps = part_begin(w->per_head * p.group, part + 1, p.sink_parts) - w->begin;
+      return w->steps > 0;
+    }
+    index -= p.sink_items;
+  }
   const int parts = kKeys ? p.parts : 1, heads = (kKeys ? p.kv_heads : p.heads) * parts;
   const int u = int(index / heads), in_tile = int(index - int64_t(u) * heads);
   w->head = in_tile / parts;
@@ -121,12 +158,19 @@ __device__ __forceinline__ bool bwd_item(const BwdParams& p, int turn, BwdItem* 
   if (w->tile * 128 >= w->at.len) return false;
   w->first = kKeys ? w->tile : 0;
   w->per_head = kKeys ? (w->at.len + 127) / 128 - w->tile : min(2 * w->tile + 2, (w->at.len + kStep - 1) / kStep);
+  if (kWindow && kKeys) {
+    if (w->tile < p.sink_tiles) return false;
+    w->per_head = seeing_tiles(w->at.len, w->tile, p.span.window);
+  } else if (kWindow) {
+    w->first = p.span.first_tile(w->tile * 128, kStep, &w->sinks);
+    w->per_head += w->sinks - w->first;
+  }
   w->begin = kKeys ? part_begin(w->per_head * p.group, w->part, parts) : 0;
   w->steps = kKeys ? part_begin(w->per_head * p.group, w->part + 1, parts) - w->begin : w->per_head;
   return w->steps > 0;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool kWindow>
 __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __grid_constant__ BwdParams p) {
   using C = QueryConfig<DP>;
   extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
@@ -173,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
       bool ok = true;
       for (int turn = 0; turn < p.turns && ok; ++turn) {
         BwdItem w;
-        if (!bwd_item<false>(p, turn, &w)) continue;
+        if (!bwd_item<false, kWindow>(p, turn, &w)) continue;
         const int kv_head = w.head / p.group;
         if (stayed > 0) ok = waiter.wait(&bar.stay_empty, (stayed - 1) & 1);
         if (!ok) break;
@@ -190,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
           const int s = filled % C::kStages;
           if (filled >= C::kStages) ok = waiter.wait(&bar.go_empty[s], (filled / C::kStages - 1) & 1);
           if (!ok) break;
-          const int at = i * kStep;
+          const int at = w.key_of<kWindow>(i);
           uint8_t* to = go + s * 2 * C::kGoBytes;
           // rows of the next sequence would meet weights of 0, but 0 * inf and 0 * NaN are not 0
           const int valid = w.at.len - at;
@@ -249,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
       };
       for (int turn = 0; turn < p.turns && ok; ++turn) {
         BwdItem w;
-        if (!bwd_item<false>(p, turn, &w)) continue;
+        if (!bwd_item<false, kWindow>(p, turn, &w)) continue;
         ok = waiter.wait(&bar.in_tmem, stayed & 1);
         if (ok) ok = both(0, used);
         if (ok && w.steps > 1) ok = both(1, used + 1);
@@ -313,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
     };
     for (int turn = 0; turn < p.turns; ++turn) {
       BwdItem w;
-      if (!bwd_item<false>(p, turn, &w)) continue;
+      if (!bwd_item<false, kWindow>(p, turn, &w)) continue;
       if (stayed == outs) into_tmem();
       const int64_t stat = w.head * p.seq.stat_rows + w.at.stat + w.tile * 128 + row;
       const float lse = p.lse[stat];
@@ -325,7 +369,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
         tc::tc_fence_after();
         // a query sees keys up to itself: of those that go by the first to `last`
         const int last = w.tile * 128 + row - i * kStep;
-        const bool diagonal = (i + 1) * kStep > w.tile * 128;
+        const bool diagonal = kWindow ? !p.span.whole(w.tile * 128, 128, w.key_of<kWindow>(i), kStep) : (i + 1) * kStep > w.tile * 128;
+        uint32_t sees = ~0u;
+        if (kWindow && diagonal) sees = p.span.sees(w.tile * 128 + row, w.key_of<kWindow>(i) + half * 32);
         uint32_t s[32], dp[32], dsw[16];
         tc::tmem_ld32(s_at, s);
         tc::tmem_ld32(dp_at, dp);
@@ -337,13 +383,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
           const float2 e = exp2_2(z);
           float2 ds = mul2(e, add2(make_float2(__uint_as_float(dp[y]), __uint_as_float(dp[y + 1])), minus_delta));
           if (diagonal) {
-            if (x > last) ds.x = 0.f;
-            if (x + 1 > last) ds.y = 0.f;
+            if (kWindow ? ((sees >> y) & 1) == 0 : x > last) ds.x = 0.f;
+            if (kWindow ? ((sees >> (y + 1)) & 1) == 0 : x + 1 > last) ds.y = 0.f;
           }
           dsw[y / 2] = pack_pair<T>(ds.x, ds.y);   // rounded to the inputs' type for its product, whose sums are in 32 bits
         }
-        if (far) far_slopes<T>(s_at, dp_at, lse, p.shifts + stat, minus_delta.x, p.scale_log2, diagonal ? last - half * 32 : 32);
-        else tc::tmem_st16(dp_at, dsw);
+        if (far) {
+          if (!kWindow && diagonal) sees = last - half * 32 >= 31 ? ~0u : last < half * 32 ? 0u : (2u << (last - half * 32)) - 1u;
+          far_slopes<T>(s_at, dp_at, lse, p.shifts + stat, minus_delta.x, p.scale_log2, sees);
+        } else {
+          tc::tmem_st16(dp_at, dsw);
+        }
         tc::tmem_wait_st();
         tc::tc_fence_before();
         __syncwarp();
@@ -357,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_queries_kernel(const __
       if (ok) ok = waiter.wait(&bar.s_full[last_set], (all[last_set] - 1) & 1);
       BwdItem next;
       for (int later = turn + 1; later < p.turns; ++later) {
-        if (bwd_item<false>(p, later, &next)) {
+        if (bwd_item<false, kWindow>(p, later, &next)) {
           into_tmem();
           break;
         }
@@ -423,16 +473,16 @@ struct KeyBars {
 };
 
 // A thread's share of a step in which a query's reference is far away: P and dS as below, with weights as in far_weight; the
-// key sees its queries from `from` on.  False where a wait ran out.
+// key is seen by those queries that have a bit.  False where a wait ran out.
 template <typename T>
 __device__ __noinline__ bool far_step(KeyBars& bar, const Waiter& waiter, uint32_t parity, uint32_t s_at, uint32_t dp_at, const float* st,
-                                      const float* shifts, float c, int from) {
+                                      const float* shifts, float c, uint32_t seen) {
   float e[32];
   uint32_t w[16], x[32];
   tc::tmem_ld32(s_at, x);
   tc::tmem_wait_ld();
 #pragma unroll
-  for (int y = 0; y < 32; ++y) e[y] = y < from ? 0.f : far_weight(x[y], st[y], shifts + y, c);
+  for (int y = 0; y < 32; ++y) e[y] = ((seen >> y) & 1) == 0 ? 0.f : far_weight(x[y], st[y], shifts + y, c);
 #pragma unroll
   for (int y = 0; y < 16; ++y) w[y] = pack_pair<T>(e[2 * y], e[2 * y + 1]);
   tc::tmem_st16(s_at, w);
@@ -445,7 +495,7 @@ __device__ __noinline__ bool far_step(KeyBars& bar, const Waiter& waiter, uint32
   tc::tmem_ld32(dp_at, x);
   tc::tmem_wait_ld();
 #pragma unroll
-  for (int y = 0; y < 32; ++y) e[y] = y < from ? 0.f : e[y] * (__uint_as_float(x[y]) + st[128 + y]);
+  for (int y = 0; y < 32; ++y) e[y] = ((seen >> y) & 1) == 0 ? 0.f : e[y] * (__uint_as_float(x[y]) + st[128 + y]);
 #pragma unroll
   for (int y = 0; y < 16; ++y) w[y] = pack_pair<T>(e[2 * y], e[2 * y + 1]);
   tc::tmem_st16(dp_at, w);
@@ -456,7 +506,7 @@ __device__ __noinline__ bool far_step(KeyBars& bar, const Waiter& waiter, uint32
   return true;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool kWindow>
 __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __grid_constant__ BwdParams p) {
   using C = KeyConfig<DP>;
   extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
@@ -506,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
       bool ok = true;
       for (int turn = 0; turn < p.turns && ok; ++turn) {
         BwdItem w;
-        if (!bwd_item<true>(p, turn, &w)) continue;
+        if (!bwd_item<true, kWindow>(p, turn, &w)) continue;
         if (stayed > 0 && !(ok = waiter.wait(&bar.stay_empty, (stayed - 1) & 1))) break;
         tc::mbar_arrive_expect_tx(&bar.stay_full, 2 * C::kTileBytes, leader);
 #pragma unroll
@@ -592,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
       };
       for (int turn = 0; turn < p.turns && ok; ++turn) {
         BwdItem w;
-        if (!bwd_item<true>(p, turn, &w)) continue;
+        if (!bwd_item<true, kWindow>(p, turn, &w)) continue;
         if (!(ok = waiter.wait(&bar.stay_full, stayed & 1))) break;
         if (!(ok = scores(used)) || !(ok = slopes(used + 1))) break;
         for (int i = 0; i < w.steps && ok; ++i) {
@@ -642,13 +692,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
     bool ok = true;
     for (int turn = 0; turn < p.turns; ++turn) {
       BwdItem w;
-      if (!bwd_item<true>(p, turn, &w)) continue;
+      if (!bwd_item<true, kWindow>(p, turn, &w)) continue;
       int in_head = w.begin % w.per_head;
       for (int i = 0; i < w.steps && ok; ++i, ++steps) {
         const float* st = stats + steps % C::kStats * 2 * 128 + part * 32;
         // queries see keys up to themselves; a head's first step is the one on the diagonal
-        const bool diagonal = in_head == 0;
         const int from = row - part * 32, query = (w.first + in_head) * 128 + part * 32;
+        const bool diagonal = kWindow ? !p.span.whole((w.first + in_head) * 128, 128, w.tile * 128, 128) : in_head == 0;
+        uint32_t seen = ~0u;   // by which of its queries
+        if (kWindow && diagonal) seen = p.span.seen(w.tile * 128 + row, query);
         if (++in_head == w.per_head) in_head = 0;
         if (!(ok = waiter.wait(&bar.s_full, steps & 1))) break;
         tc::tc_fence_after();
@@ -659,7 +711,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
         tc::tmem_wait_ld();
         if (far) {
           const float* shifts = p.shifts + (w.head * p.group + (w.begin + i) / w.per_head) * p.seq.stat_rows + w.at.stat + query;
-          if (!(ok = far_step<T>(bar, waiter, steps & 1, s_at, dp_at, st, shifts, p.scale_log2, diagonal ? from : 0))) break;
+          if (!kWindow && diagonal) seen = from >= 32 ? 0u : from <= 0 ? ~0u : ~0u << from;
+          if (!(ok = far_step<T>(bar, waiter, steps & 1, s_at, dp_at, st, shifts, p.scale_log2, seen))) break;
           continue;
         }
 #pragma unroll
@@ -673,8 +726,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
         if (diagonal) {
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
-            if (2 * y < from) e[y].x = 0.f;
-            if (2 * y + 1 < from) e[y].y = 0.f;
+            if (kWindow ? ((seen >> (2 * y)) & 1) == 0 : 2 * y < from) e[y].x = 0.f;
+            if (kWindow ? ((seen >> (2 * y + 1)) & 1) == 0 : 2 * y + 1 < from) e[y].y = 0.f;
           }
         }
         // rounded to the inputs' type for their product, whose sums are in 32 bits
@@ -699,8 +752,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
         if (diagonal) {   // 0 times what is not finite
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
-            if (2 * y < from) e[y].x = 0.f;
-            if (2 * y + 1 < from) e[y].y = 0.f;
+            if (kWindow ? ((seen >> (2 * y)) & 1) == 0 : 2 * y < from) e[y].x = 0.f;
+            if (kWindow ? ((seen >> (2 * y + 1)) & 1) == 0 : 2 * y + 1 < from) e[y].y = 0.f;
           }
         }
 #pragma unroll
@@ -720,7 +773,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
       const float by = !ok ? NAN : part < 2 ? 1.f : p.scale;
       const int64_t out_row = (w.at.row + i) * p.kv_heads + w.head;
       T* to = static_cast<T*>(part < 2 ? p.dv : p.dk) + out_row * p.dim;
+      const bool sink = kWindow && w.sinks >= 0, whole = (sink ? p.sink_parts : p.parts) == 1;
       float* partial = p.partials + ((2 * w.part + (part < 2)) * p.partial_rows + out_row) * p.dim;
+      if (sink) {
+        const int64_t rows = int64_t(p.sink_tiles) * 128;
+        partial = p.sink_partials + (((2 * w.part + (part < 2)) * p.seq.n * rows + w.sinks * rows + i) * p.kv_heads + w.head) * p.dim;
+      }
       const int col0 = (part & 1) * (DP / 2);
 #pragma unroll
       for (int x = 0; x < DP / 2; x += 16) {
@@ -731,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
 #pragma unroll
         for (int y = 0; y < 16; ++y) o[y] = __uint_as_float(raw[y]);
         if (!there) continue;
-        if (p.parts == 1) {
+        if (whole) {
           store_row16<T>(to + col0 + x, o, by, p.dim - col0 - x, p.wide);
         } else {
 #pragma unroll
@@ -801,22 +859,30 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
 // Where single items of the keys would take longer than all the rest (key_parts), each is cut into parts that sum over some
 // of its steps (heads and queries) and leave their sums in 32 bits; these are added up here in the order of the parts, four
 // channels a thread.
-template <typename T>
+// CTAs behind those of all tiles have the tiles of the sinks.
+template <typename T, bool kWindow>
 __global__ void __launch_bounds__(256) attention_parts_kernel(const __grid_constant__ BwdParams p) {
   const int pieces = p.dim / 4;
   const int64_t x = int64_t(blockIdx.y) * blockDim.x + threadIdx.x;   // (row of the tile, kv head, piece)
-  const Item it = find_item(p.seq, int(blockIdx.x) >> 1, false);
-  const int tile = 2 * it.tile + (int(blockIdx.x) & 1);
+  const int unit = int(blockIdx.x), others = kWindow && p.parts == 1 ? 0 : 2 * p.seq.tiles;
+  const bool sink = kWindow && unit >= others;
+  const int sequence = sink ? (unit - others) / p.sink_tiles : 0;
+  const Item it = sink ? find_sequence(p.seq, sequence) : find_item(p.seq, unit >> 1, false);
+  const int tile = sink ? unit - others - sequence * p.sink_tiles : 2 * it.tile + (unit & 1);
   const int i = tile * 128 + int(x / (p.kv_heads * pieces));
-  if (i >= it.len || x >= int64_t(128) * p.kv_heads * pieces) return;
+  if (i >= it.len || x >= int64_t(128) * p.kv_heads * pieces || (kWindow && !sink && tile < p.sink_tiles)) return;
   const int64_t at = ((it.row + tile * 128) * p.kv_heads * pieces + x) * 4;
-  const int steps = ((it.len + 127) / 128 - tile) * p.group;
+  const int steps = (kWindow && !sink ? seeing_tiles(it.len, tile, p.span.window) : (it.len + 127) / 128 - tile) * p.group;
+  const int parts = sink ? p.sink_parts : p.parts;
+  const int64_t sink_rows = int64_t(p.sink_tiles) * 128;
+  const float* from = sink ? p.sink_partials + ((sequence * sink_rows + tile * 128) * p.kv_heads * pieces + x) * 4 : p.partials + at;
+  const int64_t next = (sink ? p.seq.n * sink_rows * p.kv_heads : p.partial_rows) * p.dim;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {   // dk, dv
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int part = 0; part < p.parts; ++part) {
-      if (part_begin(steps, part, p.parts) == part_begin(steps, part + 1, p.parts)) continue;
-      const float4 y = *reinterpret_cast<const float4*>(p.partials + (2 * part + which) * p.partial_rows * p.dim + at);
+    for (int part = 0; part < parts; ++part) {
+      if (part_begin(steps, part, parts) == part_begin(steps, part + 1, parts)) continue;
+      const float4 y = *reinterpret_cast<const float4*>(from + (2 * part + which) * next);
       sum.x += y.x; sum.y += y.y; sum.z += y.z; sum.w += y.w;
     }
     *reinterpret_cast<uint2*>(static_cast<T*>(which ? p.dv : p.dk) + at) = make_uint2(pack_pair<T>(sum.x, sum.y), pack_pair<T>(sum.z, sum.w));
@@ -839,19 +905,28 @@ int launch_half(Kernel kernel, int bytes, const BwdParams& base, int64_t items, 
   return launch_beside(kernel, unsigned(grid), kThreads, bytes, stream, p);
 }
 
-template <typename T, int DP>
-int launch_typed(const BwdParams& p, const DeltaParams& d, cudaStream_t stream) {
+template <typename T, int DP, bool kWindow>
+int launch_typed(BwdParams& p, const DeltaParams& d, cudaStream_t stream) {
   attention_delta_kernel<T><<<unsigned(p.seq.tiles * (kTileRows / kDeltaRows) * p.heads), 256, 0, stream>>>(d);
   int status = check_launch();
   if (status != GDN2_OK) return status;
   const int64_t tiles = int64_t(p.seq.tiles) * 2;
-  status = launch_half(&attention_keys_kernel<T, DP>, KeyConfig<DP>::kBytes, p, tiles * p.kv_heads * p.parts, stream);
+  p.sink_items = kWindow ? int64_t(p.seq.n) * p.sink_tiles * p.kv_heads * p.sink_parts : 0;
+  status = launch_half(&attention_keys_kernel<T, DP, kWindow>, KeyConfig<DP>::kBytes, p, tiles * p.kv_heads * p.parts + p.sink_items, stream);
   if (status != GDN2_OK) return status;
-  status = launch_half(&attention_queries_kernel<T, DP>, QueryConfig<DP>::kBytes, p, tiles * p.heads, stream);
-  if (status != GDN2_OK || p.parts == 1) return status;
-  const int64_t threads = int64_t(128) * p.kv_heads * (p.dim / 4);
-  attention_parts_kernel<T><<<dim3(unsigned(tiles), unsigned((threads + 255) / 256)), 256, 0, stream>>>(p);
+  status = launch_half(&attention_queries_kernel<T, DP, kWindow>, QueryConfig<DP>::kBytes, p, tiles * p.heads, stream);
+  if (status != GDN2_OK) return status;
+  const unsigned per_tile = unsigned((int64_t(128) * p.kv_heads * (p.dim / 4) + 255) / 256);
+  const int64_t ctas = (p.parts > 1 ? tiles : 0) + (p.sink_parts > 1 ? int64_t(p.seq.n) * p.sink_tiles : 0);
+  if (ctas == 0) return GDN2_OK;
+  attention_parts_kernel<T, kWindow><<<dim3(unsigned(ctas), per_tile), 256, 0, stream>>>(p);
   return check_launch();
+}
+
+template <typename T>
+int launch_dim(BwdParams& p, const DeltaParams& d, cudaStream_t stream) {
+  if (p.span.window > 0) return p.dim <= 64 ? launch_typed<T, 64, true>(p, d, stream) : launch_typed<T, 128, true>(p, d, stream);
+  return p.dim <= 64 ? launch_typed<T, 64, false>(p, d, stream) : launch_typed<T, 128, false>(p, d, stream);
 }
 
 }  // namespace
@@ -861,27 +936,49 @@ int launch_typed(const BwdParams& p, const DeltaParams& d, cudaStream_t stream) 
 // SM's share of both.  16 heads; whole items / parts: 1 x 2048 tokens, 2 key heads (128 steps, a share of 29) 259 / 134 us;
 // packed 700, 1200, 300 tokens, 2 key heads (80, 18) 173 / 128; 2 x 2048, 4 key heads (64, 118) 178 / 188; below sixteen
 // steps, 1 x 1000 tokens, 8 heads (8, 4) 122 / 126.
-static int key_parts(const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, int sms) {
+// With a window of W tokens an item has a group's heads times the tiles that the window reaches, and the tiles of the sinks
+// have all; those are cut by the same rule, but not finer than the others.
+struct KeyParts { int parts, sink_tiles, sink_parts; };
+static KeyParts key_parts(const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, const Span& span, int sms) {
   const int group = heads / kv_heads;
+  const int64_t reach = span.window > 0 ? (126 + span.window) / 128 + 1 : int64_t(1) << 40;   // tiles
+  const int64_t sink_tiles = span.window > 0 ? (span.sinks + 127) / 128 : 0;
   int64_t longest = 0, all = 0;
   for (int64_t i = 0; i < (bounds != nullptr ? n_seq : 1); ++i) {
     const int64_t tiles = ((bounds != nullptr ? bounds[i + 1] - bounds[i] : time) + 127) / 128;
     longest = std::max(longest, tiles * group);
-    all += tiles * (tiles + 1) / 2 * heads;
+    const int64_t up = std::min(tiles, reach);   // items that have 1, 2, ... tiles of queries; the others have as many as is most
+    all += (up * (up + 1) / 2 + (tiles - up) * up + std::min(sink_tiles, tiles) * (tiles - up)) * heads;
   }
   if (bounds == nullptr) all *= n_seq;
   const int64_t share = std::max<int64_t>(1, 2 * all / sms);
-  return longest < 16 ? 1 : int(std::max<int64_t>(1, longest / share));
+  auto parts = [&](int64_t steps, int64_t least) { return steps < 16 ? 1 : int(std::max<int64_t>(1, steps / std::max(share, least))); };
+  const int64_t windowed = std::min(longest, span.window > 0 ? reach * group : longest);
+  const int of_others = parts(windowed, 1);
+  return {of_others, int(sink_tiles), sink_tiles > 0 ? parts(longest, std::max<int64_t>(1, windowed / of_others)) : 1};
 }
 
-// delta, then the parts' sums
-int64_t attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, int dim) {
+// delta, then the parts' sums, then those of the sinks
+struct BackwardBytes { int64_t delta, parts, sinks; };
+static int backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, int dim, const Span& span, KeyParts* k,
+                          BackwardBytes* bytes) {
   int sms = 0;
   const int status = multiprocessors(&sms);
   if (status != GDN2_OK) return status;
-  const int64_t delta = (stat_rows(bounds, n_seq, time) * heads * 4 + 15) / 16 * 16;
-  const int parts = key_parts(bounds, n_seq, time, heads, kv_heads, sms);
-  return delta + (parts == 1 ? 0 : int64_t(parts) * 2 * (bounds != nullptr ? time : n_seq * time) * kv_heads * dim * 4);
+  *k = key_parts(bounds, n_seq, time, heads, kv_heads, span, sms);
+  bytes->delta = (stat_rows(bounds, n_seq, time) * heads * 4 + 15) / 16 * 16;
+  bytes->parts = k->parts == 1 ? 0 : int64_t(k->parts) * 2 * (bounds != nullptr ? time : n_seq * time) * kv_heads * dim * 4;
+  const int64_t sequences = bounds != nullptr ? std::min<int64_t>(n_seq, kMaxSequences) : n_seq;   // of a launch
+  bytes->sinks = k->sink_parts == 1 ? 0 : int64_t(k->sink_parts) * 2 * sequences * k->sink_tiles * 128 * kv_heads * dim * 4;
+  return GDN2_OK;
+}
+
+int64_t attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, int dim, int64_t window,
+                                 int64_t sinks) {
+  KeyParts k;
+  BackwardBytes bytes;
+  const int status = backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, span_of(window, sinks, bounds, n_seq, time), &k, &bytes);
+  return status != GDN2_OK ? status : bytes.delta + bytes.parts + bytes.sinks;
 }
 
 int64_t attention_stat_rows(const int64_t* bounds, int64_t n_seq, int64_t time) { return stat_rows(bounds, n_seq, time); }
@@ -889,7 +986,7 @@ int64_t attention_stat_rows(const int64_t* bounds, int64_t n_seq, int64_t time) 
 int launch_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out,
                               const float* lse, void* scratch, void* dq, void* dk, void* dv, const int64_t* strides,
                               const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, int dim,
-                              int dtype, float scale, cudaStream_t stream) {
+                              int dtype, float scale, int64_t window, int64_t sinks, cudaStream_t stream) {
   BwdParams p;
   const int64_t batch = bounds != nullptr ? 1 : n_seq;
   struct { CUtensorMap* map; const void* base; const int64_t* strides; int heads, rows; } maps[] = {
@@ -903,11 +1000,16 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   float* delta = static_cast<float*>(scratch);
   p.lse = lse; p.delta = delta;
   p.shifts = lse + stat_rows(bounds, n_seq, time) * heads;
-  int sms = 0;
-  const int status = multiprocessors(&sms);
+  p.span = span_of(window, sinks, bounds, n_seq, time);
+  KeyParts cut;
+  BackwardBytes bytes;
+  const int status = backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, p.span, &cut, &bytes);
   if (status != GDN2_OK) return status;
-  p.parts = key_parts(bounds, n_seq, time, heads, kv_heads, sms);
-  p.partials = delta + (stat_rows(bounds, n_seq, time) * heads + 3) / 4 * 4;
+  p.parts = cut.parts;
+  p.sink_tiles = cut.sink_tiles;
+  p.sink_parts = cut.sink_parts;
+  p.partials = delta + bytes.delta / 4;
+  p.sink_partials = p.partials + bytes.parts / 4;
   p.partial_rows = batch * time * kv_heads;
   p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.dim = dim;
   p.scale = scale;
@@ -917,10 +1019,7 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   p.scale_log2 = positive_scale(scale);
   return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {
     DeltaParams d{out, d_out, {strides[9], strides[10], strides[11]}, delta, heads, dim, p.seq};
-    if (dtype == GDN2_BF16) {
-      return dim <= 64 ? launch_typed<__nv_bfloat16, 64>(p, d, stream) : launch_typed<__nv_bfloat16, 128>(p, d, stream);
-    }
-    return dim <= 64 ? launch_typed<__half, 64>(p, d, stream) : launch_typed<__half, 128>(p, d, stream);
+    return dtype == GDN2_BF16 ? launch_dim<__nv_bfloat16>(p, d, stream) : launch_dim<__half>(p, d, stream);
   });
 }
 

@@ -34,6 +34,49 @@ struct Sequences {
   Entry e[kMaxSequences];
 };
 
+// What a row sees of its sequence: with a window W and S sinks the tokens j <= i with i - j < W or j < S, and with a window
+// of 0, which stands for none, all j <= i.  Sizes are below 2^30.
+struct Span {
+  int window, sinks;
+  // The first tile of `size` keys that some of the rows from `row` on see through the window, and how many tiles of sinks
+  // lie before it; where those reach it, it is the first one of all.
+  __device__ __forceinline__ int first_tile(int row, int size, int* sink_tiles) const {
+    const int first = max(0, row - window + 1) / size, lead = (sinks + size - 1) / size;
+    const bool apart = lead < first;
+    if (sink_tiles != nullptr) *sink_tiles = apart ? lead : 0;
+    return apart ? first : 0;
+  }
+  // all of `rows` rows see all of `keys` keys
+  __device__ __forceinline__ bool whole(int row, int rows, int key, int keys) const {
+    return key + keys - 1 <= row && (row + rows - 1 - key < window || key + keys <= sinks);
+  }
+  // bit y: the row sees key + y
+  __device__ __forceinline__ uint32_t sees(int row, int key) const {
+    auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };   // the first n
+    return below(row - key + 1) & (~below(row - window + 1 - key) | below(sinks - key));
+  }
+  // bit y: query + y sees the key
+  __device__ __forceinline__ uint32_t seen(int key, int query) const {
+    auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
+    return ~below(key - query) & (key < sinks ? ~0u : below(key + window - query));
+  }
+  // scores of 32 keys: those that the row does not see become -inf
+  __device__ __forceinline__ void hide(int row, int key, uint32_t (&s)[32]) const {
+    const uint32_t see = sees(row, key);
+#pragma unroll
+    for (int y = 0; y < 32; ++y) {
+      if (((see >> y) & 1) == 0) s[y] = 0xff800000u;
+    }
+  }
+};
+// A window that reaches over the longest sequence is none.
+inline Span span_of(int64_t window, int64_t sinks, const int64_t* bounds, int64_t n_seq, int64_t time) {
+  int64_t longest = bounds != nullptr ? 0 : time;
+  for (int64_t i = 0; bounds != nullptr && i < n_seq; ++i) longest = std::max(longest, bounds[i + 1] - bounds[i]);
+  if (window <= 0 || window >= longest) return {0, 0};
+  return {int(window), int(std::min<int64_t>(sinks, longest))};
+}
+
 struct Item {
   int row0, batch;   // where the sequence's first row is in the tensor maps
   int len, tile;     // of the sequence; number of the 256-row tile in it
@@ -68,6 +111,12 @@ __device__ __forceinline__ Item find_item(const Sequences& s, int t, bool last_f
   it.row = x.row0;
   it.stat = s.stat_row0 + int64_t(x.tile0) * kTileRows;
   return it;
+}
+
+// entry `sequence` of the launch, with tile 0
+__device__ __forceinline__ Item find_sequence(const Sequences& s, int sequence) {
+  const int t = s.packed ? s.e[sequence].tile0 : sequence;   // (not packed: the first tiles of all sequences come first)
+  return find_item(s, t, false);
 }
 
 // Items are in the order of their work, the longest first.  CTA c of n takes them by turns that go up and down, c,

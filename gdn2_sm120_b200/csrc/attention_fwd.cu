@@ -48,18 +48,23 @@ struct FwdParams {
   uint32_t negate;     // the scale is negative: Q counts with its sign changed
   uint32_t polls;      // of a wait
   bool wide;           // rows of the output are 32-byte aligned
+  Span span;           // what a row sees of the tokens before it
   Sequences seq;
 };
 
 struct FwdBars {
   uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2];
   uint64_t raw;        // a tile that is mended before the products may read it
+  uint64_t told;       // all rows of an item that is done once more have what was added to them
   uint64_t drained;
   uint64_t kv_full[8], kv_empty[8];
 };
 struct FwdMarks {
   uint32_t again[32];      // items to be done once more, a bit a turn modulo 1024 (another one of that bit is done for nothing)
-  uint32_t strange[4][8];  // rows of an item's two diagonal tiles with values that are not finite, of the last four such items
+  // rows of an item's two diagonal tiles with values that are not finite, of the last four such items; with a window those
+  // of the tiles that some row sees a part of, of one item: two on the diagonal, three that the window begins in, one that
+  // the sinks end in
+  uint32_t strange[4][8];
   uint32_t tmem;
   int failed;
 };
@@ -111,6 +116,7 @@ __device__ __forceinline__ void init_bars(FwdBars& bar) {
     tc::mbar_init(&bar.o_full[t], 1);
   }
   tc::mbar_init(&bar.raw, 1);
+  tc::mbar_init(&bar.told, 16);
   tc::mbar_init(&bar.drained, 1);
   for (int s = 0; s < kStages; ++s) {
     tc::mbar_init(&bar.kv_full[s], 1);
@@ -119,8 +125,52 @@ __device__ __forceinline__ void init_bars(FwdBars& bar) {
   tc::fence_mbar_init();
 }
 
+// The tiles of 128 keys that an item goes through, step by step, and the steps that each of its two tiles of queries has
+// of them: begin[t] .. end[t] - 1.  Without a window these are all tiles from the first to the one on the diagonal.  With
+// one they come down from the diagonal, on which every row sees something, then come the tiles of the sinks, where the
+// window does not reach them, and at last the tile that the second tile of queries does not see any more: neither has a
+// gap in its steps.
+template <bool kWindow>
+struct Steps {
+  int count, begin[2], end[2];
+  int top, down, sinks, last;   // first tile and number of those on the way down, tiles of sinks behind them, the last tile
+  __device__ __forceinline__ Steps(const Item& it, const Span& span) {
+    const int q = 2 * it.tile;
+    const bool two = (q + 1) * 128 < it.len;
+    if (!kWindow) {
+      begin[0] = begin[1] = 0;
+      end[0] = q * 128 < it.len ? q + 1 : 0;
+      end[1] = two ? q + 2 : 0;
+      count = max(end[0], end[1]);
+      return;
+    }
+    top = q + two;
+    last = span.first_tile(q * 128, 128, &sinks);
+    int next = two ? span.first_tile((q + 1) * 128, 128, nullptr) : last;
+    if (sinks == 0 && last == 0 && span.sinks > 0) next = 0;   // sinks and window meet: all tiles are gone through
+    down = top - next + 1;
+    count = down + sinks + (last < next);
+    begin[0] = two;
+    end[0] = count;
+    begin[1] = 0;
+    end[1] = two ? down + sinks : 0;
+  }
+  __device__ __forceinline__ int tile(int step) const {
+    return !kWindow ? step : step < down ? top - step : step < down + sinks ? step - down : last;
+  }
+  __device__ __forceinline__ bool has(int t, int step) const { return step >= begin[t] && step < end[t]; }
+  // some row of a tile of queries that goes through it does not see all of this step's keys
+  __device__ __forceinline__ bool partial(const Item& it, const Span& span, int step) const {
+    const int k = tile(step);
+    bool any = false;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) any = any || (has(t, step) && !span.whole((2 * it.tile + t) * 128, 128, k * 128, 128));
+    return any;
+  }
+};
+
 // All items of the CTA, or the marked ones once more
-template <typename T, int DP, bool kAgain>
+template <typename T, int DP, bool kWindow, bool kAgain>
 __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem, FwdBars& bar, FwdMarks& marks, float (*told)[2][128],
                                               uint32_t tmem) {
   using C = FwdConfig<DP>;
@@ -134,10 +184,6 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
     const int t = int(index / p.heads);
     *head = int(index - int64_t(t) * p.heads);
     return find_item(p.seq, t, true);
-  };
-  auto key_tiles = [](const Item& it, int t) {  // of the first or second query tile
-    const int tile = 2 * it.tile + t;
-    return tile * 128 < it.len ? tile + 1 : 0;
   };
 
   auto marked = [&](int turn) { return ((marks.again[(turn >> 5) & 31] >> (turn & 31)) & 1) != 0; };
@@ -162,11 +208,14 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
         int head;
         const Item it = item_at(index, &head);
         const int kv_head = head / p.group;
-        const int n = max(key_tiles(it, 0), key_tiles(it, 1));
-        for (int j = 0; j < n && ok; ++j) {
-          if (j == 0) {
+        const Steps<kWindow> steps(it, p.span);
+        const int n = steps.count;
+        int sifted = 0;
+        for (int step = 0; step < n && ok; ++step) {
+          const int j = steps.tile(step);
+          if (step == 0) {
             for (int t = 0; t < 2 && ok; ++t) {
-              if (key_tiles(it, t) == 0) continue;
+              if (steps.end[t] == 0) continue;
               if (loaded[t] > 0) ok = waiter.wait(&bar.q_empty[t], (loaded[t] - 1) & 1);
               if (!ok) break;
               load(&p.q, q_tiles + t * C::kTileBytes, head, it.row0 + (2 * it.tile + t) * 128, it.batch, &bar.q_full[t]);
@@ -175,7 +224,7 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
                 const int s = filled % C::kStages;
                 if (filled >= C::kStages) ok = waiter.wait(&bar.kv_empty[s], (filled / C::kStages - 1) & 1);
                 if (!ok) break;
-                load(&p.k, kv_tiles + s * C::kTileBytes, kv_head, it.row0, it.batch, &bar.kv_full[s]);
+                load(&p.k, kv_tiles + s * C::kTileBytes, kv_head, it.row0 + (kWindow ? j * 128 : 0), it.batch, &bar.kv_full[s]);
                 ++filled;
               }
             }
@@ -192,7 +241,8 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
           if (!ok) break;
           uint8_t* to = kv_tiles + s * C::kTileBytes;
           const int valid = it.len - j * 128;   // rows of the sequence
-          const bool diagonal = kAgain && j >= 2 * it.tile;   // of one of the two tiles of queries
+          // of one of the two tiles of queries; with a window whatever some row does not see all of
+          const bool diagonal = kAgain && (kWindow ? steps.partial(it, p.span, step) : j >= 2 * it.tile);
           if (diagonal || (p.seq.packed && valid < 128)) {
             // rows of the next sequence: their weights are 0, but 0 * inf and 0 * NaN are not
             load(&p.v, to, kv_head, it.row0 + j * 128, it.batch, &bar.raw);
@@ -204,11 +254,21 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
               for (int x = valid * 8 + lane; x < 128 * 8; x += 32) lines[x] = make_uint4(0, 0, 0, 0);
             }
             if (diagonal) {
-              // (when an item's queries could be loaded, nobody reads the rows of the one three before it any more)
-              uint32_t* strange = marks.strange[redone & 3];
-              if (j == 2 * it.tile && lane < 8) strange[lane] = 0;
+              uint32_t* strange;
+              if (kWindow) {
+                // one item's rows at a time, in the order of its steps
+                if (sifted == 0 && redone > 1) ok = waiter.wait(&bar.told, (redone - 2) & 1);
+                if (!ok) break;
+                strange = marks.strange[0] + 4 * sifted++;
+                if (lane < 4) strange[lane] = 0;
+              } else {
+                // (when an item's queries could be loaded, nobody reads the rows of the one three before it any more)
+                strange = marks.strange[redone & 3];
+                if (j == 2 * it.tile && lane < 8) strange[lane] = 0;
+                strange += (j - 2 * it.tile) * 4;
+              }
               sift<T, DP>(tc::smem_u32(to), C::kSlab, 0, min(valid, 128),
-                          [&](int row) { atomicOr(&strange[(j - 2 * it.tile) * 4 + (row >> 5)], 1u << (row & 31)); });
+                          [&](int row) { atomicOr(&strange[row >> 5], 1u << (row & 31)); });
             }
             tc::fence_async_smem();
             __syncwarp();
@@ -250,17 +310,17 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
         if (index >= p.items || (kAgain && !marked(turn))) continue;
         int head;
         const Item it = item_at(index, &head);
-        const int n_t[2] = {key_tiles(it, 0), key_tiles(it, 1)};
-        const int n = max(n_t[0], n_t[1]);
+        const Steps<kWindow> steps(it, p.span);
+        const int n = steps.count;
         auto full = [&](int x) { return waiter.wait(&bar.kv_full[x % C::kStages], (x / C::kStages) & 1); };
         if (!(ok = full(used))) break;
   #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (n_t[t] == 0 || !ok) continue;
+          if (steps.end[t] == 0 || steps.begin[t] > 0 || !ok) continue;
           if (!(ok = waiter.wait(&bar.q_full[t], q_used[t] & 1))) continue;
           tc::tc_fence_after();
           scores(t, used % C::kStages);
-          if (n_t[t] == 1) tc::mma_commit(&bar.q_empty[t], leader);
+          if (steps.end[t] == 1) tc::mma_commit(&bar.q_empty[t], leader);
         }
         if (!ok) break;
         tc::mma_commit(&bar.kv_empty[used % C::kStages], leader);
@@ -271,26 +331,30 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
           const uint32_t v_tile = kv_base + (xv % C::kStages) * C::kTileBytes;
   #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (j < n_t[t] && ok) {
+            if (steps.has(t, j) && ok) {
               if (!(ok = waiter.wait(&bar.p_ready[t], p_used[t] & 1))) continue;
               ++p_used[t];
               tc::tc_fence_after();
   #pragma unroll
               for (int ks = 0; ks < 8; ++ks) {
-                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + (ks >> 2) * 64 + (ks & 3) * 8, desc_mn(v_tile, C::kSlab, ks), id_o, j > 0 || ks > 0, leader);
+                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + (ks >> 2) * 64 + (ks & 3) * 8, desc_mn(v_tile, C::kSlab, ks), id_o, j > steps.begin[t] || ks > 0, leader);
               }
-              if (j + 1 == n_t[t]) tc::mma_commit(&bar.o_full[t], leader);
+              if (j + 1 == steps.end[t]) tc::mma_commit(&bar.o_full[t], leader);
             }
             if (t == 1) tc::mma_commit(&bar.kv_empty[xv % C::kStages], leader);
-            if (j + 1 < n_t[t]) {
+            if (steps.has(t, j + 1) && (!kWindow || ok)) {
+              if (kWindow && j + 1 == steps.begin[t]) {
+                if (!(ok = waiter.wait(&bar.q_full[t], q_used[t] & 1))) continue;
+                tc::tc_fence_after();
+              }
               scores(t, xk % C::kStages);
-              if (j + 2 == n_t[t]) tc::mma_commit(&bar.q_empty[t], leader);
+              if (j + 2 == steps.end[t]) tc::mma_commit(&bar.q_empty[t], leader);
             }
           }
           if (j + 1 < n) tc::mma_commit(&bar.kv_empty[xk % C::kStages], leader);
         }
         used += 2 * n;
-        for (int t = 0; t < 2; ++t) q_used[t] += n_t[t] > 0;
+        for (int t = 0; t < 2; ++t) q_used[t] += steps.end[t] > 0;
       }
       if (!ok) {  // products under way end before the CTA does
         tc::mma_commit(&bar.drained, leader);
@@ -312,8 +376,10 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
       redone += kAgain;
       int head;
       const Item it = item_at(index, &head);
-      const int n = key_tiles(it, t);
+      const Steps<kWindow> steps(it, p.span);
+      const int begin = kWindow ? steps.begin[t] : 0, n = steps.end[t];
       if (n == 0) {
+        if (kWindow && kAgain) tc::mbar_arrive(&bar.told, lane == 0);
         if (p.lse != nullptr && half == 0) p.lse[head * p.seq.stat_rows + it.stat + (2 * it.tile + t) * 128 + row] = -INFINITY;
         continue;
       }
@@ -322,12 +388,17 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
       bool far = false;
       // The warps of a chain meet in barriers: one that waited in vain goes on as the others do, and what came of all waits is
       // asked behind the last of them.
-      for (int j = 0; j < n; ++j) {
+      for (int j = begin; j < n; ++j) {
+        // with a window: this row's place in the tile of keys, whether all rows see all of it
+        const int key0 = kWindow ? steps.tile(j) * 128 + half * 64 : 0;
+        const bool whole = !kWindow || p.span.whole((2 * it.tile + t) * 128, 128, steps.tile(j) * 128, 128);
         waiter.wait(&bar.s_full[t], seen & 1);
         ++seen;
         tc::tc_fence_after();
-        soften_half<T, DP>(pair, s_at, o_at, c, j == 0, m, sum, far, [&](int x, uint32_t (&s)[32]) {
-          if (j + 1 == n) {   // the tile on the diagonal; what lies behind the sequence's end lies behind every row
+        soften_half<T, DP>(pair, s_at, o_at, c, j == begin, m, sum, far, [&](int x, uint32_t (&s)[32]) {
+          if (kWindow) {
+            if (!whole) p.span.hide((2 * it.tile + t) * 128 + row, key0 + x * 32, s);
+          } else if (j + 1 == n) {   // the tile on the diagonal; what lies behind the sequence's end lies behind every row
 #pragma unroll
             for (int y = 0; y < 32; ++y) {
               if (half * 64 + x * 32 + y > row) s[y] = 0xff800000u;
@@ -363,6 +434,23 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
       }
       if (!kAgain) {
         if (strange != 0.f && there && ok && isfinite(sum)) atomicOr(&marks.again[(turn >> 5) & 31], 1u << (turn & 31));
+      } else if (kWindow) {
+        int sifted = 0;
+        for (int j = 0; j < steps.count && there && ok && col0 < p.dim; ++j) {
+          if (!steps.partial(it, p.span, j)) continue;
+          const uint32_t* strange = marks.strange[0] + 4 * sifted++;
+          if (j < begin || j >= n) continue;
+          const int k = steps.tile(j) * 128;
+          uint32_t sees[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sees[x] = p.span.sees(i, k + x * 32) & strange[x];
+          if ((sees[0] | sees[1] | sees[2] | sees[3]) == 0) continue;
+          const T* v = static_cast<const T*>(p.values) + it.batch * p.strides[0] + (it.row0 + int64_t(k)) * p.strides[1] +
+                       head / p.group * p.strides[2] + col0;
+          add_strange<T>(v, p.strides[1], sees, 127, to + col0, min(p.dim - col0, DP / 2));
+        }
+        __syncwarp();
+        tc::mbar_arrive(&bar.told, lane == 0);
       } else if (there && ok && col0 < p.dim) {
         const T* v = static_cast<const T*>(p.values) + it.batch * p.strides[0] + (it.row0 + int64_t(it.tile) * kTileRows) * p.strides[1] +
                      head / p.group * p.strides[2] + col0;
@@ -381,7 +469,7 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool kWindow>
 __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __grid_constant__ FwdParams p) {
   using C = FwdConfig<DP>;
   extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
@@ -404,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = marks.tmem;
-  forward_items<T, DP, false>(p, smem, bars[0], marks, told, tmem);
+  forward_items<T, DP, kWindow, false>(p, smem, bars[0], marks, told, tmem);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -412,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
   if (__any_sync(0xffffffffu, marks.again[threadIdx.x & 31] != 0) && marks.failed == 0) {
     if (threadIdx.x == 0) init_bars<C::kStages>(bars[1]);
     __syncthreads();
-    forward_items<T, DP, true>(p, smem, bars[1], marks, told, tmem);
+    forward_items<T, DP, kWindow, true>(p, smem, bars[1], marks, told, tmem);
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -420,10 +508,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_forward_kernel(const __
   if (warp == 16) tc::tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool kWindow>
 int launch_typed(const FwdParams& p, cudaStream_t stream) {
   using C = FwdConfig<DP>;
-  const void* kernel = reinterpret_cast<const void*>(&attention_forward_kernel<T, DP>);
+  const void* kernel = reinterpret_cast<const void*>(&attention_forward_kernel<T, DP, kWindow>);
   const cudaError_t err = ensure_dynamic_smem(kernel, C::kBytes);
   if (err != cudaSuccess) { record_cuda_error(err); return GDN2_ERR_LAUNCH; }
   int sms = 0;
@@ -432,15 +520,21 @@ int launch_typed(const FwdParams& p, cudaStream_t stream) {
   FwdParams q = p;
   const int64_t grid = p.items < sms ? p.items : sms;
   q.turns = int((p.items + grid - 1) / grid);
-  attention_forward_kernel<T, DP><<<unsigned(grid), kThreads, C::kBytes, stream>>>(q);
+  attention_forward_kernel<T, DP, kWindow><<<unsigned(grid), kThreads, C::kBytes, stream>>>(q);
   return check_launch();
+}
+
+template <typename T>
+int launch_dim(const FwdParams& p, cudaStream_t stream) {
+  if (p.span.window > 0) return p.dim <= 64 ? launch_typed<T, 64, true>(p, stream) : launch_typed<T, 128, true>(p, stream);
+  return p.dim <= 64 ? launch_typed<T, 64, false>(p, stream) : launch_typed<T, 128, false>(p, stream);
 }
 
 }  // namespace
 
 int launch_attention_forward(const void* q, const void* k, const void* v, void* out, float* lse, const int64_t* strides,
                              const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, int dim,
-                             int dtype, float scale, cudaStream_t stream) {
+                             int dtype, float scale, int64_t window, int64_t sinks, cudaStream_t stream) {
   FwdParams p;
   const int64_t batch = bounds != nullptr ? 1 : n_seq;
   if (!encode_heads_map(&p.q, q, strides, batch, time, heads, dim, dtype, 128) ||
@@ -456,10 +550,10 @@ int launch_attention_forward(const void* q, const void* k, const void* v, void* 
   p.polls = wait_polls();
   p.wide = wide_rows(out, dim);
   p.scale_log2 = positive_scale(scale);
+  p.span = span_of(window, sinks, bounds, n_seq, time);
   return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {
     p.items = int64_t(p.seq.tiles) * heads;
-    if (dtype == GDN2_BF16) return dim <= 64 ? launch_typed<__nv_bfloat16, 64>(p, stream) : launch_typed<__nv_bfloat16, 128>(p, stream);
-    return dim <= 64 ? launch_typed<__half, 64>(p, stream) : launch_typed<__half, 128>(p, stream);
+    return dtype == GDN2_BF16 ? launch_dim<__nv_bfloat16>(p, stream) : launch_dim<__half>(p, stream);
   });
 }
 

@@ -47,6 +47,9 @@ struct Api {
   decltype(&gdn2_attention_forward) attention_forward;
   decltype(&gdn2_attention_backward_bytes) attention_backward_bytes;
   decltype(&gdn2_attention_backward) attention_backward;
+  decltype(&gdn2_window_attention_forward) window_attention_forward;
+  decltype(&gdn2_window_attention_backward_bytes) window_attention_backward_bytes;
+  decltype(&gdn2_window_attention_backward) window_attention_backward;
 } api;
 PyObject* g_check = nullptr;     // _lib.check(status, name): raises
 PyObject* g_launches = nullptr;  // _lib.LAUNCHES
@@ -783,17 +786,27 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_CATCH
 }
 
-// attention_forward(q, k, v, bounds, scale, training) -> (output, statistics or None) or None
+// window and sinks, (0, 0) for none
+bool read_window(PyObject* const* a, int64_t* window, int64_t* sinks) {
+  int overflow[2] = {1, 1};
+  if (!PyLong_CheckExact(a[0]) || !PyLong_CheckExact(a[1])) return false;
+  *window = PyLong_AsLongLongAndOverflow(a[0], &overflow[0]);
+  *sinks = PyLong_AsLongLongAndOverflow(a[1], &overflow[1]);
+  return overflow[0] == 0 && overflow[1] == 0 && *sinks >= 0 && (*window > 0 || (*window == 0 && *sinks == 0));
+}
+
+// attention_forward(q, k, v, bounds, scale, window, sinks, training) -> (output, statistics or None) or None
 PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_TRY
   Heads h;
   float scale;
   std::vector<int64_t> bounds;
-  if (!g_bound || n != 6 || !read_heads(a, &h) || !read_bounds(a[3], h, &bounds) || !read_attention_scale(a[4], h.dim, &scale) ||
-      wants_grad({h.t[0], h.t[1], h.t[2]})) {
+  int64_t window, sinks;
+  if (!g_bound || n != 8 || !read_heads(a, &h) || !read_bounds(a[3], h, &bounds) || !read_attention_scale(a[4], h.dim, &scale) ||
+      !read_window(a + 5, &window, &sinks) || wants_grad({h.t[0], h.t[1], h.t[2]})) {
     return none();
   }
-  const bool training = a[5] == Py_True;
+  const bool training = a[7] == Py_True;
   const at::Tensor& q = *h.t[0];
   const int64_t* host = bounds.empty() ? nullptr : bounds.data();
   const int64_t n_seq = bounds.empty() ? h.batch : int64_t(bounds.size()) - 1;
@@ -808,11 +821,15 @@ PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   out = at::empty(q.sizes(), q.options());
   if (training) statistics = floats({2, h.heads, rows}, q);
-  status = api.attention_forward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out.data_ptr(),
-                                 training ? fptr(&statistics) : nullptr, h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim,
-                                 h.dtype, scale, at::cuda::getCurrentCUDAStream().stream());
+  float* stat = training ? fptr(&statistics) : nullptr;
+  void* stream = at::cuda::getCurrentCUDAStream().stream();
+  status = window == 0
+               ? api.attention_forward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out.data_ptr(), stat, h.strides, host,
+                                       n_seq, h.time, h.heads, h.kv_heads, h.dim, h.dtype, scale, stream)
+               : api.window_attention_forward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out.data_ptr(), stat, h.strides,
+                                              host, n_seq, h.time, h.heads, h.kv_heads, h.dim, window, sinks, h.dtype, scale, stream);
   others.end();
-  if (!ok(status, "gdn2_attention_forward", passes(bounds))) return nullptr;
+  if (!ok(status, window == 0 ? "gdn2_attention_forward" : "gdn2_window_attention_forward", passes(bounds))) return nullptr;
   PyObject* result = PyTuple_New(2);
   PyTuple_SET_ITEM(result, 0, wrap(out));
   PyTuple_SET_ITEM(result, 1, training ? wrap(statistics) : Py_NewRef(Py_None));
@@ -820,13 +837,15 @@ PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_CATCH
 }
 
-// attention_backward(q, k, v, output, statistics, d_output, bounds, scale) -> (dq, dk, dv) or None
+// attention_backward(q, k, v, output, statistics, d_output, bounds, scale, window, sinks) -> (dq, dk, dv) or None
 PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_TRY
   Heads h;
   float scale;
   std::vector<int64_t> bounds;
-  if (!g_bound || n != 8 || !read_heads(a, &h) || !read_bounds(a[6], h, &bounds) || !read_attention_scale(a[7], h.dim, &scale)) {
+  int64_t window, sinks;
+  if (!g_bound || n != 10 || !read_heads(a, &h) || !read_bounds(a[6], h, &bounds) || !read_attention_scale(a[7], h.dim, &scale) ||
+      !read_window(a + 8, &window, &sinks)) {
     return none();
   }
   const at::Tensor& q = *h.t[0];
@@ -841,20 +860,29 @@ PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int status;
   WithoutGil others;
   const c10::cuda::CUDAGuard guard(q.device());
-  const int64_t size = api.attention_backward_bytes(host, n_seq, h.time, h.heads, h.kv_heads, h.dim);
+  const int64_t size =
+      window == 0 ? api.attention_backward_bytes(host, n_seq, h.time, h.heads, h.kv_heads, h.dim)
+                  : api.window_attention_backward_bytes(host, n_seq, h.time, h.heads, h.kv_heads, h.dim, window, sinks);
   if (size < 0) {
     others.end();
     return none();
   }
   for (int i = 0; i < 3; ++i) grads[i] = at::empty(h.t[i]->sizes(), q.options());
   const at::Tensor scratch = bytes(size, q);
-  status = api.attention_backward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out->data_ptr(), d_out->data_ptr(),
-                                  fptr(statistics), scratch.data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(),
-                                  h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim, h.dtype, scale,
-                                  at::cuda::getCurrentCUDAStream().stream());
+  void* stream = at::cuda::getCurrentCUDAStream().stream();
+  status = window == 0
+               ? api.attention_backward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out->data_ptr(), d_out->data_ptr(),
+                                        fptr(statistics), scratch.data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(),
+                                        grads[2].data_ptr(), h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim, h.dtype, scale,
+                                        stream)
+               : api.window_attention_backward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out->data_ptr(), d_out->data_ptr(),
+                                               fptr(statistics), scratch.data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(),
+                                               grads[2].data_ptr(), h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim, window,
+                                               sinks, h.dtype, scale, stream);
   others.end();
   const bool parts = size > 2 * statistics->numel() + 15;   // sums of several CTAs are added up
-  if (!ok(status, "gdn2_attention_backward", (parts ? 4 : 3) * passes(bounds))) return nullptr;
+  const char* name = window == 0 ? "gdn2_attention_backward" : "gdn2_window_attention_backward";
+  if (!ok(status, name, (parts ? 4 : 3) * passes(bounds))) return nullptr;
   PyObject* result = PyTuple_New(3);
   for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(result, i, wrap(grads[i]));
   return result;
@@ -897,6 +925,9 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_BIND(attention_forward);
   GDN2_BIND(attention_backward_bytes);
   GDN2_BIND(attention_backward);
+  GDN2_BIND(window_attention_forward);
+  GDN2_BIND(window_attention_backward_bytes);
+  GDN2_BIND(window_attention_backward);
 #undef GDN2_BIND
   if (missing) {
     PyErr_SetString(PyExc_RuntimeError, "libgdn2_b200.so lacks an entry point");

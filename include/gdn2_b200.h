@@ -508,6 +508,23 @@ int gdn2_attention_backward(const void* q, const void* k, const void* v, const v
                             void* stream);
 
 /*
+ * The same with a sliding window: token i sees the tokens j <= i with i - j < window, itself among them, and the first
+ * `sinks` of its sequence (those that are not behind it).  window >= 1, sinks >= 0.  A window that reaches over the
+ * longest sequence is causal attention and gives its bits.
+ */
+int gdn2_window_attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics,
+                                  const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time,
+                                  int64_t heads, int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks,
+                                  int dtype, float scale, void* stream);
+int64_t gdn2_window_attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads,
+                                             int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks);
+int gdn2_window_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out,
+                                   const float* statistics, void* scratch, void* dq, void* dk, void* dv,
+                                   const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time,
+                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks,
+                                   int dtype, float scale, void* stream);
+
+/*
  * Test aid: how often a wait inside the attention kernels of later calls polls (0: it looks once; negative: as usual).
  * A CTA in which a wait runs out ends by itself and leaves NaN in place of what it has not finished.  For the process.
  */
