@@ -389,15 +389,19 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
       // The warps of a chain meet in barriers: one that waited in vain goes on as the others do, and what came of all waits is
       // asked behind the last of them.
       for (int j = begin; j < n; ++j) {
-        // with a window: this row's place in the tile of keys, whether all rows see all of it
-        const int key0 = kWindow ? steps.tile(j) * 128 + half * 64 : 0;
-        const bool whole = !kWindow || p.span.whole((2 * it.tile + t) * 128, 128, steps.tile(j) * 128, 128);
+        // with a window: the thread's first key, whether all rows are there and see all of them
+        const int row0 = (2 * it.tile + t) * 128, key0 = kWindow ? steps.tile(j) * 128 + half * 64 : 0;
+        const bool whole = !kWindow || (row0 + 128 <= it.len && p.span.whole(row0, 128, steps.tile(j) * 128, 128));
         waiter.wait(&bar.s_full[t], seen & 1);
         ++seen;
         tc::tc_fence_after();
         soften_half<T, DP>(pair, s_at, o_at, c, j == begin, m, sum, far, [&](int x, uint32_t (&s)[32]) {
           if (kWindow) {
-            if (!whole) p.span.hide((2 * it.tile + t) * 128 + row, key0 + x * 32, s);
+            if (!whole) p.span.hide(row0 + row, key0 + x * 32, s);
+            if (!whole && row0 + row >= it.len) {   // another sequence's: no score of it makes others look for their maxima
+#pragma unroll
+              for (int y = 0; y < 32; ++y) s[y] = 0;
+            }
           } else if (j + 1 == n) {   // the tile on the diagonal; what lies behind the sequence's end lies behind every row
 #pragma unroll
             for (int y = 0; y < 32; ++y) {
