@@ -76,6 +76,7 @@ _PROTOTYPES: dict[str, list] = {
     "gdn2_window_attention_forward": [_P] * 7 + [_I64] * 7 + [_INT, _F32, _P],
     "gdn2_window_attention_backward_bytes": [_P] + [_I64] * 7,
     "gdn2_window_attention_backward": [_P] * 12 + [_I64] * 7 + [_INT, _F32, _P],
+    "gdn2_window_tree_attention": [_P] * 12 + [_I64] * 13 + [_INT, _F32, _P],
     "gdn2_debug_wait_limit": [_I64],
     "gdn2_profile_enable": [_INT],
     "gdn2_profile_chunk_kernels": [_P] * 4,

@@ -1,6 +1,7 @@
 // extern "C" entry points of the operators of an attention layer: argument validation + kernel launches.
 // No allocation, no synchronisation, no exceptions cross this boundary.
 
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
@@ -14,8 +15,8 @@ int launch_append(const void*, const void*, void*, void*, const int64_t*, int64_
 int tree_ctas(int*);
 int64_t tree_workspace_bytes(int64_t, int, int);
 int launch_tree(const void*, const void*, const void*, const void*, const void*, const int*, const int*, const uint8_t*,
-                void*, void*, const int64_t*, int64_t, int64_t, int, int, int, int, int, int64_t, int, int, int, float,
-                cudaStream_t);
+                void*, void*, const int64_t*, int64_t, int64_t, int, int, int, int, int, int64_t, int, int, const int*, int64_t, int,
+                int, int, float, cudaStream_t);
 namespace attn {
 static std::atomic<uint32_t> g_wait_polls{GDN2_ATTENTION_WAIT_POLLS};
 uint32_t wait_polls() { return g_wait_polls.load(std::memory_order_relaxed); }
@@ -62,6 +63,35 @@ int check_sequences(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t 
   // pieces of 64 rows are numbered with 31 bits
   const int64_t stat = attn::attention_stat_rows(bounds, n_seq, time);
   return stat / 64 > kMost / heads ? GDN2_ERR_TOO_LARGE : GDN2_OK;
+}
+
+// Attention over a paged cache, with a window of 0 for none
+int tree_attention(const void* q, const void* k, const void* v, const void* k_pages, const void* v_pages,
+                   const int* page_table, const int* lengths, const void* mask, const int* depths, void* out,
+                   void* workspace, const int64_t* strides, int64_t table_stride, int64_t mask_stride, int64_t depth_stride,
+                   int64_t batch, int64_t drafted, int64_t heads, int64_t kv_heads, int64_t dim, int64_t pages, int64_t page,
+                   int64_t columns, int64_t window, int64_t sinks, int dtype, float scale, void* stream) {
+  if (!q || !k || !v || !k_pages || !v_pages || !page_table || !lengths || !out || !workspace || !strides) {
+    return GDN2_ERR_NULL_POINTER;
+  }
+  int status = check_heads(heads, kv_heads, dim);
+  if (status != GDN2_OK) return status;
+  if (batch <= 0 || drafted <= 0 || pages <= 0 || page <= 0 || columns < 0) return GDN2_ERR_BAD_SHAPE;
+  if (!valid_seq_dtype(dtype)) return GDN2_ERR_BAD_DTYPE;
+  // a sequence's tokens, cached and drafted, are numbered with 31 bits
+  if (batch > kMost || drafted > kMost / 2 / heads || pages > kMost || page > kMost || columns > (kMost / 2 - 128) / page) {
+    return GDN2_ERR_TOO_LARGE;
+  }
+  if ((status = check_strides(strides, 9)) != GDN2_OK) return status;
+  const void* need16[] = {q, k, v, k_pages, v_pages, out, workspace};
+  for (const void* p : need16) {
+    if (!aligned(p, 16)) return GDN2_ERR_ALIGNMENT;
+  }
+  if (!aligned(page_table, 4) || !aligned(lengths, 4) || !aligned(depths, 4)) return GDN2_ERR_ALIGNMENT;
+  return launch_tree(q, k, v, k_pages, v_pages, page_table, lengths, static_cast<const uint8_t*>(mask), out, workspace,
+                     strides, table_stride, mask_stride, int(batch), int(drafted), int(heads), int(kv_heads), int(dim),
+                     pages, int(page), int(columns), depths, depth_stride, int(std::min(window, kMost / 2)),
+                     int(std::min(sinks, kMost / 2)), dtype, scale, static_cast<cudaStream_t>(stream));
 }
 
 // Causal attention, with a window of 0 for none
@@ -163,26 +193,20 @@ int gdn2_tree_attention(const void* q, const void* k, const void* v, const void*
                         const int64_t* strides, int64_t table_stride, int64_t mask_stride, int64_t batch, int64_t drafted,
                         int64_t heads, int64_t kv_heads, int64_t dim, int64_t pages, int64_t page, int64_t columns,
                         int dtype, float scale, void* stream) {
-  if (!q || !k || !v || !k_pages || !v_pages || !page_table || !lengths || !out || !workspace || !strides) {
-    return GDN2_ERR_NULL_POINTER;
-  }
-  int status = check_heads(heads, kv_heads, dim);
-  if (status != GDN2_OK) return status;
-  if (batch <= 0 || drafted <= 0 || pages <= 0 || page <= 0 || columns < 0) return GDN2_ERR_BAD_SHAPE;
-  if (!valid_seq_dtype(dtype)) return GDN2_ERR_BAD_DTYPE;
-  // a sequence's tokens, cached and drafted, are numbered with 31 bits
-  if (batch > kMost || drafted > kMost / 2 / heads || pages > kMost || page > kMost || columns > (kMost / 2 - 128) / page) {
-    return GDN2_ERR_TOO_LARGE;
-  }
-  if ((status = check_strides(strides, 9)) != GDN2_OK) return status;
-  const void* need16[] = {q, k, v, k_pages, v_pages, out, workspace};
-  for (const void* p : need16) {
-    if (!aligned(p, 16)) return GDN2_ERR_ALIGNMENT;
-  }
-  if (!aligned(page_table, 4) || !aligned(lengths, 4)) return GDN2_ERR_ALIGNMENT;
-  return launch_tree(q, k, v, k_pages, v_pages, page_table, lengths, static_cast<const uint8_t*>(mask), out, workspace,
-                     strides, table_stride, mask_stride, int(batch), int(drafted), int(heads), int(kv_heads), int(dim),
-                     pages, int(page), int(columns), dtype, scale, static_cast<cudaStream_t>(stream));
+  return tree_attention(q, k, v, k_pages, v_pages, page_table, lengths, mask, nullptr, out, workspace, strides, table_stride,
+                        mask_stride, 0, batch, drafted, heads, kv_heads, dim, pages, page, columns, 0, 0, dtype, scale, stream);
+}
+
+int gdn2_window_tree_attention(const void* q, const void* k, const void* v, const void* k_pages, const void* v_pages,
+                               const int* page_table, const int* lengths, const void* mask, const int* depths, void* out,
+                               void* workspace, const int64_t* strides, int64_t table_stride, int64_t mask_stride,
+                               int64_t depth_stride, int64_t batch, int64_t drafted, int64_t heads, int64_t kv_heads, int64_t dim,
+                               int64_t pages, int64_t page, int64_t columns, int64_t window, int64_t sinks, int dtype, float scale,
+                               void* stream) {
+  if (window <= 0 || sinks < 0 || (mask != nullptr && depths == nullptr)) return GDN2_ERR_BAD_RANGE;
+  return tree_attention(q, k, v, k_pages, v_pages, page_table, lengths, mask, depths, out, workspace, strides, table_stride,
+                        mask_stride, depth_stride, batch, drafted, heads, kv_heads, dim, pages, page, columns, window, sinks, dtype,
+                        scale, stream);
 }
 
 int64_t gdn2_attention_stat_rows(const int64_t* bounds, int64_t n_seq, int64_t time) {

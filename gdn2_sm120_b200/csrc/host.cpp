@@ -47,6 +47,7 @@ struct Api {
   decltype(&gdn2_attention_forward) attention_forward;
   decltype(&gdn2_attention_backward_bytes) attention_backward_bytes;
   decltype(&gdn2_attention_backward) attention_backward;
+  decltype(&gdn2_window_tree_attention) window_tree_attention;
   decltype(&gdn2_window_attention_forward) window_attention_forward;
   decltype(&gdn2_window_attention_backward_bytes) window_attention_backward_bytes;
   decltype(&gdn2_window_attention_backward) window_attention_backward;
@@ -739,12 +740,22 @@ PyObject* append_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_CATCH
 }
 
-// tree_attention(q, k, v, k_pages, v_pages, page_table, lengths, mask, scale) -> output or None
+// window and sinks, (0, 0) for none
+bool read_window(PyObject* const* a, int64_t* window, int64_t* sinks) {
+  int overflow[2] = {1, 1};
+  if (!PyLong_CheckExact(a[0]) || !PyLong_CheckExact(a[1])) return false;
+  *window = PyLong_AsLongLongAndOverflow(a[0], &overflow[0]);
+  *sinks = PyLong_AsLongLongAndOverflow(a[1], &overflow[1]);
+  return overflow[0] == 0 && overflow[1] == 0 && *sinks >= 0 && (*window > 0 || (*window == 0 && *sinks == 0));
+}
+
+// tree_attention(q, k, v, k_pages, v_pages, page_table, lengths, mask, depths, window, sinks, scale) -> output or None
 PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_TRY
   Heads h;
   float scale;
-  if (!g_bound || n != 9 || !read_heads(a, &h) || !read_attention_scale(a[8], h.dim, &scale) ||
+  int64_t window, sinks;
+  if (!g_bound || n != 12 || !read_heads(a, &h) || !read_attention_scale(a[11], h.dim, &scale) || !read_window(a + 9, &window, &sinks) ||
       wants_grad({h.t[0], h.t[1], h.t[2]})) {
     return none();
   }
@@ -762,6 +773,14 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return none();
     }
   }
+  const at::Tensor* depths = nullptr;
+  if (a[8] != Py_None) {
+    const at::Tensor* t = tensor(a[8]);
+    depths = t == nullptr ? nullptr : dense(a[8], t->dim() == 1 ? 1 : 2, at::kInt, q);
+    if (depths == nullptr || window == 0 || depths->size(-1) != h.time || (depths->dim() == 2 && depths->size(0) != h.batch)) return none();
+  } else if (window > 0 && mask != nullptr) {
+    return none();
+  }
   at::Tensor out;
   int status;
   WithoutGil others;
@@ -773,26 +792,28 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   out = at::empty(q.sizes(), q.options());
   const at::Tensor workspace = bytes(size, q);
-  status = api.tree_attention(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), pages[0]->data_ptr(), pages[1]->data_ptr(),
-                              static_cast<const int*>(table->data_ptr()), static_cast<const int*>(lengths->data_ptr()),
-                              mask == nullptr ? nullptr : mask->data_ptr(), out.data_ptr(), workspace.data_ptr(), h.strides,
-                              h.batch > 1 ? table->stride(0) : table->size(1),
-                              mask == nullptr || mask->dim() == 2 ? 0 : h.time * h.time, h.batch, h.time, h.heads, h.kv_heads, h.dim,
-                              pages[0]->size(0), pages[0]->size(1), table->size(1), h.dtype, scale,
-                              at::cuda::getCurrentCUDAStream().stream());
+  const int* table_at = static_cast<const int*>(table->data_ptr());
+  const int* lengths_at = static_cast<const int*>(lengths->data_ptr());
+  const void* mask_at = mask == nullptr ? nullptr : mask->data_ptr();
+  const int64_t table_stride = h.batch > 1 ? table->stride(0) : table->size(1);
+  const int64_t mask_stride = mask == nullptr || mask->dim() == 2 ? 0 : h.time * h.time;
+  void* stream = at::cuda::getCurrentCUDAStream().stream();
+  if (window == 0) {
+    status = api.tree_attention(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), pages[0]->data_ptr(), pages[1]->data_ptr(), table_at,
+                                lengths_at, mask_at, out.data_ptr(), workspace.data_ptr(), h.strides, table_stride, mask_stride, h.batch,
+                                h.time, h.heads, h.kv_heads, h.dim, pages[0]->size(0), pages[0]->size(1), table->size(1), h.dtype, scale,
+                                stream);
+  } else {
+    status = api.window_tree_attention(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), pages[0]->data_ptr(), pages[1]->data_ptr(),
+                                       table_at, lengths_at, mask_at, depths == nullptr ? nullptr : static_cast<const int*>(depths->data_ptr()),
+                                       out.data_ptr(), workspace.data_ptr(), h.strides, table_stride, mask_stride,
+                                       depths == nullptr || depths->dim() == 1 ? 0 : h.time, h.batch, h.time, h.heads, h.kv_heads, h.dim,
+                                       pages[0]->size(0), pages[0]->size(1), table->size(1), window, sinks, h.dtype, scale, stream);
+  }
   others.end();
-  if (!ok(status, "gdn2_tree_attention", 2)) return nullptr;
+  if (!ok(status, window == 0 ? "gdn2_tree_attention" : "gdn2_window_tree_attention", 2)) return nullptr;
   return wrap(out);
   GDN2_CATCH
-}
-
-// window and sinks, (0, 0) for none
-bool read_window(PyObject* const* a, int64_t* window, int64_t* sinks) {
-  int overflow[2] = {1, 1};
-  if (!PyLong_CheckExact(a[0]) || !PyLong_CheckExact(a[1])) return false;
-  *window = PyLong_AsLongLongAndOverflow(a[0], &overflow[0]);
-  *sinks = PyLong_AsLongLongAndOverflow(a[1], &overflow[1]);
-  return overflow[0] == 0 && overflow[1] == 0 && *sinks >= 0 && (*window > 0 || (*window == 0 && *sinks == 0));
 }
 
 // attention_forward(q, k, v, bounds, scale, window, sinks, training) -> (output, statistics or None) or None
@@ -925,6 +946,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_BIND(attention_forward);
   GDN2_BIND(attention_backward_bytes);
   GDN2_BIND(attention_backward);
+  GDN2_BIND(window_tree_attention);
   GDN2_BIND(window_attention_forward);
   GDN2_BIND(window_attention_backward_bytes);
   GDN2_BIND(window_attention_backward);

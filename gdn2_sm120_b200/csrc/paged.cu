@@ -88,6 +88,11 @@ struct TreeParams {
   uint32_t negate;                           // the scale is negative: Q counts with its sign changed
   uint32_t polls;                            // of a wait
   bool wide;                                 // rows of the output are 32-byte aligned
+  // With a window a drafted token's place is its sequence's length and its depth; it sees the last `window` places, its own
+  // among them, and the first `sinks`.
+  int window, sinks;
+  const int* depths;                         // [batch or 1][drafted], or null: i
+  int64_t depth_stride;
 };
 
 // A sequence's cached tokens and then its drafted ones, in tiles; kRows rows of one key head
@@ -95,28 +100,72 @@ struct Unit {
   int b, head, block;
   int length, tiles;
   bool bad;             // the sequence's length is none that its page table can hold
+  // with a window: tiles of sinks, how many tiles behind them nobody sees, the first token that a token of depth 0 sees
+  int sink_tiles, skipped, from;
 };
 
+template <bool kWindow>
 __device__ __forceinline__ void read_length(const TreeParams& p, Unit& u) {
   const int n = u.b < p.batch ? p.lengths[u.b] : 0;
   u.bad = n < 0 || n > p.columns * p.page;
   u.length = u.bad ? 0 : n;
   u.tiles = (u.length + p.drafted + kTile - 1) / kTile;
+  if (kWindow) {
+    u.from = max(0, u.length - p.window + 1);
+    u.sink_tiles = min((p.sinks - 1) / kTile + (p.sinks > 0), u.from / kTile);
+    u.skipped = u.from / kTile - u.sink_tiles;
+    u.tiles -= u.skipped;
+  }
 }
 
+// where a unit's tile begins in its sequence
+template <bool kWindow>
+__device__ __forceinline__ int tile_token(const Unit& u, int tile) {
+  return kTile * (!kWindow || tile < u.sink_tiles ? tile : tile + u.skipped);
+}
+
+// with a window: the drafted token's depth, and the first token that it sees but for the sinks
+__device__ __forceinline__ int depth_of(const TreeParams& p, int b, int i) {
+  return p.depths == nullptr ? i : min(max(p.depths[b * p.depth_stride + i], 0), (1 << 30) - 1);
+}
+__device__ __forceinline__ int seen_from(const TreeParams& p, const Unit& u, int depth) { return u.length + depth - p.window + 1; }
+// ... whether it sees drafted token d, which its mask names
+__device__ __forceinline__ bool reaches(const TreeParams& p, const Unit& u, int depth, int d) {
+  const int at = depth_of(p, u.b, d);
+  return depth - at < p.window || u.length + at < p.sinks;
+}
+// Whether drafted token `token` sees the cached or drafted token t of its sequence; d = t - length, the drafted one's number
+template <bool kWindow>
+__device__ __forceinline__ bool sees_token(const TreeParams& p, const Unit& u, const uint8_t* mask, int token, int depth, int d) {
+  if (d < 0) return !kWindow || u.length + d >= seen_from(p, u, depth) || u.length + d < p.sinks;
+  if (d >= p.drafted || token < 0) return false;
+  return (mask == nullptr ? d <= token : mask[d] != 0) && (!kWindow || reaches(p, u, depth, d));
+}
+// ... the first token from `from` on that all drafted ones of a warp's sequence see: tokens before it are not seen by the deepest
+__device__ __forceinline__ int seen_by_all(const TreeParams& p, const Unit& u) {
+  int most = p.depths == nullptr ? p.drafted - 1 : 0;
+  if (p.depths != nullptr) {
+    for (int i = threadIdx.x & 31; i < p.drafted; i += 32) most = max(most, depth_of(p, u.b, i));
+    most = int(__reduce_max_sync(0xffffffffu, unsigned(most)));
+  }
+  return max(0, seen_from(p, u, most));
+}
+
+template <bool kWindow>
 __device__ __forceinline__ void next_unit(const TreeParams& p, Unit& u) {
   if (++u.block < p.row_blocks) return;
   u.block = 0;
   if (++u.head < p.kv_heads) return;
   u.head = 0;
   ++u.b;
-  read_length(p, u);
+  read_length<kWindow>(p, u);
 }
 
 // tiles of sequence b, for all its key heads and blocks of rows
+template <bool kWindow>
 __device__ __forceinline__ int64_t tiles_of(const TreeParams& p, int b) {
-  Unit u{b, 0, 0, 0, 0, false};
-  read_length(p, u);
+  Unit u{b, 0, 0, 0, 0, false, 0, 0, 0};
+  read_length<kWindow>(p, u);
   return int64_t(u.tiles) * p.kv_heads * p.row_blocks;
 }
 
@@ -149,12 +198,12 @@ __device__ __forceinline__ int64_t cta_scan(int64_t x, int64_t* before, int64_t*
 // This CTA's part of all tiles: its first unit and tile, and how many tiles; false if there are fewer tiles than CTAs.
 template <int kWarps>
 struct Share { int64_t scan[kWarps], found[2]; };
-template <int kWarps>
+template <bool kWindow, int kWarps>
 __device__ __forceinline__ bool part_of_cta(const TreeParams& p, Share<kWarps>& shared, Unit& u, int& tile, int& rest) {
   const int tid = threadIdx.x;
   int64_t total = 0, before, own = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32 * kWarps) {
-    own = b0 + tid < p.batch ? tiles_of(p, b0 + tid) : 0;
+    own = b0 + tid < p.batch ? tiles_of<kWindow>(p, b0 + tid) : 0;
     total += cta_scan<kWarps>(own, &before, shared.scan);
   }
   const int64_t ctas = sharing(p, total);
@@ -164,7 +213,7 @@ __device__ __forceinline__ bool part_of_cta(const TreeParams& p, Share<kWarps>& 
   for (int b0 = 0; b0 < p.batch; b0 += 32 * kWarps) {
     int64_t sum = total;
     if (p.batch > 32 * kWarps) {   // otherwise all of them have just been looked at
-      own = b0 + tid < p.batch ? tiles_of(p, b0 + tid) : 0;
+      own = b0 + tid < p.batch ? tiles_of<kWindow>(p, b0 + tid) : 0;
       sum = cta_scan<kWarps>(own, &before, shared.scan);
     }
     const int64_t from = base + before;
@@ -176,8 +225,8 @@ __device__ __forceinline__ bool part_of_cta(const TreeParams& p, Share<kWarps>& 
     if (begin < base) break;
   }
   __syncthreads();
-  u = Unit{int(shared.found[0]), 0, 0, 0, 0, false};
-  read_length(p, u);
+  u = Unit{int(shared.found[0]), 0, 0, 0, 0, false, 0, 0, 0};
+  read_length<kWindow>(p, u);
   const int64_t unit = shared.found[1] / u.tiles;
   tile = int(shared.found[1] - unit * u.tiles);
   u.head = int(unit / p.row_blocks);
@@ -243,9 +292,10 @@ __device__ __forceinline__ void tma_load_page(uint32_t to, const CUtensorMap* ma
 // The keys and values of all tiles of a CTA, brought in by kWarps warps that share the rows of every tile, in the order K0,
 // K1 V0, K2 V1, ... of a unit, into kStages places by turns.  full[] counts all their threads, empty[] says that a place has
 // been used.  *strange says that a drafted token had a value that is not finite, strange_rows (may be null) which: a bit for
-// every token modulo kStrangeRows.
+// every token modulo kStrangeRows.  With a window the cached tokens that some of the drafted ones see and some do not are
+// looked at like these (numbered back from the first drafted one), and those that none of them sees are not read.
 constexpr int kStrangeRows = 2048;
-template <typename T, int DP, int kStages, int kWarps>
+template <typename T, int DP, bool kWindow, int kStages, int kWarps>
 __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int tile, int rest, int warp, uint32_t kv_base, uint64_t* full,
                                             uint64_t* empty, const attn::Waiter& waiter, int* strange, uint32_t* strange_rows) {
   constexpr int kTileBytes = kTile * DP * 2;
@@ -255,12 +305,13 @@ __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int til
   const uint32_t leader = tc::elect_leader();
   int filled = 0;
   bool ok = true;
+  int all_from = kWindow ? seen_by_all(p, u) : 0;
   struct Pages { int of[kParts]; };    // of rows mine + lane, mine + 32 + lane, ... of a tile
   auto pages_of = [&](const Unit& x, int tile) {
     Pages r;
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
-      const int t = tile * kTile + mine + i * 32 + lane;
+      const int t = tile_token<kWindow>(x, tile) + mine + i * 32 + lane;
       r.of[i] = t < x.length ? p.table[x.b * p.table_stride + t / p.page] : 0;
     }
     return r;
@@ -271,8 +322,11 @@ __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int til
     if (!ok) return;
     ++filled;
     const uint32_t base = kv_base + s * kTileBytes;
-    const int t0 = tile * kTile + mine;
-    bool good = true;
+    const int t0 = tile_token<kWindow>(u, tile) + mine;
+    // whether some of these tokens are not seen by all drafted ones, whether some of those are seen by some
+    const bool edge = kWindow && t0 < all_from && t0 + kMine > p.sinks;
+    const bool sifted = edge && max(t0, max(u.from, p.sinks)) < min(t0 + kMine, all_from);
+    bool good = !edge;
 #pragma unroll
     for (int i = 0; i < kParts; ++i) good = good && pages.of[i] >= 0 && pages.of[i] < p.pages;
     if (p.box > 0 && t0 + kMine <= u.length && __all_sync(0xffffffffu, good)) {
@@ -296,7 +350,9 @@ __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int til
     for (int i = 0; i < kParts; ++i) {
       const int t = t0 + i * 32 + lane, j = t - u.length;
       const uint8_t* at = nullptr;
-      if (j < 0) {
+      if (edge && t < u.from && t >= p.sinks) {
+        // zeros
+      } else if (j < 0) {
         const int64_t row = (int64_t(pages.of[i]) * p.page + t % p.page) * p.kv_heads + u.head;
         if (pages.of[i] >= 0 && pages.of[i] < p.pages) at = static_cast<const uint8_t*>(keys ? p.k_pages : p.v_pages) + row * p.dim * 2;
         else if (keys) at = reinterpret_cast<const uint8_t*>(g_nan_row);
@@ -306,13 +362,13 @@ __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int til
       }
       copy_rows<DP>(base, kSlab, mine + i * 32, p.dim, at);
     }
-    if (!keys && t0 + kMine > u.length) {
+    if (!keys && (sifted || t0 + kMine > u.length)) {
       cp_async_wait_all();
       // a drafted token's values that are not finite are added to the rows that see them
-      attn::sift<T, DP>(base, kSlab, mine + max(0, u.length - t0), mine + kMine, [&](int row) {
+      attn::sift<T, DP>(base, kSlab, mine + (sifted ? 0 : max(0, u.length - t0)), mine + kMine, [&](int row) {
         *static_cast<volatile int*>(strange) = 1;
-        const int d = tile * kTile + row - u.length;
-        if (strange_rows != nullptr) atomicOr(&strange_rows[d % kStrangeRows >> 5], 1u << (d & 31));
+        const int d = t0 - mine + row - u.length;
+        if (strange_rows != nullptr) atomicOr(&strange_rows[(d & (kStrangeRows - 1)) >> 5], 1u << (d & 31));
       });
       tc::mbar_arrive(&full[s]);
     } else {
@@ -323,7 +379,7 @@ __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int til
   while (rest > 0 && ok) {
     const int n = min(rest, u.tiles - tile);
     Unit next = u;
-    if (rest > n) next_unit(p, next);
+    if (rest > n) next_unit<kWindow>(p, next);
     Pages before = pages;
     for (int x = 0; x <= n && ok; ++x) {
       const Pages now = pages;
@@ -336,6 +392,7 @@ __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int til
     }
     rest -= n;
     tile = 0;
+    if (kWindow && next.b != u.b && rest > 0) all_from = seen_by_all(p, next);
     u = next;
   }
   cp_async_wait_all();
@@ -345,6 +402,22 @@ __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int til
       for (int i = 0; i < 4096 && !tc::mbar_try_wait(&full[x % kStages], (x / kStages) & 1); ++i) {}
     }
   }
+}
+
+// With a window: where the values of token d (counted from the first drafted one) are, if drafted token `token` sees it, if it
+// is one that not all see (only those were taken out of their tiles) and in the tiles tile .. tile + n - 1; null otherwise
+template <typename T>
+__device__ __noinline__ const T* strange_value(const TreeParams& p, const Unit& u, const uint8_t* mask, int token, int depth, int d, int tile,
+                                               int n) {
+  const int t = u.length + d, t0 = t / kTile * kTile;
+  // its tile is one of the unit's, and this CTA's
+  const int of_unit = t0 / kTile < u.sink_tiles ? t0 / kTile : t0 / kTile - u.skipped;
+  if (of_unit < tile || of_unit >= tile + n || tile_token<true>(u, of_unit) != t0) return nullptr;
+  if (!sees_token<true>(p, u, mask, token, depth, d)) return nullptr;
+  if (d >= 0) return static_cast<const T*>(p.v) + u.b * p.v_stride[0] + d * p.v_stride[1] + u.head * p.v_stride[2];
+  const int page = p.table[u.b * p.table_stride + t / p.page];
+  if (page < 0 || page >= p.pages) return nullptr;
+  return static_cast<const T*>(p.v_pages) + ((int64_t(page) * p.page + t % p.page) * p.kv_heads + u.head) * p.dim;
 }
 
 template <int DP, int RT>   // RT: tiles of 128 rows that a CTA has, 1 or 2
@@ -369,7 +442,7 @@ struct TreeBars {
 };
 static_assert(sizeof(TreeBars) <= 768, "");
 
-template <typename T, int DP, int RT>
+template <typename T, int DP, int RT, bool kWindow>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ TreeParams p) {
   using C = TreeConfig<DP, RT>;
   extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
@@ -405,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   }
   Unit u;
   int tile, rest;   // the first of this CTA's tiles of the unit; how many there are left of all its tiles
-  const bool idle = !part_of_cta<kThreads / 32>(p, bar.share, u, tile, rest);
+  const bool idle = !part_of_cta<kWindow, kThreads / 32>(p, bar.share, u, tile, rest);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -502,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         if (++queries == C::kQueries) queries = 0;
         rest -= n;
         tile = 0;
-        if (rest > 0) next_unit(p, u);
+        if (rest > 0) next_unit<kWindow>(p, u);
       }
       if (!ok) {  // products under way end before the CTA does
         tc::mma_commit(&bar.drained, leader);
@@ -525,12 +598,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         cp_async_arrive(&bar.q_full[place]);
         rest -= n;
         tile = 0;
-        if (rest > 0) next_unit(p, u);
+        if (rest > 0) next_unit<kWindow>(p, u);
       }
       cp_async_wait_all();
     } else if (warp < 12) {
-      bring_tiles<T, DP, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange,
-                                              bar.strange_rows);
+      bring_tiles<T, DP, kWindow, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange,
+                                                 bar.strange_rows);
     }
   } else {
     // ---- weights: a row a thread ---------------------------------------------------------------------------
@@ -546,6 +619,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       const int token = r / p.group;
       const bool there = r < p.rows, any_there = r - lane < p.rows;
       const bool takes_part = RT == 1 || t < chains;
+      const int depth = kWindow && there ? depth_of(p, u.b, token) : 0;
+      // a tile of tokens of which no warp's row misses any: behind the window's beginning and before the drafted ones
+      const int all_from = kWindow ? max(0, seen_from(p, u, int(__reduce_max_sync(0xffffffffu, unsigned(depth))))) : 0;
       float m = -INFINITY;
       float sum = 0.f;
       int mine = 0;
@@ -554,9 +630,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         ++seen;
         tc::tc_fence_after();
         if (any_there) {   // warps without a row have nothing to do but to keep count
-          const int first_token = (tile + j) * kTile;
+          const int first_token = tile_token<kWindow>(u, tile + j);
           attn::soften<T, DP>(s_at, o_at, p.scale_log2, m, sum, [&](int x, uint32_t (&s)[32]) {
-            if (first_token + x * 32 + 32 <= u.length) return;
+            if (first_token + x * 32 + 32 <= u.length) {
+              if (!kWindow || first_token + x * 32 >= all_from || first_token + x * 32 + 32 <= p.sinks) return;
+              // (rows that are not there have a depth of 0; nothing but their zeros comes of them)
+              const attn::Span span{p.window, p.sinks};
+              span.hide(u.length + depth, first_token + x * 32, s);
+              return;
+            }
             // drafted tokens, or the end
             const uint8_t* mask = p.mask == nullptr || !there ? nullptr : p.mask + u.b * p.mask_stride + int64_t(token) * p.drafted;
             uint32_t sees = 0;
@@ -564,7 +646,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             for (int y = 0; y < 32; ++y) {
               const int d = first_token + x * 32 + y - u.length;
               bool see = d < 0;
-              if (!see && d < p.drafted && there) see = p.mask == nullptr ? d <= token : mask[d] != 0;
+              if (kWindow) see = sees_token<true>(p, u, mask, there ? token : -1, depth, d);
+              else if (!see && d < p.drafted && there) see = p.mask == nullptr ? d <= token : mask[d] != 0;
               sees |= uint32_t(see) << y;
             }
 #pragma unroll
@@ -631,16 +714,25 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           }
           if (!there) continue;
           if (strange) {
-            // of the drafted tokens in this CTA's tiles of the unit those that had such a value in some unit
-            const int first = max(0, tile * kTile - u.length);
-            const int last = min(p.mask == nullptr ? token + 1 : p.drafted, (tile + n) * kTile - u.length);
+            // of the drafted tokens in this CTA's tiles of the unit those that had such a value in some unit; with a window
+            // the cached ones, too, that not all of the drafted ones see
+            const int first = kWindow ? max(u.from - 31, 0) - u.length : max(0, tile_token<kWindow>(u, tile) - u.length);
+            const int last = min(p.mask == nullptr ? token + 1 : p.drafted, tile_token<kWindow>(u, tile + n - 1) + kTile - u.length);
+            const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + u.b * p.mask_stride + int64_t(token) * p.drafted;
             bool done = false;          // all channels are NaN
             for (int d0 = first & ~31; d0 < last && !done; d0 += 32) {
-              for (uint32_t bits = bar.strange_rows[d0 % kStrangeRows >> 5]; bits != 0 && !done; bits &= bits - 1) {
+              for (uint32_t bits = bar.strange_rows[(d0 & (kStrangeRows - 1)) >> 5]; bits != 0 && !done; bits &= bits - 1) {
                 const int d = d0 + __ffs(bits) - 1;
                 if (d < first || d >= last) continue;
-                if (p.mask != nullptr && p.mask[u.b * p.mask_stride + int64_t(token) * p.drafted + d] == 0) continue;
-                const T* v = static_cast<const T*>(p.v) + u.b * p.v_stride[0] + d * p.v_stride[1] + u.head * p.v_stride[2] + x;
+                const T* v = nullptr;
+                if (kWindow) {
+                  v = strange_value<T>(p, u, mask, token, depth, d, tile, n);
+                  if (v == nullptr) continue;
+                  v += x;
+                } else {
+                  if (mask != nullptr && mask[d] == 0) continue;
+                  v = static_cast<const T*>(p.v) + u.b * p.v_stride[0] + d * p.v_stride[1] + u.head * p.v_stride[2] + x;
+                }
 #pragma unroll
                 for (int y = 0; y < 16; y += 8) {
                   if (x + y >= p.dim) continue;
@@ -676,7 +768,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       rest -= n;
       tile = 0;
       split = false;
-      if (rest > 0) next_unit(p, u);
+      if (rest > 0) next_unit<kWindow>(p, u);
     }
   }
   tc::tc_fence_before();
@@ -734,7 +826,7 @@ struct FewBars {
 };
 static_assert(sizeof(FewBars) <= 2048, "");
 
-template <typename T, int DP>
+template <typename T, int DP, bool kWindow>
 __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_constant__ TreeParams p) {
   using C = FewConfig<DP>;
   constexpr int kKSteps = DP / 16, kDB = DP / 8;
@@ -755,16 +847,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
   }
   Unit u;
   int tile, rest;
-  if (!part_of_cta<kFewThreads / 32>(p, bar.share, u, tile, rest)) return;
+  if (!part_of_cta<kWindow, kFewThreads / 32>(p, bar.share, u, tile, rest)) return;
   const attn::Waiter waiter{&bar.failed, p.polls};
   if (warp >= 8) {
-    bring_tiles<T, DP, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange, nullptr);
+    bring_tiles<T, DP, kWindow, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange, nullptr);
     return;
   }
 
   uint32_t qf[kKSteps][4];
   const uint32_t sign = p.negate ? 0x80008000u : 0u;   // the scale's goes to the queries
   int token_of[2];
+  int depth[2] = {0, 0}, all_from = 0;   // with a window: depths of the two tokens, the first token that all rows see
   auto queries = [&](const Unit& x) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -772,6 +865,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       const bool there = r < p.rows;
       const int n = there ? r / p.group : 0, g = there ? r - n * p.group : 0;
       token_of[half] = there ? n : -1;
+      if (kWindow) depth[half] = there ? depth_of(p, x.b, n) : 0;
       const T* row = static_cast<const T*>(p.q) + x.b * p.q_stride[0] + n * p.q_stride[1] + int64_t(x.head * p.group + g) * p.q_stride[2];
 #pragma unroll
       for (int s = 0; s < kKSteps; ++s) {
@@ -782,6 +876,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
         }
       }
     }
+    if (kWindow) all_from = max(0, seen_from(p, x, int(__reduce_max_sync(0xffffffffu, unsigned(max(depth[0], depth[1]))))));
   };
   queries(u);
   const float c = p.scale_log2;
@@ -811,16 +906,20 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       }
       __syncwarp();
       tc::mbar_arrive(&bar.kv_empty[xk % C::kStages], lane == 0);
-      const int first_token = (tile + j) * kTile + warp * 16;
+      const int first_token = tile_token<kWindow>(u, tile + j) + warp * 16;
       float s[2][4];
 #pragma unroll
       for (int x = 0; x < 8; ++x) s[x >> 2][x & 3] = s2[0][x >> 2][x & 3] + s2[1][x >> 2][x & 3];
-      if (first_token + 16 > u.length) {   // drafted tokens, or the end
+      // drafted tokens, or the end; tokens that not all rows see
+      if (first_token + 16 > u.length || (kWindow && first_token < all_from && first_token + 16 > p.sinks)) {
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           const int d = first_token + (x >> 2) * 8 + in_quad * 2 + (x & 1) - u.length, token = token_of[(x >> 1) & 1];
           bool see = d < 0;
-          if (!see && d < p.drafted && token >= 0) {
+          if (kWindow) {
+            const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + u.b * p.mask_stride + int64_t(max(token, 0)) * p.drafted;
+            see = sees_token<true>(p, u, mask, token, depth[(x >> 1) & 1], d);
+          } else if (!see && d < p.drafted && token >= 0) {
             see = p.mask == nullptr ? d <= token : p.mask[u.b * p.mask_stride + int64_t(token) * p.drafted + d] != 0;
           }
           if (!see) s[x >> 2][x & 3] = -INFINITY;
@@ -863,7 +962,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
     used += 2 * n;
     Unit next = u;
     if (rest > n) {
-      next_unit(p, next);
+      next_unit<kWindow>(p, next);
       queries(next);   // on their way while the warps join
     }
 
@@ -921,9 +1020,18 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
         const float inv = !ok || u.bad ? NAN : !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
         const int i = r / p.group, g = r - i * p.group;
         if (strange) {
-          for (int d = max(0, tile * kTile - u.length); d < min(p.drafted, (tile + n) * kTile - u.length); ++d) {
-            if (!(p.mask == nullptr ? d <= i : p.mask[u.b * p.mask_stride + int64_t(i) * p.drafted + d] != 0)) continue;
-            const T* v = static_cast<const T*>(p.v) + u.b * p.v_stride[0] + d * p.v_stride[1] + u.head * p.v_stride[2];
+          const int first = kWindow ? max(u.from - 31, 0) - u.length : max(0, tile * kTile - u.length);
+          const int last = min(p.drafted, tile_token<kWindow>(u, tile + n - 1) + kTile - u.length);
+          for (int d = first; d < last; ++d) {
+            const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + u.b * p.mask_stride + int64_t(i) * p.drafted;
+            const T* v;
+            if (kWindow) {
+              v = strange_value<T>(p, u, mask, i, depth_of(p, u.b, i), d, tile, n);
+              if (v == nullptr) continue;
+            } else {
+              if (!(mask == nullptr ? d <= i : mask[d] != 0)) continue;
+              v = static_cast<const T*>(p.v) + u.b * p.v_stride[0] + d * p.v_stride[1] + u.head * p.v_stride[2];
+            }
 #pragma unroll
             for (int x = 0; x < 2 * kDB; ++x) {
               const int col = (x >> 1) * 8 + in_quad * 2 + (x & 1);
@@ -955,7 +1063,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
 }
 
 // Joins what several CTAs have of a unit: a warp a row, in the order of the tiles.
-template <typename T, int DP>
+template <typename T, int DP, bool kWindow>
 __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ TreeParams p, int block_rows, int ctas_of_unit) {
   __shared__ int64_t scan[kJoinThreads / 32];
   const int unit = int(blockIdx.x) / ctas_of_unit;
@@ -963,12 +1071,12 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
   int64_t total = 0, from = 0, before;
   for (int b0 = 0; b0 < p.batch; b0 += kJoinThreads) {
     const int x = b0 + int(threadIdx.x);
-    const int64_t own = x < p.batch ? tiles_of(p, x) : 0;
+    const int64_t own = x < p.batch ? tiles_of<kWindow>(p, x) : 0;
     total += cta_scan<kJoinThreads / 32>(own, &before, scan);
     from += cta_scan<kJoinThreads / 32>(x < b ? own : 0, &before, scan);
   }
-  Unit u{b, 0, 0, 0, 0, false};
-  read_length(p, u);
+  Unit u{b, 0, 0, 0, 0, false, 0, 0, 0};
+  read_length<kWindow>(p, u);
   const int64_t t0 = from + (int64_t(head) * p.row_blocks + block) * u.tiles, t1 = t0 + u.tiles;
   const int64_t ctas = sharing(p, total), c0 = ((t0 + 1) * ctas - 1) / total, c1 = (t1 * ctas - 1) / total;
   // Until here only lengths were read, which stood before the other kernel began; the parts are there when it has ended
@@ -1025,39 +1133,39 @@ int block_rows(int64_t rows) { return rows <= kFewRows ? kFewRows : rows <= 128 
 // the CTAs of tree_join_kernel for a unit
 int joining_ctas(const TreeParams& p, int rows) { return (std::min(p.rows, rows) + kJoinThreads / 32 - 1) / (kJoinThreads / 32); }
 
-template <typename T, int DP>
+template <typename T, int DP, bool kWindow>
 int launch_join(const TreeParams& p, int rows, cudaStream_t stream) {
   const int per_unit = joining_ctas(p, rows);
-  return launch_beside(&tree_join_kernel<T, DP>, unsigned(p.batch * p.kv_heads * p.row_blocks * per_unit), kJoinThreads, 0, stream, p,
+  return launch_beside(&tree_join_kernel<T, DP, kWindow>, unsigned(p.batch * p.kv_heads * p.row_blocks * per_unit), kJoinThreads, 0, stream, p,
                        rows, per_unit);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool kWindow>
 int launch_few(const TreeParams& p, cudaStream_t stream) {
   constexpr int kBytes = FewConfig<DP>::kBytes;
-  const cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(&tree_few_kernel<T, DP>), kBytes);
+  const cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(&tree_few_kernel<T, DP, kWindow>), kBytes);
   if (err != cudaSuccess) { record_cuda_error(err); return GDN2_ERR_LAUNCH; }
-  tree_few_kernel<T, DP><<<unsigned(p.ctas), kFewThreads, kBytes, stream>>>(p);
+  tree_few_kernel<T, DP, kWindow><<<unsigned(p.ctas), kFewThreads, kBytes, stream>>>(p);
   const int status = check_launch();
-  return status != GDN2_OK ? status : launch_join<T, DP>(p, kFewRows, stream);
+  return status != GDN2_OK ? status : launch_join<T, DP, kWindow>(p, kFewRows, stream);
 }
 
-template <typename T, int DP, int RT>
+template <typename T, int DP, int RT, bool kWindow>
 int launch_tree_typed(const TreeParams& p, cudaStream_t stream) {
   using C = TreeConfig<DP, RT>;
-  const void* kernel = reinterpret_cast<const void*>(&tree_kernel<T, DP, RT>);
+  const void* kernel = reinterpret_cast<const void*>(&tree_kernel<T, DP, RT, kWindow>);
   const cudaError_t err = ensure_dynamic_smem(kernel, C::kBytes);
   if (err != cudaSuccess) { record_cuda_error(err); return GDN2_ERR_LAUNCH; }
-  tree_kernel<T, DP, RT><<<unsigned(p.ctas), kThreads, C::kBytes, stream>>>(p);
+  tree_kernel<T, DP, RT, kWindow><<<unsigned(p.ctas), kThreads, C::kBytes, stream>>>(p);
   const int status = check_launch();
-  return status != GDN2_OK ? status : launch_join<T, DP>(p, C::kRows, stream);
+  return status != GDN2_OK ? status : launch_join<T, DP, kWindow>(p, C::kRows, stream);
 }
 
-template <typename T>
+template <typename T, bool kWindow>
 int launch_tree_dim(const TreeParams& p, cudaStream_t stream) {
-  if (p.rows <= kFewRows) return p.dim <= 64 ? launch_few<T, 64>(p, stream) : launch_few<T, 128>(p, stream);
-  if (p.dim <= 64) return p.rows <= 128 ? launch_tree_typed<T, 64, 1>(p, stream) : launch_tree_typed<T, 64, 2>(p, stream);
-  return p.rows <= 128 ? launch_tree_typed<T, 128, 1>(p, stream) : launch_tree_typed<T, 128, 2>(p, stream);
+  if (p.rows <= kFewRows) return p.dim <= 64 ? launch_few<T, 64, kWindow>(p, stream) : launch_few<T, 128, kWindow>(p, stream);
+  if (p.dim <= 64) return p.rows <= 128 ? launch_tree_typed<T, 64, 1, kWindow>(p, stream) : launch_tree_typed<T, 64, 2, kWindow>(p, stream);
+  return p.rows <= 128 ? launch_tree_typed<T, 128, 1, kWindow>(p, stream) : launch_tree_typed<T, 128, 2, kWindow>(p, stream);
 }
 
 }  // namespace
@@ -1097,13 +1205,15 @@ int64_t tree_workspace_bytes(int64_t rows, int dim, int ctas) {
 int launch_tree(const void* q, const void* k, const void* v, const void* k_pages, const void* v_pages, const int* table,
                 const int* lengths, const uint8_t* mask, void* out, void* workspace, const int64_t* strides,
                 int64_t table_stride, int64_t mask_stride, int batch, int drafted, int heads, int kv_heads, int dim,
-                int64_t pages, int page, int columns, int dtype, float scale, cudaStream_t stream) {
+                int64_t pages, int page, int columns, const int* depths, int64_t depth_stride, int window, int sinks, int dtype, float scale,
+                cudaStream_t stream) {
   TreeParams p{};
   p.q = q; p.k = k; p.v = v; p.k_pages = k_pages; p.v_pages = v_pages; p.out = out;
   p.table = table; p.lengths = lengths; p.mask = mask;
   p.partials = static_cast<float*>(workspace);
   for (int i = 0; i < 3; ++i) { p.q_stride[i] = strides[i]; p.k_stride[i] = strides[3 + i]; p.v_stride[i] = strides[6 + i]; }
   p.table_stride = table_stride; p.mask_stride = mask_stride; p.pages = pages;
+  p.depths = depths; p.depth_stride = depth_stride; p.window = window; p.sinks = sinks;
   p.batch = batch; p.drafted = drafted; p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads;
   p.dim = dim; p.page = page; p.columns = columns;
   p.rows = drafted * p.group;
@@ -1127,7 +1237,8 @@ int launch_tree(const void* q, const void* k, const void* v, const void* k_pages
   p.polls = attn::wait_polls();
   p.wide = attn::wide_rows(out, dim);
   p.scale_log2 = attn::positive_scale(scale);
-  return dtype == GDN2_BF16 ? launch_tree_dim<__nv_bfloat16>(p, stream) : launch_tree_dim<__half>(p, stream);
+  if (window > 0) return dtype == GDN2_BF16 ? launch_tree_dim<__nv_bfloat16, true>(p, stream) : launch_tree_dim<__half, true>(p, stream);
+  return dtype == GDN2_BF16 ? launch_tree_dim<__nv_bfloat16, false>(p, stream) : launch_tree_dim<__half, false>(p, stream);
 }
 
 }  // namespace gdn2

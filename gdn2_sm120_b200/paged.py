@@ -115,10 +115,14 @@ def tree_attention(
     stay on the device: no call waits for it, and a captured graph may be replayed with other contents.  A page number
     outside the cache or a length beyond ``columns`` pages makes the sequence's output NaN.  Inference only."""
 
+    return _tree_attention("tree_attention", q, k, v, k_pages, v_pages, page_table, lengths, mask, None, (0, 0), scale)
+
+
+def _tree_attention(what, q, k, v, k_pages, v_pages, page_table, lengths, mask, depths, window, scale):
     if forward_ad._current_level >= 0:
-        _validate.refuse_tangents("tree_attention", q, k, v, k_pages, v_pages)
+        _validate.refuse_tangents(what, q, k, v, k_pages, v_pages)
     if _lib.KERNEL_EVENTS is None and getattr(q, "is_cuda", False):
-        done = _lib.host().tree_attention(q, k, v, k_pages, v_pages, page_table, lengths, mask, scale)
+        done = _lib.host().tree_attention(q, k, v, k_pages, v_pages, page_table, lengths, mask, depths, *window, scale)
         if done is not None:
             return done
     if not isinstance(q, torch.Tensor):
@@ -154,8 +158,17 @@ def tree_attention(
             raise ValueError("all inputs must be CUDA tensors on the same device")
         if mask.shape not in ((drafted, drafted), (batch, drafted, drafted)):
             raise ValueError("mask must have shape [B, N, N] or [N, N]")
+    if depths is not None:
+        if not isinstance(depths, torch.Tensor) or depths.dtype != torch.int32:
+            raise TypeError("depths must be a torch.int32 tensor or None")
+        if depths.device != q.device:
+            raise ValueError("all inputs must be CUDA tensors on the same device")
+        if depths.shape not in ((drafted,), (batch, drafted)):
+            raise ValueError("depths must have shape [B, N] or [N]")
+    elif mask is not None and window != (0, 0):
+        raise ValueError("a mask needs the depths of the drafted tokens")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        raise RuntimeError("tree_attention has no gradient: call it under torch.no_grad() or with detached inputs")
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or with detached inputs")
     _lib.require_b200(q.device)
     scale = _validate.float32_scale(scale, dim)
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
@@ -166,17 +179,21 @@ def tree_attention(
     lengths = lengths.contiguous()
     if mask is not None:
         mask = mask.contiguous()
+    more = ((), (), ())
+    if window != (0, 0):
+        depths = depths if depths is None else depths.contiguous()
+        more = ((_lib.ptr(depths),), (0 if depths is None or depths.ndim == 1 else drafted,), window)
     with torch.cuda.device(q.device):
         size = _lib.lib().gdn2_tree_workspace_bytes(drafted, heads, kv_heads, dim)
     if size < 0:
         _lib.check(int(size), "gdn2_tree_workspace_bytes")
     workspace = torch.empty(size, device=q.device, dtype=torch.uint8)
     strides = _lib.int64s(*(s for x in (q, k, v) for s in _validate.head_strides(x)))
-    _lib.call("gdn2_tree_attention", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pages.data_ptr(),
-              v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), _lib.ptr(mask), out.data_ptr(),
+    _lib.call(f"gdn2_{what}", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pages.data_ptr(),
+              v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), _lib.ptr(mask), *more[0], out.data_ptr(),
               workspace.data_ptr(), strides, page_table.stride(0) if batch > 1 else page_table.shape[1],
-              0 if mask is None or mask.ndim == 2 else drafted * drafted, batch, drafted, heads, kv_heads, dim,
-              k_pages.shape[0], k_pages.shape[1], page_table.shape[1], _lib.dtype_code(q.dtype), scale,
+              0 if mask is None or mask.ndim == 2 else drafted * drafted, *more[1], batch, drafted, heads, kv_heads, dim,
+              k_pages.shape[0], k_pages.shape[1], page_table.shape[1], *more[2], _lib.dtype_code(q.dtype), scale,
               _lib.stream_ptr(q.device), kernels=2)
     return out
 

@@ -5,8 +5,9 @@ ones as far as they are not behind it.
 
 ``window_attention``          a batch of equally long sequences
 ``window_attention_varlen``   sequences of any lengths packed along time
+``window_tree_attention``     drafted tokens, or single ones, over a paged cache, of which the window and the sinks are read
 
-Both are differentiable and run on the kernels of causal attention (csrc/attention_fwd.cu, csrc/attention_bwd.cu), which pass over
+The first two are differentiable and run on the kernels of causal attention (csrc/attention_fwd.cu, csrc/attention_bwd.cu), which pass over
 the tiles that no row of theirs sees; what is said in attention.py about types, heads, roundings and values that are not finite
 holds here, with tiles that the window's edge or the sinks' end crosses beside those on the diagonal.  A window that reaches over
 the longest sequence is causal attention, bit for bit.
@@ -19,6 +20,7 @@ import operator
 import torch
 
 from .attention import _attention, _packed_bounds
+from .paged import _tree_attention
 
 _MOST = 2 ** 30     # tokens are numbered with fewer
 
@@ -70,4 +72,30 @@ def window_attention_varlen(
     return _attention(q, k, v, _packed_bounds(q, cu_seqlens), scale, _window(window, sinks))
 
 
-__all__ = ["window_attention", "window_attention_varlen"]
+def window_tree_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    window: int,
+    mask: torch.Tensor | None = None,
+    depths: torch.Tensor | None = None,
+    *,
+    sinks: int = 0,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """``tree_attention`` in which a drafted token sees the ``window`` last places, its own among them, and the first ``sinks``.
+
+    A drafted token's place is ``lengths[b]`` plus its depth in the tree: ``depths`` (int32, ``[B, N]`` or ``[N]``, on the
+    device; negative ones count as 0), which a ``mask`` needs; a chain (``mask=None``) has depths of ``0 .. N - 1`` where none
+    are given.  Of the tokens that it would see without a window it sees those that lie less than ``window`` places before it,
+    or on one of the first ``sinks`` places.  Pages that hold nothing but cached tokens that no drafted one sees are not read, so
+    that they, and their entries in ``page_table``, may be anything.  Inference only."""
+
+    return _tree_attention("window_tree_attention", q, k, v, k_pages, v_pages, page_table, lengths, mask, depths, _window(window, sinks), scale)
+
+
+__all__ = ["window_attention", "window_attention_varlen", "window_tree_attention"]

@@ -525,6 +525,20 @@ int gdn2_window_attention_backward(const void* q, const void* k, const void* v, 
                                    int dtype, float scale, void* stream);
 
 /*
+ * gdn2_tree_attention with a window.  The place of cached token t is t, that of drafted token i of sequence b is
+ * lengths[b] + depths[b * depth_stride + i], or lengths[b] + i where depths is NULL (then mask has to be NULL too);
+ * depths below 0 count as 0.  A drafted token sees those of the tokens that it would see otherwise whose place is less than
+ * `window` before its own or among the first `sinks`.  Cached tokens that no drafted one sees, and their entries in the page
+ * table, may be anything.  The workspace is gdn2_tree_workspace_bytes.
+ */
+int gdn2_window_tree_attention(const void* q, const void* k, const void* v, const void* k_pages,
+                               const void* v_pages, const int* page_table, const int* lengths, const void* mask,
+                               const int* depths, void* out, void* workspace, const int64_t* strides,
+                               int64_t table_stride, int64_t mask_stride, int64_t depth_stride, int64_t batch,
+                               int64_t drafted, int64_t heads, int64_t kv_heads, int64_t dim, int64_t pages, int64_t page,
+                               int64_t columns, int64_t window, int64_t sinks, int dtype, float scale, void* stream);
+
+/*
  * Test aid: how often a wait inside the attention kernels of later calls polls (0: it looks once; negative: as usual).
  * A CTA in which a wait runs out ends by itself and leaves NaN in place of what it has not finished.  For the process.
  */
