@@ -77,6 +77,12 @@ _PROTOTYPES: dict[str, list] = {
     "gdn2_window_attention_backward_bytes": [_P] + [_I64] * 7,
     "gdn2_window_attention_backward": [_P] * 12 + [_I64] * 7 + [_INT, _F32, _P],
     "gdn2_window_tree_attention": [_P] * 12 + [_I64] * 13 + [_INT, _F32, _P],
+    "gdn2_attention_weights_bytes": [_P] + [_I64] * 4,
+    "gdn2_attention_weights": [_P] * 7 + [_I64] * 5 + [_INT, _F32, _P],
+    "gdn2_weighed_token_workspace_bytes": [_I64] * 7,
+    "gdn2_weighed_token_attention": [_P] * 12 + [_I64] * 9 + [_F32, _INT, _F32, _P],
+    "gdn2_evict_workspace_bytes": [_I64] * 3,
+    "gdn2_evict_tokens": [_P] * 8 + [_I64] * 12 + [_INT, _P],
     "gdn2_debug_wait_limit": [_I64],
     "gdn2_profile_enable": [_INT],
     "gdn2_profile_chunk_kernels": [_P] * 4,
@@ -85,7 +91,8 @@ _RESTYPES = {"gdn2_status_string": ctypes.c_char_p, "gdn2_last_cuda_error": ctyp
              "gdn2_chunk_workspace_bytes": ctypes.c_int64, "gdn2_chunk_scratch_bytes": ctypes.c_int64,
              "gdn2_tensor_maps_encoded": ctypes.c_int64, "gdn2_tree_workspace_bytes": ctypes.c_int64,
              "gdn2_attention_stat_rows": ctypes.c_int64, "gdn2_attention_backward_bytes": ctypes.c_int64,
-             "gdn2_window_attention_backward_bytes": ctypes.c_int64}
+             "gdn2_window_attention_backward_bytes": ctypes.c_int64, "gdn2_attention_weights_bytes": ctypes.c_int64,
+             "gdn2_weighed_token_workspace_bytes": ctypes.c_int64, "gdn2_evict_workspace_bytes": ctypes.c_int64}
 
 
 def library_path() -> pathlib.Path:
@@ -133,6 +140,7 @@ class _PythonWay:
 
     forward = train_forward = train_backward = prologue_forward = prologue_backward = staticmethod(lambda *_: None)
     rotary = append_tokens = tree_attention = attention_forward = attention_backward = staticmethod(lambda *_: None)
+    weighed_token_attention = evict_tokens = staticmethod(lambda *_: None)
 
 
 _host_module = None

@@ -17,6 +17,12 @@ int64_t tree_workspace_bytes(int64_t, int, int);
 int launch_tree(const void*, const void*, const void*, const void*, const void*, const int*, const int*, const uint8_t*,
                 void*, void*, const int64_t*, int64_t, int64_t, int, int, int, int, int, int64_t, int, int, const int*, int64_t, int,
                 int, int, float, cudaStream_t);
+int64_t weighed_workspace_bytes(int, int, int, int, int, int, int);
+int launch_weighed(const void*, const void*, const void*, const void*, const void*, float*, const int*, const int*, const int64_t*,
+                   void*, void*, const int64_t*, int64_t, int, int, int, int, int, int64_t, int, int, float, int, float, cudaStream_t);
+int64_t evict_workspace_bytes(int64_t, int64_t, int64_t);
+int launch_evict(void*, void*, float*, const int*, const int*, const int*, int*, void*, int64_t, int64_t, int, int64_t, int, int, int,
+                 int, int, int, int, int, cudaStream_t);
 namespace attn {
 static std::atomic<uint32_t> g_wait_polls{GDN2_ATTENTION_WAIT_POLLS};
 uint32_t wait_polls() { return g_wait_polls.load(std::memory_order_relaxed); }
@@ -27,6 +33,9 @@ int64_t attention_backward_bytes(const int64_t*, int64_t, int64_t, int, int, int
 int launch_attention_backward(const void*, const void*, const void*, const void*, const void*, const float*, void*, void*,
                               void*, void*, const int64_t*, const int64_t*, int64_t, int64_t, int, int, int, int, float,
                               int64_t, int64_t, cudaStream_t);
+int64_t attention_weights_bytes(const int64_t*, int64_t, int64_t, int, int);
+int launch_attention_weights(const void*, const void*, const float*, float*, void*, const int64_t*, const int64_t*, int64_t, int64_t,
+                             int, int, int, int, float, cudaStream_t);
 }  // namespace attn
 
 namespace {
@@ -92,6 +101,17 @@ int tree_attention(const void* q, const void* k, const void* v, const void* k_pa
                      strides, table_stride, mask_stride, int(batch), int(drafted), int(heads), int(kv_heads), int(dim),
                      pages, int(page), int(columns), depths, depth_stride, int(std::min(window, kMost / 2)),
                      int(std::min(sinks, kMost / 2)), dtype, scale, static_cast<cudaStream_t>(stream));
+}
+
+int check_weighed(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page, int64_t columns) {
+  const int status = check_heads(heads, kv_heads, dim);
+  if (status != GDN2_OK) return status;
+  if (batch <= 0 || tokens <= 0 || page <= 0 || columns <= 0) return GDN2_ERR_BAD_SHAPE;
+  // a sequence's tokens, cached and new, are numbered with 31 bits
+  if (batch > kMost / heads || tokens > GDN2_WEIGHED_MAX_ROWS / (heads / kv_heads) || page > kMost || columns > (kMost / 2 - 512) / page) {
+    return GDN2_ERR_TOO_LARGE;
+  }
+  return GDN2_OK;
 }
 
 // Causal attention, with a window of 0 for none
@@ -255,6 +275,91 @@ int gdn2_window_attention_backward(const void* q, const void* k, const void* v, 
   if (window <= 0 || sinks < 0) return GDN2_ERR_BAD_RANGE;
   return attention_backward(q, k, v, out, d_out, statistics, scratch, dq, dk, dv, strides, bounds, n_seq, time, heads, kv_heads, dim,
                             window, sinks, dtype, scale, stream);
+}
+
+int64_t gdn2_attention_weights_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads) {
+  int status = check_heads(heads, kv_heads, 8);
+  if (status == GDN2_OK) status = check_sequences(bounds, n_seq, time, heads);
+  return status != GDN2_OK ? status : attn::attention_weights_bytes(bounds, n_seq, time, int(heads), int(kv_heads));
+}
+
+int gdn2_attention_weights(const void* q, const void* k, const float* statistics, float* weights, void* scratch,
+                           const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads,
+                           int64_t kv_heads, int64_t dim, int dtype, float scale, void* stream) {
+  if (!q || !k || !statistics || !weights || !strides) return GDN2_ERR_NULL_POINTER;
+  int status = check_heads(heads, kv_heads, dim);
+  if (status != GDN2_OK) return status;
+  if (!valid_seq_dtype(dtype)) return GDN2_ERR_BAD_DTYPE;
+  if ((status = check_sequences(bounds, n_seq, time, heads)) != GDN2_OK) return status;
+  if ((status = check_strides(strides, 6)) != GDN2_OK) return status;
+  const void* need16[] = {q, k, statistics};
+  for (const void* p : need16) {
+    if (!aligned(p, 16)) return GDN2_ERR_ALIGNMENT;
+  }
+  if (!aligned(weights, 4) || !aligned(scratch, 4)) return GDN2_ERR_ALIGNMENT;
+  return attn::launch_attention_weights(q, k, statistics, weights, scratch, strides, bounds, n_seq, time, int(heads), int(kv_heads),
+                                        int(dim), dtype, scale, static_cast<cudaStream_t>(stream));
+}
+
+int64_t gdn2_weighed_token_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim,
+                                           int64_t page, int64_t columns) {
+  const int status = check_weighed(batch, tokens, heads, kv_heads, dim, page, columns);
+  return status != GDN2_OK ? status
+                           : weighed_workspace_bytes(int(batch), int(tokens), int(heads), int(kv_heads), int(dim), int(page), int(columns));
+}
+
+int gdn2_weighed_token_attention(const void* q, const void* k, const void* v, const void* k_pages, const void* v_pages,
+                                 float* weight_pages, const int* page_table, const int* lengths, const int64_t* slots, void* out,
+                                 void* workspace, const int64_t* strides, int64_t table_stride, int64_t batch, int64_t tokens,
+                                 int64_t heads, int64_t kv_heads, int64_t dim, int64_t pages, int64_t page, int64_t columns,
+                                 float decay, int dtype, float scale, void* stream) {
+  if (!q || !k || !v || !k_pages || !v_pages || !weight_pages || !page_table || !lengths || !slots || !out || !workspace || !strides) {
+    return GDN2_ERR_NULL_POINTER;
+  }
+  int status = check_weighed(batch, tokens, heads, kv_heads, dim, page, columns);
+  if (status != GDN2_OK) return status;
+  if (pages <= 0) return GDN2_ERR_BAD_SHAPE;
+  if (pages > kMost) return GDN2_ERR_TOO_LARGE;
+  if (!valid_seq_dtype(dtype)) return GDN2_ERR_BAD_DTYPE;
+  if ((status = check_strides(strides, 9)) != GDN2_OK) return status;
+  const void* need16[] = {q, k, v, k_pages, v_pages, out, workspace};
+  for (const void* p : need16) {
+    if (!aligned(p, 16)) return GDN2_ERR_ALIGNMENT;
+  }
+  if (!aligned(page_table, 4) || !aligned(lengths, 4) || !aligned(weight_pages, 4) || !aligned(slots, 8)) return GDN2_ERR_ALIGNMENT;
+  return launch_weighed(q, k, v, k_pages, v_pages, weight_pages, page_table, lengths, slots, out, workspace, strides, table_stride,
+                        int(batch), int(tokens), int(heads), int(kv_heads), int(dim), pages, int(page), int(columns), decay, dtype,
+                        scale, static_cast<cudaStream_t>(stream));
+}
+
+int64_t gdn2_evict_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t keep) {
+  if (batch <= 0 || kv_heads <= 0 || keep <= 0) return GDN2_ERR_BAD_SHAPE;
+  if (keep > kMost / 2 || batch > kMost / kv_heads) return GDN2_ERR_TOO_LARGE;
+  return evict_workspace_bytes(batch, kv_heads, keep);
+}
+
+int gdn2_evict_tokens(void* k_pages, void* v_pages, float* weight_pages, const int* page_table, const int* lengths,
+                      const int* new_table, int* new_lengths, void* workspace, int64_t table_stride, int64_t new_stride,
+                      int64_t batch, int64_t pages, int64_t page, int64_t kv_heads, int64_t dim, int64_t columns,
+                      int64_t new_columns, int64_t keep, int64_t sinks, int64_t recent, int dtype, void* stream) {
+  if (!k_pages || !v_pages || !weight_pages || !page_table || !lengths || !new_table || !new_lengths || !workspace) {
+    return GDN2_ERR_NULL_POINTER;
+  }
+  if (batch <= 0 || pages <= 0 || page <= 0 || kv_heads <= 0 || dim <= 0 || columns <= 0 || new_columns <= 0) return GDN2_ERR_BAD_SHAPE;
+  if (dtype != GDN2_BF16 && dtype != GDN2_FP16 && dtype != GDN2_FP32) return GDN2_ERR_BAD_DTYPE;
+  if (pages > kMost || page > kMost || kv_heads > 65535 || dim > 65535 || kv_heads * dim > kMost / 4 || batch > kMost / kv_heads ||
+      columns > kMost / 2 / page || new_columns > kMost / 2 / page) {
+    return GDN2_ERR_TOO_LARGE;
+  }
+  if (keep <= 0 || sinks < 0 || recent < 0 || sinks > keep || recent > keep - sinks || keep > new_columns * page) return GDN2_ERR_BAD_RANGE;
+  const uintptr_t es = uintptr_t(element_size(dtype));
+  if (!aligned(k_pages, es) || !aligned(v_pages, es) || !aligned(weight_pages, 4) || !aligned(page_table, 4) || !aligned(lengths, 4) ||
+      !aligned(new_table, 4) || !aligned(new_lengths, 4) || !aligned(workspace, 4)) {
+    return GDN2_ERR_ALIGNMENT;
+  }
+  return launch_evict(k_pages, v_pages, weight_pages, page_table, lengths, new_table, new_lengths, workspace, table_stride, new_stride,
+                      int(batch), pages, int(page), int(kv_heads), int(dim), int(columns), int(keep), int(sinks), int(recent), int(es),
+                      static_cast<cudaStream_t>(stream));
 }
 
 int gdn2_debug_wait_limit(int64_t polls) {

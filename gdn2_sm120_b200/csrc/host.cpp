@@ -47,6 +47,10 @@ struct Api {
   decltype(&gdn2_attention_forward) attention_forward;
   decltype(&gdn2_attention_backward_bytes) attention_backward_bytes;
   decltype(&gdn2_attention_backward) attention_backward;
+  decltype(&gdn2_weighed_token_workspace_bytes) weighed_token_workspace_bytes;
+  decltype(&gdn2_weighed_token_attention) weighed_token_attention;
+  decltype(&gdn2_evict_workspace_bytes) evict_workspace_bytes;
+  decltype(&gdn2_evict_tokens) evict_tokens;
   decltype(&gdn2_window_tree_attention) window_tree_attention;
   decltype(&gdn2_window_attention_forward) window_attention_forward;
   decltype(&gdn2_window_attention_backward_bytes) window_attention_backward_bytes;
@@ -816,6 +820,125 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_CATCH
 }
 
+// int32 [batch, columns] on q's device
+const at::Tensor* read_table(PyObject* o, int64_t batch, const at::Tensor& like) {
+  const at::Tensor* t = strided(o, 2);
+  return t != nullptr && t->scalar_type() == at::kInt && t->device() == like.device() && t->size(0) == batch && t->size(1) > 0 ? t : nullptr;
+}
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// the weights of a cache's tokens
+const at::Tensor* read_weights(PyObject* o, const at::Tensor& pages) {
+  const at::Tensor* t = dense(o, 3, at::kFloat, pages);
+  return t != nullptr && t->size(0) == pages.size(0) && t->size(1) == pages.size(2) && t->size(2) == pages.size(1) ? t : nullptr;
+}
+
+bool overlaps(const at::Tensor& x, std::initializer_list<const at::Tensor*> others) {
+  for (const at::Tensor* o : others) {
+    if (Extent(x).meets(Extent(*o))) return true;
+  }
+  return false;
+}
+
+// a backward that has saved them must not use them any more
+void bump(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* x : tensors) {
+    if (!x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+  }
+}
+
+// weighed_token_attention(q, k, v, k_pages, v_pages, weight_pages, page_table, lengths, slots, decay, scale) -> output or None
+PyObject* weighed_token_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  GDN2_TRY
+  Heads h;
+  float scale;
+  if (!g_bound || n != 11 || !read_heads(a, &h) || !PyFloat_Check(a[9]) || !read_attention_scale(a[10], h.dim, &scale)) return none();
+  const float decay = static_cast<float>(PyFloat_AS_DOUBLE(a[9]));
+  if (!(decay >= 0.f && decay <= 1.f) || h.time > GDN2_WEIGHED_MAX_ROWS / (h.heads / h.kv_heads)) return none();
+  const at::Tensor &q = *h.t[0], *pages[2];
+  if (!read_pages(a + 3, q, h.kv_heads, h.dim, pages) || !aligned(*pages[0]) || !aligned(*pages[1])) return none();
+  const at::Tensor *weights = read_weights(a[5], *pages[0]), *table = read_table(a[6], h.batch, q), *lengths = dense(a[7], 1, at::kInt, q),
+                   *slots = dense(a[8], 2, at::kLong, q);
+  if (weights == nullptr || table == nullptr || lengths == nullptr || lengths->size(0) != h.batch || slots == nullptr ||
+      slots->size(0) != h.batch || slots->size(1) != h.time || wants_grad({h.t[0], h.t[1], h.t[2], pages[0], pages[1], weights}) ||
+      overlaps(*weights, {h.t[0], h.t[1], h.t[2], pages[0], pages[1], table, lengths, slots})) {
+    return none();
+  }
+  at::Tensor out;
+  int status;
+  WithoutGil others;
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int64_t page = pages[0]->size(1), columns = table->size(1);
+  const int64_t size = api.weighed_token_workspace_bytes(h.batch, h.time, h.heads, h.kv_heads, h.dim, page, columns);
+  if (size <= 0 || size >= kCheckedBytes) {
+    others.end();
+    return none();
+  }
+  out = at::empty(q.sizes(), q.options());
+  const at::Tensor workspace = bytes(size, q);
+  status = api.weighed_token_attention(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), pages[0]->data_ptr(), pages[1]->data_ptr(),
+                                       static_cast<float*>(weights->data_ptr()), static_cast<const int*>(table->data_ptr()),
+                                       static_cast<const int*>(lengths->data_ptr()), static_cast<const int64_t*>(slots->data_ptr()),
+                                       out.data_ptr(), workspace.data_ptr(), h.strides, row_stride(*table), h.batch, h.time, h.heads,
+                                       h.kv_heads, h.dim, pages[0]->size(0), page, columns, decay, h.dtype, scale,
+                                       at::cuda::getCurrentCUDAStream().stream());
+  others.end();
+  if (!ok(status, "gdn2_weighed_token_attention", 2)) return nullptr;
+  bump({weights});
+  return wrap(out);
+  GDN2_CATCH
+}
+
+// evict_tokens(k_pages, v_pages, weight_pages, page_table, lengths, new_table, keep, sinks, recent) -> new lengths or None
+PyObject* evict_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  GDN2_TRY
+  if (!g_bound || n != 9) return none();
+  int64_t sizes[3];
+  for (int i = 0; i < 3; ++i) {
+    int overflow = 1;
+    if (!PyLong_CheckExact(a[6 + i])) return none();
+    sizes[i] = PyLong_AsLongLongAndOverflow(a[6 + i], &overflow);
+    if (overflow != 0) return none();
+  }
+  const at::Tensor *k = strided(a[0], 4), *pages[2], *lengths = k == nullptr ? nullptr : dense(a[4], 1, at::kInt, *k);
+  if (k == nullptr || dtype_code(k->scalar_type()) < 0 || lengths == nullptr || lengths->size(0) <= 0 ||
+      !read_pages(a, *k, k->size(2), k->size(3), pages) || !b200(k->device().index())) {
+    return none();
+  }
+  const int64_t batch = lengths->size(0), page = k->size(1);
+  const at::Tensor *weights = read_weights(a[2], *k), *table = read_table(a[3], batch, *k), *to = read_table(a[5], batch, *k);
+  if (weights == nullptr || table == nullptr || to == nullptr || sizes[0] <= 0 || to->size(1) < (sizes[0] - 1) / page + 1 ||
+      wants_grad({pages[0], pages[1], weights})) {
+    return none();
+  }
+  if (overlaps(*pages[0], {pages[1], weights, table, lengths, to}) || overlaps(*pages[1], {weights, table, lengths, to}) ||
+      overlaps(*weights, {table, lengths, to})) {
+    return none();
+  }
+  at::Tensor kept;
+  int status;
+  WithoutGil others;
+  const c10::cuda::CUDAGuard guard(k->device());
+  const int64_t size = api.evict_workspace_bytes(batch, k->size(2), sizes[0]);
+  if (size <= 0 || size >= kCheckedBytes) {
+    others.end();
+    return none();
+  }
+  kept = at::empty({batch}, lengths->options());
+  const at::Tensor workspace = bytes(size, *k);
+  status = api.evict_tokens(pages[0]->data_ptr(), pages[1]->data_ptr(), static_cast<float*>(weights->data_ptr()),
+                            static_cast<const int*>(table->data_ptr()), static_cast<const int*>(lengths->data_ptr()),
+                            static_cast<const int*>(to->data_ptr()), static_cast<int*>(kept.data_ptr()), workspace.data_ptr(),
+                            row_stride(*table), row_stride(*to), batch, k->size(0), page, k->size(2), k->size(3), table->size(1),
+                            to->size(1), sizes[0], sizes[1], sizes[2], dtype_code(k->scalar_type()),
+                            at::cuda::getCurrentCUDAStream().stream());
+  others.end();
+  if (!ok(status, "gdn2_evict_tokens", 2)) return nullptr;
+  bump({pages[0], pages[1], weights});
+  return wrap(kept);
+  GDN2_CATCH
+}
+
 // attention_forward(q, k, v, bounds, scale, window, sinks, training) -> (output, statistics or None) or None
 PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_TRY
@@ -946,6 +1069,10 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_BIND(attention_forward);
   GDN2_BIND(attention_backward_bytes);
   GDN2_BIND(attention_backward);
+  GDN2_BIND(weighed_token_workspace_bytes);
+  GDN2_BIND(weighed_token_attention);
+  GDN2_BIND(evict_workspace_bytes);
+  GDN2_BIND(evict_tokens);
   GDN2_BIND(window_tree_attention);
   GDN2_BIND(window_attention_forward);
   GDN2_BIND(window_attention_backward_bytes);
@@ -972,6 +1099,8 @@ PyMethodDef methods[] = {
     {"rotary", reinterpret_cast<PyCFunction>(rotary), METH_FASTCALL, nullptr},
     {"append_tokens", reinterpret_cast<PyCFunction>(append_tokens), METH_FASTCALL, nullptr},
     {"tree_attention", reinterpret_cast<PyCFunction>(tree_attention), METH_FASTCALL, nullptr},
+    {"weighed_token_attention", reinterpret_cast<PyCFunction>(weighed_token_attention), METH_FASTCALL, nullptr},
+    {"evict_tokens", reinterpret_cast<PyCFunction>(evict_tokens), METH_FASTCALL, nullptr},
     {"attention_forward", reinterpret_cast<PyCFunction>(attention_forward), METH_FASTCALL, nullptr},
     {"attention_backward", reinterpret_cast<PyCFunction>(attention_backward), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -118,6 +118,38 @@ def tree_attention(
     return _tree_attention("tree_attention", q, k, v, k_pages, v_pages, page_table, lengths, mask, None, (0, 0), scale)
 
 
+def _check_table(page_table, lengths, batch, device):
+    for name, x, dims in (("page_table", page_table, 2), ("lengths", lengths, 1)):
+        if not isinstance(x, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if x.dtype != torch.int32:
+            raise TypeError(f"{name} must use torch.int32")
+        if x.device != device:
+            raise ValueError("all inputs must be CUDA tensors on the same device")
+        if x.ndim != dims or x.shape[0] != batch:
+            raise ValueError("page_table must have shape [B, columns] and lengths [B]")
+    if page_table.shape[1] == 0:
+        raise ValueError("page_table must have a column")
+
+
+def _check_fresh(q, k, v):
+    """Queries, keys and values of tokens that are not in the cache: ``(batch, tokens, heads, kv_heads, dim)``."""
+
+    if not isinstance(q, torch.Tensor):
+        raise TypeError("q must be a torch.Tensor")
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        _validate.heads_tensor(name, x, q.device, q.dtype)
+    batch, tokens, heads, dim = q.shape
+    if k.shape != v.shape or k.shape[:2] != (batch, tokens) or k.shape[3] != dim:
+        raise ValueError("k and v must have the same shape, and q's [B, N] and D")
+    kv_heads = k.shape[2]
+    if min(batch, heads, kv_heads) <= 0:
+        raise ValueError("batch and heads must be positive")
+    if heads % kv_heads:
+        raise ValueError("the number of query heads must be a multiple of that of key heads")
+    return batch, tokens, heads, kv_heads, dim
+
+
 def _tree_attention(what, q, k, v, k_pages, v_pages, page_table, lengths, mask, depths, window, scale):
     if forward_ad._current_level >= 0:
         _validate.refuse_tangents(what, q, k, v, k_pages, v_pages)
@@ -125,32 +157,11 @@ def _tree_attention(what, q, k, v, k_pages, v_pages, page_table, lengths, mask, 
         done = _lib.host().tree_attention(q, k, v, k_pages, v_pages, page_table, lengths, mask, depths, *window, scale)
         if done is not None:
             return done
-    if not isinstance(q, torch.Tensor):
-        raise TypeError("q must be a torch.Tensor")
-    for name, x in (("q", q), ("k", k), ("v", v)):
-        _validate.heads_tensor(name, x, q.device, q.dtype)
-    batch, drafted, heads, dim = q.shape
-    if k.shape != v.shape or k.shape[:2] != (batch, drafted) or k.shape[3] != dim:
-        raise ValueError("k and v must have the same shape, and q's [B, N] and D")
-    kv_heads = k.shape[2]
-    if min(batch, heads, kv_heads) <= 0:
-        raise ValueError("batch and heads must be positive")
-    if heads % kv_heads:
-        raise ValueError("the number of query heads must be a multiple of that of key heads")
+    batch, drafted, heads, kv_heads, dim = _check_fresh(q, k, v)
     _check_pages(k_pages, v_pages, q.dtype, q.device, kv_heads, dim)
     if k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
         raise ValueError("k_pages and v_pages must be 16-byte aligned")
-    for name, x, shape in (("page_table", page_table, (batch, None)), ("lengths", lengths, (batch,))):
-        if not isinstance(x, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
-        if x.dtype != torch.int32:
-            raise TypeError(f"{name} must use torch.int32")
-        if x.device != q.device:
-            raise ValueError("all inputs must be CUDA tensors on the same device")
-        if x.ndim != len(shape) or x.shape[0] != batch:
-            raise ValueError("page_table must have shape [B, columns] and lengths [B]")
-    if page_table.shape[1] == 0:
-        raise ValueError("page_table must have a column")
+    _check_table(page_table, lengths, batch, q.device)
     if mask is not None:
         if not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool:
             raise TypeError("mask must be a torch.bool tensor or None")

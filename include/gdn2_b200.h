@@ -539,6 +539,53 @@ int gdn2_window_tree_attention(const void* q, const void* k, const void* v, cons
                                int64_t columns, int64_t window, int64_t sinks, int dtype, float scale, void* stream);
 
 /*
+ * What weight every token of a prompt got from causal attention: weights[row][kv head] (fp32, contiguous), the sum of the
+ * softmax weights that the queries at and behind the token, of all heads of a group, gave it.  `statistics` is what
+ * gdn2_attention_forward left for the same q, k, bounds and scale.  scratch: gdn2_attention_weights_bytes, which may be 0
+ * (the device is the current one), dead when the call's kernels have run.  strides: batch, token and head of q, k.
+ */
+int64_t gdn2_attention_weights_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads,
+                                     int64_t kv_heads);
+int gdn2_attention_weights(const void* q, const void* k, const float* statistics, float* weights, void* scratch,
+                           const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time,
+                           int64_t heads, int64_t kv_heads, int64_t dim, int dtype, float scale, void* stream);
+
+/*
+ * Attention of `tokens` new tokens of each sequence over its cached ones and over each other (j <= i), as
+ * gdn2_tree_attention without a mask, and the weight that every token gets from them, summed over their heads of a group
+ * and over them.  weight_pages [pages][kv_heads][page] (fp32) belongs to the cache: a cached token's weight becomes
+ * decay * weight + what it got (with a decay of 0 it is not read), that of a new one is put to slots[b * tokens + i]
+ * (page number * page + place; negative or behind the cache: left out), which must not be a cached token's.  A page whose
+ * weights change belongs to one sequence.  tokens * heads / kv_heads <= GDN2_WEIGHED_MAX_ROWS.  A sequence whose output is NaN
+ * gets weights of NaN; one whose length is bad changes none but those of its new tokens.
+ */
+#define GDN2_WEIGHED_MAX_ROWS 256
+int64_t gdn2_weighed_token_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                           int64_t dim, int64_t page, int64_t columns);
+int gdn2_weighed_token_attention(const void* q, const void* k, const void* v, const void* k_pages,
+                                 const void* v_pages, float* weight_pages, const int* page_table, const int* lengths,
+                                 const int64_t* slots, void* out, void* workspace, const int64_t* strides,
+                                 int64_t table_stride, int64_t batch, int64_t tokens, int64_t heads,
+                                 int64_t kv_heads, int64_t dim, int64_t pages, int64_t page, int64_t columns,
+                                 float decay, int dtype, float scale, void* stream);
+
+/*
+ * Copies of every sequence and key head the `keep` cached tokens of the largest weights, with these, to the pages that
+ * new_table names, in their order: token j of them to page new_table[b * new_stride + j / page] at j % page.  The first
+ * `sinks` and the last `recent` tokens of a sequence are among them (sinks + recent <= keep <= new_columns * page), and
+ * all tokens of one that has no more than `keep`.  Of equal weights the earlier token's counts more, NaN counts more than any
+ * number.  new_lengths[b]: how many were kept; -1, and nothing is copied, where the length or a page number of the sequence is
+ * none of the cache.  Tokens whose new page is none of the cache are left out.  No page that is written to may be one that
+ * any sequence's page table names, or another sequence's new one.  workspace: gdn2_evict_workspace_bytes.
+ */
+int64_t gdn2_evict_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t keep);
+int gdn2_evict_tokens(void* k_pages, void* v_pages, float* weight_pages, const int* page_table, const int* lengths,
+                      const int* new_table, int* new_lengths, void* workspace, int64_t table_stride,
+                      int64_t new_stride, int64_t batch, int64_t pages, int64_t page, int64_t kv_heads, int64_t dim,
+                      int64_t columns, int64_t new_columns, int64_t keep, int64_t sinks, int64_t recent, int dtype,
+                      void* stream);
+
+/*
  * Test aid: how often a wait inside the attention kernels of later calls polls (0: it looks once; negative: as usual).
  * A CTA in which a wait runs out ends by itself and leaves NaN in place of what it has not finished.  For the process.
  */
