@@ -140,7 +140,7 @@ class _PythonWay:
 
     forward = train_forward = train_backward = prologue_forward = prologue_backward = staticmethod(lambda *_: None)
     rotary = append_tokens = tree_attention = attention_forward = attention_backward = staticmethod(lambda *_: None)
-    weighed_token_attention = evict_tokens = staticmethod(lambda *_: None)
+    weighed_attention = weighed_token_attention = evict_tokens = staticmethod(lambda *_: None)
 
 
 _host_module = None

@@ -92,6 +92,38 @@ __device__ __noinline__ float far_sum(uint32_t s_at, const float* st, const floa
   return sum;
 }
 
+// The sum of a row's weights; kPartial: columns first .. last - 1 count
+template <bool kPartial>
+__device__ __forceinline__ float row_sum(uint32_t s_at, const float* st, float2 by, int first, int last) {
+  float2 sum[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+  uint32_t s[2][32];
+  tc::tmem_ld32(s_at, s[0]);
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    tc::tmem_wait_ld();
+    if (x < 3) tc::tmem_ld32(s_at + (x + 1) * 32, s[(x + 1) & 1]);
+    const uint32_t(&v)[32] = s[x & 1];
+#pragma unroll
+    for (int y = 0; y < 32; y += 4) {
+      const float4 l = *reinterpret_cast<const float4*>(st + x * 32 + y);
+      const float2 a = fma2(make_float2(__uint_as_float(v[y]), __uint_as_float(v[y + 1])), by, make_float2(l.x, l.y));
+      const float2 b = fma2(make_float2(__uint_as_float(v[y + 2]), __uint_as_float(v[y + 3])), by, make_float2(l.z, l.w));
+      float2 e = exp2_2(a), f = (y & 4) != 0 ? exp2_fma(b) : exp2_2(b);
+      if (kPartial) {
+        const int col = x * 32 + y;
+        if (col < first || col >= last) e.x = 0.f;
+        if (col + 1 < first || col + 1 >= last) e.y = 0.f;
+        if (col + 2 < first || col + 2 >= last) f.x = 0.f;
+        if (col + 3 < first || col + 3 >= last) f.y = 0.f;
+      }
+      sum[(y >> 1) & 2] = add2(sum[(y >> 1) & 2], e);
+      sum[((y >> 1) & 2) + 1] = add2(sum[((y >> 1) & 2) + 1], f);
+    }
+  }
+  const float2 all = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+  return all.x + all.y;
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) attention_weights_kernel(const __grid_constant__ WeightParams p) {
   using C = WeightConfig<DP>;
@@ -230,32 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_weights_kernel(const __
         if (__builtin_expect(far, 0)) {
           total += far_sum(s_at, st, p.shifts + (w.head * p.group + g) * p.seq.stat_rows + w.at.stat + at, p.scale_log2, first, last);
         } else {
-          float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-          uint32_t s[2][32];
-          tc::tmem_ld32(s_at, s[0]);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            tc::tmem_wait_ld();
-            if (x < 3) tc::tmem_ld32(s_at + (x + 1) * 32, s[(x + 1) & 1]);
-            const uint32_t(&v)[32] = s[x & 1];
-#pragma unroll
-            for (int y = 0; y < 32; y += 4) {
-              const float4 l = *reinterpret_cast<const float4*>(st + x * 32 + y);
-              const float2 a = fma2(make_float2(__uint_as_float(v[y]), __uint_as_float(v[y + 1])), by, make_float2(l.x, l.y));
-              const float2 b = fma2(make_float2(__uint_as_float(v[y + 2]), __uint_as_float(v[y + 3])), by, make_float2(l.z, l.w));
-              float2 e = exp2_2(a), f = (y & 4) != 0 ? exp2_fma(b) : exp2_2(b);
-              if (partial) {
-                const int col = x * 32 + y;
-                if (col < first || col >= last) e.x = 0.f;
-                if (col + 1 < first || col + 1 >= last) e.y = 0.f;
-                if (col + 2 < first || col + 2 >= last) f.x = 0.f;
-                if (col + 3 < first || col + 3 >= last) f.y = 0.f;
-              }
-              sum[0] = add2(sum[0], e);
-              sum[1] = add2(sum[1], f);
-            }
-          }
-          total += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          total += partial ? row_sum<true>(s_at, st, by, first, last) : row_sum<false>(s_at, st, by, 0, 128);
         }
         tc::tc_fence_before();
         __syncwarp();

@@ -212,6 +212,24 @@ inline int launch_beside(void (*kernel)(Params...), unsigned blocks, int threads
   return GDN2_ERR_LAUNCH;
 }
 
+// Quotients by a number that a launch knows, for numbers from 0 to 2^31 - 1: n / d is the upper part of n times
+// ceil(2^(31 + l) / d), where 2^(l - 1) < d <= 2^l; what that is too large by, below 1 / 2^(31 + l) times n, is less than 1 / d.
+struct Divisor {
+  uint32_t d, factor, shift;
+  __device__ __forceinline__ int quotient(int n) const { return d == 1 ? n : int(__umulhi(uint32_t(n), factor) >> shift); }
+  __device__ __forceinline__ int split(int n, int* rest) const {   // quotient, and what is left
+    const int q = quotient(n);
+    *rest = n - q * int(d);
+    return q;
+  }
+};
+inline Divisor divisor(int d) {
+  uint32_t l = 0;
+  while ((uint64_t(1) << l) < uint32_t(d)) ++l;
+  const uint64_t power = uint64_t(1) << (31 + l);
+  return {uint32_t(d), uint32_t((power + uint32_t(d) - 1) / uint32_t(d)), l == 0 ? 0 : l - 1};
+}
+
 inline bool valid_seq_dtype(int d) { return d == GDN2_BF16 || d == GDN2_FP16; }
 inline bool valid_gate_dtype(int d, int seq) { return d == seq || d == GDN2_FP32; }
 

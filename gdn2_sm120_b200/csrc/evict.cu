@@ -3,10 +3,10 @@
 //
 // select_kernel   a CTA has a sequence and head.  Which tokens are kept follows from the keep-th largest weight and, among those
 //                 that are equal to it, from their order.  Weights become whole numbers of the same order, and the one looked
-//                 for is closed in by counting them in 2048 bins over the range that is left: every pass over the weights, which
-//                 lie in shared memory where there is room, narrows the range 2048 times, and the first range reaches from the
-//                 smallest weight to the largest, so that the bins are spread where the weights are.  Then a pass writes down
-//                 the numbers of the tokens that stay.
+//                 for is closed in by counting them in 2048 bins over the range that is left, which a pass narrows 2048 times; the
+//                 first range reaches from the smallest weight to the largest, so that the bins are spread where the weights
+//                 are.  When up to 512 are left they are compared with one another.  The weights lie in shared memory where there is
+//                 room (49152), and are read once more for every pass otherwise.
 // gather_kernel   copies keys, values and weights, 64 tokens of a head a CTA.  Bound by HBM.
 // TODO-FIGURES
 
@@ -18,10 +18,12 @@ namespace gdn2 {
 
 namespace {
 
-constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32;
+constexpr int kSelectThreads = 1024;
 constexpr int kBins = 2048, kBinBits = 11;
+constexpr int kAll = 0x7fffffff;
 constexpr int kCached = 49152;        // weights that stay in shared memory
-constexpr int kGatherThreads = 256, kGatherTokens = 64;
+constexpr int kGatherThreads = 256, kGatherWarp = 8, kGatherTokens = kGatherThreads / 32 * kGatherWarp;
+constexpr int kListed = 512;          // candidates near the border that are compared with one another
 
 struct EvictParams {
   uint8_t *k_pages, *v_pages;
@@ -31,8 +33,10 @@ struct EvictParams {
   int* kept;                          // [batch][kv head]: tokens that are copied, or -1
   int* tokens;                        // [batch][kv head][keep]: which
   int64_t table_stride, new_stride, pages;
-  int batch, kv_heads, page, columns, keep, sinks, recent, cached;
+  int batch, kv_heads, page, columns, keep, sinks, recent;
+  int cached;                         // weights that stay in shared memory
   int per_row, chunks;                // packs of a row of keys; CTAs of a sequence and head
+  Divisor by_page, by_row;
 };
 
 // Whole numbers in the order of the weights: NaN above all, -0 and 0 the same
@@ -42,30 +46,31 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return (x >> 31) != 0 ? ~x : x | 0x80000000u;
 }
 
-// Sums over the CTA of two numbers a thread and over the warps before its own, by all threads
-struct WarpSums { int a[kSelectWarps], b[kSelectWarps]; };
+// Of two numbers a warp, by all threads: the sums over the warps before its own, and over all
+struct WarpSums { int a[32], b[32]; };   // those behind the last warp are 0
 __device__ __forceinline__ int2 sums_before(WarpSums& shared, int a, int b, int2* all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __syncthreads();
   if (lane == 0) { shared.a[warp] = a; shared.b[warp] = b; }
   __syncthreads();
-  int2 before = make_int2(0, 0), sum = make_int2(0, 0);
+  int x = shared.a[lane], y = shared.b[lane];
+  const int own_x = x, own_y = y;
 #pragma unroll
-  for (int w = 0; w < kSelectWarps; ++w) {
-    if (w == warp) before = sum;
-    sum.x += shared.a[w];
-    sum.y += shared.b[w];
+  for (int d = 1; d < 32; d <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, x, d), v = __shfl_up_sync(0xffffffffu, y, d);
+    if (lane >= d) { x += u; y += v; }
   }
-  *all = sum;
-  return before;
+  *all = make_int2(__shfl_sync(0xffffffffu, x, 31), __shfl_sync(0xffffffffu, y, 31));
+  return make_int2(__shfl_sync(0xffffffffu, x - own_x, warp), __shfl_sync(0xffffffffu, y - own_y, warp));
 }
 
 __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const __grid_constant__ EvictParams p) {
-  extern __shared__ uint32_t cache[];
+  extern __shared__ uint32_t cache[];   // of the candidates
   __shared__ int bins[kBins];
+  __shared__ uint32_t list[kListed];
   __shared__ WarpSums sums;
   __shared__ uint32_t range[2];
-  __shared__ int found[3];
+  __shared__ int found[3], listed;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = int(blockIdx.x) / p.kv_heads, head = int(blockIdx.x) - b * p.kv_heads;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -74,41 +79,54 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const __grid_
   const int* table = p.table + b * p.table_stride;
   bool good = sized;
   for (int c = tid; sized && c < (length + p.page - 1) / p.page; c += kSelectThreads) good = good && table[c] >= 0 && table[c] < p.pages;
-  good = __syncthreads_and(good);
-  const int kept = good ? min(length, p.keep) : -1;
-  if (tid == 0) {
-    p.kept[blockIdx.x] = kept;
-    if (head == 0) p.new_lengths[b] = kept;
+  auto tell = [&](bool good) {
+    if (tid == 0) {
+      p.kept[blockIdx.x] = good ? min(length, p.keep) : -1;
+      if (head == 0) p.new_lengths[b] = good ? min(length, p.keep) : -1;
+    }
+  };
+  if (length <= p.keep || !sized) {   // all tokens stay, or none can be read
+    tell(__syncthreads_and(good));
+    return;
   }
-  if (kept < p.keep || length == p.keep) return;   // all tokens stay, or none can be read
 
-  // candidates: neither sinks nor recent ones
+  // Candidates are neither sinks nor recent ones
   const int first = p.sinks, last = length - p.recent;
   const bool cached = last - first <= p.cached;
-  auto read = [&](int t) { return order_of(p.weight_pages[(int64_t(table[t / p.page]) * p.kv_heads + head) * p.page + t % p.page]); };
+  const float* weights = p.weight_pages + int64_t(head) * p.page;
+  const int64_t page_size = int64_t(p.kv_heads) * p.page;
+  auto read = [&](int t) {   // (without a branch, so that several are under way)
+    int place;
+    const int page = table[p.by_page.split(t, &place)];
+    const bool there = page >= 0 && page < p.pages;
+    const float w = weights[there ? page * page_size + place : 0];
+    return order_of(w);
+  };
   auto key = [&](int t) { return cached ? cache[t - first] : read(t); };
   int wanted = p.keep - p.sinks - p.recent;   // candidates that stay
   uint32_t lo = ~0u, hi = 0;
   for (int t0 = first + tid; t0 < last; t0 += 8 * kSelectThreads) {
     uint32_t x[8];
 #pragma unroll
-    for (int y = 0; y < 8; ++y) {
-      const int t = t0 + y * kSelectThreads;
-      x[y] = t < last ? read(t) : 0;
-    }
+    for (int y = 0; y < 8; ++y) x[y] = read(min(t0 + y * kSelectThreads, last - 1));
 #pragma unroll
     for (int y = 0; y < 8; ++y) {
       const int t = t0 + y * kSelectThreads;
-      if (t >= last) break;
       lo = min(lo, x[y]);
       hi = max(hi, x[y]);
-      if (cached) cache[t - first] = x[y];
+      if (cached && t < last) cache[t - first] = x[y];
     }
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
-  if (tid < 2) range[tid] = tid == 0 ? ~0u : 0u;
-  __syncthreads();
+  for (int x = tid; x < kBins; x += kSelectThreads) bins[x] = 0;
+  if (tid < 32) {
+    sums.a[tid] = sums.b[tid] = 0;
+    if (tid < 2) range[tid] = tid == 0 ? ~0u : 0u;
+  }
+  good = __syncthreads_and(good);
+  tell(good);
+  if (!good) return;
   if (lane == 0) {
     atomicMin(&range[0], lo);
     atomicMax(&range[1], hi);
@@ -119,141 +137,178 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const __grid_
 
   // The wanted-th largest is in lo .. hi; what is above hi stays
   int equal = 0;             // of those that are lo in the end, so many stay
-  if (wanted == 0) {
-    lo = ~0u;
-  } else {
-    // 2^32 numbers, then at most 2^21, 2^10 and one
-    for (int pass = 0; pass < 4; ++pass) {
-      if (lo == hi) {
-        equal = wanted;
-        break;
+  if (wanted == 0) lo = ~0u;
+  // 2^32 numbers, then at most 2^21, 2^10 and one, or few weights in what is left of the range
+  for (int pass = 0; wanted > 0 && pass < 4; ++pass) {
+    if (lo == hi) {
+      equal = wanted;
+      break;
+    }
+    const int shift = max(0, 32 - __clz(hi - lo) - kBinBits);
+    int smallest = 0;        // many weights are often the smallest one: counted without the others' atomics
+    for (int t = first + tid; t < last; t += kSelectThreads) {
+      const uint32_t x = key(t);
+      if (x == lo) ++smallest;
+      else if (x > lo && x <= hi) atomicAdd(&bins[(x - lo) >> shift], 1);
+    }
+    smallest = __reduce_add_sync(0xffffffffu, smallest);
+    if (lane == 0 && smallest > 0) atomicAdd(&bins[0], smallest);
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    // a thread's bins, from the top down
+    int own[kBins / kSelectThreads], mine = 0;
+#pragma unroll
+    for (int x = 0; x < kBins / kSelectThreads; ++x) {
+      const int bin = kBins - 1 - (tid * (kBins / kSelectThreads) + x);
+      mine += own[x] = bins[bin];
+      bins[bin] = 0;         // for the next pass
+    }
+    int up_to = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, up_to, d);
+      if (lane >= d) up_to += y;
+    }
+    int2 all;
+    int above = sums_before(sums, __shfl_sync(0xffffffffu, up_to, 31), 0, &all).x + up_to - mine;
+    if (above < wanted && above + mine >= wanted) {   // one thread of all
+#pragma unroll
+      for (int x = 0; x < kBins / kSelectThreads; ++x) {
+        if (above < wanted && above + own[x] >= wanted) {
+          found[0] = kBins - 1 - (tid * (kBins / kSelectThreads) + x);
+          found[1] = wanted - above;
+          found[2] = own[x];
+        }
+        above += own[x];
       }
-      const int shift = max(0, 32 - __clz(hi - lo) - kBinBits);
-      for (int x = tid; x < kBins; x += kSelectThreads) bins[x] = 0;
-      __syncthreads();
-      int smallest = 0;      // many weights are often the smallest one: counted without the others' atomics
+    }
+    __syncthreads();
+    wanted = found[1];
+    const int count = found[2];
+    lo += uint32_t(found[0]) << shift;
+    hi = lo + min(hi - lo, (1u << shift) - 1u);   // (lo + 2^shift may pass 2^32)
+    if (wanted == count) {   // all of the bin stay
+      equal = kAll;
+      break;
+    }
+    if (count <= kListed) {  // few are left: the one that wanted - 1 others are above is compared with all of them
       for (int t = first + tid; t < last; t += kSelectThreads) {
         const uint32_t x = key(t);
-        if (x == lo) ++smallest;
-        else if (x > lo && x <= hi) atomicAdd(&bins[(x - lo) >> shift], 1);
+        if (x >= lo && x <= hi) list[atomicAdd(&listed, 1)] = x;
       }
-      smallest = __reduce_add_sync(0xffffffffu, smallest);
-      if (lane == 0 && smallest > 0) atomicAdd(&bins[0], smallest);
       __syncthreads();
-      // a thread's bins, from the top down
-      constexpr int kEach = kBins / kSelectThreads;
-      int mine = 0;
-#pragma unroll
-      for (int x = 0; x < kEach; ++x) mine += bins[kBins - 1 - (tid * kEach + x)];
-      int up_to = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, up_to, d);
-        if (lane >= d) up_to += y;
-      }
-      int2 all;
-      int above = sums_before(sums, __shfl_sync(0xffffffffu, up_to, 31), 0, &all).x + up_to - mine;
-      if (above < wanted && above + mine >= wanted) {   // one thread of all
-#pragma unroll
-        for (int x = 0; x < kEach; ++x) {
-          const int bin = kBins - 1 - (tid * kEach + x);
-          if (above + bins[bin] >= wanted) {
-            found[0] = bin;
-            found[1] = wanted - above;
-            found[2] = bins[bin];
-            break;
-          }
-          above += bins[bin];
+      if (tid < count) {
+        const uint32_t x = list[tid];
+        int larger = 0, as_large = 0;
+#pragma unroll 4
+        for (int i = 0; i < count; ++i) {
+          larger += list[i] > x;
+          as_large += list[i] == x;
+        }
+        if (larger < wanted && larger + as_large >= wanted) {   // one, or some that are equal
+          range[0] = x;
+          found[1] = wanted - larger;
+          found[2] = as_large;
         }
       }
       __syncthreads();
-      wanted = found[1];
-      lo += uint32_t(found[0]) << shift;
-      hi = lo + min(hi - lo, (1u << shift) - 1u);   // (lo + 2^shift may pass 2^32)
-      if (wanted == found[2]) {   // all of the bin stay
-        equal = 0x7fffffff;
-        break;
-      }
-      __syncthreads();
+      lo = range[0];
+      equal = found[1] == found[2] ? kAll : found[1];
+      break;
     }
+    __syncthreads();         // found has been read by all
   }
 
-  // A warp has a range of the tokens: how many stay for their weight or their place, how many are equal to the border
-  const int each = (length + kSelectThreads - 1) / kSelectThreads * 32, begin = min(length, warp * each), end = min(length, begin + each);
-  auto look = [&](int t, bool* stays, bool* even) {
-    const bool protected_ = t < first || t >= last, candidate = t < end && !protected_;
-    const uint32_t x = candidate ? key(t) : 0;
-    *stays = t < end && (protected_ || (equal == 0x7fffffff ? x >= lo : x > lo));
-    *even = candidate && equal != 0x7fffffff && x == lo;
-  };
+  // The sinks come first and the recent ones last; a warp has a range of the candidates between them: how many stay for their
+  // weight, how many are equal to the border.  (No order_of is 0, so that the bound below all of them is no problem.)
+  const uint32_t bound = equal == kAll ? lo - 1 : lo;
+  const bool border = equal != kAll && equal > 0;
+  const int each = (last - first + kSelectThreads - 1) / kSelectThreads * 32, begin = min(last, first + warp * each), end = min(last, begin + each);
+  const uint32_t below = (1u << lane) - 1u;
+  int* to = p.tokens + int64_t(blockIdx.x) * p.keep;
+  for (int j = tid; j < p.sinks; j += kSelectThreads) to[j] = j;
+  for (int j = tid; j < p.recent; j += kSelectThreads) to[p.keep - p.recent + j] = last + j;
+  int2 all;
+  if (cached && !border) {
+    // what stays moves together where it is, token numbers in place of weights, and goes out when all warps have counted
+    uint32_t* own = cache + (begin - first);
+    int staying = 0;
+    for (int t = begin + lane; t - lane < end; t += 32) {
+      const bool stay = t < end && own[t - begin] > bound;
+      const uint32_t stays = __ballot_sync(0xffffffffu, stay);
+      __syncwarp();
+      if (stay) own[staying + __popc(stays & below)] = uint32_t(t);
+      staying += __popc(stays);
+    }
+    const int at = p.sinks + sums_before(sums, staying, 0, &all).x;
+    for (int i = lane; i < staying && at + i < p.keep; i += 32) to[at + i] = int(own[i]);
+    return;
+  }
   int staying = 0, evens = 0;
   for (int t = begin + lane; t - lane < end; t += 32) {
-    bool stays, even;
-    look(t, &stays, &even);
-    staying += __popc(__ballot_sync(0xffffffffu, stays));
-    evens += __popc(__ballot_sync(0xffffffffu, even));
+    const uint32_t x = t < end ? key(t) : 0;
+    staying += __popc(__ballot_sync(0xffffffffu, x > bound));
+    if (border) evens += __popc(__ballot_sync(0xffffffffu, x == lo));
   }
-  int2 all;
-  int2 before = sums_before(sums, staying, evens, &all);
-  int* to = p.tokens + int64_t(blockIdx.x) * p.keep;
-  const uint32_t below = (1u << lane) - 1u;
+  const int2 before = sums_before(sums, staying, evens, &all);
+  int at = p.sinks + before.x + (border ? min(before.y, equal) : 0);   // where the warp's next one goes
+  int level = before.y;
   for (int t = begin + lane; t - lane < end; t += 32) {
-    bool stays, even;
-    look(t, &stays, &even);
-    const uint32_t s = __ballot_sync(0xffffffffu, stays), e = __ballot_sync(0xffffffffu, even);
-    const int rank = before.y + __popc(e & below);
-    const int at = before.x + __popc(s & below) + min(rank, equal);
-    if ((stays || (even && rank < equal)) && at < p.keep) to[at] = t;
-    before.x += __popc(s);
-    before.y += __popc(e);
+    const uint32_t x = t < end ? key(t) : 0;
+    uint32_t stays = __ballot_sync(0xffffffffu, x > bound);
+    if (border) {
+      const uint32_t even = __ballot_sync(0xffffffffu, x == lo);
+      stays |= __ballot_sync(0xffffffffu, x == lo && level + __popc(even & below) < equal);
+      level += __popc(even);
+    }
+    const int place = at + __popc(stays & below);
+    if (((stays >> lane) & 1) != 0 && place < p.keep) to[place] = t;
+    at += __popc(stays);
   }
 }
 
+// A warp has 8 tokens of a head, wherever they are: nothing but its own loads stands between it and the next one's.
 template <typename P>
 __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ int64_t from[kGatherTokens], to[kGatherTokens];   // rows of keys, -1 for none
-  const int unit = int(blockIdx.x) / p.chunks, chunk = int(blockIdx.x) - unit * p.chunks;
-  const int b = unit / p.kv_heads, head = unit - b * p.kv_heads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // the heads of 64 places are written one beside the other
+  const int head = int(blockIdx.x) % p.kv_heads, chunk = int(blockIdx.x) / p.kv_heads % p.chunks, b = int(blockIdx.x) / p.kv_heads / p.chunks;
+  const int unit = b * p.kv_heads + head;
   const int length = p.lengths[b];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int kept = p.kept[unit], j0 = chunk * kGatherTokens, count = min(kept - j0, kGatherTokens);
+  const int kept = p.kept[unit], j0 = chunk * kGatherTokens + warp * kGatherWarp, count = min(kept - j0, kGatherWarp);
   if (count <= 0) return;
-  if (threadIdx.x < kGatherTokens) {
-    const int j = j0 + int(threadIdx.x);
-    int64_t source = -1, place = -1;
-    if (j < kept) {
-      const int t = length <= p.keep ? j : p.tokens[int64_t(unit) * p.keep + j];
-      const int page = p.new_table[b * p.new_stride + j / p.page];
-      if (page >= 0 && page < p.pages) {
-        source = p.table[b * p.table_stride + t / p.page];
-        place = page;
-        p.weight_pages[(place * p.kv_heads + head) * p.page + j % p.page] = p.weight_pages[(source * p.kv_heads + head) * p.page + t % p.page];
-        source = (source * p.page + t % p.page) * p.kv_heads + head;
-        place = (place * p.page + j % p.page) * p.kv_heads + head;
-      }
+  int64_t from = 0, to = -1;   // rows of keys of token j0 + lane, -1 for none
+  if (lane < count) {
+    const int j = j0 + lane, t = length <= p.keep ? j : p.tokens[int64_t(unit) * p.keep + j];
+    int t_place, j_place;
+    const int page = p.new_table[b * p.new_stride + p.by_page.split(j, &j_place)];
+    const int64_t source = p.table[b * p.table_stride + p.by_page.split(t, &t_place)];
+    if (page >= 0 && page < p.pages) {
+      p.weight_pages[(int64_t(page) * p.kv_heads + head) * p.page + j_place] = p.weight_pages[(source * p.kv_heads + head) * p.page + t_place];
+      from = (source * p.page + t_place) * p.kv_heads + head;
+      to = (int64_t(page) * p.page + j_place) * p.kv_heads + head;
     }
-    from[threadIdx.x] = source;
-    to[threadIdx.x] = place;
   }
-  __syncthreads();
   constexpr int kAtOnce = 8;
-  const int packs = count * p.per_row;   // of keys, then of values
-  for (int x0 = threadIdx.x; x0 < 2 * packs; x0 += kAtOnce * kGatherThreads) {
+  const int packs = kGatherWarp * p.per_row;   // of keys, then of values
+  for (int x0 = 0; x0 < 2 * packs; x0 += kAtOnce * 32) {
     P data[kAtOnce];
     int64_t place[kAtOnce];
 #pragma unroll
     for (int y = 0; y < kAtOnce; ++y) {
-      const int x = x0 + y * kGatherThreads;
-      place[y] = -1;
-      if (x >= 2 * packs) continue;
-      const int z = x < packs ? x : x - packs, row = z / p.per_row, pack = z - row * p.per_row;
-      if (to[row] < 0) continue;
-      place[y] = to[row] * p.per_row + pack;
-      data[y] = reinterpret_cast<const P*>(x < packs ? p.k_pages : p.v_pages)[from[row] * p.per_row + pack];
+      const int x = x0 + y * 32 + lane, z = x < packs ? x : x - packs, row = min(p.by_row.quotient(z), kGatherWarp - 1);
+      const int64_t source = __shfl_sync(0xffffffffu, from, row);
+      place[y] = __shfl_sync(0xffffffffu, to, row);
+      const int pack = z - row * p.per_row;
+      if (x >= 2 * packs) place[y] = -1;
+      if (place[y] < 0) continue;
+      place[y] = place[y] * p.per_row + pack;
+      data[y] = reinterpret_cast<const P*>(x < packs ? p.k_pages : p.v_pages)[source * p.per_row + pack];
     }
 #pragma unroll
     for (int y = 0; y < kAtOnce; ++y) {
-      if (place[y] >= 0) reinterpret_cast<P*>(x0 + y * kGatherThreads < packs ? p.k_pages : p.v_pages)[place[y]] = data[y];
+      if (place[y] >= 0) reinterpret_cast<P*>(x0 + y * 32 + lane < packs ? p.k_pages : p.v_pages)[place[y]] = data[y];
     }
   }
 }
@@ -261,6 +316,7 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_con
 template <typename P>
 int launch_gather(EvictParams& p, int row_bytes, cudaStream_t stream) {
   p.per_row = row_bytes / int(sizeof(P));
+  p.by_row = divisor(p.per_row);
   return launch_beside(&gather_kernel<P>, unsigned(p.batch * p.kv_heads * p.chunks), kGatherThreads, 0, stream, p);
 }
 
@@ -279,6 +335,7 @@ int launch_evict(void* k_pages, void* v_pages, float* weight_pages, const int* t
   p.tokens = p.kept + int64_t(batch) * kv_heads;
   p.table_stride = table_stride; p.new_stride = new_stride; p.pages = pages;
   p.batch = batch; p.kv_heads = kv_heads; p.page = page; p.columns = columns;
+  p.by_page = divisor(page);
   p.keep = keep; p.sinks = sinks; p.recent = recent;
   p.chunks = (keep + kGatherTokens - 1) / kGatherTokens;
   const int64_t units = int64_t(batch) * kv_heads;

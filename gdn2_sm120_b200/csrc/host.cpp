@@ -49,6 +49,8 @@ struct Api {
   decltype(&gdn2_attention_backward) attention_backward;
   decltype(&gdn2_weighed_token_workspace_bytes) weighed_token_workspace_bytes;
   decltype(&gdn2_weighed_token_attention) weighed_token_attention;
+  decltype(&gdn2_attention_weights_bytes) attention_weights_bytes;
+  decltype(&gdn2_attention_weights) attention_weights;
   decltype(&gdn2_evict_workspace_bytes) evict_workspace_bytes;
   decltype(&gdn2_evict_tokens) evict_tokens;
   decltype(&gdn2_window_tree_attention) window_tree_attention;
@@ -981,6 +983,49 @@ PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_CATCH
 }
 
+// weighed_attention(q, k, v, bounds, scale) -> (output, weights) or None
+PyObject* weighed_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  GDN2_TRY
+  Heads h;
+  float scale;
+  std::vector<int64_t> bounds;
+  if (!g_bound || n != 5 || !read_heads(a, &h) || !read_bounds(a[3], h, &bounds) || !read_attention_scale(a[4], h.dim, &scale) ||
+      wants_grad({h.t[0], h.t[1], h.t[2]})) {
+    return none();
+  }
+  const at::Tensor &q = *h.t[0], &k = *h.t[1];
+  const int64_t* host = bounds.empty() ? nullptr : bounds.data();
+  const int64_t n_seq = bounds.empty() ? h.batch : int64_t(bounds.size()) - 1;
+  at::Tensor out, weights;
+  int status, second = GDN2_OK;
+  WithoutGil others;
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int64_t rows = api.attention_stat_rows(host, n_seq, h.time);
+  const int64_t size = api.attention_weights_bytes(host, n_seq, h.time, h.heads, h.kv_heads);
+  if (rows < 0 || size < 0) {
+    others.end();
+    return none();
+  }
+  out = at::empty(q.sizes(), q.options());
+  weights = floats({h.batch, h.time, h.kv_heads}, q);
+  const at::Tensor statistics = floats({2, h.heads, rows}, q), scratch = size > 0 ? bytes(size, q) : at::Tensor();
+  void* stream = at::cuda::getCurrentCUDAStream().stream();
+  status = api.attention_forward(q.data_ptr(), k.data_ptr(), h.t[2]->data_ptr(), out.data_ptr(), fptr(&statistics), h.strides, host, n_seq,
+                                 h.time, h.heads, h.kv_heads, h.dim, h.dtype, scale, stream);
+  if (status == GDN2_OK) {
+    second = api.attention_weights(q.data_ptr(), k.data_ptr(), fptr(&statistics), fptr(&weights), size > 0 ? scratch.data_ptr() : nullptr,
+                                   h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim, h.dtype, scale, stream);
+  }
+  others.end();
+  if (!ok(status, "gdn2_attention_forward", passes(bounds))) return nullptr;
+  if (!ok(second, "gdn2_attention_weights", (size > 0 ? 2 : 1) * passes(bounds))) return nullptr;
+  PyObject* result = PyTuple_New(2);
+  PyTuple_SET_ITEM(result, 0, wrap(out));
+  PyTuple_SET_ITEM(result, 1, wrap(weights));
+  return result;
+  GDN2_CATCH
+}
+
 // attention_backward(q, k, v, output, statistics, d_output, bounds, scale, window, sinks) -> (dq, dk, dv) or None
 PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_TRY
@@ -1071,6 +1116,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_BIND(attention_backward);
   GDN2_BIND(weighed_token_workspace_bytes);
   GDN2_BIND(weighed_token_attention);
+  GDN2_BIND(attention_weights_bytes);
+  GDN2_BIND(attention_weights);
   GDN2_BIND(evict_workspace_bytes);
   GDN2_BIND(evict_tokens);
   GDN2_BIND(window_tree_attention);
@@ -1099,6 +1146,7 @@ PyMethodDef methods[] = {
     {"rotary", reinterpret_cast<PyCFunction>(rotary), METH_FASTCALL, nullptr},
     {"append_tokens", reinterpret_cast<PyCFunction>(append_tokens), METH_FASTCALL, nullptr},
     {"tree_attention", reinterpret_cast<PyCFunction>(tree_attention), METH_FASTCALL, nullptr},
+    {"weighed_attention", reinterpret_cast<PyCFunction>(weighed_attention), METH_FASTCALL, nullptr},
     {"weighed_token_attention", reinterpret_cast<PyCFunction>(weighed_token_attention), METH_FASTCALL, nullptr},
     {"evict_tokens", reinterpret_cast<PyCFunction>(evict_tokens), METH_FASTCALL, nullptr},
     {"attention_forward", reinterpret_cast<PyCFunction>(attention_forward), METH_FASTCALL, nullptr},

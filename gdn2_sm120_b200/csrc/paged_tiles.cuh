@@ -47,6 +47,7 @@ struct TreeParams {
   float* weight_pages;                       // [pages][kv head][page]
   const int64_t* slots;                      // [batch][drafted]
   float decay;
+  Divisor by_page;
   int width, slices;                         // floats of a row of scores; CTAs of weigh_kernel for a sequence and head
 };
 
@@ -484,6 +485,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
   bool ok = true, split = tile != 0;   // the unit began in another CTA
   while (rest > 0) {
     const int n = min(rest, u.tiles - tile);
+    float* scores = kWeigh ? p.scores + ((int64_t(u.b) * p.kv_heads + u.head) * p.rows + u.block * 16 + quad) * p.width : nullptr;
     float o[kDB][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < kDB; ++d) { o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f; }
@@ -523,13 +525,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
           if (!see) s[x >> 2][x & 3] = -INFINITY;
         }
       }
-      if (kWeigh) {   // scores of all tokens that there are, of rows that there are
+      if (kWeigh) {   // scores of all tokens that there are, of rows that there are (whose widths are even)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int r = quad + 8 * (x & 1) + u.block * 16, t = first_token + (x >> 1) * 8 + in_quad * 2;
-          if (r < p.rows && t < u.length + p.drafted) {   // (rows have even widths)
-            float* to = p.scores + ((int64_t(u.b) * p.kv_heads + u.head) * p.rows + r) * p.width + t;
-            *reinterpret_cast<float2*>(to) = make_float2(s[x >> 1][2 * (x & 1)], s[x >> 1][2 * (x & 1) + 1]);
+          const int t = first_token + (x >> 1) * 8 + in_quad * 2;
+          if (token_of[x & 1] >= 0 && t < u.length + p.drafted) {
+            *reinterpret_cast<float2*>(scores + (x & 1) * 8 * int64_t(p.width) + t) = make_float2(s[x >> 1][2 * (x & 1)], s[x >> 1][2 * (x & 1) + 1]);
           }
         }
       }

@@ -23,7 +23,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib, _validate
-from .attention import _check, _forward, _launches, _native, _packed_bounds, _sequences
+from .attention import _check, _forward, _launches, _packed_bounds, _sequences
 from .paged import _DTYPES, _check_fresh, _check_pages, _check_table
 
 _MOST_ROWS = 256      # new tokens times heads of a group
@@ -37,14 +37,14 @@ def _refuse_gradients(what, *tensors):
 def _weighed(what, q, k, v, bounds, scale):
     if forward_ad._current_level >= 0:
         _validate.refuse_tangents(what, q, k, v)
-    tensors = [x for x in (q, k, v) if isinstance(x, torch.Tensor)]
-    _refuse_gradients(what, *tensors)
-    q, k, v = (_validate.detached(x) if isinstance(x, torch.Tensor) else x for x in (q, k, v))
-    done = _native(q, k, v, bounds, scale, (0, 0), True)
+    if _lib.KERNEL_EVENTS is None and getattr(q, "is_cuda", False):
+        done = _lib.host().weighed_attention(q, k, v, bounds, scale)
+        if done is not None:
+            return done
     checked, scale = _check(q, k, v, bounds, scale)
-    if done is None:
-        done = _forward(q, k, v, checked, scale, (0, 0), True)
-    out, statistics = done
+    _refuse_gradients(what, q, k, v)
+    q, k, v = (_validate.detached(x) for x in (q, k, v))
+    out, statistics = _forward(q, k, v, checked, scale, (0, 0), True)
     weights = torch.empty(k.shape[:3], device=k.device, dtype=torch.float32)
     if statistics is None:
         return out, weights
