@@ -44,11 +44,12 @@ struct TreeParams {
   // weights that tokens get
   float* scores;                             // [batch][kv head][row][width], as they come out of Q K^T
   float2* stats;                             // [batch][kv head][row]: (m, l) where one CTA had all of a row
+  int2* ends;                                // [batch][kv head][block of rows]: the first and last CTA that had a part of it
   float* weight_pages;                       // [pages][kv head][page]
   const int64_t* slots;                      // [batch][drafted]
   float decay;
   Divisor by_page;
-  int width, slices;                         // floats of a row of scores; CTAs of weigh_kernel for a sequence and head
+  int width, slices;                         // floats of a row of scores; CTAs of weigh_kernel
 };
 
 // A sequence's cached tokens and then its drafted ones, in tiles; kRows rows of one key head
@@ -235,8 +236,19 @@ __device__ __forceinline__ void copy_rows(uint32_t base, uint32_t slab, int firs
 }
 
 // a tiled copy into shared memory that is given by its address there
+// (kOnce: it leaves L2 before anything else)
+template <bool kOnce>
 __device__ __forceinline__ void tma_load_page(uint32_t to, const CUtensorMap* map, int c, int head, int row, int page,
                                               uint64_t* full, uint32_t leader) {
+  if (kOnce) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t.reg .b64 once;\n\tsetp.ne.b32 q, %7, 0;\n\tcreatepolicy.fractional.L2::evict_first.b64 once, 1.0;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], "
+        "[%1, {%2, %3, %4, %5}], [%6], once;\n\t}"
+        ::"r"(to), "l"(map), "r"(c), "r"(head), "r"(row), "r"(page), "r"(tc::smem_u32(full)), "r"(leader)
+        : "memory");
+    return;
+  }
   asm volatile(
       "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %7, 0;\n\t"
       "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
@@ -251,7 +263,7 @@ __device__ __forceinline__ void tma_load_page(uint32_t to, const CUtensorMap* ma
 // every token modulo kStrangeRows.  With a window the cached tokens that some of the drafted ones see and some do not are
 // looked at like these (numbered back from the first drafted one), and those that none of them sees are not read.
 constexpr int kStrangeRows = 2048;
-template <typename T, int DP, bool kWindow, int kStages, int kWarps>
+template <typename T, int DP, bool kWindow, bool kOnce, int kStages, int kWarps>
 __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int tile, int rest, int warp, uint32_t kv_base, uint64_t* full,
                                             uint64_t* empty, const attn::Waiter& waiter, int* strange, uint32_t* strange_rows) {
   constexpr int kTileBytes = kTile * DP * 2;
@@ -295,7 +307,7 @@ __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int til
           const int page = __shfl_sync(0xffffffffu, pages.of[i], r), row = (t0 + i * 32 + r) % p.page;
 #pragma unroll
           for (int slab = 0; slab < DP / 64; ++slab) {
-            tma_load_page(base + slab * kSlab + uint32_t(mine + i * 32 + r) * 128u, keys ? &p.k_map : &p.v_map, slab * 64, u.head, row, page, &full[s],
+            tma_load_page<kOnce>(base + slab * kSlab + uint32_t(mine + i * 32 + r) * 128u, keys ? &p.k_map : &p.v_map, slab * 64, u.head, row, page, &full[s],
                           leader);
           }
         }
@@ -449,7 +461,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
   if (!part_of_cta<kWindow, kFewThreads / 32>(p, bar.share, u, tile, rest)) return;
   const attn::Waiter waiter{&bar.failed, p.polls};
   if (warp >= 8) {
-    bring_tiles<T, DP, kWindow, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange, nullptr);
+    bring_tiles<T, DP, kWindow, kWeigh, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange, nullptr);
     return;
   }
 
@@ -618,6 +630,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       const bool whole = !split && tile + n == u.tiles, strange = *static_cast<volatile int*>(&bar.strange) != 0;
       const int64_t slot = int64_t(blockIdx.x) * 2 + (split ? 0 : 1);
       ok = ok && waiter.nobody_failed();   // none of the eight
+      if (kWeigh && lane == 0) {
+        int2* ends = p.ends + (int64_t(u.b) * p.kv_heads + u.head) * p.row_blocks + u.block;
+        if (!split) ends->x = int(blockIdx.x);
+        if (tile + n == u.tiles) ends->y = int(blockIdx.x);
+      }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int local = quad + 8 * half, r = local + (kWeigh ? u.block * 16 : 0);

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       }
       cp_async_wait_all();
     } else if (warp < 12) {
-      bring_tiles<T, DP, kWindow, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange,
+      bring_tiles<T, DP, kWindow, false, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange,
                                                  bar.strange_rows);
     }
   } else {
