@@ -88,6 +88,7 @@ __device__ __forceinline__ int depth_of(const TreeParams& p, int b, int i) {
 __device__ __forceinline__ int seen_from(const TreeParams& p, const Unit& u, int depth) { return u.length + depth - p.window + 1; }
 // ... whether it sees drafted token d, which its mask names
 __device__ __forceinline__ bool reaches(const TreeParams& p, const Unit& u, int depth, int d) {
+  if (depth < p.window) return true;   // (no depth is below 0)
   const int at = depth_of(p, u.b, d);
   return depth - at < p.window || u.length + at < p.sinks;
 }

@@ -219,23 +219,40 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         if (any_there) {   // warps without a row have nothing to do but to keep count
           const int first_token = tile_token<kWindow>(u, tile + j);
           attn::soften<T, DP>(s_at, o_at, p.scale_log2, m, sum, [&](int x, uint32_t (&s)[32]) {
-            if (first_token + x * 32 + 32 <= u.length) {
-              if (!kWindow || first_token + x * 32 >= all_from || first_token + x * 32 + 32 <= p.sinks) return;
-              // (rows that are not there have a depth of 0; nothing but their zeros comes of them)
-              const attn::Span span{p.window, p.sinks};
-              span.hide(u.length + depth, first_token + x * 32, s);
+            const int key = first_token + x * 32;
+            if (key + 32 <= u.length && (!kWindow || key >= all_from || key + 32 <= p.sinks)) return;
+            if (kWindow && (key + 32 <= u.length || (p.mask == nullptr && p.depths == nullptr))) {
+              // cached tokens, or a chain's, whose places are those behind them.  (Rows that are not there have a depth of 0;
+              // nothing but their zeros comes of them.)
+              attn::Span{p.window, p.sinks}.hide(u.length + depth, key, s);
               return;
             }
             // drafted tokens, or the end
             const uint8_t* mask = p.mask == nullptr || !there ? nullptr : p.mask + u.b * p.mask_stride + int64_t(token) * p.drafted;
             uint32_t sees = 0;
+            if (kWindow) {
+              const int d0 = key - u.length;
+              if (there && d0 < p.drafted) {
+#pragma unroll
+                for (int y = 0; y < 32; ++y) {   // (all loads at once)
+                  const int d = d0 + y;
+                  if (d >= 0 && d < p.drafted) sees |= uint32_t(p.mask == nullptr ? d <= token : mask[d] != 0) << y;
+                }
+              }
+              if (depth >= p.window) {           // some of them may lie a window behind
+                for (uint32_t bits = sees; bits != 0; bits &= bits - 1) {
+                  if (!reaches(p, u, depth, d0 + __ffs(bits) - 1)) sees &= ~(bits & -bits);
+                }
+              }
+              if (d0 < 0) sees |= attn::Span{p.window, p.sinks}.sees(u.length + depth, key) & ((1u << -d0) - 1u);   // cached ones
+            } else {
 #pragma unroll 8
-            for (int y = 0; y < 32; ++y) {
-              const int d = first_token + x * 32 + y - u.length;
-              bool see = d < 0;
-              if (kWindow) see = sees_token<true>(p, u, mask, there ? token : -1, depth, d);
-              else if (!see && d < p.drafted && there) see = p.mask == nullptr ? d <= token : mask[d] != 0;
-              sees |= uint32_t(see) << y;
+              for (int y = 0; y < 32; ++y) {
+                const int d = key + y - u.length;
+                bool see = d < 0;
+                if (!see && d < p.drafted && there) see = p.mask == nullptr ? d <= token : mask[d] != 0;
+                sees |= uint32_t(see) << y;
+              }
             }
 #pragma unroll
             for (int y = 0; y < 32; ++y) {
