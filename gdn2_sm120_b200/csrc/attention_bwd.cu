@@ -129,8 +129,8 @@ template <bool kKeys, bool kWindow>
 __device__ __forceinline__ bool bwd_item(const BwdParams& p, int turn, BwdItem* w) {
   int64_t index = item_of_turn(turn);
   if (index >= p.items) return false;
-  w->sinks = -1;
   if (kKeys && kWindow) {
+    w->sinks = -1;
     if (index < p.sink_items) {
       const int part = int(index % p.sink_parts);
       index /= p.sink_parts;
@@ -472,9 +472,9 @@ struct KeyBars {
   int failed;
 };
 
-// A thread's share of a step in which a query's reference is far away: P and dS as below, with weights as in far_weight; the
-// key is seen by those queries that have a bit.  False where a wait ran out.
-template <typename T>
+// A thread's share of a step in which a query's reference is far away: P and dS as below, with weights as in far_weight.  `seen`
+// is the first of its queries that sees the key, or with kBits has a bit for every one that does.  False where a wait ran out.
+template <typename T, bool kBits>
 __device__ __noinline__ bool far_step(KeyBars& bar, const Waiter& waiter, uint32_t parity, uint32_t s_at, uint32_t dp_at, const float* st,
                                       const float* shifts, float c, uint32_t seen) {
   float e[32];
@@ -482,7 +482,7 @@ __device__ __noinline__ bool far_step(KeyBars& bar, const Waiter& waiter, uint32
   tc::tmem_ld32(s_at, x);
   tc::tmem_wait_ld();
 #pragma unroll
-  for (int y = 0; y < 32; ++y) e[y] = ((seen >> y) & 1) == 0 ? 0.f : far_weight(x[y], st[y], shifts + y, c);
+  for (int y = 0; y < 32; ++y) e[y] = (kBits ? ((seen >> y) & 1) == 0 : y < int(seen)) ? 0.f : far_weight(x[y], st[y], shifts + y, c);
 #pragma unroll
   for (int y = 0; y < 16; ++y) w[y] = pack_pair<T>(e[2 * y], e[2 * y + 1]);
   tc::tmem_st16(s_at, w);
@@ -495,7 +495,7 @@ __device__ __noinline__ bool far_step(KeyBars& bar, const Waiter& waiter, uint32
   tc::tmem_ld32(dp_at, x);
   tc::tmem_wait_ld();
 #pragma unroll
-  for (int y = 0; y < 32; ++y) e[y] = ((seen >> y) & 1) == 0 ? 0.f : e[y] * (__uint_as_float(x[y]) + st[128 + y]);
+  for (int y = 0; y < 32; ++y) e[y] = (kBits ? ((seen >> y) & 1) == 0 : y < int(seen)) ? 0.f : e[y] * (__uint_as_float(x[y]) + st[128 + y]);
 #pragma unroll
   for (int y = 0; y < 16; ++y) w[y] = pack_pair<T>(e[2 * y], e[2 * y + 1]);
   tc::tmem_st16(dp_at, w);
@@ -711,8 +711,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
         tc::tmem_wait_ld();
         if (far) {
           const float* shifts = p.shifts + (w.head * p.group + (w.begin + i) / w.per_head) * p.seq.stat_rows + w.at.stat + query;
-          if (!kWindow && diagonal) seen = from >= 32 ? 0u : from <= 0 ? ~0u : ~0u << from;
-          if (!(ok = far_step<T>(bar, waiter, steps & 1, s_at, dp_at, st, shifts, p.scale_log2, seen))) break;
+          if (!(ok = far_step<T, kWindow>(bar, waiter, steps & 1, s_at, dp_at, st, shifts, p.scale_log2,
+                                          kWindow ? seen : uint32_t(diagonal ? from : 0)))) break;
           continue;
         }
 #pragma unroll
