@@ -18,6 +18,10 @@
 //
 // Training 4 x 2048 tokens, 16 heads of 128 channels, 4 heads a group, each kernel by itself: delta 11 us, keys 121, queries 120, forward 73.
 
+//
+// With a window (kWindow) each of the two goes over the tiles that its rows see or are seen by, and those of the sinks: 4 x 2048
+// tokens as above, a window of 512 and 16 sinks: keys and queries 155 us together, forward 61.
+
 #include <algorithm>
 
 #include "attention_common.cuh"

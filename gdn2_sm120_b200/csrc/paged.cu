@@ -6,28 +6,8 @@
 // append_kernel   copies the keys and values of tokens to their slots (slot = page number * page size + place in the
 //                 page; a slot that is not in the cache is left out).  Bound by HBM.
 //
-// tree_kernel     N drafted tokens of each sequence, given beside the cache, see all its cached tokens and those
-//                 drafted ones that their mask row names (their ancestors in a tree of drafts); N = 1 is plain decoding:
-//
-//                   o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i),   s_ij = scale q_i . k_j,  m_i = max_j s_ij
-//
-//                 and 0 where nothing is seen.  One pass with a running maximum and sum.  The heads of a group are rows
-//                 of one product with their shared key head, so a key is read once for 256 rows (drafted tokens x heads
-//                 of a group).  Bound by HBM: the 64 KiB of a tile of 128 tokens take an SM's share of HBM 2700 clocks,
-//                 its products 1024 for up to 128 rows and 2048 for up to 256, the few rows of plain decoding too.
-//                 All (sequence, key head, block of rows, tile) are one list that the CTAs share evenly, so neither
-//                 unequal lengths nor few sequences leave SMs idle, and the host need not know the lengths.  A CTA
-//                 whose part begins or ends inside a sequence leaves (O, m, l) in the workspace; tree_join_kernel joins
-//                 these in the order of the tiles: the same inputs give the same bits.
-//
-// A CTA of tree_kernel: two chains of four warps turn scores into weights, a row a thread.  Up to 128 rows both work on the
-// same rows, on every other tile, and their (O, m, l) are joined at the end; above, each has 128 rows and all tiles.  Four
-// warps bring in keys and values, in boxes of a tiled copy where the pages allow it and row by row with 16-byte asynchronous
-// copies elsewhere; one brings queries, one issues the products.  TMEM: S0 S1 O0 O1, 128 columns each, P over S.  48 drafted
-// tokens of 8 sequences over up to 16000 cached ones, 4 heads a group (192 rows): 106 us, 3.4 TB/s (a call in a loop, with the
-// join of the parts, 128 to 132); what bounds it is a chain's round trip between the tensor cores and its warps (of an older form
-// that took 142 us, 108 remained without the copies, 116 without the weights).
-// tree_few_kernel has up to 16 rows (below).
+// Attention over it: paged_tree.cuh (drafted tokens, any number of rows), paged_tiles.cuh (up to 16 rows, and what all kernels
+// share), paged_window.cu (with a window), paged_weigh.cu (with the weights that tokens get).
 
 #include "paged_tree.cuh"
 

@@ -1,11 +1,35 @@
-// The kernels of tree attention for any number of rows, and their launches, without a window and with one.
+// Attention of drafted tokens over a paged cache: the kernel for any number of rows, the joining of what several CTAs have, and the
+// launches, without a window and with one.
+//
+// tree_kernel     N drafted tokens of each sequence, given beside the cache, see all its cached tokens and those
+//                 drafted ones that their mask row names (their ancestors in a tree of drafts); N = 1 is plain decoding:
+//
+//                   o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i),   s_ij = scale q_i . k_j,  m_i = max_j s_ij
+//
+//                 and 0 where nothing is seen.  One pass with a running maximum and sum.  The heads of a group are rows
+//                 of one product with their shared key head, so a key is read once for 256 rows (drafted tokens x heads
+//                 of a group).  Bound by HBM: the 64 KiB of a tile of 128 tokens take an SM's share of HBM 2700 clocks,
+//                 its products 1024 for up to 128 rows and 2048 for up to 256, the few rows of plain decoding too.
+//                 All (sequence, key head, block of rows, tile) are one list that the CTAs share evenly, so neither
+//                 unequal lengths nor few sequences leave SMs idle, and the host need not know the lengths.  A CTA
+//                 whose part begins or ends inside a sequence leaves (O, m, l) in the workspace; tree_join_kernel joins
+//                 these in the order of the tiles: the same inputs give the same bits.
+//
+// A CTA of tree_kernel: two chains of four warps turn scores into weights, a row a thread.  Up to 128 rows both work on the
+// same rows, on every other tile, and their (O, m, l) are joined at the end; above, each has 128 rows and all tiles.  Four
+// warps bring in keys and values, in boxes of a tiled copy where the pages allow it and row by row with 16-byte asynchronous
+// copies elsewhere; one brings queries, one issues the products.  TMEM: S0 S1 O0 O1, 128 columns each, P over S.  48 drafted
+// tokens of 8 sequences over up to 16000 cached ones, 4 heads a group (192 rows): 106 us, 3.4 TB/s (a call in a loop, with the
+// join of the parts, 128 to 132); what bounds it is a chain's round trip between the tensor cores and its warps (of an older form
+// that took 142 us, 108 remained without the copies, 116 without the weights).
+// With a window the tiles between the sinks and the first token that any row sees are passed over (which of them, the drafted tokens'
+// number does not say: their depths move the window's edge, so that a tile at the edge is masked row by row).
 #pragma once
 
 #include "paged_tiles.cuh"
 
 namespace gdn2 {
 namespace paged {
-
 
 template <int DP, int RT>   // RT: tiles of 128 rows that a CTA has, 1 or 2
 struct TreeConfig {
