@@ -73,9 +73,9 @@ _PROTOTYPES: dict[str, list] = {
     "gdn2_attention_forward": [_P] * 7 + [_I64] * 5 + [_INT, _F32, _P],
     "gdn2_attention_backward_bytes": [_P] + [_I64] * 5,
     "gdn2_attention_backward": [_P] * 12 + [_I64] * 5 + [_INT, _F32, _P],
-    "gdn2_window_attention_forward": [_P] * 7 + [_I64] * 7 + [_INT, _F32, _P],
+    "gdn2_window_attention_forward": [_P] * 8 + [_I64] * 7 + [_INT, _F32, _P],
     "gdn2_window_attention_backward_bytes": [_P] + [_I64] * 7,
-    "gdn2_window_attention_backward": [_P] * 12 + [_I64] * 7 + [_INT, _F32, _P],
+    "gdn2_window_attention_backward": [_P] * 13 + [_I64] * 7 + [_INT, _F32, _P],
     "gdn2_window_tree_attention": [_P] * 12 + [_I64] * 13 + [_INT, _F32, _P],
     "gdn2_attention_weights_bytes": [_P] + [_I64] * 4,
     "gdn2_attention_weights": [_P] * 7 + [_I64] * 5 + [_INT, _F32, _P],

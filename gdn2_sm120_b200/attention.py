@@ -67,7 +67,7 @@ def _entry(name, window):
 def _forward(q, k, v, bounds, scale, window, training):
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     if q.shape[1] == 0:
-        return out, None
+        return out, None, None
     host, n_seq, rows = _sequences(q, bounds)
     statistics = None
     if training:
@@ -77,10 +77,11 @@ def _forward(q, k, v, bounds, scale, window, training):
         statistics = torch.empty((2, q.shape[2], each), device=q.device, dtype=torch.float32)
     strides = _lib.int64s(*(s for x in (q, k, v) for s in _validate.head_strides(x)))
     name, more = _entry("attention_forward", window)
+    rest = torch.empty_like(out) if training and more else None    # what the output's rounding leaves over
     _lib.call(name, q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-              _lib.ptr(statistics), strides, host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], *more,
+              _lib.ptr(statistics), *((_lib.ptr(rest),) if more else ()), strides, host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], *more,
               _lib.dtype_code(q.dtype), scale, _lib.stream_ptr(q.device), kernels=_launches(bounds))
-    return out, statistics
+    return out, statistics, rest
 
 
 class _CausalAttention(torch.autograd.Function):
@@ -90,17 +91,17 @@ class _CausalAttention(torch.autograd.Function):
         if done is None:
             bounds, scale = _check(q, k, v, bounds, scale)
             done = _forward(*(_validate.detached(x) for x in (q, k, v)), bounds, scale, window, True)
-        out, statistics = done
-        ctx.save_for_backward(q, k, v, out, statistics)
+        out, statistics, rest = done
+        ctx.save_for_backward(q, k, v, out, statistics, rest)
         ctx.bounds, ctx.scale, ctx.window = bounds, scale, window
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        q, k, v, out, statistics = ctx.saved_tensors
+        q, k, v, out, statistics, rest = ctx.saved_tensors
         if statistics is not None and _lib.KERNEL_EVENTS is None:
-            done = _lib.host().attention_backward(q, k, v, out, statistics, d_out, ctx.bounds, ctx.scale, *ctx.window)
+            done = _lib.host().attention_backward(q, k, v, out, statistics, d_out, ctx.bounds, ctx.scale, *ctx.window, rest)
             if done is not None:
                 return (*done, None, None, None)
         scale = _validate.float32_scale(ctx.scale, q.shape[3])
@@ -120,14 +121,14 @@ class _CausalAttention(torch.autograd.Function):
             _lib.check(int(size), name + "_bytes")
         scratch = torch.empty(size, device=q.device, dtype=torch.uint8)
         _lib.call(name, q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                  d_out.data_ptr(), statistics.data_ptr(), scratch.data_ptr(), *(x.data_ptr() for x in grads), strides,
+                  *((_lib.ptr(rest),) if more else ()), d_out.data_ptr(), statistics.data_ptr(), scratch.data_ptr(), *(x.data_ptr() for x in grads), strides,
                   host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], *more, _lib.dtype_code(q.dtype), scale,
                   _lib.stream_ptr(q.device), kernels=(3 + (size > 2 * statistics.numel() + 15)) * _launches(ctx.bounds))
         return (*grads, None, None, None)
 
 
 def _native(q, k, v, bounds, scale, window, training):
-    """The call on the native host path, ``(output, statistics)``; None where it is not the plain case."""
+    """The call on the native host path, ``(output, statistics, rest)``; None where it is not the plain case."""
 
     if _lib.KERNEL_EVENTS is not None or not getattr(q, "is_cuda", False):
         return None

@@ -27,10 +27,10 @@ namespace attn {
 static std::atomic<uint32_t> g_wait_polls{GDN2_ATTENTION_WAIT_POLLS};
 uint32_t wait_polls() { return g_wait_polls.load(std::memory_order_relaxed); }
 int64_t attention_stat_rows(const int64_t*, int64_t, int64_t);
-int launch_attention_forward(const void*, const void*, const void*, void*, float*, const int64_t*, const int64_t*, int64_t,
+int launch_attention_forward(const void*, const void*, const void*, void*, float*, void*, const int64_t*, const int64_t*, int64_t,
                              int64_t, int, int, int, int, float, int64_t, int64_t, cudaStream_t);
 int64_t attention_backward_bytes(const int64_t*, int64_t, int64_t, int, int, int, int64_t, int64_t);
-int launch_attention_backward(const void*, const void*, const void*, const void*, const void*, const float*, void*, void*,
+int launch_attention_backward(const void*, const void*, const void*, const void*, const void*, const void*, const float*, void*, void*,
                               void*, void*, const int64_t*, const int64_t*, int64_t, int64_t, int, int, int, int, float,
                               int64_t, int64_t, cudaStream_t);
 int64_t attention_weights_bytes(const int64_t*, int64_t, int64_t, int, int);
@@ -115,7 +115,7 @@ int check_weighed(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads
 }
 
 // Causal attention, with a window of 0 for none
-int attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics, const int64_t* strides,
+int attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics, void* rest, const int64_t* strides,
                       const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads, int64_t dim,
                       int64_t window, int64_t sinks, int dtype, float scale, void* stream) {
   if (!q || !k || !v || !out || !strides) return GDN2_ERR_NULL_POINTER;
@@ -124,11 +124,11 @@ int attention_forward(const void* q, const void* k, const void* v, void* out, fl
   if (!valid_seq_dtype(dtype)) return GDN2_ERR_BAD_DTYPE;
   if ((status = check_sequences(bounds, n_seq, time, heads)) != GDN2_OK) return status;
   if ((status = check_strides(strides, 9)) != GDN2_OK) return status;
-  const void* need16[] = {q, k, v, out, statistics};
+  const void* need16[] = {q, k, v, out, statistics, rest};
   for (const void* p : need16) {
     if (!aligned(p, 16)) return GDN2_ERR_ALIGNMENT;
   }
-  return attn::launch_attention_forward(q, k, v, out, statistics, strides, bounds, n_seq, time, int(heads), int(kv_heads),
+  return attn::launch_attention_forward(q, k, v, out, statistics, rest, strides, bounds, n_seq, time, int(heads), int(kv_heads),
                                         int(dim), dtype, scale, window, sinks, static_cast<cudaStream_t>(stream));
 }
 
@@ -139,7 +139,7 @@ int64_t attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t t
   return status != GDN2_OK ? status : attn::attention_backward_bytes(bounds, n_seq, time, int(heads), int(kv_heads), int(dim), window, sinks);
 }
 
-int attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out, const float* statistics,
+int attention_backward(const void* q, const void* k, const void* v, const void* out, const void* rest, const void* d_out, const float* statistics,
                        void* scratch, void* dq, void* dk, void* dv, const int64_t* strides, const int64_t* bounds, int64_t n_seq,
                        int64_t time, int64_t heads, int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks, int dtype,
                        float scale, void* stream) {
@@ -151,11 +151,11 @@ int attention_backward(const void* q, const void* k, const void* v, const void* 
   if (!valid_seq_dtype(dtype)) return GDN2_ERR_BAD_DTYPE;
   if ((status = check_sequences(bounds, n_seq, time, heads)) != GDN2_OK) return status;
   if ((status = check_strides(strides, 12)) != GDN2_OK) return status;
-  const void* need16[] = {q, k, v, out, d_out, statistics, scratch, dq, dk, dv};
+  const void* need16[] = {q, k, v, out, rest, d_out, statistics, scratch, dq, dk, dv};
   for (const void* p : need16) {
     if (!aligned(p, 16)) return GDN2_ERR_ALIGNMENT;
   }
-  return attn::launch_attention_backward(q, k, v, out, d_out, statistics, scratch, dq, dk, dv, strides, bounds, n_seq, time,
+  return attn::launch_attention_backward(q, k, v, out, rest, d_out, statistics, scratch, dq, dk, dv, strides, bounds, n_seq, time,
                                          int(heads), int(kv_heads), int(dim), dtype, scale, window, sinks,
                                          static_cast<cudaStream_t>(stream));
 }
@@ -237,7 +237,7 @@ int64_t gdn2_attention_stat_rows(const int64_t* bounds, int64_t n_seq, int64_t t
 int gdn2_attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics,
                            const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads,
                            int64_t kv_heads, int64_t dim, int dtype, float scale, void* stream) {
-  return attention_forward(q, k, v, out, statistics, strides, bounds, n_seq, time, heads, kv_heads, dim, 0, 0, dtype, scale, stream);
+  return attention_forward(q, k, v, out, statistics, nullptr, strides, bounds, n_seq, time, heads, kv_heads, dim, 0, 0, dtype, scale, stream);
 }
 
 int64_t gdn2_attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads,
@@ -249,16 +249,16 @@ int gdn2_attention_backward(const void* q, const void* k, const void* v, const v
                             const float* statistics, void* scratch, void* dq, void* dk, void* dv, const int64_t* strides,
                             const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads, int64_t dim,
                             int dtype, float scale, void* stream) {
-  return attention_backward(q, k, v, out, d_out, statistics, scratch, dq, dk, dv, strides, bounds, n_seq, time, heads, kv_heads, dim,
+  return attention_backward(q, k, v, out, nullptr, d_out, statistics, scratch, dq, dk, dv, strides, bounds, n_seq, time, heads, kv_heads, dim,
                             0, 0, dtype, scale, stream);
 }
 
-int gdn2_window_attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics,
+int gdn2_window_attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics, void* rest,
                                   const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads,
                                   int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks, int dtype, float scale,
                                   void* stream) {
   if (window <= 0 || sinks < 0) return GDN2_ERR_BAD_RANGE;
-  return attention_forward(q, k, v, out, statistics, strides, bounds, n_seq, time, heads, kv_heads, dim, window, sinks, dtype, scale,
+  return attention_forward(q, k, v, out, statistics, rest, strides, bounds, n_seq, time, heads, kv_heads, dim, window, sinks, dtype, scale,
                            stream);
 }
 
@@ -268,12 +268,12 @@ int64_t gdn2_window_attention_backward_bytes(const int64_t* bounds, int64_t n_se
   return attention_backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, window, sinks);
 }
 
-int gdn2_window_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out,
-                                   const float* statistics, void* scratch, void* dq, void* dk, void* dv, const int64_t* strides,
+int gdn2_window_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* rest,
+                                   const void* d_out, const float* statistics, void* scratch, void* dq, void* dk, void* dv, const int64_t* strides,
                                    const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads, int64_t kv_heads,
                                    int64_t dim, int64_t window, int64_t sinks, int dtype, float scale, void* stream) {
   if (window <= 0 || sinks < 0) return GDN2_ERR_BAD_RANGE;
-  return attention_backward(q, k, v, out, d_out, statistics, scratch, dq, dk, dv, strides, bounds, n_seq, time, heads, kv_heads, dim,
+  return attention_backward(q, k, v, out, rest, d_out, statistics, scratch, dq, dk, dv, strides, bounds, n_seq, time, heads, kv_heads, dim,
                             window, sinks, dtype, scale, stream);
 }
 

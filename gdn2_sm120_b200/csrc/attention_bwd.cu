@@ -19,8 +19,11 @@
 // Training 4 x 2048 tokens, 16 heads of 128 channels, 4 heads a group, each kernel by itself: delta 11 us, keys 121, queries 120, forward 73.
 
 //
-// With a window (kWindow) each of the two goes over the tiles that its rows see or are seen by, and those of the sinks: 4 x 2048
-// tokens as above, a window of 512 and 16 sinks: keys and queries 155 us together, forward 61.
+// With a window (kWindow) delta is taken from the output and what its rounding has left over: where rows see few tokens delta's
+// own error counts most.  Gradients' errors in the 2-norm without it and with it, in roundings: a window of 2 tokens 2.3 and 1.5, 4
+// 1.8 and 1.5, 10 1.6 and 1.45, 100 1.48 and 1.43; it costs 13 us of the 242 of the training step below (in 8 bits, whose rows are
+// half sectors, 18).  Each of the two goes over the tiles that its rows see or are seen by, and those of the sinks: 4 x 2048
+// tokens as above, a window of 512 and 16 sinks: keys and queries 155 us together, forward 69, delta 16.
 
 #include <algorithm>
 
@@ -818,14 +821,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_keys_kernel(const __gri
 // -delta_i = -do_i . o_i in 32 bits, 0 for the rows behind a sequence's end: a CTA has 64 rows of a head, half a warp a row
 constexpr int kDeltaRows = 64;
 struct DeltaParams {
-  const void *out, *d_out;
+  const void *out, *d_out, *rest;   // rest: what the rounding of `out` has left over, or null
   int64_t do_stride[3];
   float* delta;
   int heads, dim;
   Sequences seq;
 };
 
-template <typename T>
+template <typename T, bool kRest>
 __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ DeltaParams p) {
   let_others_begin();
   const int unit = int(blockIdx.x) / p.heads, head = int(blockIdx.x) - unit * p.heads;
@@ -833,24 +836,27 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
   const int first = it.tile * kTileRows + unit % (kTileRows / kDeltaRows) * kDeltaRows;
   const int part = threadIdx.x & 15, group = threadIdx.x >> 4;
   constexpr int kEach = kDeltaRows / 16;
-  uint4 a[kEach], b[kEach];
+  uint4 a[kEach], b[kEach], c[kEach];
 #pragma unroll
   for (int x = 0; x < kEach; ++x) {
     const int i = first + x * 16 + group;
-    a[x] = b[x] = make_uint4(0, 0, 0, 0);
+    a[x] = b[x] = c[x] = make_uint4(0, 0, 0, 0);
     if (i < it.len && part * 8 < p.dim) {
       a[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + ((it.row + i) * p.heads + head) * p.dim + part * 8);
       b[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.d_out) + it.batch * p.do_stride[0] + int64_t(it.row0 + i) * p.do_stride[1] +
                                              head * p.do_stride[2] + part * 8);
+      if (kRest) c[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.rest) + ((it.row + i) * p.heads + head) * p.dim + part * 8);
     }
   }
 #pragma unroll
   for (int x = 0; x < kEach; ++x) {
-    const uint32_t aw[4] = {a[x].x, a[x].y, a[x].z, a[x].w}, bw[4] = {b[x].x, b[x].y, b[x].z, b[x].w};
+    const uint32_t aw[4] = {a[x].x, a[x].y, a[x].z, a[x].w}, bw[4] = {b[x].x, b[x].y, b[x].z, b[x].w}, cw[4] = {c[x].x, c[x].y, c[x].z, c[x].w};
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 u = unpack2<T>(aw[j]), v = unpack2<T>(bw[j]);
+      float2 u = unpack2<T>(aw[j]);
+      const float2 v = unpack2<T>(bw[j]);
+      if (kRest) u = add2(u, unpack2<T>(cw[j]));
       sum = fmaf(u.x, v.x, sum);
       sum = fmaf(u.y, v.y, sum);
     }
@@ -911,7 +917,9 @@ int launch_half(Kernel kernel, int bytes, const BwdParams& base, int64_t items, 
 
 template <typename T, int DP, bool kWindow>
 int launch_typed(BwdParams& p, const DeltaParams& d, cudaStream_t stream) {
-  attention_delta_kernel<T><<<unsigned(p.seq.tiles * (kTileRows / kDeltaRows) * p.heads), 256, 0, stream>>>(d);
+  const unsigned ctas = unsigned(p.seq.tiles * (kTileRows / kDeltaRows) * p.heads);
+  if (kWindow && d.rest != nullptr) attention_delta_kernel<T, true><<<ctas, 256, 0, stream>>>(d);
+  else attention_delta_kernel<T, false><<<ctas, 256, 0, stream>>>(d);
   int status = check_launch();
   if (status != GDN2_OK) return status;
   const int64_t tiles = int64_t(p.seq.tiles) * 2;
@@ -921,9 +929,9 @@ int launch_typed(BwdParams& p, const DeltaParams& d, cudaStream_t stream) {
   status = launch_half(&attention_queries_kernel<T, DP, kWindow>, QueryConfig<DP>::kBytes, p, tiles * p.heads, stream);
   if (status != GDN2_OK) return status;
   const unsigned per_tile = unsigned((int64_t(128) * p.kv_heads * (p.dim / 4) + 255) / 256);
-  const int64_t ctas = (p.parts > 1 ? tiles : 0) + (p.sink_parts > 1 ? int64_t(p.seq.n) * p.sink_tiles : 0);
-  if (ctas == 0) return GDN2_OK;
-  attention_parts_kernel<T, kWindow><<<dim3(unsigned(ctas), per_tile), 256, 0, stream>>>(p);
+  const int64_t joined = (p.parts > 1 ? tiles : 0) + (p.sink_parts > 1 ? int64_t(p.seq.n) * p.sink_tiles : 0);
+  if (joined == 0) return GDN2_OK;
+  attention_parts_kernel<T, kWindow><<<dim3(unsigned(joined), per_tile), 256, 0, stream>>>(p);
   return check_launch();
 }
 
@@ -987,7 +995,7 @@ int64_t attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t t
 
 int64_t attention_stat_rows(const int64_t* bounds, int64_t n_seq, int64_t time) { return stat_rows(bounds, n_seq, time); }
 
-int launch_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out,
+int launch_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* rest, const void* d_out,
                               const float* lse, void* scratch, void* dq, void* dk, void* dv, const int64_t* strides,
                               const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, int dim,
                               int dtype, float scale, int64_t window, int64_t sinks, cudaStream_t stream) {
@@ -1022,7 +1030,7 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   p.wide = wide_rows(dq, dim) && wide_rows(dk, dim) && wide_rows(dv, dim);
   p.scale_log2 = positive_scale(scale);
   return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {
-    DeltaParams d{out, d_out, {strides[9], strides[10], strides[11]}, delta, heads, dim, p.seq};
+    DeltaParams d{out, d_out, rest, {strides[9], strides[10], strides[11]}, delta, heads, dim, p.seq};
     return dtype == GDN2_BF16 ? launch_dim<__nv_bfloat16>(p, d, stream) : launch_dim<__half>(p, d, stream);
   });
 }

@@ -47,6 +47,7 @@ struct FwdParams {
   int64_t strides[3];  // of the values: batch, token and head, in elements
   void* out;
   float* lse;          // [heads][stat rows]: -(m + log2 l) in powers of two, then far references; or null
+  void* rest;          // with a window: what the rounding of `out` has left over, in the same type; or null
   int heads, kv_heads, group, dim, turns;
   int64_t items;
   float scale_log2;    // positive
@@ -440,6 +441,17 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
           strange = fmaf(o[y], 0.f, strange);
         }
         if (there) store_row16<T>(to + col0 + x, o, inv, p.dim - col0 - x, p.wide);
+        if (kWindow && there && p.rest != nullptr) {
+          T* left = static_cast<T*>(p.rest) + (to - static_cast<T*>(p.out)) + col0 + x;
+          // (of an output that is not finite something that is not either: its row's gradients are none in any case)
+#pragma unroll
+          for (int y = 0; y < 16; y += 2) {
+            const float2 v = mul2(make_float2(o[y], o[y + 1]), twice(inv)), r = minus2(v, unpack2<T>(pack_pair<T>(v.x, v.y)));
+            o[y] = r.x;
+            o[y + 1] = r.y;
+          }
+          store_row16<T>(left, o, 1.f, p.dim - col0 - x, p.wide);
+        }
       }
       if (!kAgain) {
         if (strange != 0.f && there && ok && isfinite(sum)) atomicOr(&marks.again[(turn >> 5) & 31], 1u << (turn & 31));
@@ -541,7 +553,7 @@ int launch_dim(const FwdParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-int launch_attention_forward(const void* q, const void* k, const void* v, void* out, float* lse, const int64_t* strides,
+int launch_attention_forward(const void* q, const void* k, const void* v, void* out, float* lse, void* rest, const int64_t* strides,
                              const int64_t* bounds, int64_t n_seq, int64_t time, int heads, int kv_heads, int dim,
                              int dtype, float scale, int64_t window, int64_t sinks, cudaStream_t stream) {
   FwdParams p;
@@ -553,11 +565,11 @@ int launch_attention_forward(const void* q, const void* k, const void* v, void* 
   }
   p.values = v;
   for (int i = 0; i < 3; ++i) p.strides[i] = strides[6 + i];
-  p.out = out; p.lse = lse;
+  p.out = out; p.lse = lse; p.rest = rest;
   p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.dim = dim;
   p.negate = scale < 0.f;
   p.polls = wait_polls();
-  p.wide = wide_rows(out, dim);
+  p.wide = wide_rows(out, dim) && wide_rows(rest, dim);
   p.scale_log2 = positive_scale(scale);
   p.span = span_of(window, sinks, bounds, n_seq, time);
   return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {

@@ -941,7 +941,7 @@ PyObject* evict_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_CATCH
 }
 
-// attention_forward(q, k, v, bounds, scale, window, sinks, training) -> (output, statistics or None) or None
+// attention_forward(q, k, v, bounds, scale, window, sinks, training) -> (output, statistics or None, rest or None) or None
 PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_TRY
   Heads h;
@@ -956,7 +956,7 @@ PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor& q = *h.t[0];
   const int64_t* host = bounds.empty() ? nullptr : bounds.data();
   const int64_t n_seq = bounds.empty() ? h.batch : int64_t(bounds.size()) - 1;
-  at::Tensor out, statistics;
+  at::Tensor out, statistics, rest;
   int status;
   int64_t rows = 0;
   WithoutGil others;
@@ -968,17 +968,20 @@ PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   out = at::empty(q.sizes(), q.options());
   if (training) statistics = floats({2, h.heads, rows}, q);
   float* stat = training ? fptr(&statistics) : nullptr;
+  const bool keeps = training && window > 0;
+  if (keeps) rest = at::empty(q.sizes(), q.options());
   void* stream = at::cuda::getCurrentCUDAStream().stream();
   status = window == 0
                ? api.attention_forward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out.data_ptr(), stat, h.strides, host,
                                        n_seq, h.time, h.heads, h.kv_heads, h.dim, h.dtype, scale, stream)
-               : api.window_attention_forward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out.data_ptr(), stat, h.strides,
-                                              host, n_seq, h.time, h.heads, h.kv_heads, h.dim, window, sinks, h.dtype, scale, stream);
+               : api.window_attention_forward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out.data_ptr(), stat,
+                                              keeps ? rest.data_ptr() : nullptr, h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim, window, sinks, h.dtype, scale, stream);
   others.end();
   if (!ok(status, window == 0 ? "gdn2_attention_forward" : "gdn2_window_attention_forward", passes(bounds))) return nullptr;
-  PyObject* result = PyTuple_New(2);
+  PyObject* result = PyTuple_New(3);
   PyTuple_SET_ITEM(result, 0, wrap(out));
   PyTuple_SET_ITEM(result, 1, training ? wrap(statistics) : Py_NewRef(Py_None));
+  PyTuple_SET_ITEM(result, 2, keeps ? wrap(rest) : Py_NewRef(Py_None));
   return result;
   GDN2_CATCH
 }
@@ -1026,14 +1029,14 @@ PyObject* weighed_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_CATCH
 }
 
-// attention_backward(q, k, v, output, statistics, d_output, bounds, scale, window, sinks) -> (dq, dk, dv) or None
+// attention_backward(q, k, v, output, statistics, d_output, bounds, scale, window, sinks, rest) -> (dq, dk, dv) or None
 PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_TRY
   Heads h;
   float scale;
   std::vector<int64_t> bounds;
   int64_t window, sinks;
-  if (!g_bound || n != 10 || !read_heads(a, &h) || !read_bounds(a[6], h, &bounds) || !read_attention_scale(a[7], h.dim, &scale) ||
+  if (!g_bound || n != 11 || !read_heads(a, &h) || !read_bounds(a[6], h, &bounds) || !read_attention_scale(a[7], h.dim, &scale) ||
       !read_window(a + 8, &window, &sinks)) {
     return none();
   }
@@ -1043,6 +1046,8 @@ PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       d_out->scalar_type() != q.scalar_type() || d_out->device() != q.device() || !aligned_rows(*d_out, h.strides + 9)) {
     return none();
   }
+  const at::Tensor* rest = a[10] == Py_None ? nullptr : dense(a[10], 4, q.scalar_type(), q);
+  if (a[10] != Py_None && (rest == nullptr || window == 0 || rest->sizes() != q.sizes())) return none();
   const int64_t* host = bounds.empty() ? nullptr : bounds.data();
   const int64_t n_seq = bounds.empty() ? h.batch : int64_t(bounds.size()) - 1;
   at::Tensor grads[3];
@@ -1064,8 +1069,8 @@ PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                         fptr(statistics), scratch.data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(),
                                         grads[2].data_ptr(), h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim, h.dtype, scale,
                                         stream)
-               : api.window_attention_backward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out->data_ptr(), d_out->data_ptr(),
-                                               fptr(statistics), scratch.data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(),
+               : api.window_attention_backward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out->data_ptr(),
+                                               rest == nullptr ? nullptr : rest->data_ptr(), d_out->data_ptr(), fptr(statistics), scratch.data_ptr(), grads[0].data_ptr(), grads[1].data_ptr(),
                                                grads[2].data_ptr(), h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim, window,
                                                sinks, h.dtype, scale, stream);
   others.end();

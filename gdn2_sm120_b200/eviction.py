@@ -44,7 +44,7 @@ def _weighed(what, q, k, v, bounds, scale):
     checked, scale = _check(q, k, v, bounds, scale)
     _refuse_gradients(what, q, k, v)
     q, k, v = (_validate.detached(x) for x in (q, k, v))
-    out, statistics = _forward(q, k, v, checked, scale, (0, 0), True)
+    out, statistics, _ = _forward(q, k, v, checked, scale, (0, 0), True)
     weights = torch.empty(k.shape[:3], device=k.device, dtype=torch.float32)
     if statistics is None:
         return out, weights

@@ -9,7 +9,7 @@ ones as far as they are not behind it.
 
 The first two are differentiable and run on the kernels of causal attention (csrc/attention_fwd.cu, csrc/attention_bwd.cu), which pass over
 the tiles that no row of theirs sees; what is said in attention.py about types, heads, roundings and values that are not finite
-holds here, with tiles that the window's edge or the sinks' end crosses beside those on the diagonal.  A window that reaches over
+holds here (but for delta, which is taken from the output and what its rounding left over, which is kept for the backward), with tiles that the window's edge or the sinks' end crosses beside those on the diagonal.  A window that reaches over
 the longest sequence is causal attention, bit for bit.
 """
 

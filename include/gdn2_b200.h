@@ -510,16 +510,18 @@ int gdn2_attention_backward(const void* q, const void* k, const void* v, const v
 /*
  * The same with a sliding window: token i sees the tokens j <= i with i - j < window, itself among them, and the first
  * `sinks` of its sequence (those that are not behind it).  window >= 1, sinks >= 0.  A window that reaches over the
- * longest sequence is causal attention and gives its bits.
+ * longest sequence is causal attention and gives its bits.  `rest` (NULL: not wanted), like `out`, gets what the rounding
+ * of `out` has left over; a backward that has it takes the sums of d_out and out from both, which matters where tokens see
+ * few others.  (Neither is read or written where the window reaches over all.)
  */
 int gdn2_window_attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics,
-                                  const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time,
+                                  void* rest, const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time,
                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks,
                                   int dtype, float scale, void* stream);
 int64_t gdn2_window_attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t time, int64_t heads,
                                              int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks);
-int gdn2_window_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* d_out,
-                                   const float* statistics, void* scratch, void* dq, void* dk, void* dv,
+int gdn2_window_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* rest,
+                                   const void* d_out, const float* statistics, void* scratch, void* dq, void* dk, void* dv,
                                    const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time,
                                    int64_t heads, int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks,
                                    int dtype, float scale, void* stream);

@@ -35,9 +35,9 @@ def test_entry_points_reject_bad_windows_without_a_gpu():
     handle, one = _lib.lib(), ctypes.c_void_p(256)
     strides = _lib.int64s(*[64] * 12)
     for window, sinks in ((0, 0), (-1, 0), (1, -1)):
-        assert handle.gdn2_window_attention_forward(*[one] * 4, None, strides, None, 1, 8, 1, 1, 64, window, sinks, 0, 1.0, None) == -4
-        assert handle.gdn2_window_attention_backward(*[one] * 10, strides, None, 1, 8, 1, 1, 64, window, sinks, 0, 1.0, None) == -4
+        assert handle.gdn2_window_attention_forward(*[one] * 4, None, None, strides, None, 1, 8, 1, 1, 64, window, sinks, 0, 1.0, None) == -4
+        assert handle.gdn2_window_attention_backward(*[one] * 11, strides, None, 1, 8, 1, 1, 64, window, sinks, 0, 1.0, None) == -4
         assert handle.gdn2_window_attention_backward_bytes(None, 1, 8, 1, 1, 64, window, sinks) == -4
-    assert handle.gdn2_window_attention_forward(*[None] * 5, strides, None, 1, 8, 1, 1, 64, 4, 0, 0, 1.0, None) == -1
-    assert handle.gdn2_window_attention_forward(*[one] * 4, None, strides, None, 1, 8, 1, 1, 60, 4, 0, 0, 1.0, None) == -2
-    assert handle.gdn2_window_attention_forward(*[one] * 4, None, strides, None, 1, 8, 1, 1, 64, 4, 0, 2, 1.0, None) == -3
+    assert handle.gdn2_window_attention_forward(*[None] * 6, strides, None, 1, 8, 1, 1, 64, 4, 0, 0, 1.0, None) == -1
+    assert handle.gdn2_window_attention_forward(*[one] * 4, None, None, strides, None, 1, 8, 1, 1, 60, 4, 0, 0, 1.0, None) == -2
+    assert handle.gdn2_window_attention_forward(*[one] * 4, None, None, strides, None, 1, 8, 1, 1, 64, 4, 0, 2, 1.0, None) == -3
