@@ -193,3 +193,30 @@ def test_two_calls_at_once():
     torch.cuda.synchronize()
     for j in range(2):
         assert all(torch.equal(x, want[j]) for x in got[j]) and torch.equal(weights[j], kept[j])
+
+
+@pytest.mark.slow
+def test_offsets_beyond_32_bits():
+    """A cache of more than 2^32 bytes and 2^31 elements, of which the last pages are used; the same in a small cache."""
+
+    page, kv_heads, dim, used = 64, 4, 128, 40
+    pages = 2 ** 31 // (page * kv_heads * dim) + 2 * used
+    small = [_normal(2 * used, page, kv_heads, dim, seed=1 + i) for i in range(2)]
+    small.append(torch.rand(2 * used, kv_heads, page, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV))
+    large = [torch.zeros(pages, *x.shape[1:], device=DEV, dtype=x.dtype) for x in small]
+    for x, y in zip(large, small):
+        x[-2 * used:] = y
+    table = torch.randperm(used, generator=torch.Generator(device=DEV).manual_seed(4), device=DEV).int().view(2, 20)
+    lengths = torch.tensor([1200, 777], device=DEV, dtype=torch.int32)
+    q, k, v = _normal(2, 1, 16, dim, seed=5), _normal(2, 1, kv_heads, dim, seed=6), _normal(2, 1, kv_heads, dim, seed=7)
+    results = []
+    for cache, first in ((small, 0), (large, pages - 2 * used)):
+        at = table + first
+        slots = at.long().gather(1, lengths.long()[:, None] // page) * page + lengths.long()[:, None] % page
+        new = torch.arange(used, used + 10, device=DEV, dtype=torch.int32).view(2, 5) + first
+        out = [weighed_token_attention(q, k, v, *cache, at, lengths, slots), window_tree_attention(q, k, v, *cache[:2], at, lengths, 300, sinks=70)]
+        append_tokens(k, v, *cache[:2], slots)
+        out.append(evict_tokens(*cache, at, lengths, new, 300, sinks=2, recent=30))
+        results.append(out + [x[first:] for x in cache])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert not any(x[:-2 * used].any() for x in large)
