@@ -9,7 +9,7 @@
 //                 room (49152), and are read once more for every pass otherwise.
 // gather_kernel   copies keys, values and weights, 8 tokens of a head a warp.  Bound by HBM.
 //
-// 8 sequences of up to 16384 tokens, 8 heads of 128 channels, 4096 kept: 14.5 and 50 us, the latter 5.4 TB/s both ways in pieces
+// 8 sequences of up to 16384 tokens, 8 heads of 128 channels, 4096 kept: 14.5 and 46 us, the latter 5.9 TB/s both ways in pieces
 // of 256 bytes that lie where the weights have them.  What select_kernel takes is latency: 64 CTAs, of 24 thousand clocks 7
 // for the weights' arrival, 4 for the first pass, 5 for what is left of it, 5 for the tokens' numbers.  (Two or four CTAs of a cluster
 // for a sequence and head 41 us, where their barriers and one another's bins took more than they saved.)
@@ -26,6 +26,7 @@ constexpr int kSelectThreads = 1024;
 constexpr int kBins = 2048, kBinBits = 11;
 constexpr int kAll = 0x7fffffff;
 constexpr int kCached = 49152;        // weights that stay in shared memory
+constexpr int kAtOnce = 4;            // pieces of keys, and of values, that a lane has under way
 constexpr int kGatherThreads = 256, kGatherWarp = 8, kGatherTokens = kGatherThreads / 32 * kGatherWarp;
 constexpr int kListed = 512;          // candidates near the border that are compared with one another
 
@@ -271,9 +272,11 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const __grid_
   }
 }
 
-// A warp has 8 tokens of a head, wherever they are: nothing but its own loads stands between it and the next one's.
+// A warp has 8 tokens of a head, wherever they are: nothing but its own loads stands between it and the next one's.  (8 sequences as
+// above: pieces of keys and of values at the same places of both 46 us, one after the other 50; 16 tokens a warp 47, more warps with
+// fewer registers 53 to 55.)
 template <typename P>
-__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_constant__ EvictParams p) {
+__global__ void __launch_bounds__(kGatherThreads, 4) gather_kernel(const __grid_constant__ EvictParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // the heads of 64 places are written one beside the other
   const int head = int(blockIdx.x) % p.kv_heads, chunk = int(blockIdx.x) / p.kv_heads % p.chunks, b = int(blockIdx.x) / p.kv_heads / p.chunks;
@@ -294,25 +297,28 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_con
       to = (int64_t(page) * p.page + j_place) * p.kv_heads + head;
     }
   }
-  constexpr int kAtOnce = 8;
-  const int packs = kGatherWarp * p.per_row;   // of keys, then of values
-  for (int x0 = 0; x0 < 2 * packs; x0 += kAtOnce * 32) {
-    P data[kAtOnce];
+  from *= p.per_row;
+  to *= p.per_row;   // (of -1 something below 0)
+  const int packs = kGatherWarp * p.per_row;
+  for (int x0 = 0; x0 < packs; x0 += kAtOnce * 32) {
+    P key[kAtOnce], value[kAtOnce];
     int64_t place[kAtOnce];
 #pragma unroll
     for (int y = 0; y < kAtOnce; ++y) {
-      const int x = x0 + y * 32 + lane, z = x < packs ? x : x - packs, row = min(p.by_row.quotient(z), kGatherWarp - 1);
-      const int64_t source = __shfl_sync(0xffffffffu, from, row);
+      const int x = x0 + y * 32 + lane, row = min(p.by_row.quotient(x), kGatherWarp - 1), pack = x - row * p.per_row;
+      const int64_t source = __shfl_sync(0xffffffffu, from, row) + pack;
       place[y] = __shfl_sync(0xffffffffu, to, row);
-      const int pack = z - row * p.per_row;
-      if (x >= 2 * packs) place[y] = -1;
+      if (x >= packs) place[y] = -1;
       if (place[y] < 0) continue;
-      place[y] = place[y] * p.per_row + pack;
-      data[y] = reinterpret_cast<const P*>(x < packs ? p.k_pages : p.v_pages)[source * p.per_row + pack];
+      place[y] += pack;
+      key[y] = reinterpret_cast<const P*>(p.k_pages)[source];
+      value[y] = reinterpret_cast<const P*>(p.v_pages)[source];
     }
 #pragma unroll
     for (int y = 0; y < kAtOnce; ++y) {
-      if (place[y] >= 0) reinterpret_cast<P*>(x0 + y * 32 + lane < packs ? p.k_pages : p.v_pages)[place[y]] = data[y];
+      if (place[y] < 0) continue;
+      reinterpret_cast<P*>(p.k_pages)[place[y]] = key[y];
+      reinterpret_cast<P*>(p.v_pages)[place[y]] = value[y];
     }
   }
 }
