@@ -164,9 +164,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_weights_kernel(const __
   tc::tc_fence_after();
   const uint32_t tmem = bar.tmem;
   const Waiter waiter{&bar.failed, p.polls};
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the forward's statistics
+  let_others_begin();
 
   if (warp == 4 * kSets + 1) {
     // ---- copies --------------------------------------------------------------------------------------------
+    tc::fence_async_all();   // they were written by threads, and are read by bulk copies
     const uint32_t leader = tc::elect_leader();
     int filled = 0, items = 0;
     bool ok = true;
@@ -295,9 +298,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_weights_kernel(const __
 
 // Sums of an item's parts, in their order: a thread a key and head
 __global__ void __launch_bounds__(256) attention_weights_parts_kernel(const __grid_constant__ WeightParams p) {
-  const int x = int(blockIdx.y) * blockDim.x + threadIdx.x;   // (row of the tile, kv head)
-  const Item it = find_item(p.seq, int(blockIdx.x) >> 1, false);
-  const int tile = 2 * it.tile + (int(blockIdx.x) & 1), i = tile * 128 + x / p.kv_heads;
+  const int per_tile = (128 * p.kv_heads + 255) / 256, unit = int(blockIdx.x) / per_tile;
+  const int x = (int(blockIdx.x) - unit * per_tile) * int(blockDim.x) + int(threadIdx.x);   // (row of the tile, kv head)
+  const Item it = find_item(p.seq, unit >> 1, false);
+  const int tile = 2 * it.tile + (unit & 1), i = tile * 128 + x / p.kv_heads;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (i >= it.len || x >= 128 * p.kv_heads) return;
   const int64_t at = (it.row + tile * 128) * p.kv_heads + x;
   const int steps = ((it.len + 127) / 128 - tile) * p.group;
@@ -321,11 +326,12 @@ int launch_typed(const WeightParams& base, cudaStream_t stream) {
   p.items = tiles * p.kv_heads * p.parts;
   const int64_t grid = p.items < sms ? p.items : sms;
   p.turns = int((p.items + grid - 1) / grid);
-  attention_weights_kernel<T, DP><<<unsigned(grid), kThreads, C::kBytes, stream>>>(p);
-  status = check_launch();
+  // each is there when the one before it ends: 20 short packed prompts 37 us and not 39.5
+  status = launch_beside(&attention_weights_kernel<T, DP>, unsigned(grid), kThreads, C::kBytes, stream, p);
   if (status != GDN2_OK || p.parts == 1) return status;
-  attention_weights_parts_kernel<<<dim3(unsigned(tiles), unsigned((128 * p.kv_heads + 255) / 256)), 256, 0, stream>>>(p);
-  return check_launch();
+  const int64_t ctas = tiles * ((128 * p.kv_heads + 255) / 256);
+  if (ctas > int64_t(0x7fffffff)) return GDN2_ERR_TOO_LARGE;
+  return launch_beside(&attention_weights_parts_kernel, unsigned(ctas), 256, 0, stream, p);
 }
 
 // Parts of an item, as of the backward's items of keys: as many as bring the longest one down to an SM's share
