@@ -989,7 +989,7 @@ int64_t attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t t
                                  int64_t sinks) {
   KeyParts k;
   BackwardBytes bytes;
-  const int status = backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, span_of(window, sinks, bounds, n_seq, time), &k, &bytes);
+  const int status = backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, span_of(window, sinks, bounds, n_seq, time, true), &k, &bytes);
   return status != GDN2_OK ? status : bytes.delta + bytes.parts + bytes.sinks;
 }
 
@@ -1012,7 +1012,7 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   float* delta = static_cast<float*>(scratch);
   p.lse = lse; p.delta = delta;
   p.shifts = lse + stat_rows(bounds, n_seq, time) * heads;
-  p.span = span_of(window, sinks, bounds, n_seq, time);
+  p.span = span_of(window, sinks, bounds, n_seq, time, rest != nullptr);
   KeyParts cut;
   BackwardBytes bytes;
   const int status = backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, p.span, &cut, &bytes);

@@ -69,10 +69,14 @@ struct Span {
     }
   }
 };
-// A window that reaches over the longest sequence is none.
-inline Span span_of(int64_t window, int64_t sinks, const int64_t* bounds, int64_t n_seq, int64_t time) {
+// A window that reaches over the longest sequence is none.  But where that is one tile and the output's rest is kept for
+// a backward, it goes the window's way: with few keys the rounding of delta that the rest undoes counts most (gradients off by
+// 2.1 roundings at 3 tokens, 1.8 at 11, 1.6 at 100, and by 1.5 with it), for an eighth of a training step (64 x 128 tokens, 16
+// heads, 4 key heads: 136 us for 120).  Two tiles are gone through in another order than without a window, and give other bits.
+inline Span span_of(int64_t window, int64_t sinks, const int64_t* bounds, int64_t n_seq, int64_t time, bool rest) {
   int64_t longest = bounds != nullptr ? 0 : time;
   for (int64_t i = 0; bounds != nullptr && i < n_seq; ++i) longest = std::max(longest, bounds[i + 1] - bounds[i]);
+  if (rest && window >= longest && longest <= kTileRows / 2) return {int(longest), 0};
   if (window <= 0 || window >= longest) return {0, 0};
   return {int(window), int(std::min<int64_t>(sinks, longest))};
 }

@@ -7,10 +7,11 @@ ones as far as they are not behind it.
 ``window_attention_varlen``   sequences of any lengths packed along time
 ``window_tree_attention``     drafted tokens, or single ones, over a paged cache, of which the window and the sinks are read
 
-The first two are differentiable and run on the kernels of causal attention (csrc/attention_fwd.cu, csrc/attention_bwd.cu), which pass over
-the tiles that no row of theirs sees; what is said in attention.py about types, heads, roundings and values that are not finite
-holds here (but for delta, which is taken from the output and what its rounding left over, which is kept for the backward), with tiles that the window's edge or the sinks' end crosses beside those on the diagonal.  A window that reaches over
-the longest sequence is causal attention, bit for bit.
+The first two are differentiable and run on the kernels of causal attention (csrc/attention_fwd.cu, csrc/attention_bwd.cu), which
+pass over the tiles that no row of theirs sees.  What is said in attention.py about types, heads, roundings and values that are
+not finite holds here, with tiles that the window's edge or the sinks' end crosses beside those on the diagonal.  Delta alone is
+taken more exactly: from the output and what its rounding left over, which is kept for the backward.  A window that reaches over
+the longest sequence is causal attention, bit for bit; but where that has at most 128 tokens, gradients are taken the window's way.
 """
 
 from __future__ import annotations

@@ -509,10 +509,10 @@ int gdn2_attention_backward(const void* q, const void* k, const void* v, const v
 
 /*
  * The same with a sliding window: token i sees the tokens j <= i with i - j < window, itself among them, and the first
- * `sinks` of its sequence (those that are not behind it).  window >= 1, sinks >= 0.  A window that reaches over the
- * longest sequence is causal attention and gives its bits.  `rest` (NULL: not wanted), like `out`, gets what the rounding
- * of `out` has left over; a backward that has it takes the sums of d_out and out from both, which matters where tokens see
- * few others.  (Neither is read or written where the window reaches over all.)
+ * `sinks` of its sequence (those that are not behind it).  window >= 1, sinks >= 0.  `rest` (NULL: not wanted), like `out`,
+ * gets what the rounding of `out` has left over; a backward that has it takes the sums of d_out and out from both, which
+ * matters where tokens see few others.  A window that reaches over the longest sequence is causal attention and gives its
+ * bits; `rest` is read and written all the same where that sequence has at most 128 tokens, and not where it has more.
  */
 int gdn2_window_attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics,
                                   void* rest, const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time,

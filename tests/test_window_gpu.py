@@ -119,6 +119,47 @@ def test_a_window_over_everything_is_causal_attention(window):
     assert torch.equal(window_attention_varlen(q[:1], k[:1], v[:1], bounds, window), causal_attention_varlen(q[:1], k[:1], v[:1], bounds))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("time,window,sinks,heads,kv_heads,dim", [
+    (1, 1, 0, 2, 1, 64), (1, 5, 2 ** 40, 2, 2, 128), (2, 2, 1, 4, 2, 40), (5, 2 ** 70, 3, 2, 1, 128), (127, 127, 200, 2, 1, 64), (128, 500, 0, 4, 1, 96),
+    (129, 129, 4, 2, 2, 128), (255, 256, 0, 8, 1, 64), (256, 256, 9, 2, 1, 128), (257, 257, 9, 2, 1, 128),
+])
+def test_a_window_over_short_sequences(dtype, time, window, sinks, heads, kv_heads, dim):
+    q, k, v, do = _inputs((3, time), heads, kv_heads, dim, dtype, seed=time)
+    got = _run(q, k, v, do, window, sinks)
+    assert torch.equal(window_attention(q, k, v, window, sinks=sinks), got[0])
+    for b in range(3):
+        _check_sequence([x[b] for x in got], q[b], k[b], v[b], do[b], min(window, time), min(sinks, time), f"sequence {b}")
+    lengths = [time, 0, time // 2, 1, time]
+    bounds = [sum(lengths[:i]) for i in range(6)]
+    q, k, v, do = _inputs((1, bounds[-1]), heads, kv_heads, dim, dtype, seed=time + 1)
+    got = _run(q, k, v, do, window, sinks, bounds)
+    for i, length in enumerate(lengths):
+        part = slice(bounds[i], bounds[i + 1])
+        if length:
+            _check_sequence([x[0, part] for x in got], q[0, part], k[0, part], v[0, part], do[0, part], min(window, time), min(sinks, time), f"packed sequence {i}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("time,window", [(3, 3), (3, 2), (11, 11), (11, 100), (100, 100), (100, 20), (600, 4)])
+def test_gradients_of_few_keys_are_off_by_two_roundings(dtype, time, window):
+    # dq and dk sum products of dS, which is rounded once, and are rounded once: the square root of two roundings in the 2-norm,
+    # where a rounding of dS, whose values may lie elsewhere between two powers of two, is one of dq to a sixth (1 / sqrt(12) of
+    # a step that is 2^-8 .. 2^-7 of the value): sqrt(1 + (7/6)^2) = 1.54, and 1.65 with a share for P, the statistics and the
+    # order of 100000 samples.  Delta from the rounded output alone adds a rounding of that for every key: 1.8 to 2.3 with few of them.
+    heads, dim = 8, 64
+    batch = max(1, 2400 // time)
+    q, k, v, do = _inputs((batch, time), heads, heads, dim, dtype, seed=5)
+    got = _run(q, k, v, do, window, 0)
+    leaves = [x.double().transpose(1, 2).requires_grad_(True) for x in (q, k, v)]
+    scores = (leaves[0] @ leaves[1].transpose(-1, -2) * dim ** -0.5).masked_fill(~_seen(time, window, 0), -math.inf)
+    want = torch.autograd.grad(scores.softmax(-1) @ leaves[2], leaves, do.double().transpose(1, 2))
+    for name, x, y in zip(("dq", "dk"), got[1:3], want):
+        y = y.transpose(1, 2)
+        rounding = (y.to(dtype).double() - y).norm()
+        assert (x.double() - y).norm() < 1.65 * rounding, name
+
+
 @pytest.mark.parametrize("sinks", [599, 600, 2 ** 33])
 def test_sinks_over_everything_see_all(sinks):
     q, k, v, do = _inputs((1, 600), 2, 1, 64, FP16, seed=2)
