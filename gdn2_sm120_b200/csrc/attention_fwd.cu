@@ -61,7 +61,7 @@ struct FwdParams {
 struct FwdBars {
   uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2];
   uint64_t raw;        // a tile that is mended before the products may read it
-  uint64_t told;       // all rows of an item that is done once more have what was added to them
+  uint64_t told;       // all rows of an item that is done once more have what was added to them: 16 warps, or 8 twice
   uint64_t drained;
   uint64_t kv_full[8], kv_empty[8];
 };
@@ -385,7 +385,6 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
       const Steps<kWindow> steps(it, p.span);
       const int begin = kWindow ? steps.begin[t] : 0, n = steps.end[t];
       if (n == 0) {
-        if (kWindow && kAgain) tc::mbar_arrive(&bar.told, lane == 0);
         if (p.lse != nullptr && half == 0) p.lse[head * p.seq.stat_rows + it.stat + (2 * it.tile + t) * 128 + row] = -INFINITY;
         continue;
       }
@@ -472,6 +471,9 @@ __device__ __forceinline__ void forward_items(const FwdParams& p, uint8_t* smem,
         }
         __syncwarp();
         tc::mbar_arrive(&bar.told, lane == 0);
+        // An item without a second tile of queries: this warp arrives for that of the other chain too, which passes it over.
+        // (If that one arrived by itself it could do so for several such items before this chain has read the first one's rows.)
+        if (t == 0 && steps.end[1] == 0) tc::mbar_arrive(&bar.told, lane == 0);
       } else if (there && ok && col0 < p.dim) {
         const T* v = static_cast<const T*>(p.values) + it.batch * p.strides[0] + (it.row0 + int64_t(it.tile) * kTileRows) * p.strides[1] +
                      head / p.group * p.strides[2] + col0;
