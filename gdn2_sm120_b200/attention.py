@@ -50,12 +50,26 @@ def _sequences(q, bounds):
     return _lib.int64s(*bounds), len(bounds) - 1, q.shape[1]
 
 
-def _launches(bounds) -> int:
-    """Launches of a pass: one, or one for every 256 packed sequences of which any has a token."""
+_SHORT = 128     # GDN2_WINDOW_SHORT_ROWS
+
+
+def _launches(bounds, apart=False) -> int:
+    """Launches of a pass: one, or one for every 256 packed sequences of which any has a token; with `apart` another one for
+    short sequences beside longer ones."""
 
     if bounds is None:
         return 1
-    return sum(bounds[i] < bounds[min(i + 256, len(bounds) - 1)] for i in range(0, len(bounds) - 1, 256))
+    lengths = [b - a for a, b in zip(bounds, bounds[1:])]
+    groups = [lengths[i:i + 256] for i in range(0, len(lengths), 256)]
+    if not apart:
+        return sum(any(group) for group in groups)
+    return sum(len({n > _SHORT for n in group if n > 0}) for group in groups)
+
+
+def _apart(q, bounds, window) -> bool:
+    """Whether a training step with a window takes short sequences apart: the window reaches over all of them."""
+
+    return window != (0, 0) and window[0] >= (q.shape[1] if bounds is None else max(b - a for a, b in zip(bounds, bounds[1:])))
 
 
 def _entry(name, window):
@@ -80,7 +94,7 @@ def _forward(q, k, v, bounds, scale, window, training):
     rest = torch.empty_like(out) if training and more else None    # what the output's rounding leaves over
     _lib.call(name, q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
               _lib.ptr(statistics), *((_lib.ptr(rest),) if more else ()), strides, host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], *more,
-              _lib.dtype_code(q.dtype), scale, _lib.stream_ptr(q.device), kernels=_launches(bounds))
+              _lib.dtype_code(q.dtype), scale, _lib.stream_ptr(q.device), kernels=_launches(bounds, rest is not None and _apart(q, bounds, window)))
     return out, statistics, rest
 
 
@@ -123,7 +137,7 @@ class _CausalAttention(torch.autograd.Function):
         _lib.call(name, q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                   *((_lib.ptr(rest),) if more else ()), d_out.data_ptr(), statistics.data_ptr(), scratch.data_ptr(), *(x.data_ptr() for x in grads), strides,
                   host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], *more, _lib.dtype_code(q.dtype), scale,
-                  _lib.stream_ptr(q.device), kernels=(3 + (size > 2 * statistics.numel() + 15)) * _launches(ctx.bounds))
+                  _lib.stream_ptr(q.device), kernels=(3 + (size > 2 * statistics.numel() + 15)) * _launches(ctx.bounds, rest is not None and _apart(q, ctx.bounds, ctx.window)))
         return (*grads, None, None, None)
 
 

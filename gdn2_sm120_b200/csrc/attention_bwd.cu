@@ -989,7 +989,7 @@ int64_t attention_backward_bytes(const int64_t* bounds, int64_t n_seq, int64_t t
                                  int64_t sinks) {
   KeyParts k;
   BackwardBytes bytes;
-  const int status = backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, span_of(window, sinks, bounds, n_seq, time, true), &k, &bytes);
+  const int status = backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, ways_of(window, sinks, bounds, n_seq, time, false).span, &k, &bytes);
   return status != GDN2_OK ? status : bytes.delta + bytes.parts + bytes.sinks;
 }
 
@@ -1012,10 +1012,10 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   float* delta = static_cast<float*>(scratch);
   p.lse = lse; p.delta = delta;
   p.shifts = lse + stat_rows(bounds, n_seq, time) * heads;
-  p.span = span_of(window, sinks, bounds, n_seq, time, rest != nullptr);
+  const Ways ways = ways_of(window, sinks, bounds, n_seq, time, rest != nullptr);
   KeyParts cut;
   BackwardBytes bytes;
-  const int status = backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, p.span, &cut, &bytes);
+  const int status = backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, ways.span, &cut, &bytes);
   if (status != GDN2_OK) return status;
   p.parts = cut.parts;
   p.sink_tiles = cut.sink_tiles;
@@ -1029,7 +1029,8 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   p.polls = wait_polls();
   p.wide = wide_rows(dq, dim) && wide_rows(dk, dim) && wide_rows(dv, dim);
   p.scale_log2 = positive_scale(scale);
-  return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {
+  return for_groups(bounds, n_seq, time, ways.apart, &p.seq, [&](bool short_ones) -> int {
+    p.span = short_ones ? kShortSpan : ways.span;
     DeltaParams d{out, d_out, rest, {strides[9], strides[10], strides[11]}, delta, heads, dim, p.seq};
     return dtype == GDN2_BF16 ? launch_dim<__nv_bfloat16>(p, d, stream) : launch_dim<__half>(p, d, stream);
   });

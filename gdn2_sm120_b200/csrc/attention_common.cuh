@@ -69,16 +69,21 @@ struct Span {
     }
   }
 };
-// A window that reaches over the longest sequence is none.  But where that is one tile and the output's rest is kept for
-// a backward, it goes the window's way: with few keys the rounding of delta that the rest undoes counts most (gradients off by
-// 2.1 roundings at 3 tokens, 1.8 at 11, 1.6 at 100, and by 1.5 with it), for an eighth of a training step (64 x 128 tokens, 16
-// heads, 4 key heads: 136 us for 120).  Two tiles are gone through in another order than without a window, and give other bits.
-inline Span span_of(int64_t window, int64_t sinks, const int64_t* bounds, int64_t n_seq, int64_t time, bool rest) {
+// What the rows of a call see.  A window that reaches over the longest sequence is none.  But where the output's rest is kept for
+// a backward, sequences of one tile of queries go the window's way (`apart`), in launches of their own where there are longer
+// ones, so that a sequence's gradients do not depend on what it is packed with: with few keys the rounding of delta that the
+// rest undoes counts most (gradients off by 2.1 roundings at 3 tokens, 1.8 at 11, 1.6 at 100, and by 1.5 with it), for an
+// eighth of a training step (64 x 128 tokens, 16 heads, 4 key heads: 136 us for 120).  Two tiles are gone through in another
+// order than without a window, and give other bits.
+constexpr int kShortRows = GDN2_WINDOW_SHORT_ROWS;
+static_assert(kShortRows == kTileRows / 2, "");
+constexpr Span kShortSpan{kShortRows, 0};
+struct Ways { Span span; bool apart; };
+inline Ways ways_of(int64_t window, int64_t sinks, const int64_t* bounds, int64_t n_seq, int64_t time, bool rest) {
   int64_t longest = bounds != nullptr ? 0 : time;
   for (int64_t i = 0; bounds != nullptr && i < n_seq; ++i) longest = std::max(longest, bounds[i + 1] - bounds[i]);
-  if (rest && window >= longest && longest <= kTileRows / 2) return {int(longest), 0};
-  if (window <= 0 || window >= longest) return {0, 0};
-  return {int(window), int(std::min<int64_t>(sinks, longest))};
+  if (window <= 0 || window >= longest) return {{0, 0}, rest && window > 0};
+  return {{int(window), int(std::min<int64_t>(sinks, longest))}, false};
 }
 
 struct Item {
@@ -513,10 +518,11 @@ inline int64_t stat_rows(const int64_t* bounds, int64_t n_seq, int64_t time) {
 }
 
 // The launches of a call: one for a batch of equally long sequences (bounds null, `time` rows each), one for every
-// kMaxSequences packed ones.  Fills *s for each and calls launch(); it follows from the bounds alone, so that forward
-// and backward agree on where a row's statistics are.
+// kMaxSequences packed ones; with `apart` another one for those of up to kShortRows rows beside longer ones.  Fills *s for
+// each and calls launch(short); it follows from the bounds alone, so that forward and backward agree on where a row's
+// statistics are.
 template <typename Launch>
-inline int for_groups(const int64_t* bounds, int64_t n_seq, int64_t time, Sequences* s, Launch launch) {
+inline int for_groups(const int64_t* bounds, int64_t n_seq, int64_t time, bool apart, Sequences* s, Launch launch) {
   s->stat_rows = stat_rows(bounds, n_seq, time);
   s->stat_row0 = 0;
   if (bounds == nullptr) {
@@ -525,7 +531,7 @@ inline int for_groups(const int64_t* bounds, int64_t n_seq, int64_t time, Sequen
     s->time = int(time);
     s->tiles_each = int((time + kTileRows - 1) / kTileRows);
     s->tiles = s->tiles_each * s->n;
-    return launch();
+    return launch(apart && time <= kShortRows);
   }
   s->packed = 1;
   s->time = 0;
@@ -536,18 +542,21 @@ inline int for_groups(const int64_t* bounds, int64_t n_seq, int64_t time, Sequen
     int order[kMaxSequences];
     for (int i = 0; i < count; ++i) order[i] = i;
     std::stable_sort(order, order + count, [&](int x, int y) { return b[x + 1] - b[x] > b[y + 1] - b[y]; });
-    s->n = s->tiles = 0;
-    for (int i = 0; i < count; ++i) {
-      const int len = int(b[order[i] + 1] - b[order[i]]);
-      if (len == 0) break;   // sorted: nothing but empty ones from here on
-      s->e[s->n++] = Sequences::Entry{int(b[order[i]]), len, s->tiles, 0};
-      s->tiles += (len + kTileRows - 1) / kTileRows;
+    int at = 0;
+    for (const bool short_ones : {false, true}) {   // sorted: short ones are behind the longer ones, and then empty ones
+      s->n = s->tiles = 0;
+      for (; at < count; ++at) {
+        const int len = int(b[order[at] + 1] - b[order[at]]);
+        if (len == 0 || (apart && len <= kShortRows) != short_ones) break;
+        s->e[s->n++] = Sequences::Entry{int(b[order[at]]), len, s->tiles, 0};
+        s->tiles += (len + kTileRows - 1) / kTileRows;
+      }
+      if (s->n > 0) {
+        const int status = launch(short_ones);
+        if (status != GDN2_OK) return status;
+      }
+      s->stat_row0 += int64_t(s->tiles) * kTileRows;
     }
-    if (s->n > 0) {
-      const int status = launch();
-      if (status != GDN2_OK) return status;
-    }
-    s->stat_row0 += int64_t(s->tiles) * kTileRows;
   }
   return GDN2_OK;
 }

@@ -573,8 +573,9 @@ int launch_attention_forward(const void* q, const void* k, const void* v, void* 
   p.polls = wait_polls();
   p.wide = wide_rows(out, dim) && wide_rows(rest, dim);
   p.scale_log2 = positive_scale(scale);
-  p.span = span_of(window, sinks, bounds, n_seq, time, rest != nullptr);
-  return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {
+  const Ways ways = ways_of(window, sinks, bounds, n_seq, time, rest != nullptr);
+  return for_groups(bounds, n_seq, time, ways.apart, &p.seq, [&](bool short_ones) -> int {
+    p.span = short_ones ? kShortSpan : ways.span;
     p.items = int64_t(p.seq.tiles) * heads;
     return dtype == GDN2_BF16 ? launch_dim<__nv_bfloat16>(p, stream) : launch_dim<__half>(p, stream);
   });

@@ -379,7 +379,7 @@ int launch_attention_weights(const void* q, const void* k, const float* lse, flo
   p.negate = scale < 0.f;
   p.polls = wait_polls();
   p.scale_log2 = positive_scale(scale);
-  return for_groups(bounds, n_seq, time, &p.seq, [&]() -> int {
+  return for_groups(bounds, n_seq, time, false, &p.seq, [&](bool) -> int {
     if (dtype == GDN2_BF16) return dim <= 64 ? launch_typed<__nv_bfloat16, 64>(p, stream) : launch_typed<__nv_bfloat16, 128>(p, stream);
     return dim <= 64 ? launch_typed<__half, 64>(p, stream) : launch_typed<__half, 128>(p, stream);
   });

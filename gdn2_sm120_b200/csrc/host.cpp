@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <initializer_list>
@@ -637,13 +638,30 @@ bool read_bounds(PyObject* o, const Heads& h, std::vector<int64_t>* bounds) {
   return bounds->front() == 0 && bounds->back() == h.time;
 }
 
-// launches of a pass: one, or one for every GDN2_PACKED_MAX_SEQUENCES packed sequences of which any has a token
-long passes(const std::vector<int64_t>& bounds) {
+// launches of a pass: one, or one for every GDN2_PACKED_MAX_SEQUENCES packed sequences of which any has a token; with `apart`
+// another one for short sequences beside longer ones
+long passes(const std::vector<int64_t>& bounds, bool apart = false) {
   if (bounds.empty()) return 1;
   long count = 0;
   const size_t n = bounds.size() - 1, most = GDN2_PACKED_MAX_SEQUENCES;
-  for (size_t i = 0; i < n; i += most) count += bounds[i] < bounds[i + most < n ? i + most : n];
+  for (size_t i = 0; i < n; i += most) {
+    bool longer = false, shorter = false;
+    for (size_t j = i; j < n && j < i + most; ++j) {
+      const int64_t length = bounds[j + 1] - bounds[j];
+      longer = longer || (apart ? length > GDN2_WINDOW_SHORT_ROWS : length > 0);
+      shorter = shorter || (apart && length > 0 && length <= GDN2_WINDOW_SHORT_ROWS);
+    }
+    count += longer + shorter;
+  }
   return count;
+}
+
+// the rows of the longest sequence
+int64_t longest(const std::vector<int64_t>& bounds, int64_t time) {
+  if (bounds.empty()) return time;
+  int64_t most = 0;
+  for (size_t i = 0; i + 1 < bounds.size(); ++i) most = std::max(most, bounds[i + 1] - bounds[i]);
+  return most;
 }
 
 // rotary(q, k, cos, sin, positions, interleaved, inverse) -> (q, k) or None
@@ -977,7 +995,8 @@ PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
                : api.window_attention_forward(q.data_ptr(), h.t[1]->data_ptr(), h.t[2]->data_ptr(), out.data_ptr(), stat,
                                               keeps ? rest.data_ptr() : nullptr, h.strides, host, n_seq, h.time, h.heads, h.kv_heads, h.dim, window, sinks, h.dtype, scale, stream);
   others.end();
-  if (!ok(status, window == 0 ? "gdn2_attention_forward" : "gdn2_window_attention_forward", passes(bounds))) return nullptr;
+  if (!ok(status, window == 0 ? "gdn2_attention_forward" : "gdn2_window_attention_forward",
+          passes(bounds, keeps && window >= longest(bounds, h.time)))) return nullptr;
   PyObject* result = PyTuple_New(3);
   PyTuple_SET_ITEM(result, 0, wrap(out));
   PyTuple_SET_ITEM(result, 1, training ? wrap(statistics) : Py_NewRef(Py_None));
@@ -1076,7 +1095,7 @@ PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   others.end();
   const bool parts = size > 2 * statistics->numel() + 15;   // sums of several CTAs are added up
   const char* name = window == 0 ? "gdn2_attention_backward" : "gdn2_window_attention_backward";
-  if (!ok(status, name, (parts ? 4 : 3) * passes(bounds))) return nullptr;
+  if (!ok(status, name, (parts ? 4 : 3) * passes(bounds, rest != nullptr && window >= longest(bounds, h.time)))) return nullptr;
   PyObject* result = PyTuple_New(3);
   for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(result, i, wrap(grads[i]));
   return result;

@@ -512,8 +512,9 @@ int gdn2_attention_backward(const void* q, const void* k, const void* v, const v
  * `sinks` of its sequence (those that are not behind it).  window >= 1, sinks >= 0.  `rest` (NULL: not wanted), like `out`,
  * gets what the rounding of `out` has left over; a backward that has it takes the sums of d_out and out from both, which
  * matters where tokens see few others.  A window that reaches over the longest sequence is causal attention and gives its
- * bits; `rest` is read and written all the same where that sequence has at most 128 tokens, and not where it has more.
+ * bits; there `rest` is read and written for sequences of at most GDN2_WINDOW_SHORT_ROWS tokens, and not for longer ones.
  */
+#define GDN2_WINDOW_SHORT_ROWS 128
 int gdn2_window_attention_forward(const void* q, const void* k, const void* v, void* out, float* statistics,
                                   void* rest, const int64_t* strides, const int64_t* bounds, int64_t n_seq, int64_t time,
                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks,
