@@ -72,6 +72,14 @@ def _apart(q, bounds, window) -> bool:
     return window != (0, 0) and window[0] >= (q.shape[1] if bounds is None else max(b - a for a, b in zip(bounds, bounds[1:])))
 
 
+def _keeps_rest(q, bounds, window) -> bool:
+    """Whether a backward with a window reads what the output's rounding has left over: of all sequences, or of short ones."""
+
+    if not _apart(q, bounds, window):
+        return window != (0, 0)
+    return q.shape[1] <= _SHORT if bounds is None else any(a < b <= a + _SHORT for a, b in zip(bounds, bounds[1:]))
+
+
 def _entry(name, window):
     """The entry point ``name`` of attention without a window or with one, and what says so."""
 
@@ -91,7 +99,7 @@ def _forward(q, k, v, bounds, scale, window, training):
         statistics = torch.empty((2, q.shape[2], each), device=q.device, dtype=torch.float32)
     strides = _lib.int64s(*(s for x in (q, k, v) for s in _validate.head_strides(x)))
     name, more = _entry("attention_forward", window)
-    rest = torch.empty_like(out) if training and more else None    # what the output's rounding leaves over
+    rest = torch.empty_like(out) if training and _keeps_rest(q, bounds, window) else None    # what the output's rounding leaves over
     _lib.call(name, q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
               _lib.ptr(statistics), *((_lib.ptr(rest),) if more else ()), strides, host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], *more,
               _lib.dtype_code(q.dtype), scale, _lib.stream_ptr(q.device), kernels=_launches(bounds, rest is not None and _apart(q, bounds, window)))

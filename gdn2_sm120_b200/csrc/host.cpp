@@ -664,6 +664,14 @@ int64_t longest(const std::vector<int64_t>& bounds, int64_t time) {
   return most;
 }
 
+// whether a backward with a window reads what the output's rounding has left over: of all sequences, or of short ones
+bool keeps_rest(const std::vector<int64_t>& bounds, int64_t time, int64_t window) {
+  if (window <= 0 || window < longest(bounds, time)) return window > 0;
+  bool any = bounds.empty() && time <= GDN2_WINDOW_SHORT_ROWS;
+  for (size_t i = 0; i + 1 < bounds.size(); ++i) any = any || (bounds[i] < bounds[i + 1] && bounds[i + 1] - bounds[i] <= GDN2_WINDOW_SHORT_ROWS);
+  return any;
+}
+
 // rotary(q, k, cos, sin, positions, interleaved, inverse) -> (q, k) or None
 PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   GDN2_TRY
@@ -986,7 +994,7 @@ PyObject* attention_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   out = at::empty(q.sizes(), q.options());
   if (training) statistics = floats({2, h.heads, rows}, q);
   float* stat = training ? fptr(&statistics) : nullptr;
-  const bool keeps = training && window > 0;
+  const bool keeps = training && keeps_rest(bounds, h.time, window);
   if (keeps) rest = at::empty(q.sizes(), q.options());
   void* stream = at::cuda::getCurrentCUDAStream().stream();
   status = window == 0
