@@ -373,6 +373,10 @@ __device__ __forceinline__ void bring_tiles(const TreeParams& p, Unit u, int til
   }
 }
 
+// With a window: behind which token, counted from the first drafted one, no cached one was taken out of a unit's tiles: a warp's 32
+// are looked at where any of them is not seen by all drafted ones.  By whole warps.
+__device__ __forceinline__ int edge_of(const TreeParams& p, const Unit& u) { return min(0, seen_by_all(p, u) + 31 - u.length); }
+
 // With a window: where the values of token d (counted from the first drafted one) are, if drafted token `token` sees it, if it
 // is one that not all see (only those were taken out of their tiles) and in the tiles tile .. tile + n - 1; null otherwise
 template <typename T>
@@ -432,6 +436,7 @@ struct FewBars {
   uint64_t kv_full[10], kv_empty[10];
   Share<kFewThreads / 32> share;
   int failed, strange;
+  uint32_t strange_rows[kStrangeRows / 32];
   float m[8][16], l[8][16];
 };
 static_assert(sizeof(FewBars) <= 2048, "");
@@ -442,6 +447,7 @@ template <typename T, int DP, bool kWindow, bool kWeigh>
 __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_constant__ TreeParams p) {
   using C = FewConfig<DP>;
   constexpr int kKSteps = DP / 16, kDB = DP / 8;
+  constexpr bool kBits = kWindow || kWeigh;   // more tokens than a few to look through for values that are not finite
   extern __shared__ __align__(1024) uint8_t smem[];   // swizzled tiles: 1024-byte aligned, there is no static shared memory
   const uint32_t kv_base = tc::smem_u32(smem);
   float* join = reinterpret_cast<float*>(smem + C::kStages * C::kTileBytes);
@@ -457,12 +463,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
     bar.failed = bar.strange = 0;
     tc::fence_mbar_init();
   }
+  if (kBits && tid < kStrangeRows / 32) bar.strange_rows[tid] = 0;
   Unit u;
   int tile, rest;
   if (!part_of_cta<kWindow, kFewThreads / 32>(p, bar.share, u, tile, rest)) return;
   const attn::Waiter waiter{&bar.failed, p.polls};
   if (warp >= 8) {
-    bring_tiles<T, DP, kWindow, kWeigh, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange, nullptr);
+    bring_tiles<T, DP, kWindow, kWeigh, C::kStages, 4>(p, u, tile, rest, warp - 8, kv_base, bar.kv_full, bar.kv_empty, waiter, &bar.strange,
+                                                       kBits ? bar.strange_rows : nullptr);
     return;
   }
 
@@ -628,7 +636,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
       if (with > 1) sync();
     }
     if (warp == 0) {
-      const bool whole = !split && tile + n == u.tiles, strange = *static_cast<volatile int*>(&bar.strange) != 0;
+      const bool whole = !split && tile + n == u.tiles;
+      const bool told = *static_cast<volatile int*>(&bar.strange) != 0, strange = kWindow ? __any_sync(0xffffffffu, told) : told;
+      const int edge = kWindow && strange ? edge_of(p, u) : 0;
       const int64_t slot = int64_t(blockIdx.x) * 2 + (split ? 0 : 1);
       ok = ok && waiter.nobody_failed();   // none of the eight
       if (kWeigh && lane == 0) {
@@ -649,14 +659,15 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
         if (strange) {
           const int first = kWindow ? max(u.from - 31, 0) - u.length : max(0, tile * kTile - u.length);
           const int last = min(p.drafted, tile_token<kWindow>(u, tile + n - 1) + kTile - u.length);
-          for (int d = first; d < last; ++d) {
-            const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + u.b * p.mask_stride + int64_t(i) * p.drafted;
+          const int deep = kWindow ? depth_of(p, u.b, i) : 0;
+          auto add = [&](int d) {
+            const uint8_t* mask = kWeigh || p.mask == nullptr ? nullptr : p.mask + u.b * p.mask_stride + int64_t(i) * p.drafted;
             const T* v;
             if (kWindow) {
-              v = strange_value<T>(p, u, mask, i, depth_of(p, u.b, i), d, tile, n);
-              if (v == nullptr) continue;
+              v = strange_value<T>(p, u, mask, i, deep, d, tile, n);
+              if (v == nullptr) return;
             } else {
-              if (!(mask == nullptr ? d <= i : mask[d] != 0)) continue;
+              if (!(mask == nullptr ? d <= i : mask[d] != 0)) return;
               v = static_cast<const T*>(p.v) + u.b * p.v_stride[0] + d * p.v_stride[1] + u.head * p.v_stride[2];
             }
 #pragma unroll
@@ -665,6 +676,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) tree_few_kernel(const __grid_c
               const float value = col < p.dim ? to_float(v[col]) : 0.f;
               if (!isfinite(value)) o[x >> 1][2 * half + (x & 1)] += value;
             }
+          };
+          if (kBits) {   // those that had such a value in some unit of the CTA, but for cached ones behind the window's edge
+            for (int d0 = first & ~31; d0 < last; d0 += 32) {
+              if (kWindow && d0 >= edge && d0 < 0) d0 = 0;
+              for (uint32_t bits = bar.strange_rows[(d0 & (kStrangeRows - 1)) >> 5]; bits != 0; bits &= bits - 1) {
+                const int d = d0 + __ffs(bits) - 1;
+                if (d >= first && d < last) add(d);
+              }
+            }
+          } else {
+            for (int d = first; d < last; ++d) add(d);
           }
         }
         T* to = static_cast<T*>(p.out) + (int64_t(u.b) * p.drafted + i) * p.heads * p.dim + int64_t(u.head * p.group + g) * p.dim;

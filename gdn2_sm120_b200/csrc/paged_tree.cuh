@@ -318,7 +318,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       const float inv = !ok || u.bad ? NAN : !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
       const int64_t slot = int64_t(blockIdx.x) * 2 + (split ? 0 : 1);
       float* part = p.partials + (slot * C::kRows + local) * DP;
-      const bool strange = *static_cast<volatile int*>(&bar.strange) != 0;
+      const bool told_strange = *static_cast<volatile int*>(&bar.strange) != 0, strange = kWindow ? __any_sync(0xffffffffu, told_strange) : told_strange;
+      const int edge = kWindow && strange ? edge_of(p, u) : 0;
       if (takes_part && any_there) {
         const int g = r - token * p.group;
         T* to = static_cast<T*>(p.out) + (int64_t(u.b) * p.drafted + token) * p.heads * p.dim + int64_t(u.head * p.group + g) * p.dim;
@@ -349,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + u.b * p.mask_stride + int64_t(token) * p.drafted;
             bool done = false;          // all channels are NaN
             for (int d0 = first & ~31; d0 < last && !done; d0 += 32) {
+              if (kWindow && d0 >= edge && d0 < 0) d0 = 0;
               for (uint32_t bits = bar.strange_rows[(d0 & (kStrangeRows - 1)) >> 5]; bits != 0 && !done; bits &= bits - 1) {
                 const int d = d0 + __ffs(bits) - 1;
                 if (d < first || d >= last) continue;
