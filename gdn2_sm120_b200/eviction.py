@@ -66,8 +66,8 @@ def weighed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scal
     """``causal_attention``, and the weight that every token got: ``(output, weights)``.
 
     ``weights [B, T, Hkv]`` (fp32): the softmax weights that a token was given by itself and by the tokens behind it, summed over
-    these and over the heads of a group.  They are formed from scores in 32 bits.  A query whose output is NaN makes
-    the weights of the tokens that it sees NaN.  No gradients."""
+    these and over the heads of a group.  They are formed from scores in 32 bits.  A query that has a score of NaN or +inf
+    makes the weights of the tokens that it sees NaN; values do not enter them.  No gradients."""
 
     return _weighed("weighed_attention", q, k, v, None, scale)
 
@@ -129,7 +129,8 @@ def weighed_token_attention(
     ``slots`` (int64 ``[B, N]``), the place that ``append_tokens`` puts its key and value to; no cached token may have it, and a
     negative one, or one behind the cache, leaves it out.  A page of a sequence must not be another one's too.
     ``page_table`` and ``lengths`` as in ``tree_attention``; where those make a sequence's output NaN its weights become NaN, but
-    for a bad length only those of its new tokens."""
+    for a bad length only those of its new tokens.  Scores of NaN or +inf make their sequence's and key head's
+    weights NaN; values do not enter them."""
 
     if forward_ad._current_level >= 0:
         _validate.refuse_tangents("weighed_token_attention", q, k, v, k_pages, v_pages, weight_pages)

@@ -543,7 +543,7 @@ int gdn2_window_tree_attention(const void* q, const void* k, const void* v, cons
 
 /*
  * What weight every token of a prompt got from causal attention: weights[row][kv head] (fp32, contiguous), the sum of the
- * softmax weights that the queries at and behind the token, of all heads of a group, gave it.  `statistics` is what
+ * softmax weights that the queries at and behind the token, of all heads of a group, gave it; values do not enter it.  `statistics` is what
  * gdn2_attention_forward left for the same q, k, bounds and scale.  scratch: gdn2_attention_weights_bytes, which may be 0
  * (the device is the current one), dead when the call's kernels have run.  strides: batch, token and head of q, k.
  */
@@ -559,8 +559,9 @@ int gdn2_attention_weights(const void* q, const void* k, const float* statistics
  * and over them.  weight_pages [pages][kv_heads][page] (fp32) belongs to the cache: a cached token's weight becomes
  * decay * weight + what it got (with a decay of 0 it is not read), that of a new one is put to slots[b * tokens + i]
  * (page number * page + place; negative or behind the cache: left out), which must not be a cached token's.  A page whose
- * weights change belongs to one sequence.  tokens * heads / kv_heads <= GDN2_WEIGHED_MAX_ROWS.  A sequence whose output is NaN
- * gets weights of NaN; one whose length is bad changes none but those of its new tokens.
+ * weights change belongs to one sequence.  tokens * heads / kv_heads <= GDN2_WEIGHED_MAX_ROWS.  A sequence with a score
+ * of NaN or +inf gets weights of NaN in its key head, one with a page number that is none of the cache in all of them (values
+ * do not enter them); one whose length is bad changes none but those of its new tokens.
  */
 #define GDN2_WEIGHED_MAX_ROWS 256
 int64_t gdn2_weighed_token_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
