@@ -66,7 +66,8 @@ def weighed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scal
     """``causal_attention``, and the weight that every token got: ``(output, weights)``.
 
     ``weights [B, T, Hkv]`` (fp32): the softmax weights that a token was given by itself and by the tokens behind it, summed over
-    these and over the heads of a group.  They are formed from scores in 32 bits.  A query that has a score of NaN or +inf
+    these and over the heads of a group.  They are formed from scores in 32 bits,
+    by exponentials of which a quarter is good to 7e-6.  A query that has a score of NaN or +inf
     makes the weights of the tokens that it sees NaN; values do not enter them.  No gradients."""
 
     return _weighed("weighed_attention", q, k, v, None, scale)
@@ -130,7 +131,12 @@ def weighed_token_attention(
     negative one, or one behind the cache, leaves it out.  A page of a sequence must not be another one's too.
     ``page_table`` and ``lengths`` as in ``tree_attention``; where those make a sequence's output NaN its weights become NaN, but
     for a bad length only those of its new tokens.  Scores of NaN or +inf make their sequence's and key head's
-    weights NaN; values do not enter them."""
+    weights NaN; values do not enter them.
+
+    The call's workspace has 4 bytes for every query head, new token and token that ``page_table`` has room for, however long the
+    sequences are (64 sequences, 32 heads, room for 131072 tokens: 1.1 GB).  A table with more columns than the longest sequence
+    needs is better passed as ``page_table[:, :needed]``.  Keys and values are read once for every 16 rows (new tokens times heads
+    of a group)."""
 
     if forward_ad._current_level >= 0:
         _validate.refuse_tangents("weighed_token_attention", q, k, v, k_pages, v_pages, weight_pages)
@@ -198,10 +204,11 @@ def evict_tokens(
     A sequence of no more than ``keep`` tokens keeps all.  Their keys, values and weights are copied: token ``j`` of those that
     stay to page ``new_table[b, j // page]`` at ``j % page``.  ``new_table`` (int32 ``[B, columns]``, room for ``keep``) names
     pages of the same cache that no sequence uses: neither ``page_table`` nor another row of it; what lies in the old pages stays
-    as it was, so that sequences may share them.  A new page number outside the cache leaves its tokens out (-1 in a row's
-    entries passes a sequence by).  Keys and values are fp16, bf16 or fp32.  The new lengths (int32 ``[B]``) are the
-    smaller of ``lengths`` and ``keep``, and -1, with nothing copied, where a length or a page number of ``page_table`` is none of the
-    cache.  Like ``page_table``, ``lengths`` and ``new_table`` they stay on the device."""
+    as it was, so that sequences may share them.  A new page number outside the cache leaves its tokens out; a row of -1 passes a
+    sequence by.  Keys and values are fp16, bf16 or fp32.  The new lengths (int32 ``[B]``) are the smaller of ``lengths`` and
+    ``keep``, of a sequence that is passed by too: it is where it was, and its old length is the one to go on with.  They are -1,
+    with nothing copied, where a length or a page number of ``page_table`` is none of the cache.  Like ``page_table``, ``lengths``
+    and ``new_table`` they stay on the device."""
 
     if forward_ad._current_level >= 0:
         _validate.refuse_tangents("evict_tokens", k_pages, v_pages, weight_pages)

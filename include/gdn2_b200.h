@@ -579,7 +579,8 @@ int gdn2_weighed_token_attention(const void* q, const void* k, const void* v, co
  * `sinks` and the last `recent` tokens of a sequence are among them (sinks + recent <= keep <= new_columns * page), and
  * all tokens of one that has no more than `keep`.  Of equal weights the earlier token's counts more, NaN counts more than any
  * number.  new_lengths[b]: how many were kept; -1, and nothing is copied, where the length or a page number of the sequence is
- * none of the cache.  Tokens whose new page is none of the cache are left out.  No page that is written to may be one that
+ * none of the cache.  Tokens whose new page is none of the cache are left out; a sequence of which none was copied for that is
+ * where it was, and new_lengths[b] is no length of it.  No page that is written to may be one that
  * any sequence's page table names, or another sequence's new one.  workspace: gdn2_evict_workspace_bytes.
  */
 int64_t gdn2_evict_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t keep);
