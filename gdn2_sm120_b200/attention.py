@@ -54,7 +54,7 @@ _SHORT = 128     # GDN2_WINDOW_SHORT_ROWS
 
 
 def _launches(bounds, apart=False) -> int:
-    """Launches of a pass: one, or one for every 256 packed sequences of which any has a token; with `apart` another one for
+    """Launches of a pass: one, or one for every 256 packed sequences of which any has a token; with ``apart`` another one for
     short sequences beside longer ones."""
 
     if bounds is None:
@@ -67,7 +67,7 @@ def _launches(bounds, apart=False) -> int:
 
 
 def _apart(q, bounds, window) -> bool:
-    """Whether a training step with a window takes short sequences apart: the window reaches over all of them."""
+    """Whether a training forward with a window takes short sequences apart: the window reaches over all of them."""
 
     return window != (0, 0) and window[0] >= (q.shape[1] if bounds is None else max(b - a for a, b in zip(bounds, bounds[1:])))
 
@@ -145,7 +145,7 @@ class _CausalAttention(torch.autograd.Function):
         _lib.call(name, q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                   *((_lib.ptr(rest),) if more else ()), d_out.data_ptr(), statistics.data_ptr(), scratch.data_ptr(), *(x.data_ptr() for x in grads), strides,
                   host, n_seq, rows, q.shape[2], k.shape[2], q.shape[3], *more, _lib.dtype_code(q.dtype), scale,
-                  _lib.stream_ptr(q.device), kernels=(3 + (size > 2 * statistics.numel() + 15)) * _launches(ctx.bounds, rest is not None and _apart(q, ctx.bounds, ctx.window)))
+                  _lib.stream_ptr(q.device), kernels=(3 + (size > 2 * statistics.numel() + 15)) * _launches(ctx.bounds))
         return (*grads, None, None, None)
 
 

@@ -26,6 +26,7 @@
 // tokens as above, a window of 512 and 16 sinks: keys and queries 155 us together, forward 69, delta 16.
 
 #include <algorithm>
+#include <climits>
 
 #include "attention_common.cuh"
 
@@ -825,6 +826,7 @@ struct DeltaParams {
   int64_t do_stride[3];
   float* delta;
   int heads, dim;
+  int rest_rows;                    // of sequences of up to so many rows
   Sequences seq;
 };
 
@@ -845,7 +847,7 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
       a[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + ((it.row + i) * p.heads + head) * p.dim + part * 8);
       b[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.d_out) + it.batch * p.do_stride[0] + int64_t(it.row0 + i) * p.do_stride[1] +
                                              head * p.do_stride[2] + part * 8);
-      if (kRest) c[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.rest) + ((it.row + i) * p.heads + head) * p.dim + part * 8);
+      if (kRest && it.len <= p.rest_rows) c[x] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.rest) + ((it.row + i) * p.heads + head) * p.dim + part * 8);
     }
   }
 #pragma unroll
@@ -918,7 +920,7 @@ int launch_half(Kernel kernel, int bytes, const BwdParams& base, int64_t items, 
 template <typename T, int DP, bool kWindow>
 int launch_typed(BwdParams& p, const DeltaParams& d, cudaStream_t stream) {
   const unsigned ctas = unsigned(p.seq.tiles * (kTileRows / kDeltaRows) * p.heads);
-  if (kWindow && d.rest != nullptr) attention_delta_kernel<T, true><<<ctas, 256, 0, stream>>>(d);
+  if (d.rest != nullptr) attention_delta_kernel<T, true><<<ctas, 256, 0, stream>>>(d);
   else attention_delta_kernel<T, false><<<ctas, 256, 0, stream>>>(d);
   int status = check_launch();
   if (status != GDN2_OK) return status;
@@ -1013,6 +1015,7 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   p.lse = lse; p.delta = delta;
   p.shifts = lse + stat_rows(bounds, n_seq, time) * heads;
   const Ways ways = ways_of(window, sinks, bounds, n_seq, time, rest != nullptr);
+  p.span = ways.span;
   KeyParts cut;
   BackwardBytes bytes;
   const int status = backward_bytes(bounds, n_seq, time, heads, kv_heads, dim, ways.span, &cut, &bytes);
@@ -1029,9 +1032,8 @@ int launch_attention_backward(const void* q, const void* k, const void* v, const
   p.polls = wait_polls();
   p.wide = wide_rows(dq, dim) && wide_rows(dk, dim) && wide_rows(dv, dim);
   p.scale_log2 = positive_scale(scale);
-  return for_groups(bounds, n_seq, time, ways.apart, &p.seq, [&](bool short_ones) -> int {
-    p.span = short_ones ? kShortSpan : ways.span;
-    DeltaParams d{out, d_out, rest, {strides[9], strides[10], strides[11]}, delta, heads, dim, p.seq};
+  return for_groups(bounds, n_seq, time, false, &p.seq, [&](bool) -> int {
+    DeltaParams d{out, d_out, rest, {strides[9], strides[10], strides[11]}, delta, heads, dim, ways.apart ? kShortRows : INT_MAX, p.seq};
     return dtype == GDN2_BF16 ? launch_dim<__nv_bfloat16>(p, d, stream) : launch_dim<__half>(p, d, stream);
   });
 }

@@ -70,11 +70,10 @@ struct Span {
   }
 };
 // What the rows of a call see.  A window that reaches over the longest sequence is none.  But where the output's rest is kept for
-// a backward, sequences of one tile of queries go the window's way (`apart`), in launches of their own where there are longer
-// ones, so that a sequence's gradients do not depend on what it is packed with: with few keys the rounding of delta that the
-// rest undoes counts most (gradients off by 2.1 roundings at 3 tokens, 1.8 at 11, 1.6 at 100, and by 1.5 with it), for an
-// eighth of a training step (64 x 128 tokens, 16 heads, 4 key heads: 136 us for 120).  Two tiles are gone through in another
-// order than without a window, and give other bits.
+// a backward, that of sequences of one tile of queries is (`apart`), whatever else there is in the call: with few keys the
+// rounding of delta that it undoes counts most (gradients off by 2.1 roundings at 3 tokens, 1.8 at 11, 1.6 at 100, and by 1.5
+// with it).  In the forward they go the window's way for it, in a launch of their own where there are longer ones, since two
+// tiles are gone through in another order than without a window, and give other bits.
 constexpr int kShortRows = GDN2_WINDOW_SHORT_ROWS;
 static_assert(kShortRows == kTileRows / 2, "");
 constexpr Span kShortSpan{kShortRows, 0};

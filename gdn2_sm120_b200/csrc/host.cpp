@@ -1103,7 +1103,7 @@ PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   others.end();
   const bool parts = size > 2 * statistics->numel() + 15;   // sums of several CTAs are added up
   const char* name = window == 0 ? "gdn2_attention_backward" : "gdn2_window_attention_backward";
-  if (!ok(status, name, (parts ? 4 : 3) * passes(bounds, rest != nullptr && window >= longest(bounds, h.time)))) return nullptr;
+  if (!ok(status, name, (parts ? 4 : 3) * passes(bounds))) return nullptr;
   PyObject* result = PyTuple_New(3);
   for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(result, i, wrap(grads[i]));
   return result;

@@ -11,8 +11,8 @@ The first two are differentiable and run on the kernels of causal attention (csr
 pass over the tiles that no row of theirs sees.  What is said in attention.py about types, heads, roundings and values that are
 not finite holds here, with tiles that the window's edge or the sinks' end crosses beside those on the diagonal.  Delta alone is
 taken more exactly: from the output and what its rounding left over, which is kept for the backward.  A window that reaches over
-the longest sequence is causal attention, bit for bit; but there the gradients of sequences of at most 128 tokens are taken the
-window's way, whatever they are packed with.
+the longest sequence is causal attention, bit for bit; but there, too, the gradients of sequences of at most 128 tokens have
+delta with what rounding left over, whatever they are packed with.
 """
 
 from __future__ import annotations
