@@ -159,7 +159,7 @@ def _native(q, k, v, bounds, scale, window, training):
 
 def _attention(q, k, v, bounds, scale, window=(0, 0)):
     if forward_ad._current_level >= 0:
-        _validate.refuse_tangents("causal attention", q, k, v)
+        _validate.refuse_tangents("causal attention" if window == (0, 0) else "attention with a window", q, k, v)
     if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v)):
         return _CausalAttention.apply(q, k, v, bounds, scale, window)
     done = _native(q, k, v, bounds, scale, window, False)
