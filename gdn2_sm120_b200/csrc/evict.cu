@@ -199,7 +199,10 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const __grid_
     if (count <= kListed) {  // few are left: the one that wanted - 1 others are above is compared with all of them
       for (int t = first + tid; t < last; t += kSelectThreads) {
         const uint32_t x = key(t);
-        if (x >= lo && x <= hi) list[atomicAdd(&listed, 1)] = x;
+        if (x >= lo && x <= hi) {
+          const int at = atomicAdd(&listed, 1);
+          if (at < kListed) list[at] = x;   // (as many as were counted, unless somebody writes weights meanwhile)
+        }
       }
       __syncthreads();
       if (tid < count) {
@@ -287,11 +290,12 @@ __global__ void __launch_bounds__(kGatherThreads, 4) gather_kernel(const __grid_
   if (count <= 0) return;
   int64_t from = 0, to = -1;   // rows of keys of token j0 + lane, -1 for none
   if (lane < count) {
-    const int j = j0 + lane, t = length <= p.keep ? j : p.tokens[int64_t(unit) * p.keep + j];
+    // (a token of the sequence and a page of the cache, unless somebody writes lengths, weights or tables meanwhile)
+    const int j = j0 + lane, t = min(max(length <= p.keep ? j : p.tokens[int64_t(unit) * p.keep + j], 0), p.columns * p.page - 1);
     int t_place, j_place;
     const int page = p.new_table[b * p.new_stride + p.by_page.split(j, &j_place)];
     const int64_t source = p.table[b * p.table_stride + p.by_page.split(t, &t_place)];
-    if (page >= 0 && page < p.pages) {
+    if (page >= 0 && page < p.pages && source >= 0 && source < p.pages) {
       p.weight_pages[(int64_t(page) * p.kv_heads + head) * p.page + j_place] = p.weight_pages[(source * p.kv_heads + head) * p.page + t_place];
       from = (source * p.page + t_place) * p.kv_heads + head;
       to = (int64_t(page) * p.page + j_place) * p.kv_heads + head;
