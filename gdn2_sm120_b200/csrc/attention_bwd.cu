@@ -17,13 +17,14 @@
 // before it in its tile, a query dk and a cotangent dv of the keys behind it there.  (Another sequence's rows never.)
 //
 // Training 4 x 2048 tokens, 16 heads of 128 channels, 4 heads a group, each kernel by itself: delta 11 us, keys 121, queries 120, forward 73.
-
 //
 // With a window (kWindow) delta is taken from the output and what its rounding has left over: where rows see few tokens delta's
 // own error counts most.  Gradients' errors in the 2-norm without it and with it, in roundings: a window of 2 tokens 2.3 and 1.5, 4
 // 1.8 and 1.5, 10 1.6 and 1.45, 100 1.48 and 1.43; it costs 13 us of the 242 of the training step below (in 8 bits, whose rows are
 // half sectors, 18).  Each of the two goes over the tiles that its rows see or are seen by, and those of the sinks: 4 x 2048
-// tokens as above, a window of 512 and 16 sinks: keys and queries 155 us together, forward 69, delta 16.
+// tokens as above, a window of 512 and 16 sinks: keys and queries 155 us together, forward 69, delta 16.  Where a
+// window reaches over everything, the gradients of sequences of one tile have their delta taken that way, too; the rest is as
+// without one.
 
 #include <algorithm>
 #include <climits>

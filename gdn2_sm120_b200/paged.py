@@ -9,7 +9,8 @@ business: a row of ``page_table`` names them, its cached token ``t`` lies in pag
                      plain decoding
 
 A step of speculative decoding: ``tree_attention`` with the drafts' keys and values beside the cache, then
-``append_tokens`` with the slots of the accepted ones (-1 for the others).  Kernels: csrc/paged.cu.
+``append_tokens`` with the slots of the accepted ones (-1 for the others).  Kernels: csrc/paged.cu,
+csrc/paged_tiles.cuh, csrc/paged_tree.cuh.
 """
 
 from __future__ import annotations
