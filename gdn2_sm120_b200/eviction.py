@@ -66,9 +66,9 @@ def weighed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scal
     """``causal_attention``, and the weight that every token got: ``(output, weights)``.
 
     ``weights [B, T, Hkv]`` (fp32): the softmax weights that a token was given by itself and by the tokens behind it, summed over
-    these and over the heads of a group.  They are formed from scores in 32 bits,
-    by exponentials of which a quarter is good to 7e-6.  A query that has a score of NaN or +inf
-    makes the weights of the tokens that it sees NaN; values do not enter them.  No gradients."""
+    these and over the heads of a group.  They are formed from scores in 32 bits, by exponentials of which a quarter is good to
+    7e-6.  A query that has a score of NaN or +inf makes the weights of the tokens that it sees NaN; values do not enter them.
+    No gradients."""
 
     return _weighed("weighed_attention", q, k, v, None, scale)
 

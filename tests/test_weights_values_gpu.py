@@ -82,3 +82,29 @@ def test_a_page_number_outside_the_cache_makes_its_sequences_weights_nan(tokens,
             assert torch.isnan(got[~lost]).all() and torch.equal(got[lost], before[pages, :, t % 16][lost])
         touched[pages, :, t % 16] = True
     assert torch.equal(cache[2][~touched], before[~touched])
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_scores_that_are_nan_or_infinite_make_weights_nan(what):
+    """Those of the tokens that a query with such a score sees, in its key head, and no others."""
+
+    q, k, v = _inputs((1, 300), 4, 2, 64)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    want = weighed_attention(q, k, v)[1]
+    strange = k.clone()
+    strange[0, 299, 1, 0] = what          # the last query alone sees it
+    weights = weighed_attention(q, strange, v)[1]
+    assert torch.isnan(weights[0, :, 1]).all() and torch.equal(weights[0, :, 0], want[0, :, 0])
+    cache, slots = _cache(2, 300, 3)
+    q, k, v = _inputs((2, 3), 4, 2, 64)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    clean = [x.clone() for x in cache]
+    weighed_token_attention(q, k, v, *clean, slots)
+    cache[0][cache[3][0, 4].long(), 3, 1, 0] = what
+    weighed_token_attention(q, k, v, *cache, slots)
+    places = torch.arange(303, device=DEV)
+    for b in range(2):
+        pages = cache[3][b, places // 16].long()
+        got, kept = cache[2][pages, :, places % 16], clean[2][pages, :, places % 16]
+        assert torch.equal(got[:, 0], kept[:, 0])
+        assert torch.isnan(got[:, 1]).all() if b == 0 else torch.equal(got[:, 1], kept[:, 1])

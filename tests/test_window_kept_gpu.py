@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import gc
+
 import pytest
 import torch
 
@@ -29,6 +31,7 @@ def test_nothing_is_kept_that_the_backward_does_not_read(lengths, python):
     bounds = _bounds(lengths)
     q, k, v, _ = _inputs((1, bounds[-1]), 4, 2, 64, BF16, seed=8)
     q.requires_grad_(True)
+    gc.collect()      # what earlier tests have left does not go away meanwhile
 
     def held(call, *args):
         before = torch.cuda.memory_allocated()
